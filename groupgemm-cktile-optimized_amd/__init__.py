@@ -25,7 +25,7 @@ LIB_PATH = os.path.join(PKG_DIR, "lib", "libgg_mi355x.so")
 
 GG_OK, GG_ERR_UNSUPPORTED, GG_ERR_INVALID, GG_ERR_HIP, GG_ERR_WORKSPACE = 0, 1, 2, 3, 4
 
-# Every symbol include/gg_grouped_gemm.h declares, with its ctypes signature.
+# Every symbol include/gg_grouped_gemm.h and include/gg_moe_layer.h declare, with its ctypes signature.
 C_API = {
     "gg_prepare": (ctypes.c_int, [ctypes.c_int, ctypes.c_int, ctypes.c_int64, ctypes.c_int64,
                                   ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p, ctypes.c_void_p,
@@ -85,6 +85,29 @@ C_API = {
                                             ctypes.c_int64, ctypes.POINTER(ctypes.c_int64), ctypes.c_void_p,
                                             ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                             ctypes.c_void_p, ctypes.POINTER(ctypes.c_void_p)]),
+    # include/gg_moe_layer.h
+    "gg_layer_last_error": (ctypes.c_char_p, []),
+    "gg_rms_norm": (ctypes.c_int, [ctypes.c_int] * 4 + [ctypes.c_int64] * 2 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_int64,
+                                   ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int64]
+                    + [ctypes.c_void_p] * 5),
+    "gg_rms_norm_backward_workspace": (ctypes.c_size_t, [ctypes.c_int64] * 2),
+    "gg_rms_norm_backward": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_int64,
+                                            ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                            ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
+                                            ctypes.c_void_p]),
+    "gg_route_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
+    "gg_route": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                ctypes.c_int64] + [ctypes.c_void_p] * 10 + [ctypes.c_size_t, ctypes.c_void_p]),
+    "gg_route_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                         ctypes.c_int64] + [ctypes.c_void_p] * 8),
+    "gg_dispatch": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                   ctypes.c_int64] + [ctypes.c_void_p] * 4),
+    "gg_dispatch_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64]
+                             + [ctypes.c_void_p] * 4),
+    "gg_combine": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64] + [ctypes.c_void_p] * 5),
+    "gg_combine_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int,
+                                           ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 7),
+    "gg_gemm_w4": (ctypes.c_int, [ctypes.c_int, ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_int] + [ctypes.c_void_p] * 8),
 }
 
 _lib: Optional[ctypes.CDLL] = None
@@ -787,3 +810,19 @@ def grouped_gemm(x, w, group_m, out=None, stream: Optional[int] = None, group_of
     finally:
         be.release()
     return out
+
+
+# The operators around the grouped GEMM in a mixture-of-experts layer (moe_layer.py). Loaded on first use: that
+# module imports torch, which a process that times the hipBLASLt baselines must not.
+_LAYER = ("NormOutput", "Routing", "W4Weights", "combine", "combine_backward", "dispatch", "dispatch_backward",
+          "grouped_gemm_w4", "pack_w4", "quantize_w4", "rms_norm", "rms_norm_backward", "route", "route_backward")
+
+
+def __getattr__(name):
+    if name not in _LAYER:
+        raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
+    from . import moe_layer
+
+    for n in _LAYER:
+        globals()[n] = getattr(moe_layer, n)
+    return globals()[name]

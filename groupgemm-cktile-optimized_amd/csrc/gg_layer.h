@@ -1,0 +1,99 @@
+// Shared pieces of the layer operators (gg_norm.hip, gg_route.hip, gg_rows.hip, gg_w4.hip): the
+// message of the last failed call, argument checks, 16-byte vectors of 16-bit values as float32 and
+// reductions over the lanes of a wave.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <type_traits>
+
+#include "gg_moe_layer.h"
+
+namespace gg {
+namespace layer {
+
+// A fixed buffer, so that no entry point can throw. Defined in gg_norm.hip.
+extern thread_local char g_error[256];
+
+inline int fail(int status, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(g_error, sizeof(g_error), fmt, ap);
+    va_end(ap);
+    return status;
+}
+
+// One launch on `stream`; its own status, not one that an earlier call of the process left behind.
+template <typename... P>
+int launch(const char *what, void (*kernel)(P...), int64_t grid, int threads, hipStream_t stream,
+           std::type_identity_t<P>... args) {
+    void            *ptrs[] = {&args...};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(static_cast<unsigned>(grid)),
+                                         dim3(static_cast<unsigned>(threads)), ptrs, 0, stream);
+    return e == hipSuccess ? static_cast<int>(GG_OK) : fail(GG_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
+}
+
+inline bool aligned(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
+inline bool is16(int dtype) { return dtype == GG_DTYPE_BF16 || dtype == GG_DTYPE_FP16; }
+inline bool is8(int dtype) { return dtype == GG_DTYPE_FP8_E4M3 || dtype == GG_DTYPE_FP8_E5M2; }
+
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef float    f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16   bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// 16-bit element types. pair: two of them from the halves of a word; word: the reverse, rounded to nearest even.
+struct BF16 {
+    static __device__ __forceinline__ void pair(unsigned w, float &lo, float &hi) {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xffff0000u);
+    }
+    static __device__ __forceinline__ unsigned word(float lo, float hi) {
+        return __builtin_bit_cast(unsigned, bf16x2{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
+    }
+};
+struct F16 {
+    static __device__ __forceinline__ void pair(unsigned w, float &lo, float &hi) {
+        const f16x2 v = __builtin_bit_cast(f16x2, w);
+        lo            = static_cast<float>(v[0]);
+        hi            = static_cast<float>(v[1]);
+    }
+    static __device__ __forceinline__ unsigned word(float lo, float hi) {
+        return __builtin_bit_cast(unsigned, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
+    }
+};
+
+// Eight values of 16 bytes.
+template <typename T> __device__ __forceinline__ void unpack8(const u32x4 &w, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        T::pair(w[i], v[2 * i], v[2 * i + 1]);
+}
+template <typename T> __device__ __forceinline__ u32x4 pack8(const float (&v)[8]) {
+    u32x4 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        w[i] = T::word(v[2 * i], v[2 * i + 1]);
+    return w;
+}
+
+// Sum over the wave, in every lane; the same order in every run.
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        v += __shfl_xor(v, d);
+    return v;
+}
+__device__ __forceinline__ unsigned wave_max(unsigned v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        v = max(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), d)));
+    return v;
+}
+
+} // namespace layer
+} // namespace gg

@@ -1,0 +1,560 @@
+// RMS norm with the residual's addition, 16-bit or fp8 output, and its gradients (gg_rms_norm,
+// gg_rms_norm_backward in include/gg_moe_layer.h).
+//
+// Forward: h = round(x + r), rstd = (mean h^2 + eps)^-1/2, y = h rstd w. A row stays in the registers
+// of the waves that work on it (one wave up to 1024 values, four up to 16384, sixteen up to 32768), so
+// x and r are read once and h and y written once: bound by HBM. The tensor scale needs the largest |y|
+// of all rows before the first value is rounded: a first pass writes h, rstd and one maximum per
+// workgroup, a second reads h again and rounds.
+//
+// The norm is taken of the rounded h, the value that later layers and the backward pass read, so the
+// passes agree whatever the scale.
+#include "gg_layer.h"
+
+#include <algorithm>
+
+namespace gg {
+namespace layer {
+
+thread_local char g_error[256] = "";
+
+namespace {
+
+constexpr int kMaxParts = GG_NORM_WORKSPACE / 4; // workgroups of a tensor scale's first pass
+
+struct NormArgs {
+    const void *x, *residual, *weight;
+    void       *h, *y;
+    float      *rstd, *scale, *parts;
+    int64_t     rows, x_stride, r_stride, h_stride;
+    int         hidden, mode, n_parts;
+    float       eps;
+    bool        w32, e5m2;
+};
+
+// Eight weights from element i on, as float32.
+template <typename T> __device__ __forceinline__ void load_w(const void *w, bool w32, int i, float (&v)[8]) {
+    if (w32) {
+        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(w) + i);
+        const f32x4  a = p[0], b = p[1];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[j]     = a[j];
+            v[4 + j] = b[j];
+        }
+    } else {
+        unpack8<T>(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(w) + i), v);
+    }
+}
+
+// Saturates (the conversion would give NaN past the largest value); a NaN stays one.
+__device__ __forceinline__ float saturate(float v, float top) { return v != v ? v : fminf(fmaxf(v, -top), top); }
+
+__device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], bool e5m2) {
+    u32x2 w;
+    const float top = e5m2 ? 57344.f : 448.f;
+    float s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        s[i] = saturate(v[i], top);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        int q = 0;
+        if (e5m2) {
+            q = __builtin_amdgcn_cvt_pk_bf8_f32(s[4 * i], s[4 * i + 1], q, false);
+            q = __builtin_amdgcn_cvt_pk_bf8_f32(s[4 * i + 2], s[4 * i + 3], q, true);
+        } else {
+            q = __builtin_amdgcn_cvt_pk_fp8_f32(s[4 * i], s[4 * i + 1], q, false);
+            q = __builtin_amdgcn_cvt_pk_fp8_f32(s[4 * i + 2], s[4 * i + 3], q, true);
+        }
+        w[i] = static_cast<unsigned>(q);
+    }
+    return w;
+}
+
+// Scale of the largest |y| (bits of a float >= 0 or NaN): 1 where the quotient is zero or subnormal, whose
+// reciprocal would be infinite.
+__device__ __forceinline__ float scale_of(unsigned top_bits, bool e5m2) {
+    const float s = __uint_as_float(top_bits) / (e5m2 ? 57344.f : 448.f);
+    return s < 1.17549435e-38f ? 1.f : s;
+}
+
+// Reductions over the WPR waves of a row; `turn` alternates so that one barrier per call is enough.
+template <int WPR> struct RowReduce {
+    float    sums[2][WPR];
+    unsigned tops[2][WPR];
+};
+template <int WPR> __device__ __forceinline__ float row_sum(RowReduce<WPR> &m, int turn, float v, int wave, int lane) {
+    v = wave_sum(v);
+    if constexpr (WPR == 1)
+        return v;
+    if (lane == 0)
+        m.sums[turn][wave] = v;
+    __syncthreads();
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < WPR; ++i)
+        s += m.sums[turn][i];
+    return s;
+}
+template <int WPR> __device__ __forceinline__ unsigned row_max(RowReduce<WPR> &m, int turn, unsigned v, int wave, int lane) {
+    v = wave_max(v);
+    if constexpr (WPR == 1)
+        return v;
+    if (lane == 0)
+        m.tops[turn][wave] = v;
+    __syncthreads();
+    unsigned s = 0;
+#pragma unroll
+    for (int i = 0; i < WPR; ++i)
+        s = max(s, m.tops[turn][i]);
+    return s;
+}
+
+constexpr int block_threads(int wpr) { return wpr == 1 ? 256 : 64 * wpr; }
+constexpr int rows_per_block(int wpr) { return wpr == 1 ? 4 : 1; }
+
+// One pass over the rows. FIRST: the first pass of a tensor scale (no y; the workgroup's largest |y|).
+template <typename T, int WPR, int U, bool FIRST>
+__global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs a) {
+    __shared__ RowReduce<WPR> m;
+    __shared__ unsigned       block_top[4];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t    = WPR == 1 ? lane : static_cast<int>(threadIdx.x); // thread of the row
+    unsigned  top  = 0;
+    int       turn = 0;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * rows_per_block(WPR);
+    // every wave of a block that shares a row makes the same trips, so the barriers match
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0); row < a.rows;
+         row += step, turn ^= 1) {
+        float v[U][8];
+        float sq = 0.f;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * 64 * WPR + t) * 8;
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[u][j] = 0.f;
+            if (i < a.hidden) {
+                const u32x4 xw = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.x) + row * a.x_stride + i);
+                unpack8<T>(xw, v[u]);
+                if (a.residual != nullptr) {
+                    float r[8];
+                    unpack8<T>(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.residual) + row * a.r_stride + i), r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        v[u][j] += r[j];
+                    const u32x4 hw = pack8<T>(v[u]);
+                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.h) + row * a.h_stride + i) = hw;
+                    unpack8<T>(hw, v[u]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    sq = fmaf(v[u][j], v[u][j], sq);
+            }
+        }
+        sq = row_sum<WPR>(m, turn, sq, wave, lane);
+        const float rstd = 1.f / sqrtf(sq / static_cast<float>(a.hidden) + a.eps);
+        if (t == 0 && a.rstd != nullptr)
+            a.rstd[row] = rstd;
+        unsigned row_top = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * 64 * WPR + t) * 8;
+            if (i < a.hidden) {
+                float w[8];
+                load_w<T>(a.weight, a.w32, i, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[u][j] = v[u][j] * rstd * w[j];
+                    row_top = max(row_top, __float_as_uint(fabsf(v[u][j])));
+                }
+            }
+        }
+        if constexpr (FIRST) {
+            top = max(top, row_top);
+        } else {
+            float inv = 1.f;
+            if (a.mode == GG_NORM_SCALE_ROW) {
+                const float s = scale_of(row_max<WPR>(m, turn, row_top, wave, lane), a.e5m2);
+                inv           = 1.f / s;
+                if (t == 0)
+                    a.scale[row] = s;
+            } else if (a.mode == GG_NORM_SCALE_GIVEN) {
+                inv = 1.f / a.scale[0];
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = (u * 64 * WPR + t) * 8;
+                if (i < a.hidden) {
+                    if (a.mode == GG_NORM_PLAIN) {
+                        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.y) + row * a.hidden + i) = pack8<T>(v[u]);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            v[u][j] *= inv;
+                        *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v[u], a.e5m2);
+                    }
+                }
+            }
+        }
+    }
+    if constexpr (FIRST) {
+        top = wave_max(top);
+        constexpr int waves = block_threads(WPR) / 64;
+        static_assert(waves <= 16, "");
+        if constexpr (WPR == 1) {
+            if (lane == 0)
+                block_top[wave] = top;
+        } else {
+            __syncthreads(); // the last row's tops are read
+            if (lane == 0)
+                m.tops[0][wave] = top;
+        }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            unsigned s = 0;
+            for (int i = 0; i < waves; ++i)
+                s = max(s, WPR == 1 ? block_top[i & 3] : m.tops[0][i % WPR]);
+            reinterpret_cast<unsigned *>(a.parts)[blockIdx.x] = s;
+        }
+    }
+}
+
+// The tensor scale's second pass: the largest of the first pass's maxima, then y from h and rstd.
+template <typename T> __global__ void __launch_bounds__(256) quantize_kernel(const NormArgs a) {
+    __shared__ unsigned tops[4];
+    unsigned            top = 0;
+    for (int i = threadIdx.x; i < a.n_parts; i += 256)
+        top = max(top, reinterpret_cast<const unsigned *>(a.parts)[i]);
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0)
+        tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    const float s   = scale_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])), a.e5m2);
+    const float inv = 1.f / s;
+    if (blockIdx.x == 0 && threadIdx.x == 0)
+        a.scale[0] = s;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float rstd = a.rstd[row];
+        for (int i = threadIdx.x * 8; i < a.hidden; i += 2048) {
+            float v[8], w[8];
+            unpack8<T>(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i), v);
+            load_w<T>(a.weight, a.w32, i, w);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[j] = v[j] * rstd * w[j] * inv;
+            *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v, a.e5m2);
+        }
+    }
+}
+
+struct BackArgs {
+    const void  *g, *h, *weight, *gh;
+    const float *rstd;
+    void        *gx;
+    float       *parts; // [waves' or workgroups' rows][hidden] partial sums of grad_weight
+    int64_t      rows, g_stride, h_stride, gh_stride;
+    int          hidden;
+    bool         w32;
+};
+
+// grad_x row by row; grad_weight's partial sums stay in registers over the rows of a workgroup (of a wave
+// where a wave has a row) and are written once.
+template <typename T, int WPR, int U>
+__global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const BackArgs a) {
+    __shared__ RowReduce<WPR> m;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t    = WPR == 1 ? lane : static_cast<int>(threadIdx.x);
+    float     dw[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            dw[u][j] = 0.f;
+    int           turn = 0;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * rows_per_block(WPR);
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0); row < a.rows;
+         row += step, turn ^= 1) {
+        u32x4 gw[U], hw[U], rw[U];
+        float dot = 0.f;
+        const float rstd = a.rstd[row];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * 64 * WPR + t) * 8;
+            if (i < a.hidden) {
+                gw[u] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.g) + row * a.g_stride + i);
+                hw[u] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i);
+                if (a.gh != nullptr)
+                    rw[u] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.gh) + row * a.gh_stride + i);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * 64 * WPR + t) * 8;
+            if (i < a.hidden) {
+                float g[8], h[8], w[8];
+                unpack8<T>(gw[u], g);
+                unpack8<T>(hw[u], h);
+                load_w<T>(a.weight, a.w32, i, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    dot      = fmaf(g[j] * w[j], h[j], dot);
+                    dw[u][j] = fmaf(g[j] * h[j], rstd, dw[u][j]);
+                }
+            }
+        }
+        dot = row_sum<WPR>(m, turn, dot, wave, lane);
+        const float c = rstd * rstd * rstd * (dot / static_cast<float>(a.hidden));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * 64 * WPR + t) * 8;
+            if (i < a.hidden) {
+                float g[8], h[8], w[8], r[8];
+                unpack8<T>(gw[u], g);
+                unpack8<T>(hw[u], h);
+                load_w<T>(a.weight, a.w32, i, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    g[j] = rstd * (g[j] * w[j]) - h[j] * c;
+                if (a.gh != nullptr) {
+                    unpack8<T>(rw[u], r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        g[j] += r[j];
+                }
+                *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.gx) + row * a.hidden + i) = pack8<T>(g);
+            }
+        }
+    }
+    float *part = a.parts + (static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0)) * a.hidden;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = (u * 64 * WPR + t) * 8;
+        if (i < a.hidden) {
+            f32x4 *p = reinterpret_cast<f32x4 *>(part + i);
+            p[0]     = f32x4{dw[u][0], dw[u][1], dw[u][2], dw[u][3]};
+            p[1]     = f32x4{dw[u][4], dw[u][5], dw[u][6], dw[u][7]};
+        }
+    }
+}
+
+// grad_weight: the sum of the partial sums of each column, in their order; 64 columns by 16 slices a workgroup.
+template <typename T>
+__global__ void __launch_bounds__(1024) weight_sum_kernel(const float *parts, int n_parts, int hidden, void *out, bool w32) {
+    __shared__ float sums[16][64];
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
+    const int per = (n_parts + 15) / 16;
+    float     s   = 0.f;
+    if (col < hidden)
+        for (int p = slice * per; p < min(n_parts, (slice + 1) * per); ++p)
+            s += parts[static_cast<int64_t>(p) * hidden + col];
+    sums[slice][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (slice == 0 && col < hidden) {
+        for (int i = 1; i < 16; ++i)
+            s += sums[i][threadIdx.x];
+        if (w32)
+            static_cast<float *>(out)[col] = s;
+        else
+            static_cast<uint16_t *>(out)[col] = static_cast<uint16_t>(T::word(s, 0.f));
+    }
+}
+
+int waves_per_row(int64_t hidden) { return hidden <= 1024 ? 1 : hidden <= 16384 ? 4 : 16; }
+
+int64_t row_blocks(int64_t rows, int64_t hidden) {
+    const int per = rows_per_block(waves_per_row(hidden));
+    return (rows + per - 1) / per;
+}
+
+// f(WPR, U) of the instance for `hidden` values a row: U pieces of 8 per lane.
+template <typename F> int with_shape(int64_t hidden, F f) {
+    using std::integral_constant;
+    const int wpr = waves_per_row(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+#define GG_SHAPE(W, N)                                                                                                 \
+    if (wpr == W && u <= N)                                                                                            \
+        return f(integral_constant<int, W>{}, integral_constant<int, N>{});
+    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(4, 4) GG_SHAPE(4, 6) GG_SHAPE(4, 8)
+#undef GG_SHAPE
+    return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+}
+
+constexpr int64_t kMaxBlocks = int64_t(1) << 20;
+
+template <typename T> int run_norm(const NormArgs &a, hipStream_t s) {
+    const int64_t blocks = row_blocks(a.rows, a.hidden);
+    if (a.mode != GG_NORM_SCALE_TENSOR)
+        return with_shape(a.hidden, [&](auto wpr, auto u) {
+            return launch("rms_norm", norm_kernel<T, wpr.value, u.value, false>, std::min(blocks, kMaxBlocks),
+                          block_threads(wpr.value), s, a);
+        });
+    NormArgs b = a;
+    b.n_parts  = static_cast<int>(std::min<int64_t>(blocks, kMaxParts));
+    if (b.residual == nullptr) { // h is x
+        b.h        = const_cast<void *>(b.x);
+        b.h_stride = b.x_stride;
+    }
+    const int st = with_shape(a.hidden, [&](auto wpr, auto u) {
+        return launch("rms_norm", norm_kernel<T, wpr.value, u.value, true>, b.n_parts, block_threads(wpr.value), s, b);
+    });
+    return st ? st : launch("rms_norm", quantize_kernel<T>, std::min<int64_t>(b.rows, 8192), 256, s, b);
+}
+
+// Workgroups of the backward pass: enough to fill the GPU four times over, few enough that their partial sums
+// are a small part of what is read.
+constexpr int64_t kBackBlocks = 1024;
+int64_t back_blocks(int64_t rows, int64_t hidden) {
+    const int64_t b = row_blocks(rows, hidden);
+    return b < kBackBlocks ? b : kBackBlocks;
+}
+int64_t back_parts(int64_t rows, int64_t hidden) {
+    return back_blocks(rows, hidden) * rows_per_block(waves_per_row(hidden));
+}
+
+template <typename T> int run_back(const BackArgs &a, void *grad_weight, hipStream_t s) {
+    const int st = with_shape(a.hidden, [&](auto wpr, auto u) {
+        return launch("rms_norm_backward", norm_back_kernel<T, wpr.value, u.value>, back_blocks(a.rows, a.hidden),
+                      block_threads(wpr.value), s, a);
+    });
+    return st ? st : launch("rms_norm_backward", weight_sum_kernel<T>, (a.hidden + 63) / 64, 1024, s, a.parts,
+                            static_cast<int>(back_parts(a.rows, a.hidden)), a.hidden, grad_weight, a.w32);
+}
+
+// Rules shared by both passes.
+int check_norm(int dtype, int weight_dtype, int64_t rows, int64_t hidden) {
+    if (!is16(dtype))
+        return fail(GG_ERR_INVALID, "dtype must be GG_DTYPE_BF16 or GG_DTYPE_FP16");
+    if (weight_dtype != dtype && weight_dtype != GG_DTYPE_FP32)
+        return fail(GG_ERR_INVALID, "weight_dtype must be dtype or GG_DTYPE_FP32");
+    if (rows < 0 || hidden < 1)
+        return fail(GG_ERR_INVALID, "rows must be >= 0 and hidden >= 1");
+    if (hidden % 8 != 0 || hidden > 32768)
+        return fail(GG_ERR_UNSUPPORTED, "hidden must be a multiple of 8 and at most 32768");
+    return GG_OK;
+}
+// A matrix operand: rows at least hidden apart, 16-byte pieces.
+int check_rows(const char *name, const void *p, int64_t stride, int64_t rows) {
+    if (rows > 0 && p == nullptr)
+        return fail(GG_ERR_INVALID, "%s is null", name);
+    if (rows > 1 && stride < 0)
+        return fail(GG_ERR_INVALID, "%s has a negative row stride", name);
+    if (!aligned(p, 16) || (rows > 1 && stride % 8 != 0))
+        return fail(GG_ERR_UNSUPPORTED, "%s must be 16-byte aligned with row strides of multiples of 8", name);
+    return GG_OK;
+}
+
+} // namespace
+} // namespace layer
+} // namespace gg
+
+using namespace gg::layer;
+
+extern "C" {
+
+const char *gg_layer_last_error(void) { return g_error; }
+
+int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
+                const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight,
+                void *h, int64_t h_stride, void *y, float *rstd, float *scale, void *workspace, void *stream) {
+    g_error[0] = 0;
+    if (const int st = check_norm(dtype, weight_dtype, rows, hidden))
+        return st;
+    if (scale_mode < GG_NORM_PLAIN || scale_mode > GG_NORM_SCALE_GIVEN)
+        return fail(GG_ERR_INVALID, "scale_mode must be a gg_norm_scale");
+    if (scale_mode == GG_NORM_PLAIN ? out_dtype != dtype : !is8(out_dtype))
+        return fail(GG_ERR_INVALID, "out_dtype must be dtype, or an fp8 type with a scale");
+    if (scale_mode != GG_NORM_PLAIN && scale == nullptr)
+        return fail(GG_ERR_INVALID, "scale is null");
+    if (rows == 0 && scale_mode != GG_NORM_SCALE_TENSOR)
+        return GG_OK;
+    if (weight == nullptr || (rows > 0 && y == nullptr))
+        return fail(GG_ERR_INVALID, "weight and y must be device pointers");
+    if (scale_mode == GG_NORM_SCALE_TENSOR && (workspace == nullptr || (rows > 0 && rstd == nullptr)))
+        return fail(GG_ERR_INVALID, "a tensor scale needs workspace and rstd");
+    if (const int st = check_rows("x", x, x_stride, rows))
+        return st;
+    if (residual != nullptr) {
+        if (const int st = check_rows("residual", residual, residual_stride, rows))
+            return st;
+        if (const int st = check_rows("h", h, h_stride, rows))
+            return st;
+        if (rows > 1 && h_stride < hidden)
+            return fail(GG_ERR_INVALID, "rows of h overlap");
+    }
+    if (!aligned(weight, 16) || !aligned(y, scale_mode == GG_NORM_PLAIN ? 16 : 8) || !aligned(workspace, 4))
+        return fail(GG_ERR_UNSUPPORTED, "weight and y must be 16-byte aligned (fp8 y: 8)");
+    NormArgs a{};
+    a.x        = x;
+    a.residual = residual;
+    a.weight   = weight;
+    a.h        = h;
+    a.y        = y;
+    a.rstd     = rstd;
+    a.scale    = scale;
+    a.parts    = static_cast<float *>(workspace);
+    a.rows     = rows;
+    a.x_stride = x_stride;
+    a.r_stride = residual_stride;
+    a.h_stride = h_stride;
+    a.hidden   = static_cast<int>(hidden);
+    a.mode     = scale_mode;
+    a.eps      = eps;
+    a.w32      = weight_dtype == GG_DTYPE_FP32;
+    a.e5m2     = out_dtype == GG_DTYPE_FP8_E5M2;
+    if (rows == 0) { // no maximum: the scale alone
+        return launch("rms_norm", quantize_kernel<BF16>, 1, 256, static_cast<hipStream_t>(stream), a);
+    }
+    return dtype == GG_DTYPE_BF16 ? run_norm<BF16>(a, static_cast<hipStream_t>(stream))
+                                  : run_norm<F16>(a, static_cast<hipStream_t>(stream));
+}
+
+size_t gg_rms_norm_backward_workspace(int64_t rows, int64_t hidden) {
+    if (rows < 1 || hidden < 1 || hidden > 32768)
+        return 0;
+    return static_cast<size_t>(back_parts(rows, hidden)) * static_cast<size_t>(hidden) * 4;
+}
+
+int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidden, const void *grad_y,
+                         int64_t grad_y_stride, const void *h, int64_t h_stride, const void *weight, const float *rstd,
+                         const void *grad_h, int64_t grad_h_stride, void *grad_x, void *grad_weight, void *workspace,
+                         size_t workspace_bytes, void *stream) {
+    g_error[0] = 0;
+    if (const int st = check_norm(dtype, weight_dtype, rows, hidden))
+        return st;
+    if (weight == nullptr || grad_weight == nullptr || (rows > 0 && (grad_x == nullptr || rstd == nullptr)))
+        return fail(GG_ERR_INVALID, "weight, rstd, grad_x and grad_weight must be device pointers");
+    if (const int st = check_rows("grad_y", grad_y, grad_y_stride, rows))
+        return st;
+    if (const int st = check_rows("h", h, h_stride, rows))
+        return st;
+    if (grad_h != nullptr)
+        if (const int st = check_rows("grad_h", grad_h, grad_h_stride, rows))
+            return st;
+    if (!aligned(weight, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 4))
+        return fail(GG_ERR_UNSUPPORTED, "weight and grad_x must be 16-byte aligned, grad_weight 4-byte");
+    if (workspace_bytes < gg_rms_norm_backward_workspace(rows, hidden) || (rows > 0 && (workspace == nullptr || !aligned(workspace, 16))))
+        return fail(GG_ERR_WORKSPACE, "workspace must be 16-byte aligned and of gg_rms_norm_backward_workspace(rows, hidden) bytes");
+    BackArgs a{};
+    a.g         = grad_y;
+    a.h         = h;
+    a.weight    = weight;
+    a.gh        = grad_h;
+    a.rstd      = rstd;
+    a.gx        = grad_x;
+    a.parts     = static_cast<float *>(workspace);
+    a.rows      = rows;
+    a.g_stride  = grad_y_stride;
+    a.h_stride  = h_stride;
+    a.gh_stride = grad_h_stride;
+    a.hidden    = static_cast<int>(hidden);
+    a.w32       = weight_dtype == GG_DTYPE_FP32;
+    if (rows == 0) { // the sums of no rows
+        return launch("rms_norm_backward", weight_sum_kernel<BF16>, (a.hidden + 63) / 64, 1024,
+                      static_cast<hipStream_t>(stream), nullptr, 0, a.hidden, grad_weight, a.w32);
+    }
+    return dtype == GG_DTYPE_BF16 ? run_back<BF16>(a, grad_weight, static_cast<hipStream_t>(stream))
+                                  : run_back<F16>(a, grad_weight, static_cast<hipStream_t>(stream));
+}
+
+} // extern "C"
