@@ -22,64 +22,57 @@ _NORM_WORKSPACE = 8192  # GG_NORM_WORKSPACE
 _PLAIN, _TENSOR, _ROW, _GIVEN = 0, 1, 2, 3  # gg_norm_scale
 
 
-def _done(status: int) -> None:
-    if status != GG_OK:
-        raise GGError(status, load_library().gg_layer_last_error().decode())
+_lib = load_library()
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 
-def _matrix(name: str, t, cols: Optional[int] = None):
+def _call(fn, dev, stream: Optional[int], args, tensors) -> None:
+    """fn(*args, stream): on the current stream of `dev` or on a given one, with `dev` the current device. A
+    stream that is not torch's current one is told of the tensors it uses."""
+    current = _raw_stream(dev.index)
+    if dev.index == _current_device():
+        st = fn(*args, current if stream is None else stream)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, current if stream is None else stream)
+    if st != GG_OK:
+        raise GGError(st, _lib.gg_layer_last_error().decode())
+    if stream is not None and stream != current:
+        # (handle 0 is the default stream)
+        other = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
+        for t in tensors:
+            if t is not None:
+                t.record_stream(other)
+
+
+def _matrix(name: str, t):
     """Row stride of a device matrix whose rows are contiguous."""
     if t.dim() != 2 or not t.is_cuda:
         raise ValueError(f"{name} must be a device matrix")
-    if cols is not None and t.shape[1] != cols:
-        raise ValueError(f"{name} has {t.shape[1]} columns, not {cols}")
-    if t.stride(1) != 1 and t.shape[1] > 1:
+    rows, cols = t.stride()
+    if cols != 1 and t.shape[1] > 1:
         raise ValueError(f"{name} must have contiguous rows")
-    return t.stride(0)
+    return rows
 
 
-def _flat(name: str, t, dtype, shape, device) -> None:
+def _flat(name: str, t, dtype, shape, dev) -> None:
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}")
-    if t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous tensor of shape {list(shape)} on {device}")
+    if t.shape != shape or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of shape {list(shape)} on {dev}")
 
 
-def _out(name: str, t, dtype, shape, device):
+def _like(name: str, t, ref) -> None:
+    if t.dtype != ref.dtype or t.shape != ref.shape or t.device != ref.device:
+        raise ValueError(f"{name} must have the type, shape and device of its counterpart")
+
+
+def _out(t, dtype, shape, dev):
     if t is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _flat(name, t, dtype, shape, device)
+        return torch.empty(shape, dtype=dtype, device=dev)
+    _flat("out", t, dtype, shape, dev)
     return t
-
-
-class _On:
-    """The stream of a call on `device`, with that device current while it is entered. Tensors given to
-    use() are recorded on a stream that is not torch's current one."""
-
-    def __init__(self, device, stream: Optional[int]):
-        self.other = None
-        self.guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-        current = torch.cuda.current_stream(device)
-        self.stream = current.cuda_stream
-        if stream is not None and stream != self.stream:
-            self.stream = stream
-            # (the default stream has no tensors of its own to record: handle 0)
-            self.other = torch.cuda.ExternalStream(stream, device=device) if stream else torch.cuda.default_stream(device)
-
-    def use(self, *tensors) -> None:
-        if self.other is not None:
-            for t in tensors:
-                if t is not None:
-                    t.record_stream(self.other)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
 
 
 def _ptr(t) -> int:
@@ -107,36 +100,36 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
     "tensor": the x_scale of grouped_gemm_fp8), one for each row ("row"), or divided by a given device
     float32 scale [1]. out: y's buffer; out_h: h's, which may be x or residual itself.
     """
-    dt = _T16.get(x.dtype)
+    dtype = x.dtype
+    dt = _T16.get(dtype)
     if dt is None:
         raise TypeError("x must be bfloat16 or float16")
     xs = _matrix("x", x)
     (m, n), dev = x.shape, x.device
-    if weight.dtype not in (x.dtype, torch.float32):
+    wd = weight.dtype
+    if wd != dtype and wd != torch.float32:
         raise TypeError("weight must be of x's type or float32")
-    _flat("weight", weight, weight.dtype, (n,), dev)
-    rs = hs = 0
+    _flat("weight", weight, wd, (n,), dev)
+    rs = hs = hp = 0
+    h = x
     if residual is not None:
-        if residual.dtype != x.dtype or residual.device != dev or residual.shape != x.shape:
-            raise ValueError("residual must match x")
+        _like("residual", residual, x)
         rs = _matrix("residual", residual)
         if out_h is None:
-            h = torch.empty((m, n), dtype=x.dtype, device=dev)
+            h = torch.empty((m, n), dtype=dtype, device=dev)
+            hs = n
         else:
             h = out_h
-            if h.dtype != x.dtype or h.device != dev or h.shape != x.shape:
-                raise ValueError("out_h must match x")
-        hs = _matrix("out_h", h)
-    else:
-        if out_h is not None:
-            raise ValueError("out_h goes with a residual")
-        h = x
-    rstd = torch.empty(m, dtype=torch.float32, device=dev)
+            _like("out_h", h, x)
+            hs = _matrix("out_h", h)
+        hp = h.data_ptr()
+    elif out_h is not None:
+        raise ValueError("out_h goes with a residual")
     ws = s = None
-    if out_dtype is None or out_dtype == x.dtype:
+    if out_dtype is None or out_dtype == dtype:
         if scale is not None:
             raise ValueError("scale goes with an fp8 out_dtype")
-        out_dtype, od, mode = x.dtype, dt, _PLAIN
+        out_dtype, od, mode = dtype, dt, _PLAIN
     else:
         od = _T8.get(out_dtype)
         if od is None:
@@ -152,12 +145,12 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
             mode, s = _GIVEN, scale
             if s.dtype != torch.float32 or s.numel() != 1 or s.device != dev:
                 raise ValueError("scale must be 'tensor', 'row' or a device float32 tensor of one value")
-    y = _out("out", out, out_dtype, (m, n), dev)
-    with _On(dev, stream) as on:
-        _done(load_library().gg_rms_norm(dt, dt if weight.dtype == x.dtype else _FP32, od, mode, m, n, eps, x.data_ptr(), xs,
-                                         _ptr(residual), rs, weight.data_ptr(), 0 if residual is None else h.data_ptr(), hs,
-                                         y.data_ptr(), rstd.data_ptr(), _ptr(s), _ptr(ws), on.stream))
-        on.use(x, residual, weight, h, y, rstd, s, ws)
+    y = _out(out, out_dtype, (m, n), dev)
+    rstd = torch.empty(m, dtype=torch.float32, device=dev)
+    _call(_lib.gg_rms_norm, dev, stream, (dt, dt if wd == dtype else _FP32, od, mode, m, n, eps, x.data_ptr(), xs,
+                                          _ptr(residual), rs,
+                                          weight.data_ptr(), hp, hs, y.data_ptr(), rstd.data_ptr(), _ptr(s), _ptr(ws)),
+          (x, residual, weight, h, y, rstd, s, ws))
     return NormOutput(y, h, rstd, s)
 
 
@@ -165,29 +158,31 @@ def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Op
     """(grad_x, grad_weight) of rms_norm from its h and rstd (gg_rms_norm_backward). grad_x is the gradient
     of x and of residual; grad_h, the gradient that reaches h past the norm, is added to it. grad_y and
     grad_h are of h's type (an fp8 y is differentiated as if it were not rounded)."""
-    dt = _T16.get(h.dtype)
+    dtype = h.dtype
+    dt = _T16.get(dtype)
     if dt is None:
         raise TypeError("h must be bfloat16 or float16")
     hs = _matrix("h", h)
     (m, n), dev = h.shape, h.device
-    for name, t in (("grad_y", grad_y), ("grad_h", grad_h)):
-        if t is not None and (t.dtype != h.dtype or t.device != dev or t.shape != h.shape):
-            raise ValueError(f"{name} must match h")
-    gs = _matrix("grad_y", grad_y)
-    ghs = 0 if grad_h is None else _matrix("grad_h", grad_h)
-    if weight.dtype not in (h.dtype, torch.float32):
+    _like("grad_y", grad_y, h)
+    gs, ghs = _matrix("grad_y", grad_y), 0
+    if grad_h is not None:
+        _like("grad_h", grad_h, h)
+        ghs = _matrix("grad_h", grad_h)
+    wd = weight.dtype
+    if wd != dtype and wd != torch.float32:
         raise TypeError("weight must be of h's type or float32")
-    _flat("weight", weight, weight.dtype, (n,), dev)
+    _flat("weight", weight, wd, (n,), dev)
     _flat("rstd", rstd, torch.float32, (m,), dev)
-    gx = _out("out", out, h.dtype, (m, n), dev)
-    gw = torch.empty(n, dtype=weight.dtype, device=dev)
-    lib = load_library()
-    ws = torch.empty(lib.gg_rms_norm_backward_workspace(m, n), dtype=torch.uint8, device=dev)
-    with _On(dev, stream) as on:
-        _done(lib.gg_rms_norm_backward(dt, dt if weight.dtype == h.dtype else _FP32, m, n, grad_y.data_ptr(), gs, h.data_ptr(),
-                                       hs, weight.data_ptr(), rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(), gw.data_ptr(),
-                                       ws.data_ptr(), ws.numel(), on.stream))
-        on.use(grad_y, h, weight, rstd, grad_h, gx, gw, ws)
+    gx = _out(out, dtype, (m, n), dev)
+    gw = torch.empty(n, dtype=wd, device=dev)
+    need = _lib.gg_rms_norm_backward_workspace(m, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(_lib.gg_rms_norm_backward, dev, stream, (dt, dt if wd == dtype else _FP32, m, n, grad_y.data_ptr(), gs,
+                                                   h.data_ptr(), hs,
+                                                   weight.data_ptr(), rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(),
+                                                   gw.data_ptr(), ws.data_ptr(), need),
+          (grad_y, h, weight, rstd, grad_h, gx, gw, ws))
     return gx, gw
 
 
@@ -231,7 +226,6 @@ def route(logits, top_k: int, mask=None, renormalize: bool = True, balance: bool
         _flat("mask", mask, torch.bool, (t,), dev)
     if not 1 <= top_k <= e:
         raise ValueError("top_k must be in 1 .. E")
-    lib = load_library()
     experts = torch.empty((t, top_k), dtype=torch.int32, device=dev)
     rows = torch.empty((t, top_k), dtype=torch.int32, device=dev)
     weights = torch.empty((t, top_k), dtype=torch.float32, device=dev)
@@ -242,14 +236,14 @@ def route(logits, top_k: int, mask=None, renormalize: bool = True, balance: bool
     if balance:
         slope = torch.empty(e, dtype=torch.float32, device=dev)
         loss = torch.empty((), dtype=torch.float32, device=dev)
-    need = lib.gg_route_workspace(t, e, top_k)
+    need = _lib.gg_route_workspace(t, e, top_k)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    with _On(dev, stream) as on:
-        _done(lib.gg_route(dt, t, e, top_k, int(renormalize), logits.data_ptr(), stride, _ptr(mask), experts.data_ptr(),
-                           weights.data_ptr(), counts.data_ptr(), offs.data_ptr(), rows.data_ptr(), lse.data_ptr(), _ptr(loss),
-                           _ptr(slope), _ptr(ws), need, on.stream))
-        on.use(logits, mask, experts, weights, counts, offs, rows, lse, loss, slope, ws)
+    _call(_lib.gg_route, dev, stream, (dt, t, e, top_k, int(renormalize), logits.data_ptr(), stride, _ptr(mask),
+                                       experts.data_ptr(),
+                                       weights.data_ptr(), counts.data_ptr(), offs.data_ptr(), rows.data_ptr(), lse.data_ptr(),
+                                       _ptr(loss), _ptr(slope), _ptr(ws), need),
+          (logits, mask, experts, weights, counts, offs, rows, lse, loss, slope, ws))
     return Routing(experts, weights, counts, offs, rows, lse, slope, loss, bool(renormalize))
 
 
@@ -271,12 +265,12 @@ def route_backward(logits, routing: Routing, grad_weights=None, grad_loss=None, 
         _flat("routing.slope", r.slope, torch.float32, (e,), dev)
         if grad_loss.dtype != torch.float32 or grad_loss.numel() != 1 or grad_loss.device != dev:
             raise ValueError("grad_loss must be a device float32 tensor of one value")
-    g = _out("out", out, logits.dtype, (t, e), dev)
-    with _On(dev, stream) as on:
-        _done(load_library().gg_route_backward(dt, t, e, k, int(r.renormalize), logits.data_ptr(), stride, r.experts.data_ptr(),
-                                               r.weights.data_ptr(), r.lse.data_ptr(), _ptr(grad_weights), _ptr(grad_loss),
-                                               0 if grad_loss is None else r.slope.data_ptr(), g.data_ptr(), on.stream))
-        on.use(logits, r.experts, r.weights, r.lse, r.slope, grad_weights, grad_loss, g)
+    g = _out(out, logits.dtype, (t, e), dev)
+    _call(_lib.gg_route_backward, dev, stream, (dt, t, e, k, int(r.renormalize), logits.data_ptr(), stride,
+                                                r.experts.data_ptr(),
+                                                r.weights.data_ptr(), r.lse.data_ptr(), _ptr(grad_weights), _ptr(grad_loss),
+                                                0 if grad_loss is None else r.slope.data_ptr(), g.data_ptr()),
+          (logits, r.experts, r.weights, r.lse, r.slope, grad_weights, grad_loss, g))
     return g
 
 
@@ -311,19 +305,18 @@ def dispatch(x, routing: Routing, out=None, stream: Optional[int] = None):
     n = x.shape[1]
     if x.element_size() not in (1, 2, 4):
         raise TypeError("x must be of a type of 1, 2 or 4 bytes")
-    xs = _out("out", out, x.dtype, (t * k, n), dev)
-    with _On(dev, stream) as on:
-        _done(load_library().gg_dispatch(x.element_size(), t, k, n, offs.numel() - 1, x.data_ptr(), stride, rows.data_ptr(),
-                                         offs.data_ptr(), xs.data_ptr(), on.stream))
-        on.use(x, rows, offs, xs)
+    xs = _out(out, x.dtype, (t * k, n), dev)
+    _call(_lib.gg_dispatch, dev, stream, (x.element_size(), t, k, n, offs.numel() - 1, x.data_ptr(), stride,
+                                          rows.data_ptr(), offs.data_ptr(), xs.data_ptr()),
+          (x, rows, offs, xs))
     return xs
 
 
 def _pairs(name: str, y, t: int, k: int):
     if y.dtype not in _T16:
         raise TypeError(f"{name} must be bfloat16 or float16")
-    if y.dim() != 2 or y.shape[0] != t * k or not y.is_contiguous():
-        raise ValueError(f"{name} must be contiguous with a row for each (token, slot) pair of the routing")
+    if y.dim() != 2 or not y.is_cuda or y.shape[0] != t * k or not y.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous device matrix with a row for each (token, slot) pair of the routing")
     return y.shape[1]
 
 
@@ -332,11 +325,10 @@ def dispatch_backward(grad_xs, routing: Routing, out=None, stream: Optional[int]
     dev = grad_xs.device
     rows, t, k = _rows(routing, dev)
     n = _pairs("grad_xs", grad_xs, t, k)
-    gx = _out("out", out, grad_xs.dtype, (t, n), dev)
-    with _On(dev, stream) as on:
-        _done(load_library().gg_dispatch_backward(_T16[grad_xs.dtype], t, k, n, grad_xs.data_ptr(), rows.data_ptr(),
-                                                  gx.data_ptr(), on.stream))
-        on.use(grad_xs, rows, gx)
+    gx = _out(out, grad_xs.dtype, (t, n), dev)
+    _call(_lib.gg_dispatch_backward, dev, stream, (_T16[grad_xs.dtype], t, k, n, grad_xs.data_ptr(), rows.data_ptr(),
+                                                   gx.data_ptr()),
+          (grad_xs, rows, gx))
     return gx
 
 
@@ -346,11 +338,10 @@ def combine(y, routing: Routing, out=None, stream: Optional[int] = None):
     rows, t, k = _rows(routing, dev)
     n = _pairs("y", y, t, k)
     _flat("routing.weights", routing.weights, torch.float32, (t, k), dev)
-    o = _out("out", out, y.dtype, (t, n), dev)
-    with _On(dev, stream) as on:
-        _done(load_library().gg_combine(_T16[y.dtype], t, k, n, y.data_ptr(), rows.data_ptr(), routing.weights.data_ptr(),
-                                        o.data_ptr(), on.stream))
-        on.use(y, rows, routing.weights, o)
+    o = _out(out, y.dtype, (t, n), dev)
+    _call(_lib.gg_combine, dev, stream, (_T16[y.dtype], t, k, n, y.data_ptr(), rows.data_ptr(), routing.weights.data_ptr(),
+                                         o.data_ptr()),
+          (y, rows, routing.weights, o))
     return o
 
 
@@ -365,13 +356,12 @@ def combine_backward(grad_out, y, routing: Routing, out=None, stream: Optional[i
     if grad_out.dtype != y.dtype or grad_out.device != dev or tuple(grad_out.shape) != (t, n):
         raise ValueError("grad_out must be [T, H] of y's type")
     stride = _matrix("grad_out", grad_out)
-    gy = _out("out", out, y.dtype, (t * k, n), dev)
+    gy = _out(out, y.dtype, (t * k, n), dev)
     gw = torch.empty((t, k), dtype=torch.float32, device=dev)
-    with _On(dev, stream) as on:
-        _done(load_library().gg_combine_backward(_T16[y.dtype], t, k, n, offs.numel() - 1, grad_out.data_ptr(), stride,
-                                                 y.data_ptr(), rows.data_ptr(), offs.data_ptr(), routing.weights.data_ptr(),
-                                                 gy.data_ptr(), gw.data_ptr(), on.stream))
-        on.use(grad_out, y, rows, offs, routing.weights, gy, gw)
+    _call(_lib.gg_combine_backward, dev, stream, (_T16[y.dtype], t, k, n, offs.numel() - 1, grad_out.data_ptr(), stride,
+                                                  y.data_ptr(), rows.data_ptr(), offs.data_ptr(),
+                                                  routing.weights.data_ptr(), gy.data_ptr(), gw.data_ptr()),
+          (grad_out, y, rows, offs, routing.weights, gy, gw))
     return gy, gw
 
 
@@ -473,10 +463,9 @@ def grouped_gemm_w4(x, w: W4Weights, group_m, out=None, stream: Optional[int] = 
         group_m = torch.tensor(list(group_m), dtype=torch.int64, device=dev)
     elif group_m.device != dev or (group_offs is not None and group_offs.device != dev):
         raise ValueError("group sizes must be on x's device")
-    o = _out("out", out, x.dtype, (x.shape[0], w.n), dev)
-    with _On(dev, stream) as on:
-        _done(load_library().gg_gemm_w4(dt, b, x.shape[0], w.n, w.k, w.group, group_m.data_ptr(), _ptr(group_offs),
-                                        x.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), _ptr(w.zeros), o.data_ptr(),
-                                        on.stream))
-        on.use(x, w.packed, w.scales, w.zeros, group_m, group_offs, o)
+    o = _out(out, x.dtype, (x.shape[0], w.n), dev)
+    _call(_lib.gg_gemm_w4, dev, stream, (dt, b, x.shape[0], w.n, w.k, w.group, group_m.data_ptr(), _ptr(group_offs),
+                                         x.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), _ptr(w.zeros),
+                                         o.data_ptr()),
+          (x, w.packed, w.scales, w.zeros, group_m, group_offs, o))
     return o
