@@ -81,6 +81,12 @@ template <typename T> __device__ __forceinline__ u32x4 pack8(const float (&v)[8]
     return w;
 }
 
+// Between LDS accesses of one wave's lanes to each other's values (the hardware keeps a wave's own order).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
 // Sum over the wave, in every lane; the same order in every run.
 __device__ __forceinline__ float wave_sum(float v) {
 #pragma unroll

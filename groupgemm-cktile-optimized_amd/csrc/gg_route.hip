@@ -416,12 +416,6 @@ __global__ void __launch_bounds__(kThreads) empty_kernel(const RouteArgs a) {
         a.loss[0] = 0.f;
 }
 
-// Between LDS accesses of one wave's lanes to each other's values (the hardware keeps a wave's own order).
-__device__ __forceinline__ void wave_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-}
-
 struct BackArgs {
     const void  *logits;
     const int   *experts_of;

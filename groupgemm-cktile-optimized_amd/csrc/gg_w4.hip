@@ -1,13 +1,14 @@
 // Grouped products of few rows with 4-bit weights (gg_gemm_w4 in include/gg_moe_layer.h):
 // out[m, n] = sum_k x[m, k] s (q[n, k] - z), s and z of each `group` consecutive k.
 //
-// What bounds it: the packed weights of the groups that have rows, read once. A wave takes 16 weight rows
-// (NT such tiles) and every W-th tile of 128 k; a tile is one 16-byte load per lane, 1 KB in a row, and
-// the operand of four 16x16x32 matrix instructions. A nibble becomes a 16-bit float by three bit
-// operations on a word, two nibbles at a time: rotated to the top of the mantissa of 16.0 it is 16 + q,
-// exact in bf16 and fp16. The products therefore sum x (16 + q); the scale's share of the sum,
-// s (sum x (16 + q) - (16 + z) sum x), takes sum x from one more matrix instruction whose weights are
-// ones. Nothing is rounded before the float32 sums. The W partial sums are added through LDS.
+// What bounds it: the packed weights of the groups that have rows, read once. A wave takes NT tiles of 16
+// weight rows and every W-th 128 columns of k; a tile's 16 x 128 weights are one 16-byte load per lane, 1 KB in a
+// row, and the operand of four 16x16x32 matrix instructions. A nibble becomes a 16-bit float by two bit operations
+// on a word for two of them: rotated to the top of the mantissa of 16.0 it is 16 + q, exact in bf16 and fp16. So
+// the sum of a scale's k is sum x (16 + q) - (16 + z) sum x, where the second sum comes from matrix instructions
+// too, with a constant -24 (-16 and zero points) for weights, once for the NT tiles, and starts the first one.
+// The weights are a matrix instruction's columns: a lane has one scale and zero point. Nothing is rounded before
+// the float32 sums. The W partial sums are added through LDS.
 #include <algorithm>
 
 #include "gg_layer.h"
@@ -30,77 +31,223 @@ struct W4Args {
 
 template <typename T> struct W4Type;
 template <> struct W4Type<BF16> {
-    static constexpr unsigned mask = 0x00780078u, sixteen = 0x41804180u, one = 0x3f803f80u;
+    static __device__ __forceinline__ float value(unsigned bits) { return __uint_as_float(bits << 16); }
+    static constexpr unsigned mask = 0x00780078u, sixteen = 0x41804180u, minus16 = 0xc180c180u, minus24 = 0xc1c0c1c0u;
     static constexpr int      shift = 3; // of q's lowest bit in the half word
     static __device__ __forceinline__ f32x4 mma(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
 };
 template <> struct W4Type<F16> {
-    static constexpr unsigned mask = 0x03c003c0u, sixteen = 0x4c004c00u, one = 0x3c003c00u;
+    static __device__ __forceinline__ float value(unsigned bits) {
+        return static_cast<float>(__builtin_bit_cast(_Float16, static_cast<uint16_t>(bits)));
+    }
+    static constexpr unsigned mask = 0x03c003c0u, sixteen = 0x4c004c00u, minus16 = 0xcc00cc00u, minus24 = 0xce00ce00u;
     static constexpr int      shift = 6;
     static __device__ __forceinline__ f32x4 mma(const u32x4 &a, const u32x4 &b, const f32x4 &c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
 };
 
-// Eight nibbles of a word as 16 + q: element 2 i from nibble i, 2 i + 1 from nibble i + 4.
-template <typename T> __device__ __forceinline__ u32x4 expand(unsigned w) {
+// Eight nibbles of a word as 16 + q: element 2 i from nibble i, 2 i + 1 from nibble i + 4. The two constants come in
+// registers of their own (one scalar at most): a shift and one and-or for two nibbles.
+struct Bits {
+    unsigned mask, sixteen;
+};
+template <typename T> __device__ __forceinline__ Bits expand_bits() {
+    Bits b{W4Type<T>::mask, W4Type<T>::sixteen};
+    asm("" : "+v"(b.mask));
+    asm("" : "+s"(b.sixteen));
+    return b;
+}
+template <typename T> __device__ __forceinline__ u32x4 expand(unsigned w, const Bits &b) {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const unsigned turned = __builtin_amdgcn_alignbit(w, w, (4 * i - W4Type<T>::shift) & 31);
-        r[i]                  = (turned & W4Type<T>::mask) | W4Type<T>::sixteen;
+        constexpr int up    = W4Type<T>::shift;
+        const unsigned turned = 4 * i < up ? w << (up - 4 * i) : w >> (4 * i - up);
+        r[i]                  = (turned & b.mask) | b.sixteen;
     }
     return r;
 }
 
-// The `want`-th group with rows: its number, or -1, its first row and its rows. A bad length counts as no
-// rows, a group that does not lie inside [0, total_m) has no work.
-struct Found {
-    int     group;
-    int64_t row0;
-    int     rows;
-};
-__device__ __forceinline__ Found find_group(const W4Args &a, int want, int lane) {
-    int64_t base = 0; // rows of the groups before this window of 64
-    for (int g0 = 0; g0 < a.group_num; g0 += 64) {
-        const int g   = g0 + lane;
-        int64_t   len = g < a.group_num ? a.lens[g] : 0;
-        if (len < 0 || len > INT32_MAX)
-            len = 0;
-        int64_t incl = len;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t o = __shfl_up(incl, d);
-            incl += lane >= d ? o : 0;
-        }
-        const int64_t  row0 = a.offs != nullptr ? (g < a.group_num ? a.offs[g] : 0) : base + incl - len;
-        const bool     ok   = len > 0 && row0 >= 0 && row0 <= a.total_m && len <= a.total_m - row0;
-        const uint64_t have = __ballot(ok);
-        const int      n    = __builtin_popcountll(have);
-        if (want < n) {
-            uint64_t m = have;
-            for (int i = 0; i < want; ++i)
-                m &= m - 1;
-            const int src = __builtin_ctzll(m);
-            Found     f;
-            f.group = g0 + src;
-            f.row0  = __shfl(row0, src);
-            f.rows  = static_cast<int>(__shfl(len, src));
-            return f;
-        }
-        want -= n;
-        base += __shfl(incl, 63);
-    }
-    return {-1, 0, 0};
+typedef __amdgpu_buffer_rsrc_t rsrc_t;
+__device__ __forceinline__ rsrc_t resource(const void *p, int bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, bytes, 0x00020000);
+}
+// Lane offset `v` (checked against the resource), scalar offset `s`.
+__device__ __forceinline__ u32x4 load128(rsrc_t r, int v, int s) {
+    return __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(r, v, s, 0));
+}
+__device__ __forceinline__ unsigned load16(rsrc_t r, int v, int s) { return __builtin_amdgcn_raw_buffer_load_b16(r, v, s, 0); }
+__device__ __forceinline__ unsigned load8(rsrc_t r, int v, int s) { return __builtin_amdgcn_raw_buffer_load_b8(r, v, s, 0); }
+
+// Of one register: rows (16 lanes) 0 0 2 2 and 1 1 3 3; halves 0 0 and 1 1.
+__device__ __forceinline__ u32x2 swap16(unsigned v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return u32x2{r[0], r[1]};
+}
+__device__ __forceinline__ u32x2 swap32(unsigned v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return u32x2{r[0], r[1]};
 }
 
-// Grid: workgroup (tile block of 16 NT columns, one of the groups with rows). MT row tiles of 16 at a time.
-// G: k of one scale.
-template <typename T, int MT, int NT, int W, int G> __global__ void __launch_bounds__(W * 64) w4_kernel(const W4Args a) {
+// Rows of group g, 0 for a bad length.
+__device__ __forceinline__ int64_t length_of(const W4Args &a, int g) {
+    const int64_t len = g < a.group_num ? a.lens[g] : 0;
+    return len < 0 || len > INT32_MAX ? 0 : len;
+}
+__device__ __forceinline__ int64_t read_lane(int64_t v, int src) { // into scalar registers
+    return static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), src))) |
+           (static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), src)) << 32);
+}
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1)
+        v += __shfl_xor(v, d);
+    return v;
+}
+
+// The `want`-th group with rows, or -1, and its rows. Its weights can be asked for before its first row is known.
+struct Found {
+    int group, rows;
+};
+__device__ __forceinline__ Found find_group(const W4Args &a, int want, int lane) {
+    for (int g0 = 0; g0 < a.group_num; g0 += 64) {
+        const int64_t len  = length_of(a, g0 + lane);
+        uint64_t      have = __ballot(len > 0);
+        const int     n    = __builtin_popcountll(have);
+        if (want < n) {
+            for (int i = 0; i < want; ++i)
+                have &= have - 1;
+            const int src = __builtin_ctzll(have);
+            return {g0 + src, __builtin_amdgcn_readlane(static_cast<int>(len), src)};
+        }
+        want -= n;
+    }
+    return {-1, 0};
+}
+// Its first row; -1 if its rows do not lie inside [0, total_m).
+__device__ __forceinline__ int64_t first_row(const W4Args &a, const Found &f, int lane) {
+    int64_t row0 = 0;
+    if (a.offs != nullptr) {
+        row0 = read_lane(a.offs[f.group], 0);
+    } else {
+        for (int g0 = 0; g0 < f.group; g0 += 64)
+            row0 += wave_sum64(g0 + lane < f.group ? length_of(a, g0 + lane) : 0);
+        row0 = read_lane(row0, 0);
+    }
+    return row0 >= 0 && row0 <= a.total_m && f.rows <= a.total_m - row0 ? row0 : -1;
+}
+
+// The scales (and zero points times scales) of a tile in every lane: rows 0 .. N - 1 of 16 lanes hold one each.
+template <typename T, int N, bool ZEROS>
+__device__ __forceinline__ void spread_scales(unsigned s, unsigned z, float (&scale)[N], float (&point)[N]) {
+    unsigned v[4] = {ZEROS ? s | z << 16 : s};
+    if constexpr (N > 1) {
+        const u32x2 r = swap16(v[0]); // rows 0 0 2 2, 1 1 3 3
+        v[0]          = r[0];
+        v[1]          = r[1];
+    }
+    if constexpr (N == 4) {
+        const u32x2 a = swap32(v[0]), b = swap32(v[1]);
+        v[0]          = a[0];
+        v[2]          = a[1];
+        v[1]          = b[0];
+        v[3]          = b[1];
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        scale[i] = W4Type<T>::value(v[i] & 0xffffu);
+        point[i] = ZEROS ? scale[i] * static_cast<float>(v[i] >> 16) : 0.f;
+    }
+}
+
+// What both kernels read of weight tile j (of NT) of a group: resources over its weights, scales and zero points.
+template <int NT, bool ZEROS> struct Weights {
+    rsrc_t w[NT], s[NT], z[NT];
+    __device__ __forceinline__ Weights(const W4Args &a, int group, int tile0) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int64_t tile = static_cast<int64_t>(group) * a.n_tiles + min(tile0 + j, a.n_tiles - 1); // past N: the last again
+            w[j] = resource(static_cast<const char *>(a.packed) + tile * a.k_tiles * 1024, a.k_tiles * 1024);
+            s[j] = resource(static_cast<const char *>(a.scales) + tile * a.groups * 32, a.groups * 32);
+            if constexpr (ZEROS)
+                z[j] = resource(a.zeros + tile * a.groups * 16, a.groups * 16);
+        }
+    }
+};
+template <int NT> struct TileWords {
+    u32x4 w[NT];
+};
+template <int NT> struct TileScales {
+    unsigned s[NT], z[NT]; // lanes of row (of 16) quad % kScales: the tile's scale of that number
+};
+template <int NT, bool ZEROS>
+__device__ __forceinline__ void load_words(TileWords<NT> &t, const Weights<NT, ZEROS> &w, int c, int lane) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+        t.w[j] = load128(w.w[j], lane * 16, c * 1024);
+}
+template <int NT, bool ZEROS, int kScales>
+__device__ __forceinline__ void load_scales(TileScales<NT> &t, const Weights<NT, ZEROS> &w, int c, int lane) { // past K: zeros
+    const int at = c * kScales + ((lane >> 4) & (kScales - 1));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        t.s[j] = load16(w.s[j], at * 32 + (lane & 15) * 2, 0);
+        if constexpr (ZEROS)
+            t.z[j] = load8(w.z[j], at * 16 + (lane & 15), 0);
+    }
+}
+
+// The end of a scale's k: its sums, scaled, into acc. What they lack comes first: base where they did not start
+// from it; with zero points z / 16 of base.
+template <int MT, int NT, bool ZEROS, bool BASE_FIRST, int N>
+__device__ __forceinline__ void scale_sums(f32x4 (&acc)[MT][NT], f32x4 (&sum)[MT][NT], f32x4 (&base)[MT],
+                                           const float (&scale)[NT][N], const float (&point)[NT][N], int q) {
+    if constexpr (!BASE_FIRST)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    sum[i][j][r] += base[i][r];
+    if constexpr (ZEROS)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                base[i][r] *= 0.0625f;
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                acc[i][j][r] = fmaf(scale[j][q], sum[i][j][r], acc[i][j][r]);
+                if constexpr (ZEROS)
+                    acc[i][j][r] = fmaf(point[j][q], base[i][r], acc[i][j][r]);
+            }
+    // here, and not after the tile's last step, where the compiler would gather them with every step's sums alive
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+            asm volatile("" : "+v"(acc[i][j]));
+}
+
+// Up to 16 rows of a group at a time. Grid: workgroup (tile block of 16 NT columns, one of the groups with rows), G k of
+// one scale. The W waves share out the 128-column tiles; each loads its weights D tiles ahead, scales and x one
+// tile ahead. x comes through a buffer resource that ends at the last row, so rows past it read as zeros and cost no
+// traffic.
+template <typename T, int NT, int W, int G, int D, bool ZEROS>
+__global__ void __launch_bounds__(W * 64, 2) w4_kernel(const W4Args a) {
     using X = W4Type<T>;
-    __shared__ f32x4 part[W][MT * NT][64];
+    constexpr int kSteps  = G / 32;  // matrix steps of one scale
+    constexpr int kScales = 128 / G; // scales of one tile
+    __shared__ f32x4 part[W][NT][64];
+    const Bits bits = expand_bits<T>();
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 15, quad = lane >> 4;
     const int blocks = (a.n_tiles + NT - 1) / NT;
@@ -110,128 +257,280 @@ template <typename T, int MT, int NT, int W, int G> __global__ void __launch_bou
         const Found f = find_group(a, want, lane);
         if (f.group < 0)
             return;
-        const int   tile0 = nb * NT;
-        const char *wp[NT], *sp[NT], *zp[NT];
+        const int tile0 = nb * NT;
+        const Weights<NT, ZEROS> w(a, f.group, tile0);
+        TileWords<NT>  ahead[D];
+        TileScales<NT> next_scales;
+        auto start = [&] {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const int64_t tile = static_cast<int64_t>(f.group) * a.n_tiles + min(tile0 + i, a.n_tiles - 1); // past N: the last again
-            wp[i] = static_cast<const char *>(a.packed) + tile * a.k_tiles * 1024 + lane * 16;
-            sp[i] = static_cast<const char *>(a.scales) + tile * a.groups * 32 + quad * 8;
-            zp[i] = reinterpret_cast<const char *>(a.zeros) + tile * a.groups * 16 + quad * 4;
-        }
-        for (int m0 = 0; m0 < f.rows; m0 += 16 * MT) {
-            const uint16_t *xp[MT];
-            bool            has[MT];
+            for (int d = 0; d < D; ++d)
+                if (wave + d * W < a.k_tiles)
+                    load_words(ahead[d], w, wave + d * W, lane);
+            load_scales<NT, ZEROS, kScales>(next_scales, w, wave, lane);
+        };
+        start();
+        const int64_t row0 = first_row(a, f, lane);
+        if (row0 < 0)
+            continue;
+        for (int m0 = 0; m0 < f.rows; m0 += 16) {
+            if (m0 > 0)
+                start();
+            const rsrc_t xr = resource(static_cast<const uint16_t *>(a.x) + (row0 + m0) * a.k, min(16, f.rows - m0) * a.k * 2);
+            const int    xo = col * a.k * 2 + quad * 16;
+            struct Operand {
+                u32x4 x[4];
+            };
+            auto load_x = [&](Operand &o, int c) { // past K: zeros
 #pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int m = m0 + 16 * i + col;
-                has[i]      = m < f.rows;
-                xp[i]       = static_cast<const uint16_t *>(a.x) + (f.row0 + (has[i] ? m : 0)) * a.k + quad * 8;
-            }
-            f32x4 acc[MT][NT];
+                for (int st = 0; st < 4; ++st) {
+                    const int k0 = c * 128 + st * 32;
+                    o.x[st]      = load128(xr, xo | (k0 < a.k ? 0 : static_cast<int>(0x80000000u)), k0 * 2);
+                }
+            };
+            f32x4 acc[1][NT];
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < NT; ++j)
+                acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            Operand next;
+            load_x(next, wave);
             for (int c = wave; c < a.k_tiles; c += W) {
-                u32x4 wv[NT];
+                const TileWords<NT> now = ahead[0];
+                float scale[NT][kScales], point[NT][kScales]; // of this lane's column: scale, scale * zero point
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
-                    wv[j] = *reinterpret_cast<const u32x4 *>(wp[j] + static_cast<int64_t>(c) * 1024);
-                constexpr int kSteps = G / 32; // matrix instructions of one scale
+                    spread_scales<T, kScales, ZEROS>(next_scales.s[j], next_scales.z[j], scale[j], point[j]);
+                const Operand x = next;
 #pragma unroll
-                for (int q = 0; q < 4 / kSteps; ++q) { // scales of this tile
-                    const int sg = c * (128 / G) + q;
-                    if (sg >= a.groups) // past K
-                        break;
-                    f32x4 sum[MT][NT], ones[MT];
+                for (int d = 0; d + 1 < D; ++d)
+                    ahead[d] = ahead[d + 1];
+                if (c + D * W < a.k_tiles)
+                    load_words(ahead[D - 1], w, c + D * W, lane);
+                load_scales<NT, ZEROS, kScales>(next_scales, w, c + W, lane);
+                load_x(next, c + W);
+                f32x4 sum[1][NT], base[1];
+                const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+                constexpr unsigned kMinus = ZEROS ? X::minus16 : X::minus24;
+                const u32x4 minus{kMinus, kMinus, kMinus, kMinus};
 #pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        ones[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+                for (int step = 0; step < 4; ++step) {
+                    const bool first = step % kSteps == 0;
+                    if (first) { // -24 (-16) times the scale's share of sum x, in every column: the sums start from it
+                        base[0] = zero;
 #pragma unroll
-                        for (int j = 0; j < NT; ++j)
-                            sum[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                        for (int s2 = step; s2 < step + kSteps; ++s2)
+                            base[0] = X::mma(x.x[s2], minus, base[0]);
                     }
 #pragma unroll
-                    for (int st = 0; st < kSteps; ++st) {
-                        const int step = q * kSteps + st;
-                        u32x4     xv[MT];
-#pragma unroll
-                        for (int i = 0; i < MT; ++i) {
-                            xv[i] = u32x4{0, 0, 0, 0};
-                            if (has[i])
-                                xv[i] = *reinterpret_cast<const u32x4 *>(xp[i] + static_cast<int64_t>(c) * 128 + step * 32);
-                        }
-                        const u32x4 one{X::one, X::one, X::one, X::one};
-#pragma unroll
-                        for (int i = 0; i < MT; ++i)
-                            ones[i] = X::mma(one, xv[i], ones[i]);
-#pragma unroll
-                        for (int j = 0; j < NT; ++j) {
-                            const u32x4 wf = expand<T>(wv[j][step]);
-#pragma unroll
-                            for (int i = 0; i < MT; ++i)
-                                sum[i][j] = X::mma(wf, xv[i], sum[i][j]);
-                        }
-                    }
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        float       s[4], z[4];
-                        const u32x2 sw = *reinterpret_cast<const u32x2 *>(sp[j] + static_cast<int64_t>(sg) * 32);
-                        T::pair(sw[0], s[0], s[1]);
-                        T::pair(sw[1], s[2], s[3]);
-                        if (a.zeros != nullptr) {
-                            const unsigned zw = *reinterpret_cast<const unsigned *>(zp[j] + static_cast<int64_t>(sg) * 16);
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                z[r] = static_cast<float>((zw >> (8 * r)) & 255u) + 16.f;
-                        } else {
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                z[r] = 24.f;
-                        }
-#pragma unroll
-                        for (int i = 0; i < MT; ++i)
-#pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                acc[i][j][r] = fmaf(s[r], fmaf(-z[r], ones[i][r], sum[i][j][r]), acc[i][j][r]);
-                    }
+                    for (int j = 0; j < NT; ++j)
+                        sum[0][j] = X::mma(x.x[step], expand<T>(now.w[j][step], bits), first ? base[0] : sum[0][j]);
+                    if (step % kSteps == kSteps - 1)
+                        scale_sums<1, NT, ZEROS, true, kScales>(acc, sum, base, scale, point, step / kSteps);
                 }
             }
-            // the waves' sums, in their order; each wave stores every W-th of the MT x NT tiles
+            // the waves' sums, in their order; each wave stores every W-th of the NT tiles
             __syncthreads(); // the tiles before are read
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    part[wave][i * NT + j][lane] = acc[i][j];
+            for (int j = 0; j < NT; ++j)
+                part[wave][j][lane] = acc[0][j];
             __syncthreads();
-            for (int u = wave; u < MT * NT; u += W) {
-                f32x4 v = part[0][u][lane];
+            for (int u = wave; u < NT; u += W) {
+                // a sum lies in lane 16 (row / 4) + column, word row % 4; this lane takes row `col`, columns 4 quad ..
+                float v[4];
 #pragma unroll
-                for (int w = 1; w < W; ++w)
-                    v += part[w][u][lane];
-                const int m = m0 + 16 * (u / NT) + col, n = (tile0 + u % NT) * 16 + quad * 4;
+                for (int i = 0; i < 4; ++i) {
+                    v[i] = 0.f;
+#pragma unroll
+                    for (int p = 0; p < W; ++p)
+                        v[i] += part[p][u][(col >> 2) * 16 + quad * 4 + i][col & 3];
+                }
+                const int m = m0 + col, n = (tile0 + u) * 16 + quad * 4;
                 if (m < f.rows && n < a.n) // n % 8 == 0: four columns are all there or none
-                    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + (f.row0 + m) * a.n + n) =
+                    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + (row0 + m) * a.n + n) =
                         u32x2{T::word(v[0], v[1]), T::word(v[2], v[3])};
             }
         }
     }
 }
 
-template <typename T, int MT, int NT, int W> int launch_w4(const W4Args &a, int group, hipStream_t s) {
-    const int64_t blocks = (a.n_tiles + NT - 1) / NT;
-    // at most total_m groups have rows (device offsets that overlap may give more: slots are walked in strides);
-    // HIP refuses grids of 2^32 threads
-    const int64_t slots = std::clamp<int64_t>(std::min<int64_t>(a.group_num, a.total_m), 1, (int64_t(1) << 31) / (W * 64) / blocks);
-    const int64_t grid  = blocks * slots;
-    return launch("gemm_w4", group == 128 ? w4_kernel<T, MT, NT, W, 128> : group == 64 ? w4_kernel<T, MT, NT, W, 64> : w4_kernel<T, MT, NT, W, 32>,
-                  grid, W * 64, s, a);
+// More rows of a group: 16 MT at a time, each of the four waves with NT tiles of its own, x's rows shared through two LDS
+// buffers of one 128-column tile. A row's 16-byte pieces lie at piece ^ row % 16, so the 16 rows that a matrix
+// operand takes at once are in different banks.
+template <typename T, int MT, int NT, int G, bool ZEROS>
+__global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
+    using X = W4Type<T>;
+    constexpr int kSteps  = G / 32;
+    constexpr int kScales = 128 / G;
+    constexpr bool kBaseFirst = kSteps <= 2; // two steps' x are in registers
+    constexpr int kTile   = MT * 16 * 256; // bytes of a tile of x
+    constexpr int kOut    = MT * 16 * NT * 32; // bytes of a wave's outputs
+    __shared__ __attribute__((aligned(16))) unsigned char lds[2 * kTile > 4 * kOut ? 2 * kTile : 4 * kOut];
+    const Bits bits = expand_bits<T>();
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const int blocks = (a.n_tiles + 4 * NT - 1) / (4 * NT);
+    const int nb     = static_cast<int>(blockIdx.x) % blocks;
+    const int slots  = static_cast<int>(gridDim.x) / blocks;
+    for (int want = static_cast<int>(blockIdx.x) / blocks;; want += slots) {
+        const Found f = find_group(a, want, lane);
+        if (f.group < 0)
+            return;
+        const int tile0 = (nb * 4 + wave) * NT;
+        const Weights<NT, ZEROS> w(a, f.group, tile0);
+        TileWords<NT>  ahead[2];
+        TileScales<NT> next_scales;
+        auto start = [&] {
+            load_words(ahead[0], w, 0, lane);
+            if (1 < a.k_tiles)
+                load_words(ahead[1], w, 1, lane);
+            load_scales<NT, ZEROS, kScales>(next_scales, w, 0, lane);
+        };
+        start();
+        const int64_t row0 = first_row(a, f, lane);
+        if (row0 < 0)
+            continue;
+        for (int m0 = 0; m0 < f.rows; m0 += 16 * MT) {
+            if (m0 > 0)
+                start();
+            const rsrc_t xr = resource(static_cast<const uint16_t *>(a.x) + (row0 + m0) * a.k, min(16 * MT, f.rows - m0) * a.k * 2);
+            // this thread's pieces: row 16 i + tid / 16, piece tid % 16
+            const int xrow = tid >> 4, piece = tid & 15;
+            u32x4     xin[MT];
+            auto load_x = [&](int c) { // past K: zeros
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    xin[i] = load128(xr, ((16 * i + xrow) * a.k * 2 + piece * 16) | (c * 128 + piece * 8 < a.k ? 0 : static_cast<int>(0x80000000u)),
+                                     c * 256);
+            };
+            auto store_x = [&](int c) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    *reinterpret_cast<u32x4 *>(lds + (c & 1) * kTile + (16 * i + xrow) * 256 + ((piece ^ xrow) << 4)) = xin[i];
+            };
+            f32x4 acc[MT][NT];
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+            __syncthreads(); // what was in LDS is read
+            load_x(0);
+            store_x(0);
+            __syncthreads();
+            for (int c = 0; c < a.k_tiles; ++c) {
+                const TileWords<NT> now = ahead[0];
+                float scale[NT][kScales], point[NT][kScales];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+                    spread_scales<T, kScales, ZEROS>(next_scales.s[j], next_scales.z[j], scale[j], point[j]);
+                ahead[0] = ahead[1];
+                const bool more = c + 1 < a.k_tiles;
+                if (more) {
+                    load_x(c + 1);
+                    load_scales<NT, ZEROS, kScales>(next_scales, w, c + 1, lane);
+                }
+                if (c + 2 < a.k_tiles)
+                    load_words(ahead[1], w, c + 2, lane);
+                const unsigned char *xt = lds + (c & 1) * kTile;
+                auto read_x = [&](u32x4(&x)[MT], int step) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        x[i] = *reinterpret_cast<const u32x4 *>(xt + (16 * i + col) * 256 + (((step * 4 + quad) ^ col) << 4));
+                };
+                f32x4 sum[MT][NT], base[MT];
+                const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+                constexpr unsigned kMinus = ZEROS ? X::minus16 : X::minus24;
+                const u32x4 minus{kMinus, kMinus, kMinus, kMinus};
+                u32x4 x[2][MT]; // of this step and the next
+                read_x(x[0], 0);
+#pragma unroll
+                for (int step = 0; step < 4; ++step) {
+                    const bool first = step % kSteps == 0;
+                    if (step < 3)
+                        read_x(x[(step + 1) & 1], step + 1);
+                    if (!kBaseFirst || first)
+#pragma unroll
+                        for (int s2 = step; s2 < (kBaseFirst ? step + kSteps : step + 1); ++s2)
+#pragma unroll
+                            for (int i = 0; i < MT; ++i)
+                                base[i] = X::mma(x[s2 & 1][i], minus, first && s2 == step ? zero : base[i]);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        const u32x4 wf = expand<T>(now.w[j][step], bits);
+#pragma unroll
+                        for (int i = 0; i < MT; ++i)
+                            sum[i][j] = X::mma(x[step & 1][i], wf, !first ? sum[i][j] : kBaseFirst ? base[i] : zero);
+                    }
+                    if (step % kSteps == kSteps - 1)
+                        scale_sums<MT, NT, ZEROS, kBaseFirst, kScales>(acc, sum, base, scale, point, step / kSteps);
+                    __builtin_amdgcn_sched_barrier(0); // a step's operands are not fetched earlier than this
+                }
+                if (more)
+                    store_x(c + 1);
+                __syncthreads();
+            }
+            // outputs through LDS, a wave's own part: rows of 16 NT columns, stored 16 bytes (8 columns) a lane
+            unsigned char *ot = lds + wave * kOut;
+#pragma unroll
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        *reinterpret_cast<uint16_t *>(ot + ((16 * i + quad * 4 + r) * NT * 16 + j * 16 + col) * 2) =
+                            static_cast<uint16_t>(T::word(acc[i][j][r], 0.f));
+            wave_sync();
+            for (int u = lane; u < MT * 16 * NT * 2; u += 64) {
+                const int m = u / (NT * 2), n8 = u % (NT * 2), n = tile0 * 16 + n8 * 8;
+                if (m0 + m < f.rows && n < a.n)
+                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + (row0 + m0 + m) * a.n + n) =
+                        *reinterpret_cast<const u32x4 *>(ot + (m * NT * 16 + n8 * 8) * 2);
+            }
+        }
+    }
 }
 
-template <typename T> int run_w4(const W4Args &a, int group, hipStream_t s) { return launch_w4<T, 1, 1, 8>(a, group, s); }
+template <typename K> int launch_w4(K kernel, int columns, int threads, const W4Args &a, hipStream_t s) {
+    const int64_t blocks = (static_cast<int64_t>(a.n_tiles) * 16 + columns - 1) / columns;
+    // at most total_m groups have rows where nothing is wrong with the sizes (slots are walked in strides); HIP refuses
+    // grids of 2^32 threads
+    const int64_t slots = std::clamp<int64_t>(std::min<int64_t>(a.group_num, a.total_m), 1, (int64_t(1) << 31) / threads / blocks);
+    return launch("gemm_w4", kernel, blocks * slots, threads, s, a);
+}
+
+// f(k of one scale, zero points or not)
+template <typename F> int with_format(const W4Args &a, int group, F f) {
+    using std::integral_constant;
+    auto zeros = [&](auto g) { return a.zeros != nullptr ? f(g, std::true_type{}) : f(g, std::false_type{}); };
+    return group == 128  ? zeros(integral_constant<int, 128>{})
+           : group == 64 ? zeros(integral_constant<int, 64>{})
+                         : zeros(integral_constant<int, 32>{});
+}
+template <typename T, int NT, int W, int D> int launch_few(const W4Args &a, int group, hipStream_t s) {
+    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_kernel<T, NT, W, g.value, D, z.value>, 16 * NT, 64 * W, a, s); });
+}
+template <typename T, int MT, int NT> int launch_rows(const W4Args &a, int group, hipStream_t s) {
+    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_rows_kernel<T, MT, NT, g.value, z.value>, 64 * NT, 256, a, s); });
+}
+
+// The instance by the rows that a group has on average and the workgroups there are. Measured (us; columns: a few-row
+// instance of 64, 32 and 16 columns a workgroup, then the many-row ones of 32 and 64 rows):
+//   rows per group (ragged; 32 groups of 2880 x 2880, k of a scale 32, zero points / 16 of 4096 x 4096, 128):
+//     8:  43.9 / 34.3, -, -, 49.9 / 35.0, 80.9 / 48.8       12: 56.7 / 44.0, -, -, 52.3 / 35.0, 81.6 / 47.9
+//     20: 82.9 / 71.2, -, -, 98.8 / 61.6, 113.6 / 50.4      24: 85.7 / 64.3, -, -, 89.4 / 61.5, 81.9 / 51.0
+//     48: 138.5 / 96.5, -, -, 122.6 / 79.4, 148.7 / 80.9
+//   workgroups of 64 columns (one row): 8 of 512 x 7168: 11.9, 7.5, 6.3; 32 of 2048 x 2048: 6.1, 4.8, 4.3; 128 of
+//     1024 x 7168 15.7, 9.7, 11.2; 224 of 14336 x 4096 10.7, 9.4, 13.1; 448 of 7168 x 2048 10.2, 12, 12.8
+//   the many-row ones do not split k: with fewer workgroups than CUs they lose (4 groups of 20 rows, 2048 x 4096: 16.7, 11.8,
+//     13.9, 25, 36).
+template <typename T> int run_w4(const W4Args &a, int group, hipStream_t s) {
+    const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m)), per = a.total_m / slots;
+    const int64_t wide = (a.n_tiles + 7) / 8 * slots, narrow = (a.n_tiles + 3) / 4 * slots;
+    if (per >= 12 && wide >= 256)
+        return per <= 20 ? launch_rows<T, 2, 2>(a, group, s) : launch_rows<T, 4, 2>(a, group, s);
+    return narrow >= 256  ? launch_few<T, 4, 4, 1>(a, group, s)
+           : narrow >= 64 ? launch_few<T, 2, 8, 1>(a, group, s)
+                          : launch_few<T, 1, 8, 2>(a, group, s);
+}
 
 } // namespace
 } // namespace layer

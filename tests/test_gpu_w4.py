@@ -80,6 +80,49 @@ def test_against_64_bits(pkg, dtype, zeros, n, k, group, lens):
     assert torch.equal(got, pkg.grouped_gemm_w4(x, w4, group_m))
 
 
+def _ragged(b, rows, seed):
+    """Rows of b groups that add up to `rows`: one group with many, some with none."""
+    g = torch.Generator().manual_seed(seed)
+    share = torch.rand(b, generator=g) ** 2
+    share[seed % b] += 3.0
+    share[(seed + 1) % b] = 0.0
+    lens = (share / share.sum() * rows).int().tolist()
+    lens[seed % b] += rows - sum(lens)
+    return lens
+
+
+# The kernel is chosen by the average rows and the number of workgroups: these reach every choice (the cases above
+# have few workgroups).
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group,k", [(32, 160), (64, 448), (128, 640)])
+@pytest.mark.parametrize("b,n,per", [(16, 264, 2), (16, 1048, 5), (32, 1048, 12), (32, 1000, 19), (32, 1032, 21), (32, 1016, 40)])
+def test_every_instance(pkg, dtype, zeros, group, k, b, n, per):
+    q, s, z = _weights(b, n, k, group, dtype, zeros, n + k + per)
+    w4 = pkg.pack_w4(q, s, z)
+    w, size = _dense(q, s, z, group)
+    lens = _ragged(b, b * per, per)
+    x = torch.randn(b * per, k, device=DEV, generator=_gen(k)).to(dtype)
+    out = torch.full((b * per * n + 64,), 3.0, dtype=dtype, device=DEV)
+    got = pkg.grouped_gemm_w4(x, w4, torch.tensor(lens, device=DEV), out=out[:-64].view(b * per, n))
+    offs = [sum(lens[:g]) for g in range(b)]
+    assert bool(_check(got, x, w, size, offs, lens, dtype, k).all()) and bool((out[-64:] == 3).all())
+    assert torch.equal(got, pkg.grouped_gemm_w4(x, w4, torch.tensor(lens, device=DEV)))
+    # rows elsewhere than back to back, in another order of the groups
+    order = sorted(range(b), key=lambda g: (g * 7) % b)
+    at, start = 3, [0] * (b + 1)
+    for g in order:
+        start[g], at = at, at + lens[g] + 1
+    wide = torch.zeros(at, k, dtype=dtype, device=DEV)
+    far = torch.full((at, n), 5.0, dtype=dtype, device=DEV)
+    for g in range(b):
+        wide[start[g]:start[g] + lens[g]] = x[offs[g]:offs[g] + lens[g]]
+    pkg.grouped_gemm_w4(wide, w4, torch.tensor(lens, device=DEV), out=far, group_offs=torch.tensor(start, device=DEV))
+    for g in range(b):
+        assert torch.equal(far[start[g]:start[g] + lens[g]], got[offs[g]:offs[g] + lens[g]])
+        assert bool((far[start[g] + lens[g]] == 5).all())
+
+
 @pytest.mark.parametrize("b", [63, 64, 65, 200, 1000])
 def test_many_groups_few_with_rows(pkg, b):
     n, k, group = 32, 128, 64
