@@ -87,19 +87,53 @@ __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_wave_barrier();
 }
 
-// Sum over the wave, in every lane; the same order in every run.
-__device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1)
-        v += __shfl_xor(v, d);
+// op over groups of L consecutive lanes, in every lane of the group, in the same order in every run. Within a row of
+// 16 lanes by register moves between lanes (pairs, quads, halves and rows mirrored), then by swaps of rows and halves:
+// a step costs an instruction or two, where a shuffle goes through the LDS unit.
+template <int CTRL> __device__ __forceinline__ unsigned lane_move(unsigned v) {
+    return static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, 0xf, 0xf, true));
+}
+template <int L, typename F> __device__ __forceinline__ unsigned group_reduce(unsigned v, F op) {
+    if constexpr (L >= 2)
+        v = op(v, lane_move<0xb1>(v)); // quad_perm 1 0 3 2
+    if constexpr (L >= 4)
+        v = op(v, lane_move<0x4e>(v)); // quad_perm 2 3 0 1
+    if constexpr (L >= 8)
+        v = op(v, lane_move<0x141>(v)); // row_half_mirror
+    if constexpr (L >= 16)
+        v = op(v, lane_move<0x140>(v)); // row_mirror
+    if constexpr (L >= 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        v            = op(r[0], r[1]);
+    }
+    if constexpr (L >= 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+        v            = op(r[0], r[1]);
+    }
     return v;
 }
-__device__ __forceinline__ unsigned wave_max(unsigned v) {
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1)
-        v = max(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), d)));
+template <int L> __device__ __forceinline__ unsigned group_max(unsigned v) {
+    return group_reduce<L>(v, [](unsigned x, unsigned y) { return max(x, y); });
+}
+template <int L> __device__ __forceinline__ float group_sum(float v) {
+    return __uint_as_float(group_reduce<L>(__float_as_uint(v), [](unsigned x, unsigned y) {
+        return __float_as_uint(__uint_as_float(x) + __uint_as_float(y));
+    }));
+}
+// Sum over the lanes of the same number in the wave's groups of L >= 16 lanes.
+template <int L> __device__ __forceinline__ float rows_sum(float v) {
+    if constexpr (L < 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v            = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if constexpr (L < 64) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v            = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
     return v;
 }
+__device__ __forceinline__ float    wave_sum(float v) { return group_sum<64>(v); }
+__device__ __forceinline__ unsigned wave_max(unsigned v) { return group_max<64>(v); }
 
 } // namespace layer
 } // namespace gg

@@ -1,10 +1,11 @@
 // Top-k router with counts, the sorted row of every (token, slot) pair and the balance loss, and its
 // gradients (gg_route, gg_route_backward in include/gg_moe_layer.h).
 //
-// A token belongs to L lanes, each with V consecutive experts in registers. The largest logits come out
-// one per round: the lanes' own maxima, a maximum over the L lanes, and the lowest lane that has it gives
-// up its first value of that size, so equal logits go to the lower expert. Logits are compared as
-// unsigned numbers of the same order; softmax is taken of the values (max subtracted, float32).
+// A token belongs to L lanes, each with V consecutive experts in registers. Logits are compared as unsigned numbers of
+// the same order. Packed into one word, the number's upper bits and the expert counted backwards (equal logits go to
+// the lower expert), each lane sorts its V with a network; then one value per round comes out: the largest of the
+// lanes' first ones, whose lane moves up. Where the bits that packing cuts could matter the wave takes them again by
+// their whole numbers. Softmax is taken of the values (max subtracted, float32).
 //
 // Rows are a stable counting sort. A workgroup takes a chunk of consecutive tokens, lays the experts of
 // its pairs out in LDS and ranks 64 pairs at a time: lanes with the same expert find each other with one
@@ -28,58 +29,57 @@ struct RouteArgs {
     int           *experts_out, *rows;
     float         *weights, *lse, *loss, *slope;
     int64_t       *counts, *offs;
-    int           *hist;  // [chunks][experts + 1]: pairs of each expert, then tokens that take part
-    float         *sums;  // [chunks][experts]: sums of probabilities
+    int           *hist;  // [chunks + 1][experts + 1]: pairs of each expert, then tokens that take part; then the totals
+    float         *sums;  // [chunks + 1][experts]: sums of probabilities, then their totals
     int64_t        tokens, stride;
-    int            experts, top_k, renormalize, chunk, chunks; // tokens of a chunk
+    int            dtype, experts, top_k, renormalize, chunk, chunks; // chunk: tokens of one
     bool           vec, balance;
 };
 
-template <typename T> struct Value;
-template <> struct Value<float> {
-    static __device__ __forceinline__ float load(const void *p, int64_t i) { return static_cast<const float *>(p)[i]; }
-};
-template <> struct Value<BF16> {
-    static __device__ __forceinline__ float load(const void *p, int64_t i) {
-        return __uint_as_float(static_cast<unsigned>(static_cast<const uint16_t *>(p)[i]) << 16);
-    }
-};
-template <> struct Value<F16> {
-    static __device__ __forceinline__ float load(const void *p, int64_t i) {
-        return static_cast<float>(static_cast<const _Float16 *>(p)[i]);
-    }
-};
-
-// V values from element i on (i + V inside the row), from 16-byte (8-byte: four 16-bit) pieces.
-template <typename T, int V> __device__ __forceinline__ void load_vec(const void *p, int64_t i, float (&v)[V]) {
-    if constexpr (std::is_same_v<T, float>) {
-#pragma unroll
-        for (int j = 0; j < V; j += 4) {
-            const f32x4 w = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i + j);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-                v[j + q] = w[q];
-        }
-    } else {
-#pragma unroll
-        for (int j = 0; j < V; j += 4) {
-            const u32x2 w = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + i + j);
-            T::pair(w[0], v[j], v[j + 1]);
-            T::pair(w[1], v[j + 2], v[j + 3]);
-        }
-    }
+// Element i of logits of type `dtype`.
+__device__ __forceinline__ float load_one(int dtype, const void *p, int64_t i) {
+    if (dtype == GG_DTYPE_FP32)
+        return static_cast<const float *>(p)[i];
+    const unsigned w = static_cast<const uint16_t *>(p)[i];
+    float          lo, hi;
+    if (dtype == GG_DTYPE_BF16)
+        BF16::pair(w, lo, hi);
+    else
+        F16::pair(w, lo, hi);
+    return lo;
 }
 
-// The V logits from expert e0 on; -infinity past the last expert.
-template <typename T, int V>
-__device__ __forceinline__ void load_logits(const void *p, int64_t row, int e0, int experts, bool vec, float (&v)[V]) {
+// The V logits from element `row` + e0 on; -infinity past the last expert. `vec`: rows are 16-byte aligned.
+template <int V>
+__device__ __forceinline__ void load_logits(int dtype, const void *p, int64_t row, int e0, int experts, bool vec, float (&v)[V]) {
     if (vec && e0 + V <= experts) {
-        load_vec<T, V>(p, row + e0, v);
+        if (dtype == GG_DTYPE_FP32) {
+#pragma unroll
+            for (int j = 0; j < V; j += 4) {
+                const f32x4 w = *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + row + e0 + j);
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+                    v[j + q] = w[q];
+            }
+            return;
+        }
+        const uint16_t *h = static_cast<const uint16_t *>(p) + row + e0;
+#pragma unroll
+        for (int j = 0; j < V; j += 4) {
+            const u32x2 w = *reinterpret_cast<const u32x2 *>(h + j);
+            if (dtype == GG_DTYPE_BF16) {
+                BF16::pair(w[0], v[j], v[j + 1]);
+                BF16::pair(w[1], v[j + 2], v[j + 3]);
+            } else {
+                F16::pair(w[0], v[j], v[j + 1]);
+                F16::pair(w[1], v[j + 2], v[j + 3]);
+            }
+        }
         return;
     }
 #pragma unroll
     for (int j = 0; j < V; ++j)
-        v[j] = e0 + j < experts ? Value<T>::load(p, row + e0 + j) : -__builtin_inff();
+        v[j] = e0 + j < experts ? load_one(dtype, p, row + e0 + j) : -__builtin_inff();
 }
 
 // Unsigned numbers in the order of the floats: NaN largest, the zeros equal, 0 below every one of them.
@@ -88,36 +88,57 @@ __device__ __forceinline__ unsigned key_of(float v) {
     const unsigned b = __float_as_uint(v + 0.f); // -0 + 0 = 0
     return v != v ? 0xffffffffu : b ^ (static_cast<int>(b) < 0 ? 0xffffffffu : 0x80000000u);
 }
+__device__ __forceinline__ unsigned plain_key(float v) { // of no NaN (a positive one is right, too)
+    const int b = __float_as_int(v + 0.f);
+    return static_cast<unsigned>(b) ^ (static_cast<unsigned>(b >> 31) | 0x80000000u);
+}
 __device__ __forceinline__ float value_of(unsigned k) {
     return __uint_as_float(k ^ (static_cast<int>(k) < 0 ? 0x80000000u : 0xffffffffu)); // NaN: 0x7fffffff, a NaN
 }
 
-template <int L> __device__ __forceinline__ unsigned group_max(unsigned v) {
+// exp(x) for x <= 0: the product's rounding makes it off by |x| 2^-24 at most, v_exp_f32 by one unit.
+__device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
+
+// Compare-exchanges of a sorting network for N = 4, 8 or 16 values (odd-even merges).
+template <int N> struct Network {
+    int pairs[N == 4 ? 5 : N == 8 ? 19 : 63][2] = {};
+    constexpr Network() {
+        int n = 0;
+        for (int p = 1; p < N; p *= 2)
+            for (int k = p; k >= 1; k /= 2)
+                for (int j = k % p; j + k < N; j += 2 * k)
+                    for (int i = 0; i < k; ++i)
+                        if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                            pairs[n][0] = i + j;
+                            pairs[n][1] = i + j + k;
+                            ++n;
+                        }
+    }
+};
+template <int N> __device__ __forceinline__ void sort_descending(unsigned (&v)[N]) {
+    constexpr Network<N> net;
+    constexpr int        count = sizeof(net.pairs) / sizeof(net.pairs[0]);
 #pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1)
-        v = max(v, static_cast<unsigned>(__shfl_xor(static_cast<int>(v), d)));
-    return v;
-}
-template <int L> __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int d = L / 2; d > 0; d >>= 1)
-        v += __shfl_xor(v, d);
-    return v;
+    for (int i = 0; i < count; ++i) {
+        const unsigned a = v[net.pairs[i][0]], b = v[net.pairs[i][1]];
+        v[net.pairs[i][0]] = max(a, b);
+        v[net.pairs[i][1]] = min(a, b);
+    }
 }
 
 // Exclusive prefix sums over the threads of a workgroup; `scratch` of kWaves entries.
-__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t *scratch, int64_t *total) {
+__device__ __forceinline__ int block_prefix(int v, int *scratch, int *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    int64_t   s = v;
+    int       s = v;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int64_t o = __shfl_up(s, d);
+        const int o = __shfl_up(s, d);
         s += lane >= d ? o : 0;
     }
     if (lane == 63)
         scratch[wave] = s;
     __syncthreads();
-    int64_t before = 0, all = 0;
+    int before = 0, all = 0;
     for (int i = 0; i < kWaves; ++i) {
         before += i < wave ? scratch[i] : 0;
         all += scratch[i];
@@ -146,52 +167,136 @@ __device__ __forceinline__ void write_loss(const RouteArgs &a, int64_t count, in
     }
 }
 
-// One chunk of tokens a workgroup.
-template <typename T, int L, int V> __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
-    constexpr int kPer = 64 / L, kExperts = L * V; // tokens a wave has at a time
-    __shared__ short    sel[kMaxPairs];            // expert of each pair, -1: none
+// One chunk of tokens a workgroup. KEEP: values of its own that a lane may give (its share of the top_k + 1 largest);
+// SLOTS: of the top_k + 1, those that one lane keeps (lane s % L of the token the s-th).
+template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
+    constexpr int      kPer = 64 / L, kExperts = L * V; // tokens a wave has at a time
+    constexpr unsigned kIndex = kExperts - 1;           // low bits of a packed value
+    __shared__ short    sel[kMaxPairs];                 // expert of each pair, -1: none
     __shared__ uint16_t seg_hist[kSegments][kExperts];
-    __shared__ float    sum_part[kWaves > kPer ? kWaves : kPer][kExperts];
-    __shared__ int      live_part[kWaves];
-    __shared__ int64_t  scratch[kWaves];
+    __shared__ float    sum_part[kWaves][kExperts];
+    __shared__ int      live_part[kWaves], scratch[kWaves];
     __shared__ float    fscratch[kWaves];
     const int     tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int     sub = lane & (L - 1), e0 = sub * V, base_lane = lane & ~(L - 1);
     const int64_t first  = static_cast<int64_t>(blockIdx.x) * a.chunk;
     const int     tokens = static_cast<int>(min(static_cast<int64_t>(a.chunk), a.tokens - first));
-    const int     pairs  = tokens * a.top_k;
+    const int     pairs  = tokens * a.top_k, segments = (pairs + 63) / 64;
+    unsigned      mask   = ~kIndex; // (in a register: the and-or below has a constant already)
+    asm("" : "+v"(mask));
+    const unsigned lane_bits = (L - 1 - sub) * V;
 
     float acc[V];
 #pragma unroll
     for (int j = 0; j < V; ++j)
         acc[j] = 0.f;
     int live_here = 0;
+    for (int i = tid; i < segments * kExperts; i += kThreads)
+        (&seg_hist[0][0])[i] = 0;
     for (int t = wave * kPer + lane / L; t - lane / L < tokens; t += kWaves * kPer) {
         const bool    inside = t < tokens;
-        const int64_t token  = first + (inside ? t : 0);
+        const int64_t token  = first + (inside ? t : 0), row = token * a.stride;
         const bool    wanted = inside && (a.mask == nullptr || a.mask[token] != 0);
-        float v[V];
-        load_logits<T, V>(a.logits, token * a.stride, e0, a.experts, a.vec, v);
-        unsigned key[V];
-        unsigned top = kNoKey;
+        float    v[V];
+        unsigned packed[V], top = 0, low = 0;
+        load_logits<V>(a.dtype, a.logits, row, e0, a.experts, a.vec, v); // -infinity past the last expert
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            key[j] = wanted && e0 + j < a.experts ? key_of(v[j]) : kNoKey;
-            top    = max(top, key[j]);
+            const unsigned key = plain_key(v[j]);
+            packed[j]          = (key & mask) | (V - 1 - j);
+            top                = max(top, key);
+            low |= __float_as_uint(v[j]);
         }
-        top             = group_max<L>(top);
-        const bool live = top > kNegInf;
-        // a token with a NaN has a NaN for its maximum, and so for every probability
-        const float most = value_of(top);
-        float       sum  = 0.f;
+        top        = group_max<L>(top);
+        low        = group_reduce<L>(low & kIndex, [](unsigned x, unsigned y) { return x | y; });
+        float most = value_of(top), sum = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            v[j] = e0 + j < a.experts ? expf(v[j] - most) : 0.f;
+            v[j] = exp_neg(v[j] - most);
             sum += v[j];
         }
-        sum             = group_sum<L>(sum);
-        const float inv = 1.f / sum;
-        if (live) {
+        sum       = group_sum<L>(sum);
+        bool live = wanted && top > kNegInf;
+        // the top_k + 1 largest packed values in order
+        sort_descending(packed);
+#pragma unroll
+        for (int j = 0; j < KEEP; ++j)
+            packed[j] |= lane_bits;
+        unsigned pick[SLOTS];
+#pragma unroll
+        for (int r = 0; r < SLOTS; ++r) {
+            pick[r] = 0;
+            for (int i = 0; i < L && r * L + i <= a.top_k; ++i) {
+                const unsigned best = group_max<L>(packed[0]);
+                pick[r]             = sub == i ? best : pick[r];
+                const bool mine     = packed[0] == best;
+#pragma unroll
+                for (int j = 0; j + 1 < KEEP; ++j)
+                    packed[j] = mine ? packed[j + 1] : packed[j];
+                packed[KEEP - 1] = mine ? 0 : packed[KEEP - 1];
+            }
+        }
+        // Packing cut the values' last bits: their order is right unless two that follow each other agree in the
+        // rest (top_k and the first one out among them). 16-bit logits have no such bits.
+        bool doubt = false;
+        if (__ballot(low != 0) != 0) {
+#pragma unroll
+            for (int r = 0; r < SLOTS; ++r) {
+                const unsigned up   = static_cast<unsigned>(__shfl(static_cast<int>(pick[r]), base_lane + ((sub + 1) & (L - 1))));
+                const unsigned over = r + 1 < SLOTS ? static_cast<unsigned>(__shfl(static_cast<int>(pick[r + 1 < SLOTS ? r + 1 : r]), base_lane)) : 0;
+                const unsigned next = sub + 1 < L ? up : over;
+                doubt |= r * L + sub < a.top_k && ((pick[r] ^ next) & ~kIndex) == 0;
+            }
+            doubt &= low != 0;
+        }
+        // A NaN sum: a NaN, an infinity, or nothing but -infinity. Then too the wave takes the values one by one.
+        doubt |= sum != sum;
+        int   slot[SLOTS]; // experts
+        float x[SLOTS];    // and their logits, -infinity: none
+#pragma unroll
+        for (int r = 0; r < SLOTS; ++r)
+            slot[r] = static_cast<int>(kIndex - (pick[r] & kIndex));
+        if (__ballot(doubt && wanted) != 0) {
+            unsigned key[V], exact_top = 0;
+            float    raw[V];
+            load_logits<V>(a.dtype, a.logits, row, e0, a.experts, a.vec, raw);
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                key[j]    = e0 + j < a.experts ? key_of(raw[j]) : kNoKey;
+                exact_top = max(exact_top, key[j]);
+            }
+            live = wanted && group_max<L>(exact_top) > kNegInf;
+#pragma unroll
+            for (int r = 0; r < SLOTS; ++r)
+                for (int i = 0; i < L && r * L + i < a.top_k; ++i) {
+                    unsigned own = key[0];
+#pragma unroll
+                    for (int j = 1; j < V; ++j)
+                        own = max(own, key[j]);
+                    const unsigned best = group_max<L>(own);
+                    const uint64_t have = (__ballot(own == best) >> base_lane) & (L == 64 ? ~0ull : (1ull << L) - 1);
+                    const int      from = __builtin_ctzll(have); // the lowest lane that has it, its first value of that size
+                    int            e    = 0;
+#pragma unroll
+                    for (int j = V - 1; j >= 0; --j)
+                        e = key[j] == best ? j : e;
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        key[j] = sub == from && j == e ? kNoKey : key[j];
+                    e       = from * V + __shfl(e, base_lane + from);
+                    slot[r] = sub == i ? e : slot[r];
+                }
+        }
+        float chosen = 0.f;
+#pragma unroll
+        for (int r = 0; r < SLOTS; ++r) {
+            x[r] = -__builtin_inff();
+            if (live && r * L + sub < a.top_k && slot[r] < a.experts)
+                x[r] = load_one(a.dtype, a.logits, row + slot[r]);
+            chosen += x[r] != -__builtin_inff() ? exp_neg(x[r] - most) : 0.f;
+        }
+        const float inv = 1.f / sum, scale = a.renormalize ? 1.f / group_sum<L>(chosen) : inv;
+        if (live && a.balance) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 acc[j] = fmaf(v[j], inv, acc[j]);
@@ -200,72 +305,46 @@ template <typename T, int L, int V> __global__ void __launch_bounds__(kThreads) 
             a.lse[token] = live ? most + logf(sum) : -__builtin_inff();
             live_here += live ? 1 : 0;
         }
-        // the rounds; lane s % L keeps slot s
-        float picked = 0.f, chosen_sum = 0.f;
-        for (int s = 0; s < a.top_k; ++s) {
-            unsigned own = key[0];
 #pragma unroll
-            for (int j = 1; j < V; ++j)
-                own = max(own, key[j]);
-            const unsigned best = group_max<L>(own);
-            const uint64_t have = (__ballot(own == best) >> base_lane) & (L == 64 ? ~0ull : (1ull << L) - 1);
-            const int      from = __builtin_ctzll(have);
-            int            e    = 0;
-#pragma unroll
-            for (int j = V - 1; j >= 0; --j)
-                e = key[j] == best ? j : e;
-            if (sub == from) {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    key[j] = j == e ? kNoKey : key[j];
-            }
-            e = from * V + __shfl(e, base_lane + from);
-            const bool  ok = best > kNegInf;
-            const float w  = ok ? expf(value_of(best) - most) : 0.f;
-            chosen_sum += w;
-            if (inside && sub == s % L) {
-                sel[t * a.top_k + s]                 = static_cast<short>(ok ? e : -1);
-                a.weights[token * a.top_k + s]       = w; // scaled below, by the same lane
-                a.experts_out[token * a.top_k + s]   = ok ? e : -1;
+        for (int r = 0; r < SLOTS; ++r) {
+            const int s = r * L + sub;
+            if (inside && s < a.top_k) {
+                const bool    ok = x[r] != -__builtin_inff(); // -infinity is never chosen
+                const int     i  = t * a.top_k + s;
+                const int64_t o  = first * a.top_k + i;
+                a.weights[o]     = ok ? exp_neg(x[r] - most) * scale : 0.f;
+                a.experts_out[o] = ok ? slot[r] : -1;
+                sel[i]           = static_cast<short>(ok ? slot[r] : -1);
             }
         }
-        picked = a.renormalize ? 1.f / chosen_sum : inv;
-        if (inside)
-            for (int s = sub; s < a.top_k; s += L) {
-                float *w = a.weights + token * a.top_k + s;
-                *w       = live ? *w * picked : 0.f;
-            }
     }
 
     // sums of probabilities and tokens that take part, wave by wave
     if (a.balance) {
 #pragma unroll
-        for (int d = L; d < 64; d <<= 1)
+        for (int j = 0; j < V; ++j) {
 #pragma unroll
-            for (int j = 0; j < V; ++j)
+            for (int d = L; d < 16; d <<= 1)
                 acc[j] += __shfl_xor(acc[j], d);
+            acc[j] = rows_sum<(L > 16 ? L : 16)>(acc[j]);
+        }
         if (lane < L)
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 sum_part[wave][e0 + j] = acc[j];
     }
     {
-        int n = live_here;
-#pragma unroll
-        for (int d = 32; d > 0; d >>= 1)
-            n += __shfl_xor(n, d);
+        const int n = static_cast<int>(group_reduce<64>(static_cast<unsigned>(live_here), [](unsigned x, unsigned y) { return x + y; }));
         if (lane == 0)
             live_part[wave] = n;
     }
-    for (int i = tid; i < kSegments * kExperts; i += kThreads)
-        (&seg_hist[0][0])[i] = 0;
     __syncthreads();
 
     // rank of each pair among the 64 of its segment, and the segments' histograms
     const int p = tid, seg = wave;
     const int e = p < pairs ? sel[p] : -1;
     int       rank = 0;
-    {
+    if (seg < segments) {
         uint64_t same = __ballot(e >= 0);
 #pragma unroll
         for (int b = 1; b < kExperts; b <<= 1) {
@@ -280,24 +359,23 @@ template <typename T, int L, int V> __global__ void __launch_bounds__(kThreads) 
     }
     __syncthreads();
     // running sums over the segments; the chunk's total
-    int total = 0;
+    int   total = 0, live = 0;
+    float sum   = 0.f;
     if (tid < a.experts) {
-        for (int i = 0; i < kSegments; ++i) {
+        for (int i = 0; i < segments; ++i) {
             const int n      = seg_hist[i][tid];
             seg_hist[i][tid] = static_cast<uint16_t>(total);
             total += n;
         }
+        if (a.balance)
+            for (int i = 0; i < kWaves; ++i)
+                sum += sum_part[i][tid];
     }
+    for (int i = 0; i < kWaves; ++i)
+        live += live_part[i];
     __syncthreads();
     if (e >= 0)
         rank += seg_hist[seg][e];
-    float sum = 0.f;
-    if (a.balance && tid < a.experts)
-        for (int i = 0; i < kWaves; ++i)
-            sum += sum_part[i][tid];
-    int live = 0;
-    for (int i = 0; i < kWaves; ++i)
-        live += live_part[i];
 
     const int64_t pair0 = first * a.top_k;
     if (a.chunks > 1) { // finished by the next launches
@@ -313,19 +391,16 @@ template <typename T, int L, int V> __global__ void __launch_bounds__(kThreads) 
             hist[a.experts] = live;
         return;
     }
-    int64_t       all;
-    const int64_t before = block_prefix(tid < a.experts ? total : 0, scratch, &all);
+    int       all;
+    const int before = block_prefix(tid < a.experts ? total : 0, scratch, &all);
+    int      *start  = reinterpret_cast<int *>(&sum_part[0][0]); // (sum_part is read)
     if (tid < a.experts) {
         a.counts[tid] = total;
         a.offs[tid]   = before;
+        start[tid]    = before;
     }
     if (tid == 0)
         a.offs[a.experts] = all;
-    // sum_part is read: its first row takes the experts' starts
-    __syncthreads();
-    int *start = reinterpret_cast<int *>(&sum_part[0][0]);
-    if (tid < a.experts)
-        start[tid] = static_cast<int>(before);
     __syncthreads();
     if (p < pairs)
         a.rows[pair0 + p] = e >= 0 ? start[e] + rank : -1;
@@ -333,12 +408,30 @@ template <typename T, int L, int V> __global__ void __launch_bounds__(kThreads) 
         write_loss(a, total, all, live, sum, fscratch);
 }
 
-// The chunks' histograms become running sums over the chunks; the totals go to counts and to one more row of
-// hist. 64 columns by 16 slices of the chunks a workgroup.
+// The chunks' histograms become running sums over the chunks; the totals go to one more row of hist (and to counts).
+// The sums of probabilities: only their totals, to one more row. 16 columns by 64 slices of the chunks a workgroup,
+// first the columns of hist, then those of sums.
 __global__ void __launch_bounds__(kThreads) scan_kernel(const RouteArgs a) {
-    __shared__ int part[kWaves][64];
-    const int c = threadIdx.x & 63, slice = threadIdx.x >> 6, col = blockIdx.x * 64 + c, cols = a.experts + 1;
-    const int per = (a.chunks + kWaves - 1) / kWaves, from = min(slice * per, a.chunks), to = min(from + per, a.chunks);
+    __shared__ int   part[64][16];
+    __shared__ float fpart[64][16];
+    const int c = threadIdx.x & 15, slice = threadIdx.x >> 4, cols = a.experts + 1, hist_blocks = (cols + 15) / 16;
+    const int per = (a.chunks + 63) / 64, from = min(slice * per, a.chunks), to = min(from + per, a.chunks);
+    if (static_cast<int>(blockIdx.x) >= hist_blocks) {
+        const int col = (blockIdx.x - hist_blocks) * 16 + c;
+        float     s   = 0.f;
+        if (col < a.experts)
+            for (int i = from; i < to; ++i)
+                s += a.sums[static_cast<int64_t>(i) * a.experts + col];
+        fpart[slice][c] = s;
+        __syncthreads();
+        if (slice == 0 && col < a.experts) {
+            for (int i = 1; i < 64; ++i)
+                s += fpart[i][c];
+            a.sums[static_cast<int64_t>(a.chunks) * a.experts + col] = s;
+        }
+        return;
+    }
+    const int col = blockIdx.x * 16 + c;
     int       s   = 0;
     if (col < cols)
         for (int i = from; i < to; ++i)
@@ -347,59 +440,53 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const RouteArgs a) {
     __syncthreads();
     if (col >= cols)
         return;
-    int run = 0, all = 0;
-    for (int i = 0; i < kWaves; ++i) {
-        run += i < slice ? part[i][c] : 0;
-        all += part[i][c];
-    }
+    int run = 0;
+    for (int i = 0; i < slice; ++i)
+        run += part[i][c];
     for (int i = from; i < to; ++i) {
         int      *h = a.hist + static_cast<int64_t>(i) * cols + col;
         const int n = *h;
         *h          = run;
         run += n;
     }
-    if (slice == 0) {
-        a.hist[static_cast<int64_t>(a.chunks) * cols + col] = all;
+    if (slice == 63) {
+        a.hist[static_cast<int64_t>(a.chunks) * cols + col] = run;
         if (col < a.experts)
-            a.counts[col] = all;
+            a.counts[col] = run;
     }
 }
 
 // Every pair's row: its expert's first row, the expert's pairs in earlier chunks, its rank in the chunk. One
 // workgroup more for offs and the loss.
 __global__ void __launch_bounds__(kThreads) finish_kernel(const RouteArgs a) {
-    __shared__ int     start[kThreads];
-    __shared__ int64_t scratch[kWaves];
-    __shared__ float   fscratch[kWaves];
+    __shared__ int   start[kThreads], scratch[kWaves];
+    __shared__ float fscratch[kWaves];
     const int  tid = threadIdx.x, cols = a.experts + 1;
-    const bool last  = static_cast<int>(blockIdx.x) == a.chunks;
-    const int  count = tid < a.experts ? a.hist[static_cast<int64_t>(a.chunks) * cols + tid] : 0;
-    int64_t       all;
-    const int64_t before = block_prefix(count, scratch, &all);
+    const bool last   = static_cast<int>(blockIdx.x) == a.chunks;
+    const int *totals = a.hist + static_cast<int64_t>(a.chunks) * cols;
+    const int  count  = tid < a.experts ? totals[tid] : 0;
+    // this workgroup's pairs are asked for before the sums
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * a.chunk, p = first * a.top_k + tid;
+    const bool    mine  = !last && tid < a.chunk * a.top_k && p < a.tokens * a.top_k;
+    const int     e = mine ? a.experts_out[p] : -1, rank = mine ? a.rows[p] : 0;
+    const int     earlier = !last && tid < a.experts ? a.hist[static_cast<int64_t>(blockIdx.x) * cols + tid] : 0;
+    int           all;
+    const int     before = block_prefix(count, scratch, &all);
     if (!last) {
         if (tid < a.experts)
-            start[tid] = static_cast<int>(before) + a.hist[static_cast<int64_t>(blockIdx.x) * cols + tid];
+            start[tid] = before + earlier;
         __syncthreads();
-        const int64_t first  = static_cast<int64_t>(blockIdx.x) * a.chunk;
-        const int     tokens = static_cast<int>(min(static_cast<int64_t>(a.chunk), a.tokens - first));
-        if (tid < tokens * a.top_k) {
-            const int64_t p = first * a.top_k + tid;
-            const int     e = a.experts_out[p];
-            a.rows[p]       = e >= 0 ? start[e] + a.rows[p] : -1;
-        }
+        if (mine)
+            a.rows[p] = e >= 0 ? start[e] + rank : -1;
         return;
     }
     if (tid < a.experts)
         a.offs[tid] = before;
     if (tid == 0)
         a.offs[a.experts] = all;
-    if (a.balance) {
-        float sum = 0.f;
-        if (tid < a.experts)
-            for (int i = 0; i < a.chunks; ++i)
-                sum += a.sums[static_cast<int64_t>(i) * a.experts + tid];
-        write_loss(a, count, all, a.hist[static_cast<int64_t>(a.chunks) * cols + a.experts], sum, fscratch);
-    }
+    if (a.balance)
+        write_loss(a, count, all, totals[a.experts], tid < a.experts ? a.sums[static_cast<int64_t>(a.chunks) * a.experts + tid] : 0.f,
+                   fscratch);
 }
 
 // No tokens: counts and offs of zero, a loss of zero.
@@ -415,6 +502,8 @@ __global__ void __launch_bounds__(kThreads) empty_kernel(const RouteArgs a) {
     if (threadIdx.x == 0 && a.balance)
         a.loss[0] = 0.f;
 }
+
+template <typename T> constexpr int kType = std::is_same_v<T, float> ? int(GG_DTYPE_FP32) : std::is_same_v<T, BF16> ? int(GG_DTYPE_BF16) : int(GG_DTYPE_FP16);
 
 struct BackArgs {
     const void  *logits;
@@ -439,14 +528,14 @@ template <typename T, int L, int V> __global__ void __launch_bounds__(256) route
         const bool    inside = t0 + mine < a.tokens;
         const int64_t t      = inside ? t0 + mine : a.tokens - 1;
         float v[V], g[V];
-        load_logits<T, V>(a.logits, t * a.stride, e0, a.experts, a.vec, v);
+        load_logits<V>(kType<T>, a.logits, t * a.stride, e0, a.experts, a.vec, v);
         const float lse  = a.lse[t];
         const bool  live = lse > -__builtin_inff() || lse != lse;
         float dot = 0.f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             extra[mine][e0 + j] = 0.f;
-            v[j]                = live && e0 + j < a.experts ? expf(v[j] - lse) : 0.f;
+            v[j]                = live && e0 + j < a.experts ? exp_neg(v[j] - lse) : 0.f;
             g[j]                = a.grad_loss != nullptr && e0 + j < a.experts ? gl * a.slope[e0 + j] : 0.f;
         }
         float inner = 0.f; // sum of w gw over the slots, for renormalised weights
@@ -547,12 +636,16 @@ bool vector_rows(const void *p, int64_t stride, int64_t tokens, int dtype) {
     return aligned(p, 16) && (tokens <= 1 || stride * (dtype == GG_DTYPE_FP32 ? 4 : 2) % 16 == 0);
 }
 
-template <typename T> int run_route(const RouteArgs &a, hipStream_t s) {
+int run_route(const RouteArgs &a, hipStream_t s) {
     int st = with_lanes(a.experts, [&](auto l, auto v) {
-        return launch("route", route_kernel<T, l.value, v.value>, a.chunks, kThreads, s, a);
+        constexpr int few = v.value < 9 ? v.value : 9; // of top_k + 1 <= 9 values
+        constexpr int most = l.value * v.value < 32 ? l.value * v.value + 1 : 33; // top_k + 1
+        return a.top_k <= 8
+                   ? launch("route", route_kernel<l.value, v.value, few, (9 + l.value - 1) / l.value>, a.chunks, kThreads, s, a)
+                   : launch("route", route_kernel<l.value, v.value, v.value, (most + l.value - 1) / l.value>, a.chunks, kThreads, s, a);
     });
     if (st == GG_OK && a.chunks > 1) {
-        st = launch("route", scan_kernel, (a.experts + 1 + 63) / 64, kThreads, s, a);
+        st = launch("route", scan_kernel, (a.experts + 16) / 16 + (a.balance ? (a.experts + 15) / 16 : 0), kThreads, s, a);
         if (st == GG_OK)
             st = launch("route", finish_kernel, static_cast<int64_t>(a.chunks) + 1, kThreads, s, a);
     }
@@ -582,7 +675,7 @@ size_t gg_route_workspace(int64_t tokens, int experts, int top_k) {
     if (chunks == 1)
         return 0;
     const size_t hist = ((static_cast<size_t>(chunks) + 1) * (experts + 1) * 4 + 15) / 16 * 16;
-    return hist + static_cast<size_t>(chunks) * experts * 4;
+    return hist + (static_cast<size_t>(chunks) + 1) * experts * 4;
 }
 
 int gg_route(int dtype, int64_t tokens, int experts, int top_k, int renormalize, const void *logits, int64_t stride,
@@ -612,6 +705,7 @@ int gg_route(int dtype, int64_t tokens, int experts, int top_k, int renormalize,
     a.offs        = offs;
     a.tokens      = tokens;
     a.stride      = stride;
+    a.dtype       = dtype;
     a.experts     = experts;
     a.top_k       = top_k;
     a.renormalize = renormalize;
@@ -625,9 +719,7 @@ int gg_route(int dtype, int64_t tokens, int experts, int top_k, int renormalize,
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (tokens == 0)
         return launch("route", empty_kernel, 1, kThreads, s, a);
-    return dtype == GG_DTYPE_FP32   ? run_route<float>(a, s)
-           : dtype == GG_DTYPE_BF16 ? run_route<BF16>(a, s)
-                                    : run_route<F16>(a, s);
+    return run_route(a, s);
 }
 
 int gg_route_backward(int dtype, int64_t tokens, int experts, int top_k, int renormalize, const void *logits,
