@@ -36,6 +36,16 @@ int launch(const char *what, void (*kernel)(P...), int64_t grid, int threads, hi
     return e == hipSuccess ? static_cast<int>(GG_OK) : fail(GG_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
 
+// Workgroups of a kernel that the GPU holds at once.
+template <typename... P> int resident_blocks(void (*kernel)(P...), int threads) {
+    int dev = 0, cus = 0, per_cu = 0;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, reinterpret_cast<const void *>(kernel), threads, 0) != hipSuccess ||
+        cus < 1 || per_cu < 1)
+        return 1024;
+    return cus * per_cu;
+}
+
 inline bool aligned(const void *p, uintptr_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 inline bool is16(int dtype) { return dtype == GG_DTYPE_BF16 || dtype == GG_DTYPE_FP16; }
 inline bool is8(int dtype) { return dtype == GG_DTYPE_FP8_E4M3 || dtype == GG_DTYPE_FP8_E5M2; }
@@ -66,6 +76,9 @@ struct F16 {
         return __builtin_bit_cast(unsigned, f16x2{static_cast<_Float16>(lo), static_cast<_Float16>(hi)});
     }
 };
+
+// Sixteen bytes that nothing reads again soon: they go past the caches, which keep what comes after.
+__device__ __forceinline__ u32x4 load_once(const void *p) { return __builtin_nontemporal_load(static_cast<const u32x4 *>(p)); }
 
 // Eight values of 16 bytes.
 template <typename T> __device__ __forceinline__ void unpack8(const u32x4 &w, float (&v)[8]) {

@@ -136,11 +136,11 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
             for (int j = 0; j < 8; ++j)
                 v[u][j] = 0.f;
             if (i < a.hidden) {
-                const u32x4 xw = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.x) + row * a.x_stride + i);
+                const u32x4 xw = load_once(static_cast<const uint16_t *>(a.x) + row * a.x_stride + i);
                 unpack8<T>(xw, v[u]);
                 if (a.residual != nullptr) {
                     float r[8];
-                    unpack8<T>(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.residual) + row * a.r_stride + i), r);
+                    unpack8<T>(load_once(static_cast<const uint16_t *>(a.residual) + row * a.r_stride + i), r);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
                         v[u][j] += r[j];
@@ -235,11 +235,12 @@ template <typename T> __global__ void __launch_bounds__(256) quantize_kernel(con
     const float inv = 1.f / s;
     if (blockIdx.x == 0 && threadIdx.x == 0)
         a.scale[0] = s;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    // from the last row backwards: the rows written last are still in the Infinity Cache
+    for (int64_t row = a.rows - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
         const float rstd = a.rstd[row];
         for (int i = threadIdx.x * 8; i < a.hidden; i += 2048) {
             float v[8], w[8];
-            unpack8<T>(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i), v);
+            unpack8<T>(load_once(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i), v);
             load_w<T>(a.weight, a.w32, i, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
@@ -253,14 +254,14 @@ struct BackArgs {
     const void  *g, *h, *weight, *gh;
     const float *rstd;
     void        *gx;
-    float       *parts; // [waves' or workgroups' rows][hidden] partial sums of grad_weight
+    float       *parts; // [workgroups][hidden] partial sums of grad_weight
     int64_t      rows, g_stride, h_stride, gh_stride;
     int          hidden;
     bool         w32;
 };
 
-// grad_x row by row; grad_weight's partial sums stay in registers over the rows of a workgroup (of a wave
-// where a wave has a row) and are written once.
+// grad_x row by row; grad_weight's partial sums stay in registers over the rows of a workgroup and are
+// written once.
 template <typename T, int WPR, int U>
 __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const BackArgs a) {
     __shared__ RowReduce<WPR> m;
@@ -283,10 +284,10 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const Bac
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
             if (i < a.hidden) {
-                gw[u] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.g) + row * a.g_stride + i);
-                hw[u] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i);
+                gw[u] = load_once(static_cast<const uint16_t *>(a.g) + row * a.g_stride + i);
+                hw[u] = load_once(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i);
                 if (a.gh != nullptr)
-                    rw[u] = *reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(a.gh) + row * a.gh_stride + i);
+                    rw[u] = load_once(static_cast<const uint16_t *>(a.gh) + row * a.gh_stride + i);
             }
         }
 #pragma unroll
@@ -327,7 +328,29 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const Bac
             }
         }
     }
-    float *part = a.parts + (static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0)) * a.hidden;
+    // a workgroup whose waves had rows of their own adds them up first, in their order
+    if constexpr (WPR == 1) {
+        __shared__ f32x4 mine[3][U][2][64];
+        if (wave > 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    mine[wave - 1][u][q][lane] = f32x4{dw[u][4 * q], dw[u][4 * q + 1], dw[u][4 * q + 2], dw[u][4 * q + 3]};
+        __syncthreads();
+        if (wave > 0)
+            return;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int o = 0; o < 3; ++o)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        dw[u][4 * q + j] += mine[o][u][q][lane][j];
+    }
+    float *part = a.parts + static_cast<int64_t>(blockIdx.x) * a.hidden;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int i = (u * 64 * WPR + t) * 8;
@@ -339,25 +362,30 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const Bac
     }
 }
 
-// grad_weight: the sum of the partial sums of each column, in their order; 64 columns by 16 slices a workgroup.
+// grad_weight: the sum of the partial sums of each column, in a fixed order; 32 columns by 128 slices of the parts a
+// workgroup.
 template <typename T>
 __global__ void __launch_bounds__(1024) weight_sum_kernel(const float *parts, int n_parts, int hidden, void *out, bool w32) {
-    __shared__ float sums[16][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), slice = threadIdx.x >> 6;
-    const int per = (n_parts + 15) / 16;
-    float     s   = 0.f;
+    __shared__ f32x4 sums[128][8];
+    const int c4 = threadIdx.x & 7, slice = threadIdx.x >> 3, col = blockIdx.x * 32 + c4 * 4; // hidden % 8 == 0
+    f32x4     s{0.f, 0.f, 0.f, 0.f};
     if (col < hidden)
-        for (int p = slice * per; p < min(n_parts, (slice + 1) * per); ++p)
-            s += parts[static_cast<int64_t>(p) * hidden + col];
-    sums[slice][threadIdx.x & 63] = s;
+#pragma unroll 8
+        for (int p = slice; p < n_parts; p += 128)
+            s += *reinterpret_cast<const f32x4 *>(parts + static_cast<int64_t>(p) * hidden + col);
+    sums[slice][c4] = s;
     __syncthreads();
+#pragma unroll
+    for (int half = 64; half > 0; half >>= 1) {
+        if (slice < half)
+            sums[slice][c4] = s += sums[slice + half][c4];
+        __syncthreads();
+    }
     if (slice == 0 && col < hidden) {
-        for (int i = 1; i < 16; ++i)
-            s += sums[i][threadIdx.x];
         if (w32)
-            static_cast<float *>(out)[col] = s;
+            *reinterpret_cast<f32x4 *>(static_cast<float *>(out) + col) = s;
         else
-            static_cast<uint16_t *>(out)[col] = static_cast<uint16_t>(T::word(s, 0.f));
+            *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + col) = u32x2{T::word(s[0], s[1]), T::word(s[2], s[3])};
     }
 }
 
@@ -389,27 +417,31 @@ template <typename T> int run_norm(const NormArgs &a, hipStream_t s) {
             return launch("rms_norm", norm_kernel<T, wpr.value, u.value, false>, std::min(blocks, kMaxBlocks),
                           block_threads(wpr.value), s, a);
         });
+    // The first pass: as many workgroups as fit at once, each with its share of the rows (32768 rows of 7168: 1280
+    // workgroups 405 us for both passes, 1024 439, 2048, 1.6 rounds of them, 465).
     NormArgs b = a;
-    b.n_parts  = static_cast<int>(std::min<int64_t>(blocks, kMaxParts));
     if (b.residual == nullptr) { // h is x
         b.h        = const_cast<void *>(b.x);
         b.h_stride = b.x_stride;
     }
     const int st = with_shape(a.hidden, [&](auto wpr, auto u) {
-        return launch("rms_norm", norm_kernel<T, wpr.value, u.value, true>, b.n_parts, block_threads(wpr.value), s, b);
+        constexpr auto   kernel = norm_kernel<T, wpr.value, u.value, true>;
+        static const int fit    = resident_blocks(kernel, block_threads(wpr.value));
+        b.n_parts               = static_cast<int>(std::min<int64_t>(blocks, std::min(fit, kMaxParts)));
+        return launch("rms_norm", kernel, b.n_parts, block_threads(wpr.value), s, b);
     });
     return st ? st : launch("rms_norm", quantize_kernel<T>, std::min<int64_t>(b.rows, 8192), 256, s, b);
 }
 
-// Workgroups of the backward pass: enough to fill the GPU four times over, few enough that their partial sums
-// are a small part of what is read.
-constexpr int64_t kBackBlocks = 1024;
+// Workgroups of the backward pass: at most those that the GPU holds at once (by the instances' registers, 72 to 224),
+// fewer where each would have less than four rows and their partial sums would cost more than they save. us at 1, 2
+// and 4 rows each: 64 rows of 7168 8.9, 11.3, 16.2; 512 19.9, 18.6, 21.6; 2048 46.8, 37.9, 34.2. At once against 1024:
+// 16640 rows of 2880 73.7 (1536) and 77.6, 4096 of 14336 108.5 (512) and 118.6.
 int64_t back_blocks(int64_t rows, int64_t hidden) {
-    const int64_t b = row_blocks(rows, hidden);
-    return b < kBackBlocks ? b : kBackBlocks;
-}
-int64_t back_parts(int64_t rows, int64_t hidden) {
-    return back_blocks(rows, hidden) * rows_per_block(waves_per_row(hidden));
+    const int     wpr = waves_per_row(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+    const int64_t fit = wpr == 16 ? 256 : u == 1 ? 1792 : u > 4 ? 512 : u == 2 && wpr == 4 ? 1536 : 1024;
+    const int64_t b   = row_blocks(rows, hidden);
+    return std::min(fit, std::max(b / 4, b <= 256 ? b : std::min<int64_t>(b / 2, 512)));
 }
 
 template <typename T> int run_back(const BackArgs &a, void *grad_weight, hipStream_t s) {
@@ -417,8 +449,8 @@ template <typename T> int run_back(const BackArgs &a, void *grad_weight, hipStre
         return launch("rms_norm_backward", norm_back_kernel<T, wpr.value, u.value>, back_blocks(a.rows, a.hidden),
                       block_threads(wpr.value), s, a);
     });
-    return st ? st : launch("rms_norm_backward", weight_sum_kernel<T>, (a.hidden + 63) / 64, 1024, s, a.parts,
-                            static_cast<int>(back_parts(a.rows, a.hidden)), a.hidden, grad_weight, a.w32);
+    return st ? st : launch("rms_norm_backward", weight_sum_kernel<T>, (a.hidden + 31) / 32, 1024, s, a.parts,
+                            static_cast<int>(back_blocks(a.rows, a.hidden)), a.hidden, grad_weight, a.w32);
 }
 
 // Rules shared by both passes.
@@ -512,7 +544,7 @@ int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int6
 size_t gg_rms_norm_backward_workspace(int64_t rows, int64_t hidden) {
     if (rows < 1 || hidden < 1 || hidden > 32768)
         return 0;
-    return static_cast<size_t>(back_parts(rows, hidden)) * static_cast<size_t>(hidden) * 4;
+    return static_cast<size_t>(back_blocks(rows, hidden)) * static_cast<size_t>(hidden) * 4;
 }
 
 int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidden, const void *grad_y,
@@ -531,8 +563,8 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
     if (grad_h != nullptr)
         if (const int st = check_rows("grad_h", grad_h, grad_h_stride, rows))
             return st;
-    if (!aligned(weight, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 4))
-        return fail(GG_ERR_UNSUPPORTED, "weight and grad_x must be 16-byte aligned, grad_weight 4-byte");
+    if (!aligned(weight, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 16))
+        return fail(GG_ERR_UNSUPPORTED, "weight, grad_x and grad_weight must be 16-byte aligned");
     if (workspace_bytes < gg_rms_norm_backward_workspace(rows, hidden) || (rows > 0 && (workspace == nullptr || !aligned(workspace, 16))))
         return fail(GG_ERR_WORKSPACE, "workspace must be 16-byte aligned and of gg_rms_norm_backward_workspace(rows, hidden) bytes");
     BackArgs a{};
@@ -550,7 +582,7 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
     a.hidden    = static_cast<int>(hidden);
     a.w32       = weight_dtype == GG_DTYPE_FP32;
     if (rows == 0) { // the sums of no rows
-        return launch("rms_norm_backward", weight_sum_kernel<BF16>, (a.hidden + 63) / 64, 1024,
+        return launch("rms_norm_backward", weight_sum_kernel<BF16>, (a.hidden + 31) / 32, 1024,
                       static_cast<hipStream_t>(stream), nullptr, 0, a.hidden, grad_weight, a.w32);
     }
     return dtype == GG_DTYPE_BF16 ? run_back<BF16>(a, grad_weight, static_cast<hipStream_t>(stream))
