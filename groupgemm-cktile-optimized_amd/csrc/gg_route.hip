@@ -21,6 +21,7 @@ namespace layer {
 namespace {
 
 constexpr int kThreads  = 1024, kWaves = kThreads / 64;
+constexpr int kScanless = 32; // chunks
 constexpr int kMaxPairs = 1024, kMaxTokens = 128, kSegments = kMaxPairs / 64; // of a chunk
 
 struct RouteArgs {
@@ -77,9 +78,32 @@ __device__ __forceinline__ void load_logits(int dtype, const void *p, int64_t ro
         }
         return;
     }
+    // one by one; past the last expert its value is asked for again, so that no load waits for a branch
+    int at[V];
 #pragma unroll
     for (int j = 0; j < V; ++j)
-        v[j] = e0 + j < experts ? load_one(dtype, p, row + e0 + j) : -__builtin_inff();
+        at[j] = min(e0 + j, experts - 1);
+    if (dtype == GG_DTYPE_FP32) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            v[j] = static_cast<const float *>(p)[row + at[j]];
+    } else {
+        unsigned w[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            w[j] = static_cast<const uint16_t *>(p)[row + at[j]];
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            float hi;
+            if (dtype == GG_DTYPE_BF16)
+                BF16::pair(w[j], v[j], hi);
+            else
+                F16::pair(w[j], v[j], hi);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+        v[j] = e0 + j < experts ? v[j] : -__builtin_inff();
 }
 
 // Unsigned numbers in the order of the floats: NaN largest, the zeros equal, 0 below every one of them.
@@ -457,20 +481,47 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(const RouteArgs a) {
 }
 
 // Every pair's row: its expert's first row, the expert's pairs in earlier chunks, its rank in the chunk. One
-// workgroup more for offs and the loss.
+// workgroup more for offs and the loss. Of up to kScanless chunks it adds the histograms up itself and there is no
+// scan launch.
 __global__ void __launch_bounds__(kThreads) finish_kernel(const RouteArgs a) {
     __shared__ int   start[kThreads], scratch[kWaves];
     __shared__ float fscratch[kWaves];
     const int  tid = threadIdx.x, cols = a.experts + 1;
     const bool last   = static_cast<int>(blockIdx.x) == a.chunks;
     const int *totals = a.hist + static_cast<int64_t>(a.chunks) * cols;
-    const int  count  = tid < a.experts ? totals[tid] : 0;
     // this workgroup's pairs are asked for before the sums
     const int64_t first = static_cast<int64_t>(blockIdx.x) * a.chunk, p = first * a.top_k + tid;
     const bool    mine  = !last && tid < a.chunk * a.top_k && p < a.tokens * a.top_k;
     const int     e = mine ? a.experts_out[p] : -1, rank = mine ? a.rows[p] : 0;
-    const int     earlier = !last && tid < a.experts ? a.hist[static_cast<int64_t>(blockIdx.x) * cols + tid] : 0;
-    int           all;
+    int           earlier = 0, count = 0, live = 0, all;
+    float         sum = 0.f;
+    if (a.chunks <= kScanless) { // the histograms themselves
+        if (tid < a.experts) {
+#pragma unroll 8
+            for (int i = 0; i < a.chunks; ++i) {
+                const int n = a.hist[i * cols + tid];
+                count += n;
+                earlier += i < static_cast<int>(blockIdx.x) ? n : 0;
+            }
+            if (last && a.balance)
+#pragma unroll 8
+                for (int i = 0; i < a.chunks; ++i)
+                    sum += a.sums[i * a.experts + tid];
+        }
+        if (last) {
+            for (int i = 0; i < a.chunks; ++i)
+                live += a.hist[i * cols + a.experts];
+            if (tid < a.experts)
+                a.counts[tid] = count;
+        }
+    } else {
+        if (tid < a.experts) {
+            count   = totals[tid];
+            earlier = last ? 0 : a.hist[static_cast<int64_t>(blockIdx.x) * cols + tid];
+            sum     = last && a.balance ? a.sums[static_cast<int64_t>(a.chunks) * a.experts + tid] : 0.f;
+        }
+        live = totals[a.experts];
+    }
     const int     before = block_prefix(count, scratch, &all);
     if (!last) {
         if (tid < a.experts)
@@ -485,8 +536,7 @@ __global__ void __launch_bounds__(kThreads) finish_kernel(const RouteArgs a) {
     if (tid == 0)
         a.offs[a.experts] = all;
     if (a.balance)
-        write_loss(a, count, all, totals[a.experts], tid < a.experts ? a.sums[static_cast<int64_t>(a.chunks) * a.experts + tid] : 0.f,
-                   fscratch);
+        write_loss(a, count, all, live, sum, fscratch);
 }
 
 // No tokens: counts and offs of zero, a loss of zero.
@@ -613,7 +663,17 @@ template <typename F> int with_lanes(int experts, F f) {
     return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
 }
 
-int chunk_tokens(int top_k) { return std::min(kMaxTokens, kMaxPairs / top_k); }
+// Tokens of a chunk. All of them where a workgroup takes them in two turns of its waves: one launch. Else a quarter of
+// its waves' tokens or more, so that there are about as many chunks as CUs (4096 tokens of 256 experts, top 8: 16 tokens a
+// chunk instead of 128).
+int chunk_tokens(int64_t tokens, int experts, int top_k) {
+    const int most = std::min(kMaxTokens, kMaxPairs / top_k);
+    const int turn = with_lanes(experts, [](auto l, auto) { return kWaves * 64 / l.value; }); // tokens of a workgroup's waves at a time
+    if (tokens <= std::min(most, 2 * turn))
+        return most;
+    const int64_t even = (tokens + 255) / 256, quarter = turn / 4;
+    return static_cast<int>(std::min<int64_t>(most, (even + quarter - 1) / quarter * quarter));
+}
 
 int check_route(int dtype, int64_t tokens, int experts, int top_k, const void *logits, int64_t stride) {
     if (!is16(dtype) && dtype != GG_DTYPE_FP32)
@@ -645,7 +705,8 @@ int run_route(const RouteArgs &a, hipStream_t s) {
                    : launch("route", route_kernel<l.value, v.value, v.value, (most + l.value - 1) / l.value>, a.chunks, kThreads, s, a);
     });
     if (st == GG_OK && a.chunks > 1) {
-        st = launch("route", scan_kernel, (a.experts + 16) / 16 + (a.balance ? (a.experts + 15) / 16 : 0), kThreads, s, a);
+        if (a.chunks > kScanless)
+            st = launch("route", scan_kernel, (a.experts + 16) / 16 + (a.balance ? (a.experts + 15) / 16 : 0), kThreads, s, a);
         if (st == GG_OK)
             st = launch("route", finish_kernel, static_cast<int64_t>(a.chunks) + 1, kThreads, s, a);
     }
@@ -669,9 +730,9 @@ using namespace gg::layer;
 extern "C" {
 
 size_t gg_route_workspace(int64_t tokens, int experts, int top_k) {
-    if (tokens < 1 || experts < 1 || top_k < 1 || top_k > 32)
+    if (tokens < 1 || experts < 1 || experts > 1024 || top_k < 1 || top_k > 32)
         return 0;
-    const int64_t chunk = chunk_tokens(top_k), chunks = (tokens + chunk - 1) / chunk;
+    const int64_t chunk = chunk_tokens(tokens, experts, top_k), chunks = (tokens + chunk - 1) / chunk;
     if (chunks == 1)
         return 0;
     const size_t hist = ((static_cast<size_t>(chunks) + 1) * (experts + 1) * 4 + 15) / 16 * 16;
@@ -709,7 +770,7 @@ int gg_route(int dtype, int64_t tokens, int experts, int top_k, int renormalize,
     a.experts     = experts;
     a.top_k       = top_k;
     a.renormalize = renormalize;
-    a.chunk       = chunk_tokens(top_k);
+    a.chunk       = chunk_tokens(tokens, experts, top_k);
     a.chunks      = static_cast<int>((tokens + a.chunk - 1) / a.chunk);
     a.hist        = static_cast<int *>(workspace);
     a.sums        = reinterpret_cast<float *>(static_cast<char *>(workspace) +

@@ -94,6 +94,27 @@ def test_combine_and_gradients(pkg, dtype, t, e, k, h, masked, closed):
     assert torch.equal(gy, again[0]) and torch.equal(gw, again[1])
 
 
+@pytest.mark.parametrize("t,e,k,h,masked", [(26000, 16, 2, 2056, False), (13000, 32, 4, 2048, True)])
+def test_outputs_past_the_caches(pkg, t, e, k, h, masked):
+    """More than 192 MB of rows: stores that bypass the caches, same results."""
+    r = _routing(pkg, t, e, k, 5, masked)
+    ok, at = r.rows >= 0, r.rows.clamp(min=0).long()
+    x = torch.randn(t, h, device=DEV, generator=_gen(1)).to(torch.bfloat16)
+    xs = pkg.dispatch(x, r)
+    assert xs.numel() * 2 > 192 << 20
+    assert bool((xs[int(r.offs[-1]):] == 0).all())
+    for s in range(k):
+        assert torch.equal(xs[at[ok[:, s], s]], x[ok[:, s]])
+    gy, gw = pkg.combine_backward(x, xs, r)
+    assert bool((gy[int(r.offs[-1]):] == 0).all())
+    norm = x.double().square().sum(1)
+    for s in range(k):
+        o = ok[:, s]
+        want = x[o].double() * r.weights[o, s, None].double()
+        assert bool(((gy[at[o, s]].double() - want).abs() <= HALF[torch.bfloat16] * want.abs() * 1.001).all())
+        assert bool(((gw[o, s].double() - norm[o]).abs() <= D * norm[o]).all())
+
+
 def test_gradients_against_differences(pkg):
     """combine is linear in y and in the weights: the difference along a direction is exact."""
     t, e, k, h = 9, 8, 3, 64
