@@ -75,6 +75,11 @@ def _out(t, dtype, shape, dev):
     return t
 
 
+def _new_like(x):
+    """A contiguous tensor of x's type and shape (empty_like is the quicker of the two)."""
+    return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
 def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -116,7 +121,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
         _like("residual", residual, x)
         rs = _matrix("residual", residual)
         if out_h is None:
-            h = torch.empty((m, n), dtype=dtype, device=dev)
+            h = _new_like(x)
             hs = n
         else:
             h = out_h
@@ -145,7 +150,7 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
             mode, s = _GIVEN, scale
             if s.dtype != torch.float32 or s.numel() != 1 or s.device != dev:
                 raise ValueError("scale must be 'tensor', 'row' or a device float32 tensor of one value")
-    y = _out(out, out_dtype, (m, n), dev)
+    y = _new_like(x) if out is None and mode == _PLAIN else _out(out, out_dtype, (m, n), dev)
     rstd = torch.empty(m, dtype=torch.float32, device=dev)
     _call(_lib.gg_rms_norm, dev, stream, (dt, dt if wd == dtype else _FP32, od, mode, m, n, eps, x.data_ptr(), xs,
                                           _ptr(residual), rs,
@@ -174,8 +179,8 @@ def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Op
         raise TypeError("weight must be of h's type or float32")
     _flat("weight", weight, wd, (n,), dev)
     _flat("rstd", rstd, torch.float32, (m,), dev)
-    gx = _out(out, dtype, (m, n), dev)
-    gw = torch.empty(n, dtype=wd, device=dev)
+    gx = _new_like(h) if out is None else _out(out, dtype, (m, n), dev)
+    gw = torch.empty_like(weight)
     need = _lib.gg_rms_norm_backward_workspace(m, n)
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     _call(_lib.gg_rms_norm_backward, dev, stream, (dt, dt if wd == dtype else _FP32, m, n, grad_y.data_ptr(), gs,
@@ -227,8 +232,8 @@ def route(logits, top_k: int, mask=None, renormalize: bool = True, balance: bool
     if not 1 <= top_k <= e:
         raise ValueError("top_k must be in 1 .. E")
     experts = torch.empty((t, top_k), dtype=torch.int32, device=dev)
-    rows = torch.empty((t, top_k), dtype=torch.int32, device=dev)
-    weights = torch.empty((t, top_k), dtype=torch.float32, device=dev)
+    rows = torch.empty_like(experts)
+    weights = torch.empty_like(experts, dtype=torch.float32)
     counts = torch.empty(e, dtype=torch.int64, device=dev)
     offs = torch.empty(e + 1, dtype=torch.int64, device=dev)
     lse = torch.empty(t, dtype=torch.float32, device=dev)
@@ -265,7 +270,7 @@ def route_backward(logits, routing: Routing, grad_weights=None, grad_loss=None, 
         _flat("routing.slope", r.slope, torch.float32, (e,), dev)
         if grad_loss.dtype != torch.float32 or grad_loss.numel() != 1 or grad_loss.device != dev:
             raise ValueError("grad_loss must be a device float32 tensor of one value")
-    g = _out(out, logits.dtype, (t, e), dev)
+    g = _new_like(logits) if out is None else _out(out, logits.dtype, (t, e), dev)
     _call(_lib.gg_route_backward, dev, stream, (dt, t, e, k, int(r.renormalize), logits.data_ptr(), stride,
                                                 r.experts.data_ptr(),
                                                 r.weights.data_ptr(), r.lse.data_ptr(), _ptr(grad_weights), _ptr(grad_loss),
