@@ -1,0 +1,116 @@
+"""The operators together, as moe_example.py's layer runs them, against a float64 autograd layer with the
+same routing.
+
+Bounds: about eight bf16 roundings (2^-9 each in the mean, and no cancellation in these norms) lie between input and
+any output or gradient: 2 % of the 2-norm. fp8 (e4m3: 2^-4 at most, 3 % in the mean, on both operands) 8 %; 4 bits with
+a scale for 64 normal values (a step of 0.35 standard deviations, 0.1 rms) on both products 20 %.
+"""
+import importlib
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs an MI355X", allow_module_level=True)
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+
+def _layer(pkg, **kw):
+    return importlib.import_module(pkg.__name__ + ".moe_example").MoeLayer(**kw)
+
+
+def _inputs(t, h, seed=1):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [torch.randn(t, h, device="cuda", generator=g).to(torch.bfloat16) for _ in range(4)]
+
+
+def _off(a, b):
+    b = b.detach().double()
+    return float((a.double() - b).norm() / b.norm())
+
+
+def _reference(layer, x, residual, r):
+    """(out, h, loss, leaves) in float64, the experts and counts of r held."""
+    leaves = {n: getattr(layer, n).double().requires_grad_() for n in ("norm", "router", "gate_up", "down")}
+    leaves["x"] = (x.double() + residual.double()).to(x.dtype).double().requires_grad_()
+    h = leaves["x"]
+    y = h * (h.square().mean(1, keepdim=True) + 1e-6).rsqrt() * leaves["norm"]
+    p = torch.softmax(y @ leaves["router"].t(), 1)
+    out = torch.zeros_like(y)
+    ok = r.experts >= 0
+    w = torch.take_along_dim(p, r.experts.clamp(min=0).long(), 1) * ok
+    w = w / w.sum(1, keepdim=True).clamp(min=1e-300)
+    for e in range(layer.router.shape[0]):
+        t, s = torch.nonzero(r.experts == e, as_tuple=True)
+        gu = y[t] @ leaves["gate_up"][e].t()
+        a, b = gu.chunk(2, 1)
+        out = out.index_add(0, t, (torch.nn.functional.silu(a) * b) @ leaves["down"][e].t() * w[t, s, None])
+    live = ok.any(1)
+    loss = (r.slope.double() * (p * live[:, None]).sum(0)).sum()
+    return out, h, loss, leaves
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_training_step(pkg, padded):
+    t, h = 300, 256
+    layer = _layer(pkg, hidden=h, inner=192, experts=12, top_k=3)
+    x, residual, grad, grad_h = _inputs(t, h)
+    mask = torch.arange(t, device="cuda") % 100 < 77 if padded else None
+    out, hh, loss, saved = layer.forward(x, residual, mask)
+    r = saved[4]
+    want, h64, loss64, leaves = _reference(layer, x, residual, r)
+    assert torch.equal(hh.double(), h64.detach()) and _off(out, want) < 0.02 and abs(float(loss) / float(loss64) - 1) < 0.02
+    if padded:
+        assert bool((out[~mask] == 0).all())
+    grad_loss = torch.full((), 50.0, device="cuda")
+    got = layer.backward(saved, grad, grad_h, grad_loss)
+    ((want * grad.double()).sum() + 50.0 * loss64 + (h64 * grad_h.double()).sum()).backward()
+    for name, leaf in leaves.items():
+        assert _off(got[name], leaf.grad) < 0.02, (name, _off(got[name], leaf.grad))
+
+
+def test_fp8_and_4_bit_passes(pkg):
+    t, h = 200, 512
+    layer = _layer(pkg, hidden=h, inner=256, experts=8, top_k=2)
+    layer.quantize(64)
+    x, residual, _, _ = _inputs(t, h, 3)
+    out, hh, _, saved = layer.forward(x, residual)
+    same = []
+    for f in (layer.forward_fp8, layer.decode):
+        got, h2 = f(x, residual)
+        assert torch.equal(h2, hh)
+        same.append(got)
+    # tokens whose experts are far enough apart to be the same ones in fp8
+    best = saved[3].sort(1, descending=True).values
+    sure = best[:, 1] - best[:, 2] > 0.3
+    assert int(sure.sum()) > 50
+    assert _off(same[0][sure], out[sure]) < 0.08 and _off(same[1], out) < 0.20
+
+
+def test_decode_does_not_wait_and_can_be_captured(pkg):
+    h = 512
+    layer = _layer(pkg, hidden=h, inner=256, experts=16, top_k=4)
+    layer.quantize(128)
+    x, residual, _, _ = _inputs(4, h, 5)
+    layer.decode(x, residual)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):  # a wait would fail the capture
+        out, _ = layer.decode(x, residual)
+    for seed in (6, 7, 8):
+        x.copy_(_inputs(4, h, seed)[0])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, layer.decode(x, residual)[0])
+
+
+def test_script_runs():
+    r = subprocess.run([sys.executable, os.path.join(ROOT, "groupgemm-cktile-optimized_amd", "moe_example.py"), "--tokens", "256",
+                        "--hidden", "256", "--inner", "128", "--experts", "8"], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "decode of 8, 4-bit" in r.stdout, r.stderr[-800:]
