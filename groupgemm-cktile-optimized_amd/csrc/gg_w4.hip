@@ -108,24 +108,39 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t v) {
     return v;
 }
 
-// The `want`-th group with rows, or -1, and its rows. Its weights can be asked for before its first row is known.
+// The `want`-th group with rows, or -1, and its rows. Its weights can be asked for before its first row is known. 64
+// groups are looked at first, then 256 at a time (four loads in flight; from the start they cost a call of 64 groups
+// or fewer 0.4 us).
 struct Found {
     int group, rows;
 };
-__device__ __forceinline__ Found find_group(const W4Args &a, int want, int lane) {
-    for (int g0 = 0; g0 < a.group_num; g0 += 64) {
-        const int64_t len  = length_of(a, g0 + lane);
-        uint64_t      have = __ballot(len > 0);
-        const int     n    = __builtin_popcountll(have);
+template <int N> __device__ __forceinline__ bool find_in(const W4Args &a, int g0, int &want, int lane, Found &f) {
+    int64_t len[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+        len[q] = length_of(a, g0 + 64 * q + lane);
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+        uint64_t  have = __ballot(len[q] > 0);
+        const int n    = __builtin_popcountll(have);
         if (want < n) {
             for (int i = 0; i < want; ++i)
                 have &= have - 1;
             const int src = __builtin_ctzll(have);
-            return {g0 + src, __builtin_amdgcn_readlane(static_cast<int>(len), src)};
+            f             = {g0 + 64 * q + src, __builtin_amdgcn_readlane(static_cast<int>(len[q]), src)};
+            return true;
         }
         want -= n;
     }
-    return {-1, 0};
+    return false;
+}
+__device__ __forceinline__ Found find_group(const W4Args &a, int want, int lane) {
+    Found f{-1, 0};
+    if (!find_in<1>(a, 0, want, lane, f))
+        for (int g0 = 64; g0 < a.group_num; g0 += 256)
+            if (find_in<4>(a, g0, want, lane, f))
+                break;
+    return f;
 }
 // Its first row; -1 if its rows do not lie inside [0, total_m).
 __device__ __forceinline__ int64_t first_row(const W4Args &a, const Found &f, int lane) {
@@ -133,14 +148,15 @@ __device__ __forceinline__ int64_t first_row(const W4Args &a, const Found &f, in
     if (a.offs != nullptr) {
         row0 = read_lane(a.offs[f.group], 0);
     } else {
-        for (int g0 = 0; g0 < f.group; g0 += 64)
-            row0 += wave_sum64(g0 + lane < f.group ? length_of(a, g0 + lane) : 0);
-        row0 = read_lane(row0, 0);
+        row0 = lane < f.group ? length_of(a, lane) : 0;
+        for (int g = 64 + lane; g < f.group; g += 64)
+            row0 += length_of(a, g);
+        row0 = read_lane(wave_sum64(row0), 0);
     }
     return row0 >= 0 && row0 <= a.total_m && f.rows <= a.total_m - row0 ? row0 : -1;
 }
 
-// The scales (and zero points times scales) of a tile in every lane: rows 0 .. N - 1 of 16 lanes hold one each.
+// The scales of a tile, and of zero points z 1 + z / 16, in every lane: rows 0 .. N - 1 of 16 lanes hold one each.
 template <typename T, int N, bool ZEROS>
 __device__ __forceinline__ void spread_scales(unsigned s, unsigned z, float (&scale)[N], float (&point)[N]) {
     unsigned v[4] = {ZEROS ? s | z << 16 : s};
@@ -159,7 +175,7 @@ __device__ __forceinline__ void spread_scales(unsigned s, unsigned z, float (&sc
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         scale[i] = W4Type<T>::value(v[i] & 0xffffu);
-        point[i] = ZEROS ? scale[i] * static_cast<float>(v[i] >> 16) : 0.f;
+        point[i] = ZEROS ? fmaf(static_cast<float>(v[i] >> 16), 0.0625f, 1.f) : 1.f;
     }
 }
 
@@ -200,34 +216,30 @@ __device__ __forceinline__ void load_scales(TileScales<NT> &t, const Weights<NT,
     }
 }
 
-// The end of a scale's k: its sums, scaled, into acc. What they lack comes first: base where they did not start
-// from it; with zero points z / 16 of base.
+// What a scale's sums start from: base, times 1 + z / 16 of its column with zero points.
+template <bool ZEROS> __device__ __forceinline__ f32x4 started(const f32x4 &base, float point) {
+    if constexpr (!ZEROS)
+        return base;
+    f32x4 v;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        v[r] = base[r] * point;
+    return v;
+}
+
+// The end of a scale's k: its sums, scaled, into acc. Sums that did not start from base get it here.
 template <int MT, int NT, bool ZEROS, bool BASE_FIRST, int N>
-__device__ __forceinline__ void scale_sums(f32x4 (&acc)[MT][NT], f32x4 (&sum)[MT][NT], f32x4 (&base)[MT],
+__device__ __forceinline__ void scale_sums(f32x4 (&acc)[MT][NT], f32x4 (&sum)[MT][NT], const f32x4 (&base)[MT],
                                            const float (&scale)[NT][N], const float (&point)[NT][N], int q) {
-    if constexpr (!BASE_FIRST)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    sum[i][j][r] += base[i][r];
-    if constexpr (ZEROS)
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-                base[i][r] *= 0.0625f;
 #pragma unroll
     for (int j = 0; j < NT; ++j)
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
+                if constexpr (!BASE_FIRST)
+                    sum[i][j][r] = ZEROS ? fmaf(point[j][q], base[i][r], sum[i][j][r]) : sum[i][j][r] + base[i][r];
                 acc[i][j][r] = fmaf(scale[j][q], sum[i][j][r], acc[i][j][r]);
-                if constexpr (ZEROS)
-                    acc[i][j][r] = fmaf(point[j][q], base[i][r], acc[i][j][r]);
             }
     // here, and not after the tile's last step, where the compiler would gather them with every step's sums alive
 #pragma unroll
@@ -238,11 +250,10 @@ __device__ __forceinline__ void scale_sums(f32x4 (&acc)[MT][NT], f32x4 (&sum)[MT
 }
 
 // Up to 16 rows of a group at a time. Grid: workgroup (tile block of 16 NT columns, one of the groups with rows), G k of
-// one scale. The W waves share out the 128-column tiles; each loads its weights D tiles ahead, scales and x one
-// tile ahead. x comes through a buffer resource that ends at the last row, so rows past it read as zeros and cost no
-// traffic.
-template <typename T, int NT, int W, int G, int D, bool ZEROS>
-__global__ void __launch_bounds__(W * 64, 2) w4_kernel(const W4Args a) {
+// one scale. The W waves share out the 128-column tiles; each loads weights, scales and x one tile ahead. x comes
+// through a buffer resource that ends at the last row, so rows past it read as zeros and cost no traffic.
+template <typename T, int NT, int W, int G, bool ZEROS>
+__global__ void __launch_bounds__(W * 64, NT == 4 ? 3 : 2) w4_kernel(const W4Args a) {
     using X = W4Type<T>;
     constexpr int kSteps  = G / 32;  // matrix steps of one scale
     constexpr int kScales = 128 / G; // scales of one tile
@@ -259,14 +270,12 @@ __global__ void __launch_bounds__(W * 64, 2) w4_kernel(const W4Args a) {
             return;
         const int tile0 = nb * NT;
         const Weights<NT, ZEROS> w(a, f.group, tile0);
-        TileWords<NT>  ahead[D];
-        TileScales<NT> next_scales;
+        TileWords<NT>  words[2]; // of this tile and the next, in turn
+        TileScales<NT> scales[2];
         auto start = [&] {
-#pragma unroll
-            for (int d = 0; d < D; ++d)
-                if (wave + d * W < a.k_tiles)
-                    load_words(ahead[d], w, wave + d * W, lane);
-            load_scales<NT, ZEROS, kScales>(next_scales, w, wave, lane);
+            if (wave < a.k_tiles)
+                load_words(words[0], w, wave, lane);
+            load_scales<NT, ZEROS, kScales>(scales[0], w, wave, lane);
         };
         start();
         const int64_t row0 = first_row(a, f, lane);
@@ -280,6 +289,7 @@ __global__ void __launch_bounds__(W * 64, 2) w4_kernel(const W4Args a) {
             struct Operand {
                 u32x4 x[4];
             };
+            Operand xs[2];
             auto load_x = [&](Operand &o, int c) { // past K: zeros
 #pragma unroll
                 for (int st = 0; st < 4; ++st) {
@@ -291,22 +301,18 @@ __global__ void __launch_bounds__(W * 64, 2) w4_kernel(const W4Args a) {
 #pragma unroll
             for (int j = 0; j < NT; ++j)
                 acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            Operand next;
-            load_x(next, wave);
-            for (int c = wave; c < a.k_tiles; c += W) {
-                const TileWords<NT> now = ahead[0];
-                float scale[NT][kScales], point[NT][kScales]; // of this lane's column: scale, scale * zero point
+            load_x(xs[0], wave);
+            // one tile; PHASE: which of the two buffers is its own (known here, so nothing is moved between them)
+            auto tile = [&](auto phase, int c) {
+                constexpr int kMine = decltype(phase)::value, kNext = 1 - kMine;
+                if (c + W < a.k_tiles)
+                    load_words(words[kNext], w, c + W, lane);
+                load_scales<NT, ZEROS, kScales>(scales[kNext], w, c + W, lane);
+                load_x(xs[kNext], c + W);
+                float scale[NT][kScales], point[NT][kScales]; // of this lane's column
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
-                    spread_scales<T, kScales, ZEROS>(next_scales.s[j], next_scales.z[j], scale[j], point[j]);
-                const Operand x = next;
-#pragma unroll
-                for (int d = 0; d + 1 < D; ++d)
-                    ahead[d] = ahead[d + 1];
-                if (c + D * W < a.k_tiles)
-                    load_words(ahead[D - 1], w, c + D * W, lane);
-                load_scales<NT, ZEROS, kScales>(next_scales, w, c + W, lane);
-                load_x(next, c + W);
+                    spread_scales<T, kScales, ZEROS>(scales[kMine].s[j], scales[kMine].z[j], scale[j], point[j]);
                 f32x4 sum[1][NT], base[1];
                 const f32x4 zero{0.f, 0.f, 0.f, 0.f};
                 constexpr unsigned kMinus = ZEROS ? X::minus16 : X::minus24;
@@ -318,14 +324,20 @@ __global__ void __launch_bounds__(W * 64, 2) w4_kernel(const W4Args a) {
                         base[0] = zero;
 #pragma unroll
                         for (int s2 = step; s2 < step + kSteps; ++s2)
-                            base[0] = X::mma(x.x[s2], minus, base[0]);
+                            base[0] = X::mma(xs[kMine].x[s2], minus, base[0]);
                     }
 #pragma unroll
                     for (int j = 0; j < NT; ++j)
-                        sum[0][j] = X::mma(x.x[step], expand<T>(now.w[j][step], bits), first ? base[0] : sum[0][j]);
+                        sum[0][j] = X::mma(xs[kMine].x[step], expand<T>(words[kMine].w[j][step], bits),
+                                           first ? started<ZEROS>(base[0], point[j][step / kSteps]) : sum[0][j]);
                     if (step % kSteps == kSteps - 1)
                         scale_sums<1, NT, ZEROS, true, kScales>(acc, sum, base, scale, point, step / kSteps);
                 }
+            };
+            for (int c = wave; c < a.k_tiles; c += 2 * W) {
+                tile(std::integral_constant<int, 0>{}, c);
+                if (c + W < a.k_tiles)
+                    tile(std::integral_constant<int, 1>{}, c + W);
             }
             // the waves' sums, in their order; each wave stores every W-th of the NT tiles
             __syncthreads(); // the tiles before are read
@@ -461,7 +473,10 @@ __global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
                         const u32x4 wf = expand<T>(now.w[j][step], bits);
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
-                            sum[i][j] = X::mma(x[step & 1][i], wf, !first ? sum[i][j] : kBaseFirst ? base[i] : zero);
+                            sum[i][j] = X::mma(x[step & 1][i], wf,
+                                               !first       ? sum[i][j]
+                                               : kBaseFirst ? started<ZEROS>(base[i], point[j][step / kSteps])
+                                                            : zero);
                     }
                     if (step % kSteps == kSteps - 1)
                         scale_sums<MT, NT, ZEROS, kBaseFirst, kScales>(acc, sum, base, scale, point, step / kSteps);
@@ -509,8 +524,8 @@ template <typename F> int with_format(const W4Args &a, int group, F f) {
            : group == 64 ? zeros(integral_constant<int, 64>{})
                          : zeros(integral_constant<int, 32>{});
 }
-template <typename T, int NT, int W, int D> int launch_few(const W4Args &a, int group, hipStream_t s) {
-    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_kernel<T, NT, W, g.value, D, z.value>, 16 * NT, 64 * W, a, s); });
+template <typename T, int NT, int W> int launch_few(const W4Args &a, int group, hipStream_t s) {
+    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_kernel<T, NT, W, g.value, z.value>, 16 * NT, 64 * W, a, s); });
 }
 template <typename T, int MT, int NT> int launch_rows(const W4Args &a, int group, hipStream_t s) {
     return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_rows_kernel<T, MT, NT, g.value, z.value>, 64 * NT, 256, a, s); });
@@ -531,9 +546,9 @@ template <typename T> int run_w4(const W4Args &a, int group, hipStream_t s) {
     const int64_t wide = (a.n_tiles + 7) / 8 * slots, narrow = (a.n_tiles + 3) / 4 * slots;
     if (per >= 12 && wide >= 256)
         return per <= 20 ? launch_rows<T, 2, 2>(a, group, s) : launch_rows<T, 4, 2>(a, group, s);
-    return narrow >= 256  ? launch_few<T, 4, 4, 1>(a, group, s)
-           : narrow >= 64 ? launch_few<T, 2, 8, 1>(a, group, s)
-                          : launch_few<T, 1, 8, 2>(a, group, s);
+    return narrow >= 256  ? launch_few<T, 4, 4>(a, group, s)
+           : narrow >= 64 ? launch_few<T, 2, 8>(a, group, s)
+                          : launch_few<T, 1, 8>(a, group, s);
 }
 
 } // namespace
