@@ -682,6 +682,8 @@ int check_route(int dtype, int64_t tokens, int experts, int top_k, const void *l
         return fail(GG_ERR_INVALID, "tokens must be >= 0, experts >= 1 and top_k in 1 .. experts");
     if (experts > 1024 || top_k > 32 || tokens > INT32_MAX / top_k)
         return fail(GG_ERR_UNSUPPORTED, "experts must be at most 1024, top_k at most 32 and tokens * top_k below 2^31");
+    if (tokens > 1 << 28) // HIP refuses grids of 2^32 threads: 1024 for each chunk of 128 tokens
+        return fail(GG_ERR_UNSUPPORTED, "tokens must be at most 268435456");
     if (tokens > 0 && logits == nullptr)
         return fail(GG_ERR_INVALID, "logits is null");
     if (tokens > 1 && stride < 0)

@@ -92,11 +92,11 @@ __device__ __forceinline__ u32x2 swap32(unsigned v) {
     return u32x2{r[0], r[1]};
 }
 
-// Rows of group g, 0 for a bad length.
-__device__ __forceinline__ int64_t length_of(const W4Args &a, int g) {
-    const int64_t len = g < a.group_num ? a.lens[g] : 0;
-    return len < 0 || len > INT32_MAX ? 0 : len;
+// A group's rows, 0 for a length that cannot be right.
+__device__ __forceinline__ int length(int64_t len, int64_t total_m) {
+    return len < 0 || len > total_m ? 0 : static_cast<int>(len);
 }
+__device__ __forceinline__ int length_of(const W4Args &a, int g) { return g < a.group_num ? length(a.lens[g], a.total_m) : 0; }
 __device__ __forceinline__ int64_t read_lane(int64_t v, int src) { // into scalar registers
     return static_cast<int64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), src))) |
            (static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(v >> 32), src)) << 32);
@@ -108,43 +108,73 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t v) {
     return v;
 }
 
-// The `want`-th group with rows, or -1, and its rows. Its weights can be asked for before its first row is known. 64
-// groups are looked at first, then 256 at a time (four loads in flight; from the start they cost a call of 64 groups
-// or fewer 0.4 us).
+// Sums of v over the lanes up to each one.
+template <int CTRL, int ROWS> __device__ __forceinline__ unsigned add_dpp(unsigned v) { // v plus another lane's, of rows ROWS
+    return v + static_cast<unsigned>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ unsigned wave_scan(unsigned v) {
+    v = add_dpp<0x111, 0xf>(v); // the lane 1, 2, 4, 8 before in a row of 16
+    v = add_dpp<0x112, 0xf>(v);
+    v = add_dpp<0x114, 0xf>(v);
+    v = add_dpp<0x118, 0xf>(v);
+    v = add_dpp<0x142, 0xa>(v); // a row's last lane to the next row: rows 1 and 3
+    return add_dpp<0x143, 0xc>(v); // lane 31 to rows 2 and 3
+}
+
+// The `want`-th piece of ROWS rows of the groups: its group (-1: none), the group's rows and the piece's first one. Its
+// weights can be asked for before the group's first row is known. A workgroup for each piece, not for each group, because
+// one group with more rows than the others would keep its workgroups busy after all else is done: 32 groups of 2 to 25
+// rows of 2880 x 2880 51.8 -> 43.6 us, 8 of 12 to 139 rows of 7168 x 2048 47.1 -> 41.
+// 64 groups are looked at first, then 256 at a time: 256 groups of which 29 have rows 21.2 -> 19.8 us against 64 at a time.
 struct Found {
-    int group, rows;
+    int group, rows, m0;
 };
-template <int N> __device__ __forceinline__ bool find_in(const W4Args &a, int g0, int &want, int lane, Found &f) {
-    int64_t len[N];
+template <int ROWS, int N> // N groups a lane, from g0 on
+__device__ __forceinline__ bool find_in(const W4Args &a, rsrc_t lens, int g0, unsigned &want, int lane, Found &f) {
+    int len[N];
+#pragma unroll
+    for (int q = 0; q < N; ++q) { // past the last group: 0
+        const u32x2 v = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(lens, (g0 + lane * N + q) * 8, 0, 0));
+        len[q]        = length(static_cast<int64_t>(v[0] | static_cast<uint64_t>(v[1]) << 32), a.total_m);
+    }
+    unsigned mine = 0;
 #pragma unroll
     for (int q = 0; q < N; ++q)
-        len[q] = length_of(a, g0 + 64 * q + lane);
-#pragma unroll
-    for (int q = 0; q < N; ++q) {
-        uint64_t  have = __ballot(len[q] > 0);
-        const int n    = __builtin_popcountll(have);
-        if (want < n) {
-            for (int i = 0; i < want; ++i)
-                have &= have - 1;
-            const int src = __builtin_ctzll(have);
-            f             = {g0 + 64 * q + src, __builtin_amdgcn_readlane(static_cast<int>(len[q]), src)};
-            return true;
-        }
-        want -= n;
+        mine += (static_cast<unsigned>(len[q]) + ROWS - 1) / ROWS;
+    const unsigned upto = wave_scan(mine), all = __builtin_amdgcn_readlane(upto, 63);
+    if (want >= all) {
+        want -= all;
+        return false;
     }
-    return false;
+    const int src = __builtin_ctzll(__ballot(upto > want));
+    want -= __builtin_amdgcn_readlane(upto - mine, src);
+    f = {g0 + src * N, __builtin_amdgcn_readlane(len[0], src), 0};
+#pragma unroll
+    for (int q = 1; q < N; ++q) {
+        const unsigned pieces = (static_cast<unsigned>(f.rows) + ROWS - 1) / ROWS;
+        if (f.group == g0 + src * N + q - 1 && want >= pieces) {
+            want -= pieces;
+            f.group = g0 + src * N + q;
+            f.rows  = __builtin_amdgcn_readlane(len[q], src);
+        }
+    }
+    f.m0 = static_cast<int>(want) * ROWS;
+    return true;
 }
-__device__ __forceinline__ Found find_group(const W4Args &a, int want, int lane) {
-    Found f{-1, 0};
-    if (!find_in<1>(a, 0, want, lane, f))
+template <int ROWS> __device__ __forceinline__ Found find_piece(const W4Args &a, unsigned want, int lane) {
+    const rsrc_t lens = resource(a.lens, a.group_num * 8);
+    asm volatile("" : "+v"(lane)); // or the offsets made of it stay in registers through the product (5 %)
+    Found f{-1, 0, 0};
+    if (!find_in<ROWS, 1>(a, lens, 0, want, lane, f))
         for (int g0 = 64; g0 < a.group_num; g0 += 256)
-            if (find_in<4>(a, g0, want, lane, f))
+            if (find_in<ROWS, 4>(a, lens, g0, want, lane, f))
                 break;
     return f;
 }
 // Its first row; -1 if its rows do not lie inside [0, total_m).
 __device__ __forceinline__ int64_t first_row(const W4Args &a, const Found &f, int lane) {
     int64_t row0 = 0;
+    asm volatile("" : "+v"(lane)); // as above
     if (a.offs != nullptr) {
         row0 = read_lane(a.offs[f.group], 0);
     } else {
@@ -249,8 +279,7 @@ __device__ __forceinline__ void scale_sums(f32x4 (&acc)[MT][NT], f32x4 (&sum)[MT
             asm volatile("" : "+v"(acc[i][j]));
 }
 
-// Up to 16 rows of a group at a time. Grid: workgroup (tile block of 16 NT columns, one of the groups with rows), G k of
-// one scale. The W waves share out the 128-column tiles; each loads weights, scales and x one tile ahead. x comes
+// 16 rows of a group at a time. Grid: workgroup (piece of 16 rows, block of 16 NT columns), G k of one scale. The W waves share out the 128-column tiles; each loads weights, scales and x one tile ahead. x comes
 // through a buffer resource that ends at the last row, so rows past it read as zeros and cost no traffic.
 template <typename T, int NT, int W, int G, bool ZEROS>
 __global__ void __launch_bounds__(W * 64, NT == 4 ? 3 : 2) w4_kernel(const W4Args a) {
@@ -264,108 +293,101 @@ __global__ void __launch_bounds__(W * 64, NT == 4 ? 3 : 2) w4_kernel(const W4Arg
     const int blocks = (a.n_tiles + NT - 1) / NT;
     const int nb     = static_cast<int>(blockIdx.x) % blocks;
     const int slots  = static_cast<int>(gridDim.x) / blocks;
-    for (int want = static_cast<int>(blockIdx.x) / blocks;; want += slots) {
-        const Found f = find_group(a, want, lane);
+    for (unsigned want = blockIdx.x / blocks;; want += slots) {
+        const Found f = find_piece<16>(a, want, lane);
         if (f.group < 0)
             return;
         const int tile0 = nb * NT;
         const Weights<NT, ZEROS> w(a, f.group, tile0);
         TileWords<NT>  words[2]; // of this tile and the next, in turn
         TileScales<NT> scales[2];
-        auto start = [&] {
-            if (wave < a.k_tiles)
-                load_words(words[0], w, wave, lane);
-            load_scales<NT, ZEROS, kScales>(scales[0], w, wave, lane);
-        };
-        start();
+        if (wave < a.k_tiles)
+            load_words(words[0], w, wave, lane);
+        load_scales<NT, ZEROS, kScales>(scales[0], w, wave, lane);
         const int64_t row0 = first_row(a, f, lane);
         if (row0 < 0)
             continue;
-        for (int m0 = 0; m0 < f.rows; m0 += 16) {
-            if (m0 > 0)
-                start();
-            const rsrc_t xr = resource(static_cast<const uint16_t *>(a.x) + (row0 + m0) * a.k, min(16, f.rows - m0) * a.k * 2);
-            const int    xo = col * a.k * 2 + quad * 16;
-            struct Operand {
-                u32x4 x[4];
-            };
-            Operand xs[2];
-            auto load_x = [&](Operand &o, int c) { // past K: zeros
+        const int m0 = f.m0;
+        const rsrc_t xr = resource(static_cast<const uint16_t *>(a.x) + (row0 + m0) * a.k, min(16, f.rows - m0) * a.k * 2);
+        const int    xo = col * a.k * 2 + quad * 16;
+        struct Operand {
+            u32x4 x[4];
+        };
+        Operand xs[2];
+        auto load_x = [&](Operand &o, int c) { // past K: zeros
 #pragma unroll
-                for (int st = 0; st < 4; ++st) {
-                    const int k0 = c * 128 + st * 32;
-                    o.x[st]      = load128(xr, xo | (k0 < a.k ? 0 : static_cast<int>(0x80000000u)), k0 * 2);
-                }
-            };
-            f32x4 acc[1][NT];
+            for (int st = 0; st < 4; ++st) {
+                const int k0 = c * 128 + st * 32;
+                o.x[st]      = load128(xr, xo | (k0 < a.k ? 0 : static_cast<int>(0x80000000u)), k0 * 2);
+            }
+        };
+        f32x4 acc[1][NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+            acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        load_x(xs[0], wave);
+        // one tile; PHASE: which of the two buffers is its own (known here, so nothing is moved between them)
+        auto tile = [&](auto phase, int c) {
+            constexpr int kMine = decltype(phase)::value, kNext = 1 - kMine;
+            if (c + W < a.k_tiles)
+                load_words(words[kNext], w, c + W, lane);
+            load_scales<NT, ZEROS, kScales>(scales[kNext], w, c + W, lane);
+            load_x(xs[kNext], c + W);
+            float scale[NT][kScales], point[NT][kScales]; // of this lane's column
 #pragma unroll
             for (int j = 0; j < NT; ++j)
-                acc[0][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            load_x(xs[0], wave);
-            // one tile; PHASE: which of the two buffers is its own (known here, so nothing is moved between them)
-            auto tile = [&](auto phase, int c) {
-                constexpr int kMine = decltype(phase)::value, kNext = 1 - kMine;
-                if (c + W < a.k_tiles)
-                    load_words(words[kNext], w, c + W, lane);
-                load_scales<NT, ZEROS, kScales>(scales[kNext], w, c + W, lane);
-                load_x(xs[kNext], c + W);
-                float scale[NT][kScales], point[NT][kScales]; // of this lane's column
+                spread_scales<T, kScales, ZEROS>(scales[kMine].s[j], scales[kMine].z[j], scale[j], point[j]);
+            f32x4 sum[1][NT], base[1];
+            const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+            constexpr unsigned kMinus = ZEROS ? X::minus16 : X::minus24;
+            const u32x4 minus{kMinus, kMinus, kMinus, kMinus};
+#pragma unroll
+            for (int step = 0; step < 4; ++step) {
+                const bool first = step % kSteps == 0;
+                if (first) { // -24 (-16) times the scale's share of sum x, in every column: the sums start from it
+                    base[0] = zero;
+#pragma unroll
+                    for (int s2 = step; s2 < step + kSteps; ++s2)
+                        base[0] = X::mma(xs[kMine].x[s2], minus, base[0]);
+                }
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
-                    spread_scales<T, kScales, ZEROS>(scales[kMine].s[j], scales[kMine].z[j], scale[j], point[j]);
-                f32x4 sum[1][NT], base[1];
-                const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-                constexpr unsigned kMinus = ZEROS ? X::minus16 : X::minus24;
-                const u32x4 minus{kMinus, kMinus, kMinus, kMinus};
-#pragma unroll
-                for (int step = 0; step < 4; ++step) {
-                    const bool first = step % kSteps == 0;
-                    if (first) { // -24 (-16) times the scale's share of sum x, in every column: the sums start from it
-                        base[0] = zero;
-#pragma unroll
-                        for (int s2 = step; s2 < step + kSteps; ++s2)
-                            base[0] = X::mma(xs[kMine].x[s2], minus, base[0]);
-                    }
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        sum[0][j] = X::mma(xs[kMine].x[step], expand<T>(words[kMine].w[j][step], bits),
-                                           first ? started<ZEROS>(base[0], point[j][step / kSteps]) : sum[0][j]);
-                    if (step % kSteps == kSteps - 1)
-                        scale_sums<1, NT, ZEROS, true, kScales>(acc, sum, base, scale, point, step / kSteps);
-                }
-            };
-            for (int c = wave; c < a.k_tiles; c += 2 * W) {
-                tile(std::integral_constant<int, 0>{}, c);
-                if (c + W < a.k_tiles)
-                    tile(std::integral_constant<int, 1>{}, c + W);
+                    sum[0][j] = X::mma(xs[kMine].x[step], expand<T>(words[kMine].w[j][step], bits),
+                                       first ? started<ZEROS>(base[0], point[j][step / kSteps]) : sum[0][j]);
+                if (step % kSteps == kSteps - 1)
+                    scale_sums<1, NT, ZEROS, true, kScales>(acc, sum, base, scale, point, step / kSteps);
             }
-            // the waves' sums, in their order; each wave stores every W-th of the NT tiles
-            __syncthreads(); // the tiles before are read
+        };
+        for (int c = wave; c < a.k_tiles; c += 2 * W) {
+            tile(std::integral_constant<int, 0>{}, c);
+            if (c + W < a.k_tiles)
+                tile(std::integral_constant<int, 1>{}, c + W);
+        }
+        // the waves' sums, in their order; each wave stores every W-th of the NT tiles
+        __syncthreads(); // the tiles before are read
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-                part[wave][j][lane] = acc[0][j];
-            __syncthreads();
-            for (int u = wave; u < NT; u += W) {
-                // a sum lies in lane 16 (row / 4) + column, word row % 4; this lane takes row `col`, columns 4 quad ..
-                float v[4];
+        for (int j = 0; j < NT; ++j)
+            part[wave][j][lane] = acc[0][j];
+        __syncthreads();
+        for (int u = wave; u < NT; u += W) {
+            // a sum lies in lane 16 (row / 4) + column, word row % 4; this lane takes row `col`, columns 4 quad ..
+            float v[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    v[i] = 0.f;
+            for (int i = 0; i < 4; ++i) {
+                v[i] = 0.f;
 #pragma unroll
-                    for (int p = 0; p < W; ++p)
-                        v[i] += part[p][u][(col >> 2) * 16 + quad * 4 + i][col & 3];
-                }
-                const int m = m0 + col, n = (tile0 + u) * 16 + quad * 4;
-                if (m < f.rows && n < a.n) // n % 8 == 0: four columns are all there or none
-                    *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + (row0 + m) * a.n + n) =
-                        u32x2{T::word(v[0], v[1]), T::word(v[2], v[3])};
+                for (int p = 0; p < W; ++p)
+                    v[i] += part[p][u][(col >> 2) * 16 + quad * 4 + i][col & 3];
             }
+            const int m = m0 + col, n = (tile0 + u) * 16 + quad * 4;
+            if (m < f.rows && n < a.n) // n % 8 == 0: four columns are all there or none
+                *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(a.out) + (row0 + m) * a.n + n) =
+                    u32x2{T::word(v[0], v[1]), T::word(v[2], v[3])};
         }
     }
 }
 
-// More rows of a group: 16 MT at a time, each of the four waves with NT tiles of its own, x's rows shared through two LDS
-// buffers of one 128-column tile. A row's 16-byte pieces lie at piece ^ row % 16, so the 16 rows that a matrix
+// More rows: pieces of 16 MT, each of the four waves with NT tiles of its own, x's rows shared through two LDS buffers of one 128-column tile. A row's 16-byte pieces lie at piece ^ row % 16, so the 16 rows that a matrix
 // operand takes at once are in different banks.
 template <typename T, int MT, int NT, int G, bool ZEROS>
 __global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
@@ -382,137 +404,133 @@ __global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
     const int blocks = (a.n_tiles + 4 * NT - 1) / (4 * NT);
     const int nb     = static_cast<int>(blockIdx.x) % blocks;
     const int slots  = static_cast<int>(gridDim.x) / blocks;
-    for (int want = static_cast<int>(blockIdx.x) / blocks;; want += slots) {
-        const Found f = find_group(a, want, lane);
+    for (unsigned want = blockIdx.x / blocks;; want += slots) {
+        const Found f = find_piece<16 * MT>(a, want, lane);
         if (f.group < 0)
             return;
         const int tile0 = (nb * 4 + wave) * NT;
         const Weights<NT, ZEROS> w(a, f.group, tile0);
         TileWords<NT>  ahead[2];
         TileScales<NT> next_scales;
-        auto start = [&] {
-            load_words(ahead[0], w, 0, lane);
-            if (1 < a.k_tiles)
-                load_words(ahead[1], w, 1, lane);
-            load_scales<NT, ZEROS, kScales>(next_scales, w, 0, lane);
-        };
-        start();
+        load_words(ahead[0], w, 0, lane);
+        if (1 < a.k_tiles)
+            load_words(ahead[1], w, 1, lane);
+        load_scales<NT, ZEROS, kScales>(next_scales, w, 0, lane);
         const int64_t row0 = first_row(a, f, lane);
         if (row0 < 0)
             continue;
-        for (int m0 = 0; m0 < f.rows; m0 += 16 * MT) {
-            if (m0 > 0)
-                start();
-            const rsrc_t xr = resource(static_cast<const uint16_t *>(a.x) + (row0 + m0) * a.k, min(16 * MT, f.rows - m0) * a.k * 2);
-            // this thread's pieces: row 16 i + tid / 16, piece tid % 16
-            const int xrow = tid >> 4, piece = tid & 15;
-            u32x4     xin[MT];
-            auto load_x = [&](int c) { // past K: zeros
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    xin[i] = load128(xr, ((16 * i + xrow) * a.k * 2 + piece * 16) | (c * 128 + piece * 8 < a.k ? 0 : static_cast<int>(0x80000000u)),
-                                     c * 256);
-            };
-            auto store_x = [&](int c) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    *reinterpret_cast<u32x4 *>(lds + (c & 1) * kTile + (16 * i + xrow) * 256 + ((piece ^ xrow) << 4)) = xin[i];
-            };
-            f32x4 acc[MT][NT];
+        const int m0 = f.m0;
+        const rsrc_t xr = resource(static_cast<const uint16_t *>(a.x) + (row0 + m0) * a.k, min(16 * MT, f.rows - m0) * a.k * 2);
+        // this thread's pieces: row 16 i + tid / 16, piece tid % 16
+        const int xrow = tid >> 4, piece = tid & 15;
+        u32x4     xin[MT];
+        auto load_x = [&](int c) { // past K: zeros
 #pragma unroll
             for (int i = 0; i < MT; ++i)
+                xin[i] = load128(xr, ((16 * i + xrow) * a.k * 2 + piece * 16) | (c * 128 + piece * 8 < a.k ? 0 : static_cast<int>(0x80000000u)),
+                                 c * 256);
+        };
+        auto store_x = [&](int c) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-            __syncthreads(); // what was in LDS is read
-            load_x(0);
-            store_x(0);
-            __syncthreads();
-            for (int c = 0; c < a.k_tiles; ++c) {
-                const TileWords<NT> now = ahead[0];
-                float scale[NT][kScales], point[NT][kScales];
+            for (int i = 0; i < MT; ++i)
+                *reinterpret_cast<u32x4 *>(lds + (c & 1) * kTile + (16 * i + xrow) * 256 + ((piece ^ xrow) << 4)) = xin[i];
+        };
+        f32x4 acc[MT][NT];
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
-                    spread_scales<T, kScales, ZEROS>(next_scales.s[j], next_scales.z[j], scale[j], point[j]);
-                ahead[0] = ahead[1];
-                const bool more = c + 1 < a.k_tiles;
-                if (more) {
-                    load_x(c + 1);
-                    load_scales<NT, ZEROS, kScales>(next_scales, w, c + 1, lane);
-                }
-                if (c + 2 < a.k_tiles)
-                    load_words(ahead[1], w, c + 2, lane);
-                const unsigned char *xt = lds + (c & 1) * kTile;
-                auto read_x = [&](u32x4(&x)[MT], int step) {
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-                    for (int i = 0; i < MT; ++i)
-                        x[i] = *reinterpret_cast<const u32x4 *>(xt + (16 * i + col) * 256 + (((step * 4 + quad) ^ col) << 4));
-                };
-                f32x4 sum[MT][NT], base[MT];
-                const f32x4 zero{0.f, 0.f, 0.f, 0.f};
-                constexpr unsigned kMinus = ZEROS ? X::minus16 : X::minus24;
-                const u32x4 minus{kMinus, kMinus, kMinus, kMinus};
-                u32x4 x[2][MT]; // of this step and the next
-                // the waves that multiply go before those that load and store: 8 groups of 60 rows of 7168 x 2048 30.8 ->
-                // 29.6 us, 30 rows 20.1 -> 18.9, 16 of 60 of 4096 x 4096 57.7 -> 53.4
-                __builtin_amdgcn_s_setprio(1);
-                read_x(x[0], 0);
+            for (int j = 0; j < NT; ++j)
+                acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        __syncthreads(); // what was in LDS is read
+        load_x(0);
+        store_x(0);
+        __syncthreads();
+        for (int c = 0; c < a.k_tiles; ++c) {
+            const TileWords<NT> now = ahead[0];
+            float scale[NT][kScales], point[NT][kScales];
 #pragma unroll
-                for (int step = 0; step < 4; ++step) {
-                    const bool first = step % kSteps == 0;
-                    if (step < 3)
-                        read_x(x[(step + 1) & 1], step + 1);
-                    if (!kBaseFirst || first)
+            for (int j = 0; j < NT; ++j)
+                spread_scales<T, kScales, ZEROS>(next_scales.s[j], next_scales.z[j], scale[j], point[j]);
+            ahead[0] = ahead[1];
+            const bool more = c + 1 < a.k_tiles;
+            if (more) {
+                load_x(c + 1);
+                load_scales<NT, ZEROS, kScales>(next_scales, w, c + 1, lane);
+            }
+            if (c + 2 < a.k_tiles)
+                load_words(ahead[1], w, c + 2, lane);
+            const unsigned char *xt = lds + (c & 1) * kTile;
+            auto read_x = [&](u32x4(&x)[MT], int step) {
 #pragma unroll
-                        for (int s2 = step; s2 < (kBaseFirst ? step + kSteps : step + 1); ++s2)
+                for (int i = 0; i < MT; ++i)
+                    x[i] = *reinterpret_cast<const u32x4 *>(xt + (16 * i + col) * 256 + (((step * 4 + quad) ^ col) << 4));
+            };
+            f32x4 sum[MT][NT], base[MT];
+            const f32x4 zero{0.f, 0.f, 0.f, 0.f};
+            constexpr unsigned kMinus = ZEROS ? X::minus16 : X::minus24;
+            const u32x4 minus{kMinus, kMinus, kMinus, kMinus};
+            u32x4 x[2][MT]; // of this step and the next
+            // the waves that multiply go before those that load and store: 5 to 10 % (8 groups of 30 rows of 7168 x 2048 20.1
+            // -> 18.9 us when this was added)
+            __builtin_amdgcn_s_setprio(1);
+            read_x(x[0], 0);
 #pragma unroll
-                            for (int i = 0; i < MT; ++i)
-                                base[i] = X::mma(x[s2 & 1][i], minus, first && s2 == step ? zero : base[i]);
+            for (int step = 0; step < 4; ++step) {
+                const bool first = step % kSteps == 0;
+                if (step < 3)
+                    read_x(x[(step + 1) & 1], step + 1);
+                if (!kBaseFirst || first)
 #pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        const u32x4 wf = expand<T>(now.w[j][step], bits);
+                    for (int s2 = step; s2 < (kBaseFirst ? step + kSteps : step + 1); ++s2)
 #pragma unroll
                         for (int i = 0; i < MT; ++i)
-                            sum[i][j] = X::mma(x[step & 1][i], wf,
-                                               !first       ? sum[i][j]
-                                               : kBaseFirst ? started<ZEROS>(base[i], point[j][step / kSteps])
-                                                            : zero);
-                    }
-                    if (step % kSteps == kSteps - 1)
-                        scale_sums<MT, NT, ZEROS, kBaseFirst, kScales>(acc, sum, base, scale, point, step / kSteps);
-                    __builtin_amdgcn_sched_barrier(0); // a step's operands are not fetched earlier than this
+                            base[i] = X::mma(x[s2 & 1][i], minus, first && s2 == step ? zero : base[i]);
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const u32x4 wf = expand<T>(now.w[j][step], bits);
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        sum[i][j] = X::mma(x[step & 1][i], wf,
+                                           !first       ? sum[i][j]
+                                           : kBaseFirst ? started<ZEROS>(base[i], point[j][step / kSteps])
+                                                        : zero);
                 }
-                __builtin_amdgcn_s_setprio(0);
-                if (more)
-                    store_x(c + 1);
-                __syncthreads();
+                if (step % kSteps == kSteps - 1)
+                    scale_sums<MT, NT, ZEROS, kBaseFirst, kScales>(acc, sum, base, scale, point, step / kSteps);
+                __builtin_amdgcn_sched_barrier(0); // a step's operands are not fetched earlier than this
             }
-            // outputs through LDS, a wave's own part: rows of 16 NT columns, stored 16 bytes (8 columns) a lane
-            unsigned char *ot = lds + wave * kOut;
+            __builtin_amdgcn_s_setprio(0);
+            if (more)
+                store_x(c + 1);
+            __syncthreads();
+        }
+        // outputs through LDS, a wave's own part: rows of 16 NT columns, stored 16 bytes (8 columns) a lane
+        unsigned char *ot = lds + wave * kOut;
 #pragma unroll
-            for (int i = 0; i < MT; ++i)
+        for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        *reinterpret_cast<uint16_t *>(ot + ((16 * i + quad * 4 + r) * NT * 16 + j * 16 + col) * 2) =
-                            static_cast<uint16_t>(T::word(acc[i][j][r], 0.f));
-            wave_sync();
-            for (int u = lane; u < MT * 16 * NT * 2; u += 64) {
-                const int m = u / (NT * 2), n8 = u % (NT * 2), n = tile0 * 16 + n8 * 8;
-                if (m0 + m < f.rows && n < a.n)
-                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + (row0 + m0 + m) * a.n + n) =
-                        *reinterpret_cast<const u32x4 *>(ot + (m * NT * 16 + n8 * 8) * 2);
-            }
+                for (int r = 0; r < 4; ++r)
+                    *reinterpret_cast<uint16_t *>(ot + ((16 * i + quad * 4 + r) * NT * 16 + j * 16 + col) * 2) =
+                        static_cast<uint16_t>(T::word(acc[i][j][r], 0.f));
+        wave_sync();
+        for (int u = lane; u < MT * 16 * NT * 2; u += 64) {
+            const int m = u / (NT * 2), n8 = u % (NT * 2), n = tile0 * 16 + n8 * 8;
+            if (m0 + m < f.rows && n < a.n)
+                *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.out) + (row0 + m0 + m) * a.n + n) =
+                    *reinterpret_cast<const u32x4 *>(ot + (m * NT * 16 + n8 * 8) * 2);
         }
     }
 }
 
-template <typename K> int launch_w4(K kernel, int columns, int threads, const W4Args &a, hipStream_t s) {
+// How many pieces of `rows` rows the groups have at most.
+int64_t pieces_of(const W4Args &a, int rows) { return std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m) + a.total_m / rows); }
+
+template <typename K> int launch_w4(K kernel, int rows, int columns, int threads, const W4Args &a, hipStream_t s) {
     const int64_t blocks = (static_cast<int64_t>(a.n_tiles) * 16 + columns - 1) / columns;
-    // at most total_m groups have rows where nothing is wrong with the sizes (slots are walked in strides); HIP refuses
-    // grids of 2^32 threads
-    const int64_t slots = std::clamp<int64_t>(std::min<int64_t>(a.group_num, a.total_m), 1, (int64_t(1) << 31) / threads / blocks);
+    // HIP refuses grids of 2^32 threads: past them the pieces are walked in strides
+    const int64_t slots = std::min<int64_t>(pieces_of(a, rows), (int64_t(1) << 31) / threads / blocks);
     return launch("gemm_w4", kernel, blocks * slots, threads, s, a);
 }
 
@@ -525,30 +543,31 @@ template <typename F> int with_format(const W4Args &a, int group, F f) {
                          : zeros(integral_constant<int, 32>{});
 }
 template <typename T, int NT, int W> int launch_few(const W4Args &a, int group, hipStream_t s) {
-    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_kernel<T, NT, W, g.value, z.value>, 16 * NT, 64 * W, a, s); });
+    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_kernel<T, NT, W, g.value, z.value>, 16, 16 * NT, 64 * W, a, s); });
 }
 template <typename T, int MT, int NT> int launch_rows(const W4Args &a, int group, hipStream_t s) {
-    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_rows_kernel<T, MT, NT, g.value, z.value>, 64 * NT, 256, a, s); });
+    return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_rows_kernel<T, MT, NT, g.value, z.value>, 16 * MT, 64 * NT, 256, a, s); });
 }
 
-// The instance by the rows that a group has on average and the workgroups there are. Measured (us; columns: a few-row
-// instance of 64, 32 and 16 columns a workgroup, then the many-row ones of 32 and 64 rows):
+// The instance by the rows that a group has on average and the workgroups there are. Measured (us; few-row instances of
+// 64, 32 and 16 columns a workgroup, then the many-row one, of 32 rows and 128 columns):
 //   rows per group (ragged; 32 groups of 2880 x 2880, k of a scale 32, zero points / 16 of 4096 x 4096, 128):
-//     8:  43.9 / 34.3, -, -, 49.9 / 35.0, 80.9 / 48.8       12: 56.7 / 44.0, -, -, 52.3 / 35.0, 81.6 / 47.9
-//     20: 82.9 / 71.2, -, -, 98.8 / 61.6, 113.6 / 50.4      24: 85.7 / 64.3, -, -, 89.4 / 61.5, 81.9 / 51.0
-//     48: 138.5 / 96.5, -, -, 122.6 / 79.4, 148.7 / 80.9
-//   workgroups of 64 columns (one row): 8 of 512 x 7168: 11.9, 7.5, 6.3; 32 of 2048 x 2048: 6.1, 4.8, 4.3; 128 of
-//     1024 x 7168 15.7, 9.7, 11.2; 224 of 14336 x 4096 10.7, 9.4, 13.1; 448 of 7168 x 2048 10.2, 12, 12.8
-//   the many-row ones do not split k: with fewer workgroups than CUs they lose (4 groups of 20 rows, 2048 x 4096: 16.7, 11.8,
-//     13.9, 25, 36).
+//     8: 41.1, 53.9, 82.9, 45.1 / 32.8, 41.6, 57.9, 33.8          12: 49.8, 63.2, 100.9, 44.8 / 36.8, 48.7, 71.5, 34.4
+//     24: 70.4, 94.3, 158.2, 62.2 / 49.4, 74.5, 118.7, 43.0       48: 110.8, 157.7, 271.5, 88.8 / 80.9, 131.8, 222.8, 62.5
+//     32 rows in every group of the first: 72.5, 103.6, 180.8, 49.9
+//   Many-row instances of 16, 48 and 64 rows, or of 64, 192 and 256 columns, gain 3 to 17 % where their sizes fit and
+//   lose 5 to 50 % elsewhere.
+//   workgroups of 64 columns (one row): 8 of 512 x 7168: 11.8, 7.3, 6.1; 32 of 512 x 2048: 6.3, 5.0, 4.7; 128 of
+//     4096 x 1024: 5.2, 4.7, 5.5; 224 of 14336 x 4096: 10.7, 9.6, 12.0; 448 of 7168 x 2048: 9.6, 12.0, 14.1; 4 groups of 20
+//     rows, 2048 x 4096 (288): 11.8, 13.9, 18.8
+//   the many-row one does not split k: with fewer workgroups than CUs it loses (those 4 groups: 24.0).
 template <typename T> int run_w4(const W4Args &a, int group, hipStream_t s) {
-    const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m)), per = a.total_m / slots;
-    const int64_t wide = (a.n_tiles + 7) / 8 * slots, narrow = (a.n_tiles + 3) / 4 * slots;
-    if (per >= 12 && wide >= 256)
-        return per <= 20 ? launch_rows<T, 2, 2>(a, group, s) : launch_rows<T, 4, 2>(a, group, s);
-    return narrow >= 256  ? launch_few<T, 4, 4>(a, group, s)
-           : narrow >= 64 ? launch_few<T, 2, 8>(a, group, s)
-                          : launch_few<T, 1, 8>(a, group, s);
+    const int64_t per  = a.total_m / std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m));
+    const int64_t wide = (a.n_tiles + 7) / 8 * pieces_of(a, 32), narrow = (a.n_tiles + 3) / 4 * pieces_of(a, 16);
+    return per >= 12 && wide >= 256 ? launch_rows<T, 2, 2>(a, group, s)
+           : narrow >= 256          ? launch_few<T, 4, 4>(a, group, s)
+           : narrow >= 64           ? launch_few<T, 2, 8>(a, group, s)
+                                    : launch_few<T, 1, 8>(a, group, s);
 }
 
 } // namespace
@@ -569,8 +588,8 @@ extern "C" int gg_gemm_w4(int dtype, int group_num, int64_t total_m, int64_t n, 
         return fail(GG_ERR_UNSUPPORTED, "group must be 32, 64 or 128");
     if (n % 8 != 0 || k % group != 0)
         return fail(GG_ERR_UNSUPPORTED, "N must be a multiple of 8 and K of group");
-    if (n > (1 << 21) || k > (1 << 21) || group_num > 8192)
-        return fail(GG_ERR_UNSUPPORTED, "N and K must be at most 2097152 and groups at most 8192");
+    if (n > (1 << 21) || k > (1 << 21) || group_num > 8192 || total_m > (1 << 27)) // 256 groups' pieces: in 32 bits
+        return fail(GG_ERR_UNSUPPORTED, "N and K must be at most 2097152, groups at most 8192 and rows at most 134217728");
     if (group_num == 0 || total_m == 0 || n == 0)
         return GG_OK;
     if (group_lens == nullptr || x == nullptr || packed == nullptr || scales == nullptr || out == nullptr)

@@ -40,11 +40,11 @@ typedef enum gg_norm_scale {
  * h = x + residual, rounded to x's type as the layers after this one read it (h = x without a
  * residual); rstd = 1 / sqrt(mean(h^2) + eps) of each row; y = h * rstd * weight, of the rounded h.
  * fp8: y = round(h * rstd * weight / scale), scale = max |h * rstd * weight| / (the format's largest
- * value), 1 where that is zero. A NaN in a row makes its rstd, y and (for a tensor scale, every) scale NaN.
+ * value), 1 where that is zero or subnormal. A NaN in a row makes its rstd, y and (for a tensor scale, every) scale NaN.
  *   dtype: GG_DTYPE_BF16 or GG_DTYPE_FP16 (x, residual, h; y unless fp8). weight_dtype: the same or
  *   GG_DTYPE_FP32. out_dtype: dtype, or an fp8 type with scale_mode 1-3.
  *   h: [rows, hidden]; may be x or residual itself. Not written (and may be NULL) without a residual.
- *   y: [rows, hidden] contiguous, overlapping no input. rstd: [rows] or NULL.
+ *   y: [rows, hidden] contiguous, overlapping no input. rstd: [rows], or NULL but for GG_NORM_SCALE_TENSOR.
  *   scale: written, [1] or [rows], or for GG_NORM_SCALE_GIVEN read, [1].
  *   workspace: GG_NORM_WORKSPACE bytes for GG_NORM_SCALE_TENSOR, else unused.
  * GG_ERR_UNSUPPORTED unless hidden % 8 == 0, hidden <= 32768, strides % 8 == 0 and 16-byte aligned
@@ -91,7 +91,7 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
  *               over the tokens that take part, and its derivative with respect to one token's
  *               probability of e, experts * f_e / (tokens that take part). 0 if there are none.
  *   workspace:  gg_route_workspace(tokens, experts, top_k) bytes, 16-byte aligned.
- * GG_ERR_UNSUPPORTED: more than 1024 experts, top_k > 32, tokens * top_k >= 2^31. top_k <= experts.
+ * GG_ERR_UNSUPPORTED: more than 1024 experts, top_k > 32, tokens > 2^28 or tokens * top_k >= 2^31. top_k <= experts.
  */
 size_t gg_route_workspace(int64_t tokens, int experts, int top_k);
 int gg_route(int dtype, int64_t tokens, int experts, int top_k, int renormalize, const void *logits, int64_t stride,
@@ -140,7 +140,8 @@ int gg_combine_backward(int dtype, int64_t tokens, int top_k, int64_t hidden, in
  * zero, in 0..15) for each `group` consecutive k; zero = 8 where zeros is NULL. x [total_m, k], out
  * [total_m, n], scales of dtype (bf16 or fp16), zeros bytes. For groups of few rows: decode, short prompts.
  * group_lens / group_offs: device sizes as in gg_prepare_device_lens_op; a group whose rows are not
- * inside [0, total_m) gets no work (and is not reported).
+ * inside [0, total_m) gets no work (and is not reported). The products are of 16 + q, less (16 + zero) times the sum of x,
+ * exact but for the float32 sums: an infinity in x makes its row's outputs NaN.
  *
  * Storage: n in tiles of 16 and k in tiles of 128, padded with zeros:
  *   packed [group_num][ceil(n / 16)][ceil(k / 128)][64][16] bytes: piece 16 a + r of a tile is row r,
@@ -149,7 +150,7 @@ int gg_combine_backward(int dtype, int64_t tokens, int top_k, int64_t hidden, in
  *   scales, zeros [group_num][ceil(n / 16)][k / group][16].
  * So a wave's load of a tile is 1 KB in a row, and a lane has the operand of four matrix instructions.
  * GG_ERR_UNSUPPORTED unless n % 8 == 0, group is 32, 64 or 128, k % group == 0, x, out, packed, scales
- * 16-byte and zeros 4-byte aligned, n and k at most 2097152 and group_num at most 8192.
+ * 16-byte and zeros 4-byte aligned, n and k at most 2097152, group_num at most 8192 and total_m at most 134217728.
  */
 int gg_gemm_w4(int dtype, int group_num, int64_t total_m, int64_t n, int64_t k, int group, const int64_t *group_lens,
                const int64_t *group_offs, const void *x, const void *packed, const void *scales, const uint8_t *zeros,

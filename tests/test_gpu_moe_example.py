@@ -65,7 +65,7 @@ def test_training_step(pkg, padded):
     out, hh, loss, saved = layer.forward(x, residual, mask)
     r = saved[4]
     want, h64, loss64, leaves = _reference(layer, x, residual, r)
-    assert torch.equal(hh.double(), h64.detach()) and _off(out, want) < 0.02 and abs(float(loss) / float(loss64) - 1) < 0.02
+    assert torch.equal(hh.double(), h64.detach()) and _off(out, want) < 0.02 and abs(float(loss.detach()) / float(loss64.detach()) - 1) < 0.02
     if padded:
         assert bool((out[~mask] == 0).all())
     grad_loss = torch.full((), 50.0, device="cuda")

@@ -138,6 +138,25 @@ def test_many_groups_few_with_rows(pkg, b):
     assert bool(_check(got, x, w, size, offs, lens, torch.bfloat16, k).all())
 
 
+# Pieces of 16 and 32 rows of many groups: full ones, ragged ones, groups without rows between them, few and many rows on average.
+@pytest.mark.parametrize("gaps", [False, True])
+@pytest.mark.parametrize("b,sizes", [(70, (0, 17, 1, 0, 33, 16)), (300, (5, 0, 32, 0, 0, 0, 65)), (330, (64, 31, 0, 15, 48)), (520, (0, 0, 0, 0, 47, 0, 1))])
+def test_pieces_of_many_groups(pkg, b, sizes, gaps):
+    n, k, group, dtype = 40, 160, 32, torch.float16
+    lens = [sizes[(i * i // 3) % len(sizes)] for i in range(b)]
+    offs = [sum(lens[:g]) + (g // 2 if gaps else 0) for g in range(b)]
+    total = offs[-1] + lens[-1] + 1
+    q, s, z = _weights(b, n, k, group, dtype, True, b)
+    w4 = pkg.pack_w4(q, s, z)
+    w, size = _dense(q, s, z, group)
+    x = torch.randn(total, k, device=DEV, generator=_gen(b)).to(dtype)
+    out = torch.full((total, n), 4.0, dtype=dtype, device=DEV)
+    where = torch.tensor(offs + [total], device=DEV) if gaps else None
+    pkg.grouped_gemm_w4(x, w4, torch.tensor(lens, device=DEV), out=out, group_offs=where)
+    written = _check(out, x, w, size, offs, lens, dtype, k)
+    assert bool((out[~written] == 4).all()) and int(written.sum()) == sum(lens)
+
+
 def test_offsets_gaps_and_bad_sizes(pkg):
     """Rows between groups stay as they were; a group that does not lie inside x gets no work, the others do."""
     n, k, group, dtype = 48, 256, 128, torch.bfloat16

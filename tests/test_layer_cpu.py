@@ -74,6 +74,7 @@ def test_rms_norm_backward_refusals(pkg, change, want, text):
     (dict(k=33), UNSUPPORTED, "top_k"),
     (dict(e=1025), UNSUPPORTED, "experts"),
     (dict(t=1 << 29), UNSUPPORTED, "2^31"),
+    (dict(t=(1 << 28) + 1, k=2), UNSUPPORTED, "tokens must be at most"),
     (dict(logits=None), INVALID, "logits is null"),
     (dict(logits=P + 2), UNSUPPORTED, "aligned"),
     (dict(stride=-64), INVALID, "negative"),
@@ -135,6 +136,7 @@ def test_combine_refusals(pkg):
     (dict(k=160), UNSUPPORTED, "K of group"),
     (dict(n=(1 << 21) + 8), UNSUPPORTED, "at most"),
     (dict(b=8193), UNSUPPORTED, "at most"),
+    (dict(m=(1 << 27) + 1), UNSUPPORTED, "rows at most"),
     (dict(lens=None), INVALID, "group_lens"),
     (dict(x=P + 8), UNSUPPORTED, "aligned"),
     (dict(zeros=P + 2), UNSUPPORTED, "aligned"),
