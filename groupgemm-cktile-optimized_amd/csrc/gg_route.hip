@@ -434,49 +434,76 @@ template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(k
 
 // The chunks' histograms become running sums over the chunks; the totals go to one more row of hist (and to counts).
 // The sums of probabilities: only their totals, to one more row. 16 columns by 64 slices of the chunks a workgroup,
-// first the columns of hist, then those of sums.
+// first the columns of hist, then those of sums. A slice's chunks are loaded kHeld at a time.
+template <typename N> __device__ __forceinline__ N slices_before(N s, N (*part)[16], N *total) { // of the 64: in order
+    const int c = threadIdx.x & 15, quarter = (threadIdx.x >> 4) & 3, wave = threadIdx.x >> 6;
+    const N   one = __shfl_up(s, 16), two = __shfl_up(s, 32), three = __shfl_up(s, 48);
+    const N   before = quarter == 0 ? N(0) : quarter == 1 ? one : quarter == 2 ? two + one : three + two + one;
+    if (quarter == 3)
+        part[wave][c] = before + s;
+    __syncthreads();
+    N run = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        run += i < wave ? part[i][c] : N(0);
+        all += part[i][c];
+    }
+    *total = all;
+    return run + before;
+}
 __global__ void __launch_bounds__(kThreads) scan_kernel(const RouteArgs a) {
-    __shared__ int   part[64][16];
-    __shared__ float fpart[64][16];
+    constexpr int kHeld = 4;
+    __shared__ int   part[kWaves][16];
+    __shared__ float fpart[kWaves][16];
     const int c = threadIdx.x & 15, slice = threadIdx.x >> 4, cols = a.experts + 1, hist_blocks = (cols + 15) / 16;
     const int per = (a.chunks + 63) / 64, from = min(slice * per, a.chunks), to = min(from + per, a.chunks);
     if (static_cast<int>(blockIdx.x) >= hist_blocks) {
-        const int col = (blockIdx.x - hist_blocks) * 16 + c;
-        float     s   = 0.f;
-        if (col < a.experts)
-            for (int i = from; i < to; ++i)
-                s += a.sums[static_cast<int64_t>(i) * a.experts + col];
-        fpart[slice][c] = s;
-        __syncthreads();
-        if (slice == 0 && col < a.experts) {
-            for (int i = 1; i < 64; ++i)
-                s += fpart[i][c];
-            a.sums[static_cast<int64_t>(a.chunks) * a.experts + col] = s;
+        const int col = min(static_cast<int>((blockIdx.x - hist_blocks) * 16 + c), a.experts - 1); // past the last: it again
+        float     s   = 0.f, all;
+        for (int i = from; i < to; i += kHeld) {
+            float v[kHeld];
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                v[j] = a.sums[static_cast<int64_t>(min(i + j, to - 1)) * a.experts + col];
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                s += i + j < to ? v[j] : 0.f;
         }
+        slices_before(s, fpart, &all);
+        if (slice == 0)
+            a.sums[static_cast<int64_t>(a.chunks) * a.experts + col] = all;
         return;
     }
-    const int col = blockIdx.x * 16 + c;
-    int       s   = 0;
-    if (col < cols)
-        for (int i = from; i < to; ++i)
-            s += a.hist[static_cast<int64_t>(i) * cols + col];
-    part[slice][c] = s;
-    __syncthreads();
-    if (col >= cols)
-        return;
-    int run = 0;
-    for (int i = 0; i < slice; ++i)
-        run += part[i][c];
-    for (int i = from; i < to; ++i) {
-        int      *h = a.hist + static_cast<int64_t>(i) * cols + col;
-        const int n = *h;
-        *h          = run;
-        run += n;
+    const int col = min(static_cast<int>(blockIdx.x) * 16 + c, cols - 1);
+    const bool mine = static_cast<int>(blockIdx.x) * 16 + c < cols;
+    int       v[kHeld], s = 0, all;
+    for (int i = from; i < to; i += kHeld) {
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            v[j] = a.hist[static_cast<int64_t>(min(i + j, to - 1)) * cols + col];
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            s += i + j < to ? v[j] : 0;
     }
-    if (slice == 63) {
-        a.hist[static_cast<int64_t>(a.chunks) * cols + col] = run;
+    int run = slices_before(s, part, &all);
+    if (!mine)
+        return;
+    for (int i = from; i < to; i += kHeld) {
+        if (per > kHeld)
+#pragma unroll
+            for (int j = 0; j < kHeld; ++j)
+                v[j] = a.hist[static_cast<int64_t>(min(i + j, to - 1)) * cols + col];
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+            if (i + j < to) {
+                a.hist[static_cast<int64_t>(i + j) * cols + col] = run;
+                run += v[j];
+            }
+    }
+    if (slice == 0) {
+        a.hist[static_cast<int64_t>(a.chunks) * cols + col] = all;
         if (col < a.experts)
-            a.counts[col] = run;
+            a.counts[col] = all;
     }
 }
 
@@ -652,23 +679,31 @@ template <typename T, int L, int V> __global__ void __launch_bounds__(256) route
     }
 }
 
-// f(L, V) for a number of experts.
-template <typename F> int with_lanes(int experts, F f) {
+// f(L, V) for a number of experts. Of 129 to 256 in the forward pass, 32 lanes of 8 are faster than 16 of 16 while there are few tokens for
+// each workgroup, as they take half the time between a turn's loads and its outputs (top 8: 128 tokens 12.7 -> 9.2 us, 4096
+// 17.0 -> 14.6, 16384 21.3 -> 20.3; but 33 7.4 -> 7.9, in two turns, and 32768 27.3 -> 28.1, 131072 77 -> 88).
+template <typename F> int with_lanes(int experts, bool halves, F f) {
     using std::integral_constant;
 #define GG_LANES(l, v)                                                                                                 \
     if (experts <= l * v)                                                                                              \
         return f(integral_constant<int, l>{}, integral_constant<int, v>{});
-    GG_LANES(4, 4) GG_LANES(8, 4) GG_LANES(16, 4) GG_LANES(16, 8) GG_LANES(16, 16) GG_LANES(32, 16)
+    GG_LANES(4, 4) GG_LANES(8, 4) GG_LANES(16, 4) GG_LANES(16, 8)
+    if (halves) {
+        GG_LANES(32, 8)
+    }
+    GG_LANES(16, 16) GG_LANES(32, 16)
 #undef GG_LANES
     return f(integral_constant<int, 64>{}, integral_constant<int, 16>{});
 }
+
+bool halves(int64_t tokens) { return tokens > 64 && tokens <= 16384; }
 
 // Tokens of a chunk. All of them where a workgroup takes them in two turns of its waves: one launch. Else a quarter of
 // its waves' tokens or more, so that there are about as many chunks as CUs (4096 tokens of 256 experts, top 8: 16 tokens a
 // chunk instead of 128).
 int chunk_tokens(int64_t tokens, int experts, int top_k) {
     const int most = std::min(kMaxTokens, kMaxPairs / top_k);
-    const int turn = with_lanes(experts, [](auto l, auto) { return kWaves * 64 / l.value; }); // tokens of a workgroup's waves at a time
+    const int turn = with_lanes(experts, halves(tokens), [](auto l, auto) { return kWaves * 64 / l.value; }); // tokens of a workgroup's waves at a time
     if (tokens <= std::min(most, 2 * turn))
         return most;
     const int64_t even = (tokens + 255) / 256, quarter = turn / 4;
@@ -699,7 +734,7 @@ bool vector_rows(const void *p, int64_t stride, int64_t tokens, int dtype) {
 }
 
 int run_route(const RouteArgs &a, hipStream_t s) {
-    int st = with_lanes(a.experts, [&](auto l, auto v) {
+    int st = with_lanes(a.experts, halves(a.tokens), [&](auto l, auto v) {
         constexpr int few = v.value < 9 ? v.value : 9; // of top_k + 1 <= 9 values
         constexpr int most = l.value * v.value < 32 ? l.value * v.value + 1 : 33; // top_k + 1
         return a.top_k <= 8
@@ -716,7 +751,7 @@ int run_route(const RouteArgs &a, hipStream_t s) {
 }
 
 template <typename T> int run_back(const BackArgs &a, hipStream_t s) {
-    return with_lanes(a.experts, [&](auto l, auto v) {
+    return with_lanes(a.experts, false, [&](auto l, auto v) {
         const int64_t per = 4 * (64 / l.value);
         return launch("route_backward", route_back_kernel<T, l.value, v.value>,
                       std::min((a.tokens + per - 1) / per, int64_t(1) << 20), 256, s, a);

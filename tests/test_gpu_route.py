@@ -86,6 +86,16 @@ def test_route(pkg, dtype, t, e, k):
         assert all(torch.equal(a, b) for a, b in zip(r[:8], again[:8]) if a is not None)
 
 
+# Either side of where 129 to 256 experts take other lanes; chunks beyond what the scan holds in registers at once.
+@pytest.mark.parametrize("t,e,k", [(64, 200, 6), (65, 200, 6), (300, 256, 20), (64, 256, 12), (16384, 256, 8), (16385, 130, 9), (40000, 200, 3), (70001, 16, 1),
+                                   (140000, 6, 2)])
+def test_route_sizes_that_choose(pkg, t, e, k):
+    g = _gen(t + e)
+    logits = 2 * torch.randn(t, e, device=DEV, generator=g)
+    mask = torch.rand(t, device=DEV, generator=g) < 0.9
+    _check(pkg.route(logits, k, mask, True, True), _reference(logits, k, mask, True), True)
+
+
 @pytest.mark.parametrize("t,e,k", [(1, 8, 2), (7, 33, 4), (200, 64, 8), (1500, 256, 8), (140, 1024, 12)])
 def test_mask_hides_garbage(pkg, t, e, k):
     """Masked tokens hold NaN and infinities, masked experts -infinity; some tokens have no expert left, one
