@@ -279,8 +279,13 @@ __device__ __forceinline__ void scale_sums(f32x4 (&acc)[MT][NT], f32x4 (&sum)[MT
             asm volatile("" : "+v"(acc[i][j]));
 }
 
-// 16 rows of a group at a time. Grid: workgroup (piece of 16 rows, block of 16 NT columns), G k of one scale. The W waves share out the 128-column tiles; each loads weights, scales and x one tile ahead. x comes
-// through a buffer resource that ends at the last row, so rows past it read as zeros and cost no traffic.
+// Grid: workgroup (piece of 16 rows, block of 16 NT columns), G k of one scale. The W waves share out the 128-column tiles;
+// each loads weights, scales and x one tile ahead, into two sets of registers in turn. x comes through a buffer resource
+// that ends at the last row, so rows past it read as zeros and cost no traffic. Three workgroups a CU: 168 registers, which
+// the compiler passes into accumulation registers, with moves, unless it is told. 16 groups of 8 rows of 4096 x 4096 (k of
+// a scale 128): 32.2 us, 4.3 TB/s of packed weights and scales; 32 of 8 rows of 2880 x 2880 (32, zero points) 42.7, 3.7 TB/s.
+// Long k comes nearer to the memory's 5.3 TB/s (32 of 8 rows, 2880 x 5632: 55.0 us, 4.9): a call spends 6 to 8 us on the
+// launch, the search for its rows, the first loads and the sum over the waves.
 template <typename T, int NT, int W, int G, bool ZEROS>
 __global__ void __launch_bounds__(W * 64, NT == 4 ? 3 : 2) w4_kernel(const W4Args a) {
     using X = W4Type<T>;
@@ -387,10 +392,13 @@ __global__ void __launch_bounds__(W * 64, NT == 4 ? 3 : 2) w4_kernel(const W4Arg
     }
 }
 
-// More rows: pieces of 16 MT, each of the four waves with NT tiles of its own, x's rows shared through two LDS buffers of one 128-column tile. A row's 16-byte pieces lie at piece ^ row % 16, so the 16 rows that a matrix
-// operand takes at once are in different banks.
+// More rows: pieces of 16 MT, each of the four waves with NT tiles of its own, x's rows shared through two LDS buffers of
+// one 128-column tile. A row's 16-byte pieces lie at piece ^ row % 16, so the 16 rows that a matrix operand takes at once
+// are in different banks. Four workgroups a CU (128 registers) against three: 64 groups of 16 rows of 2048 x 1408 28.9 ->
+// 25.1 us, 16 of 48 rows of 4096 x 4096 65.5 -> 57.8, 32 of 12 rows of 2880 x 2880 50.0 -> 49.0; a third set of weights in
+// flight takes that back. What bounds it: matrix and vector instructions, which take about as long, hardly overlap.
 template <typename T, int MT, int NT, int G, bool ZEROS>
-__global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
+__global__ void __launch_bounds__(256, 4) w4_rows_kernel(const W4Args a) {
     using X = W4Type<T>;
     constexpr int kSteps  = G / 32;
     constexpr int kScales = 128 / G;
@@ -410,11 +418,9 @@ __global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
             return;
         const int tile0 = (nb * 4 + wave) * NT;
         const Weights<NT, ZEROS> w(a, f.group, tile0);
-        TileWords<NT>  ahead[2];
+        TileWords<NT>  words[2];
         TileScales<NT> next_scales;
-        load_words(ahead[0], w, 0, lane);
-        if (1 < a.k_tiles)
-            load_words(ahead[1], w, 1, lane);
+        load_words(words[0], w, 0, lane);
         load_scales<NT, ZEROS, kScales>(next_scales, w, 0, lane);
         const int64_t row0 = first_row(a, f, lane);
         if (row0 < 0)
@@ -445,20 +451,19 @@ __global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
         load_x(0);
         store_x(0);
         __syncthreads();
-        for (int c = 0; c < a.k_tiles; ++c) {
-            const TileWords<NT> now = ahead[0];
+        // one tile; PHASE as above
+        auto tile = [&](auto phase, int c) {
+            constexpr int kMine = decltype(phase)::value, kNext = 1 - kMine;
             float scale[NT][kScales], point[NT][kScales];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
                 spread_scales<T, kScales, ZEROS>(next_scales.s[j], next_scales.z[j], scale[j], point[j]);
-            ahead[0] = ahead[1];
             const bool more = c + 1 < a.k_tiles;
             if (more) {
                 load_x(c + 1);
                 load_scales<NT, ZEROS, kScales>(next_scales, w, c + 1, lane);
+                load_words(words[kNext], w, c + 1, lane);
             }
-            if (c + 2 < a.k_tiles)
-                load_words(ahead[1], w, c + 2, lane);
             const unsigned char *xt = lds + (c & 1) * kTile;
             auto read_x = [&](u32x4(&x)[MT], int step) {
 #pragma unroll
@@ -487,7 +492,7 @@ __global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
                             base[i] = X::mma(x[s2 & 1][i], minus, first && s2 == step ? zero : base[i]);
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const u32x4 wf = expand<T>(now.w[j][step], bits);
+                    const u32x4 wf = expand<T>(words[kMine].w[j][step], bits);
 #pragma unroll
                     for (int i = 0; i < MT; ++i)
                         sum[i][j] = X::mma(x[step & 1][i], wf,
@@ -503,6 +508,11 @@ __global__ void __launch_bounds__(256, 2) w4_rows_kernel(const W4Args a) {
             if (more)
                 store_x(c + 1);
             __syncthreads();
+        };
+        for (int c = 0; c < a.k_tiles; c += 2) {
+            tile(std::integral_constant<int, 0>{}, c);
+            if (c + 1 < a.k_tiles)
+                tile(std::integral_constant<int, 1>{}, c + 1);
         }
         // outputs through LDS, a wave's own part: rows of 16 NT columns, stored 16 bytes (8 columns) a lane
         unsigned char *ot = lds + wave * kOut;
@@ -552,19 +562,20 @@ template <typename T, int MT, int NT> int launch_rows(const W4Args &a, int group
 // The instance by the rows that a group has on average and the workgroups there are. Measured (us; few-row instances of
 // 64, 32 and 16 columns a workgroup, then the many-row one, of 32 rows and 128 columns):
 //   rows per group (ragged; 32 groups of 2880 x 2880, k of a scale 32, zero points / 16 of 4096 x 4096, 128):
-//     8: 41.1, 53.9, 82.9, 45.1 / 32.8, 41.6, 57.9, 33.8          12: 49.8, 63.2, 100.9, 44.8 / 36.8, 48.7, 71.5, 34.4
-//     24: 70.4, 94.3, 158.2, 62.2 / 49.4, 74.5, 118.7, 43.0       48: 110.8, 157.7, 271.5, 88.8 / 80.9, 131.8, 222.8, 62.5
-//     32 rows in every group of the first: 72.5, 103.6, 180.8, 49.9
+//     8: 44.6, 54.6, 82.4, 47.4 / 32.5, 42.0, 57.4, 40.5          12: 50.1, 63.2, 100.9, 49.3 / 36.8, 48.7, 70.7, 38.0
+//     16: 54.5, 70.8, 114.9, 52.8 / 40.3, 56.1, 84.6, 41.6        20: 66.0, 84.0, 138.2, 58.9 / 49.0, 68.7, 104.7, 47.6
+//     24: 71.8, 95.5, 157.6, 65.2 / 52.7, 74.3, 118.0, 48.3       48: 120.1, 162.1, 269.7, 98.5 / 87.3, 133.5, 221.8, 63.1
+//     16 rows in every group of the first: 45.0, 60.3, 100.5, 50.0; 24: 71.0, 94.2, 157.3, 51.0
 //   Many-row instances of 16, 48 and 64 rows, or of 64, 192 and 256 columns, gain 3 to 17 % where their sizes fit and
 //   lose 5 to 50 % elsewhere.
-//   workgroups of 64 columns (one row): 8 of 512 x 7168: 11.8, 7.3, 6.1; 32 of 512 x 2048: 6.3, 5.0, 4.7; 128 of
-//     4096 x 1024: 5.2, 4.7, 5.5; 224 of 14336 x 4096: 10.7, 9.6, 12.0; 448 of 7168 x 2048: 9.6, 12.0, 14.1; 4 groups of 20
-//     rows, 2048 x 4096 (288): 11.8, 13.9, 18.8
-//   the many-row one does not split k: with fewer workgroups than CUs it loses (those 4 groups: 24.0).
+//   workgroups of 64 columns (one row): 8 of 512 x 7168: 11.9, 7.3, 6.1; 32 of 512 x 2048: 6.3, 5.0, 4.6; 128 of
+//     4096 x 1024: 5.2, 4.7, 5.5; 224 of 14336 x 4096: 10.8, 9.5, 12.0; 448 of 7168 x 2048: 9.7, 11.9, 13.8; 4 groups of 20
+//     rows, 2048 x 4096 (288): 11.6, 13.7, 18.8
+//   the many-row one does not split k: with fewer workgroups than CUs it loses (those 4 groups: 25.7).
 template <typename T> int run_w4(const W4Args &a, int group, hipStream_t s) {
     const int64_t per  = a.total_m / std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m));
     const int64_t wide = (a.n_tiles + 7) / 8 * pieces_of(a, 32), narrow = (a.n_tiles + 3) / 4 * pieces_of(a, 16);
-    return per >= 12 && wide >= 256 ? launch_rows<T, 2, 2>(a, group, s)
+    return per > 16 && wide >= 256 ? launch_rows<T, 2, 2>(a, group, s)
            : narrow >= 256          ? launch_few<T, 4, 4>(a, group, s)
            : narrow >= 64           ? launch_few<T, 2, 8>(a, group, s)
                                     : launch_few<T, 1, 8>(a, group, s);
