@@ -13,7 +13,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import GG_OK, DType, GGError, load_library
+from . import GG_OK, DType, GGError, _device_sizes, load_library
 
 _T16 = {torch.bfloat16: int(DType.BF16), torch.float16: int(DType.FP16)}
 _T8 = {torch.float8_e4m3fn: int(DType.FP8_E4M3), torch.float8_e5m2: int(DType.FP8_E5M2)}
@@ -446,31 +446,31 @@ def grouped_gemm_w4(x, w: W4Weights, group_m, out=None, stream: Optional[int] = 
     """out [sum(M), N] = x[rows of g] @ w[g]^T for 4-bit weights (gg_gemm_w4), x bf16 or fp16 [sum(M), K] of
     the scales' type. group_m as in grouped_gemm: a host sequence of row counts, or a device int64 tensor [B]
     that is never read on the host (with optional device offsets); a device group that does not lie inside x
-    gets no work. For groups of few rows: every 16 to 64 rows of a group read its weights once."""
-    from . import _device_sizes
-
+    gets no work. For groups of few rows: every 16 or 32 rows of a group read its weights once."""
     dt = _T16.get(x.dtype)
     if dt is None:
         raise TypeError("x must be bfloat16 or float16")
     dev = x.device
-    b, nt = w.packed.shape[0], (w.n + 15) // 16
-    if w.scales.dtype != x.dtype:
+    packed, scales, zeros, n, k, group = w
+    b, nt = packed.shape[0], (n + 15) // 16
+    if scales.dtype != x.dtype:
         raise TypeError("the scales must be of x's type")
-    _flat("w.packed", w.packed, torch.uint8, (b, nt, (w.k + 127) // 128, 64, 16), dev)
-    _flat("w.scales", w.scales, x.dtype, (b, nt, w.k // w.group, 16), dev)
-    if w.zeros is not None:
-        _flat("w.zeros", w.zeros, torch.uint8, (b, nt, w.k // w.group, 16), dev)
-    if x.dim() != 2 or x.shape[1] != w.k or not x.is_cuda or not x.is_contiguous():
+    _flat("w.packed", packed, torch.uint8, (b, nt, (k + 127) // 128, 64, 16), dev)
+    shape = (b, nt, k // group, 16)
+    _flat("w.scales", scales, x.dtype, shape, dev)
+    if zeros is not None:
+        _flat("w.zeros", zeros, torch.uint8, shape, dev)
+    if x.dim() != 2 or not x.is_cuda or x.shape[1] != k or not x.is_contiguous():
         raise ValueError("x must be a contiguous device matrix with K columns")
+    m = x.shape[0]
     if not _device_sizes(group_m, group_offs, b):
-        if len(group_m) != b or any(m < 0 for m in group_m) or sum(group_m) != x.shape[0]:
+        if len(group_m) != b or any(r < 0 for r in group_m) or sum(group_m) != m:
             raise ValueError("shape mismatch between x, w and group_m")
         group_m = torch.tensor(list(group_m), dtype=torch.int64, device=dev)
     elif group_m.device != dev or (group_offs is not None and group_offs.device != dev):
         raise ValueError("group sizes must be on x's device")
-    o = _out(out, x.dtype, (x.shape[0], w.n), dev)
-    _call(_lib.gg_gemm_w4, dev, stream, (dt, b, x.shape[0], w.n, w.k, w.group, group_m.data_ptr(), _ptr(group_offs),
-                                         x.data_ptr(), w.packed.data_ptr(), w.scales.data_ptr(), _ptr(w.zeros),
-                                         o.data_ptr()),
-          (x, w.packed, w.scales, w.zeros, group_m, group_offs, o))
+    o = _out(out, x.dtype, (m, n), dev)
+    _call(_lib.gg_gemm_w4, dev, stream, (dt, b, m, n, k, group, group_m.data_ptr(), _ptr(group_offs), x.data_ptr(),
+                                         packed.data_ptr(), scales.data_ptr(), _ptr(zeros), o.data_ptr()),
+          (x, packed, scales, zeros, group_m, group_offs, o))
     return o
