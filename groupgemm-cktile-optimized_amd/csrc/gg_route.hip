@@ -12,6 +12,12 @@
 // ballot per bit of its number. A chunk's histogram goes to memory, a second launch turns the histograms
 // into running sums, a third adds each pair's start. One chunk needs only the first launch. The
 // probabilities' sums for the loss follow the same way, chunk by chunk in a fixed order.
+//
+// What bounds it: not the bytes (32768 tokens of 256 experts, float32: 7 us at 5.3 TB/s) but vector instructions and the
+// steps that wait for each other. Those tokens, top 8 with the loss: 27 us, 20 for the first launch (about 10 of them the
+// issue of its 6.1 million vector instructions, the rest loads, barriers and ranks with one workgroup a CU), 4 for the
+// second, 3.5 for the third. 33 tokens, one launch: 7.4; one token 5.5. Asking for the next turn's logits ahead
+// (29.6 us) loses: the registers are full. Backward 16640 tokens of 32 experts 3.7.
 #include <algorithm>
 
 #include "gg_layer.h"

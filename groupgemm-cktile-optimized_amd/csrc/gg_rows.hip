@@ -3,7 +3,8 @@
 //
 // Every kernel moves rows of hidden values in 16-byte pieces between a token's row and the top_k rows
 // that its slots have in expert order. Bound by HBM: the tokens' rows are read or written once, the
-// experts' rows once.
+// experts' rows once. Measured, 4096 tokens of 7168 to 8 experts each: dispatch of fp8 46 us (5.7 TB/s), combine of bf16 108
+// (4.9); 4160 tokens of 2880 to 4: combine_backward 34 (6.3 TB/s: part of y comes from the Infinity Cache).
 #include <algorithm>
 
 #include "gg_layer.h"
