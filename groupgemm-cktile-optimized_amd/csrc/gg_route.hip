@@ -27,7 +27,7 @@ namespace layer {
 namespace {
 
 constexpr int kThreads  = 1024, kWaves = kThreads / 64;
-constexpr int kScanless = 32; // chunks
+constexpr int kScanless = 32; // chunks whose histograms the last launch adds up itself (of 256: 30 us with the loss, scanned 26)
 constexpr int kMaxPairs = 1024, kMaxTokens = 128, kSegments = kMaxPairs / 64; // of a chunk
 
 struct RouteArgs {
