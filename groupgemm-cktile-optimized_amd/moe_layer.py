@@ -446,7 +446,8 @@ def grouped_gemm_w4(x, w: W4Weights, group_m, out=None, stream: Optional[int] = 
     """out [sum(M), N] = x[rows of g] @ w[g]^T for 4-bit weights (gg_gemm_w4), x bf16 or fp16 [sum(M), K] of
     the scales' type. group_m as in grouped_gemm: a host sequence of row counts, or a device int64 tensor [B]
     that is never read on the host (with optional device offsets); a device group that does not lie inside x
-    gets no work. For groups of few rows: every 16 or 32 rows of a group read its weights once."""
+    gets no work, and rows of no group are not written. For groups of few rows: every 16 or 32 rows of a group read
+    its weights once."""
     dt = _T16.get(x.dtype)
     if dt is None:
         raise TypeError("x must be bfloat16 or float16")

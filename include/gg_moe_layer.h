@@ -140,7 +140,7 @@ int gg_combine_backward(int dtype, int64_t tokens, int top_k, int64_t hidden, in
  * zero, in 0..15) for each `group` consecutive k; zero = 8 where zeros is NULL. x [total_m, k], out
  * [total_m, n], scales of dtype (bf16 or fp16), zeros bytes. For groups of few rows: decode, short prompts.
  * group_lens / group_offs: device sizes as in gg_prepare_device_lens_op; a group whose rows are not
- * inside [0, total_m) gets no work (and is not reported). The products are of 16 + q, less (16 + zero) times the sum of x,
+ * inside [0, total_m) gets no work (and is not reported); rows of out that belong to no group are not written. The products are of 16 + q, less (16 + zero) times the sum of x,
  * exact but for the float32 sums: an infinity in x makes its row's outputs NaN.
  *
  * Storage: n in tiles of 16 and k in tiles of 128, padded with zeros:
