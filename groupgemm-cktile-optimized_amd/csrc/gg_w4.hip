@@ -571,11 +571,13 @@ template <typename T, int MT, int NT> int launch_rows(const W4Args &a, int group
 //   workgroups of 64 columns (one row): 8 of 512 x 7168: 11.9, 7.3, 6.1; 32 of 512 x 2048: 6.3, 5.0, 4.6; 128 of
 //     4096 x 1024: 5.2, 4.7, 5.5; 224 of 14336 x 4096: 10.8, 9.5, 12.0; 448 of 7168 x 2048: 9.7, 11.9, 13.8; 4 groups of 20
 //     rows, 2048 x 4096 (288): 11.6, 13.7, 18.8
-//   the many-row one does not split k: with fewer workgroups than CUs it loses (those 4 groups: 25.7).
+//   the many-row one does not split k: with few workgroups it loses (64-column few-row and many-row instance; workgroups of the
+//     latter): 160 of 24 rows, 4096 x 4096 17.6, 26.8; 320 27.5, 30.8 (k 9600: 63.7, 75.8; 1024: 12.2, 11.2); 448 of 14336 x
+//     4096 41.3, 34.6; 510 of 1280 x 5120 60.0, 50.5. Half a piece for each group and the rows / 32: about as many as there are.
 template <typename T> int run_w4(const W4Args &a, int group, hipStream_t s) {
-    const int64_t per  = a.total_m / std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m));
-    const int64_t wide = (a.n_tiles + 7) / 8 * pieces_of(a, 32), narrow = (a.n_tiles + 3) / 4 * pieces_of(a, 16);
-    return per > 16 && wide >= 256 ? launch_rows<T, 2, 2>(a, group, s)
+    const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m)), per = a.total_m / slots;
+    const int64_t wide = (a.n_tiles + 7) / 8 * (slots + a.total_m / 16) / 2, narrow = (a.n_tiles + 3) / 4 * pieces_of(a, 16);
+    return per > 16 && wide >= 384 ? launch_rows<T, 2, 2>(a, group, s)
            : narrow >= 256          ? launch_few<T, 4, 4>(a, group, s)
            : narrow >= 64           ? launch_few<T, 2, 8>(a, group, s)
                                     : launch_few<T, 1, 8>(a, group, s);
