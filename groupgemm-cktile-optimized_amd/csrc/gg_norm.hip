@@ -2,7 +2,7 @@
 // gg_rms_norm_backward in include/gg_moe_layer.h).
 //
 // Forward: h = round(x + r), rstd = (mean h^2 + eps)^-1/2, y = h rstd w. A row stays in the registers
-// of the waves that work on it (one wave up to 1024 values, four up to 16384, sixteen up to 32768), so
+// of the waves that work on it (one wave up to 1024 values, four up to 16384, of few rows up to 2048, else sixteen), so
 // x and r are read once and h and y written once: bound by HBM. The tensor scale needs the largest |y|
 // of all rows before the first value is rounded: a first pass writes h, rstd and one maximum per
 // workgroup, a second reads h again and rounds.
@@ -11,8 +11,8 @@
 // passes agree whatever the scale.
 //
 // Measured: 32768 rows of 7168, bf16 with residual to fp8 with a tensor scale, 377 us: 248 for the first pass (x and r
-// read, h written: 5.7 TB/s) and 130 for the second (h read, y written: 5.4); 5 rows to bf16 5.0, the latency of a launch,
-// a row's loads and two barriers. Backward 16640 x 2880 with a gradient past the norm: 75 us, 5.1 TB/s (69 row by row, 6 for
+// read, h written: 5.7 TB/s) and 130 for the second (h read, y written: 5.4); 5 rows to bf16 3.9, the latency of a launch,
+// a row's loads and a barrier. Backward 16640 x 2880 with a gradient past the norm: 75 us, 5.1 TB/s (69 row by row, 6 for
 // the weight's gradient).
 #include "gg_layer.h"
 
@@ -227,23 +227,26 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
 }
 
 // The tensor scale's second pass: the largest of the first pass's maxima, then y from h and rstd.
-template <typename T> __global__ void __launch_bounds__(256) quantize_kernel(const NormArgs a) {
-    __shared__ unsigned tops[4];
+template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) quantize_kernel(const NormArgs a) {
+    __shared__ unsigned tops[THREADS / 64];
     unsigned            top = 0;
-    for (int i = threadIdx.x; i < a.n_parts; i += 256)
+    for (int i = threadIdx.x; i < a.n_parts; i += THREADS)
         top = max(top, reinterpret_cast<const unsigned *>(a.parts)[i]);
     top = wave_max(top);
     if ((threadIdx.x & 63) == 0)
         tops[threadIdx.x >> 6] = top;
     __syncthreads();
-    const float s   = scale_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])), a.e5m2);
+#pragma unroll
+    for (int i = 0; i < THREADS / 64; ++i)
+        top = max(top, tops[i]);
+    const float s   = scale_of(top, a.e5m2);
     const float inv = 1.f / s;
     if (blockIdx.x == 0 && threadIdx.x == 0)
         a.scale[0] = s;
     // from the last row backwards: the rows written last are still in the Infinity Cache
     for (int64_t row = a.rows - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
         const float rstd = a.rstd[row];
-        for (int i = threadIdx.x * 8; i < a.hidden; i += 2048) {
+        for (int i = threadIdx.x * 8; i < a.hidden; i += THREADS * 8) {
             float v[8], w[8];
             unpack8<T>(load_once(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i), v);
             load_w<T>(a.weight, a.w32, i, w);
@@ -267,7 +270,7 @@ struct BackArgs {
 
 // grad_x row by row; grad_weight's partial sums stay in registers over the rows of a workgroup and are
 // written once.
-template <typename T, int WPR, int U>
+template <typename T, int WPR, int U, bool SUMS>
 __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const BackArgs a) {
     __shared__ RowReduce<WPR> m;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -306,7 +309,8 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const Bac
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     dot      = fmaf(g[j] * w[j], h[j], dot);
-                    dw[u][j] = fmaf(g[j] * h[j], rstd, dw[u][j]);
+                    if constexpr (SUMS)
+                        dw[u][j] = fmaf(g[j] * h[j], rstd, dw[u][j]);
                 }
             }
         }
@@ -333,6 +337,8 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const Bac
             }
         }
     }
+    if constexpr (!SUMS)
+        return;
     // a workgroup whose waves had rows of their own adds them up first, in their order
     if constexpr (WPR == 1) {
         __shared__ f32x4 mine[3][U][2][64];
@@ -367,6 +373,48 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const Bac
     }
 }
 
+// grad_weight from g and h themselves: 64 columns (a line of 128 bytes a row) by 128 slices of the rows a workgroup.
+template <typename T> __global__ void __launch_bounds__(1024) weight_strip_kernel(const BackArgs a, void *out) {
+    __shared__ f32x4 sums[2][128][8];
+    const int c8 = threadIdx.x & 7, slice = threadIdx.x >> 3, col = blockIdx.x * 64 + c8 * 8; // hidden % 8 == 0
+    f32x4     s[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+    if (col < a.hidden) {
+        const uint16_t *g = static_cast<const uint16_t *>(a.g) + col, *h = static_cast<const uint16_t *>(a.h) + col;
+#pragma unroll 4
+        for (int64_t row = slice; row < a.rows; row += 128) {
+            float gv[8], hv[8];
+            unpack8<T>(*reinterpret_cast<const u32x4 *>(g + row * a.g_stride), gv);
+            unpack8<T>(*reinterpret_cast<const u32x4 *>(h + row * a.h_stride), hv);
+            const float rstd = a.rstd[row];
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                s[j / 4][j % 4] = fmaf(gv[j] * hv[j], rstd, s[j / 4][j % 4]);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+        sums[q][slice][c8] = s[q];
+    __syncthreads();
+#pragma unroll
+    for (int half = 64; half > 0; half >>= 1) {
+        if (slice < half)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                sums[q][slice][c8] = s[q] += sums[q][slice + half][c8];
+        __syncthreads();
+    }
+    if (slice == 0 && col < a.hidden) {
+        if (a.w32) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+                reinterpret_cast<f32x4 *>(static_cast<float *>(out) + col)[q] = s[q];
+        } else {
+            const float v[8] = {s[0][0], s[0][1], s[0][2], s[0][3], s[1][0], s[1][1], s[1][2], s[1][3]};
+            *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(out) + col) = pack8<T>(v);
+        }
+    }
+}
+
 // grad_weight: the sum of the partial sums of each column, in a fixed order; 32 columns by 128 slices of the parts a
 // workgroup.
 template <typename T>
@@ -394,31 +442,42 @@ __global__ void __launch_bounds__(1024) weight_sum_kernel(const float *parts, in
     }
 }
 
-int waves_per_row(int64_t hidden) { return hidden <= 1024 ? 1 : hidden <= 16384 ? 4 : 16; }
+// Few rows: a row's latency counts, and not how many are in flight. Then (WIDE) sixteen waves take a row of more than 2048
+// values, and grad_weight is summed from g and h again, which are in the caches, instead of from partial sums, which would be
+// as many bytes as the rows. us, sixteen waves and four: norm of 5 rows of 7168 3.9, 5.1, of 256 5.5, 7.3, 512 8.4, 10.8, 1024
+// 14.5, 14.8; of 512 rows of 4096 5.7, 5.6, 1024 10.8, 9.5; 256 of 14336 8.5, 14.0. Backward, with the sums and without:
+// 64 of 7168 7.1, 9.1, 481 of 13456 22.2, 34.3, 512 of 7168 16.6, 18.1, 512 of 4096 13.9, 12.4, 1024 of 8192 27.6, 27.4.
+bool few(int64_t rows, int64_t hidden) { return hidden > 1024 && rows <= (hidden > 5120 ? 512 : 256); }
 
-int64_t row_blocks(int64_t rows, int64_t hidden) {
-    const int per = rows_per_block(waves_per_row(hidden));
-    return (rows + per - 1) / per;
+template <bool WIDE> int waves_per_row(int64_t hidden) {
+    return hidden <= 1024 ? 1 : hidden <= (WIDE ? 2048 : 16384) ? 4 : 16;
 }
 
+int64_t row_blocks(int64_t rows, int64_t hidden) { return hidden <= 1024 ? (rows + 3) / 4 : rows; }
+
 // f(WPR, U) of the instance for `hidden` values a row: U pieces of 8 per lane.
-template <typename F> int with_shape(int64_t hidden, F f) {
+template <bool WIDE, typename F> int with_shape(int64_t hidden, F f) {
     using std::integral_constant;
-    const int wpr = waves_per_row(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+    const int wpr = waves_per_row<WIDE>(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
 #define GG_SHAPE(W, N)                                                                                                 \
     if (wpr == W && u <= N)                                                                                            \
         return f(integral_constant<int, W>{}, integral_constant<int, N>{});
-    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(4, 4) GG_SHAPE(4, 6) GG_SHAPE(4, 8)
+    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1)
+    if constexpr (WIDE) {
+        GG_SHAPE(16, 1) GG_SHAPE(16, 2)
+    } else {
+        GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(4, 4) GG_SHAPE(4, 6) GG_SHAPE(4, 8)
+    }
 #undef GG_SHAPE
     return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
 }
 
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;
 
-template <typename T> int run_norm(const NormArgs &a, hipStream_t s) {
+template <typename T, bool WIDE> int run_norm(const NormArgs &a, hipStream_t s) {
     const int64_t blocks = row_blocks(a.rows, a.hidden);
     if (a.mode != GG_NORM_SCALE_TENSOR)
-        return with_shape(a.hidden, [&](auto wpr, auto u) {
+        return with_shape<WIDE>(a.hidden, [&](auto wpr, auto u) {
             return launch("rms_norm", norm_kernel<T, wpr.value, u.value, false>, std::min(blocks, kMaxBlocks),
                           block_threads(wpr.value), s, a);
         });
@@ -429,29 +488,37 @@ template <typename T> int run_norm(const NormArgs &a, hipStream_t s) {
         b.h        = const_cast<void *>(b.x);
         b.h_stride = b.x_stride;
     }
-    const int st = with_shape(a.hidden, [&](auto wpr, auto u) {
+    const int st = with_shape<WIDE>(a.hidden, [&](auto wpr, auto u) {
         constexpr auto   kernel = norm_kernel<T, wpr.value, u.value, true>;
         static const int fit    = resident_blocks(kernel, block_threads(wpr.value));
         b.n_parts               = static_cast<int>(std::min<int64_t>(blocks, std::min(fit, kMaxParts)));
         return launch("rms_norm", kernel, b.n_parts, block_threads(wpr.value), s, b);
     });
-    return st ? st : launch("rms_norm", quantize_kernel<T>, std::min<int64_t>(b.rows, 8192), 256, s, b);
+    constexpr int kThreads = WIDE ? 1024 : 256;
+    return st ? st : launch("rms_norm", quantize_kernel<T, kThreads>, std::min<int64_t>(b.rows, 8192), kThreads, s, b);
 }
 
 // Workgroups of the backward pass: at most those that the GPU holds at once (by the instances' registers, 72 to 224),
 // fewer where each would have less than four rows and their partial sums would cost more than they save. us at 1, 2
-// and 4 rows each: 64 rows of 7168 8.9, 11.3, 16.2; 512 19.9, 18.6, 21.6; 2048 46.8, 37.9, 34.2. At once against 1024:
+// and 4 rows each, of 7168: 512 rows 19.9, 18.6, 21.6; 2048 46.8, 37.9, 34.2. At once against 1024:
 // 16640 rows of 2880 73.7 (1536) and 77.6, 4096 of 14336 108.5 (512) and 118.6.
 int64_t back_blocks(int64_t rows, int64_t hidden) {
-    const int     wpr = waves_per_row(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+    const int     wpr = waves_per_row<false>(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
     const int64_t fit = wpr == 16 ? 256 : u == 1 ? 1792 : u > 4 ? 512 : u == 2 && wpr == 4 ? 1536 : 1024;
     const int64_t b   = row_blocks(rows, hidden);
     return std::min(fit, std::max(b / 4, b <= 256 ? b : std::min<int64_t>(b / 2, 512)));
 }
 
 template <typename T> int run_back(const BackArgs &a, void *grad_weight, hipStream_t s) {
-    const int st = with_shape(a.hidden, [&](auto wpr, auto u) {
-        return launch("rms_norm_backward", norm_back_kernel<T, wpr.value, u.value>, back_blocks(a.rows, a.hidden),
+    if (few(a.rows, a.hidden)) { // (grad_weight first: grad_x may take the place of an input)
+        const int st = launch("rms_norm_backward", weight_strip_kernel<T>, (a.hidden + 63) / 64, 1024, s, a, grad_weight);
+        return st ? st : with_shape<true>(a.hidden, [&](auto wpr, auto u) {
+            return launch("rms_norm_backward", norm_back_kernel<T, wpr.value, u.value, false>, row_blocks(a.rows, a.hidden),
+                          block_threads(wpr.value), s, a);
+        });
+    }
+    const int st = with_shape<false>(a.hidden, [&](auto wpr, auto u) {
+        return launch("rms_norm_backward", norm_back_kernel<T, wpr.value, u.value, true>, back_blocks(a.rows, a.hidden),
                       block_threads(wpr.value), s, a);
     });
     return st ? st : launch("rms_norm_backward", weight_sum_kernel<T>, (a.hidden + 31) / 32, 1024, s, a.parts,
@@ -540,14 +607,17 @@ int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int6
     a.w32      = weight_dtype == GG_DTYPE_FP32;
     a.e5m2     = out_dtype == GG_DTYPE_FP8_E5M2;
     if (rows == 0) { // no maximum: the scale alone
-        return launch("rms_norm", quantize_kernel<BF16>, 1, 256, static_cast<hipStream_t>(stream), a);
+        return launch("rms_norm", quantize_kernel<BF16, 256>, 1, 256, static_cast<hipStream_t>(stream), a);
     }
-    return dtype == GG_DTYPE_BF16 ? run_norm<BF16>(a, static_cast<hipStream_t>(stream))
-                                  : run_norm<F16>(a, static_cast<hipStream_t>(stream));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    const bool        wide = few(rows, hidden);
+    if (dtype == GG_DTYPE_BF16)
+        return wide ? run_norm<BF16, true>(a, st) : run_norm<BF16, false>(a, st);
+    return wide ? run_norm<F16, true>(a, st) : run_norm<F16, false>(a, st);
 }
 
 size_t gg_rms_norm_backward_workspace(int64_t rows, int64_t hidden) {
-    if (rows < 1 || hidden < 1 || hidden > 32768)
+    if (rows < 1 || hidden < 1 || hidden > 32768 || few(rows, hidden))
         return 0;
     return static_cast<size_t>(back_blocks(rows, hidden)) * static_cast<size_t>(hidden) * 4;
 }
@@ -570,7 +640,8 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
             return st;
     if (!aligned(weight, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 16))
         return fail(GG_ERR_UNSUPPORTED, "weight, grad_x and grad_weight must be 16-byte aligned");
-    if (workspace_bytes < gg_rms_norm_backward_workspace(rows, hidden) || (rows > 0 && (workspace == nullptr || !aligned(workspace, 16))))
+    const size_t need = gg_rms_norm_backward_workspace(rows, hidden);
+    if (workspace_bytes < need || (need > 0 && (workspace == nullptr || !aligned(workspace, 16))))
         return fail(GG_ERR_WORKSPACE, "workspace must be 16-byte aligned and of gg_rms_norm_backward_workspace(rows, hidden) bytes");
     BackArgs a{};
     a.g         = grad_y;

@@ -182,11 +182,11 @@ def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Op
     gx = _new_like(h) if out is None else _out(out, dtype, (m, n), dev)
     gw = torch.empty_like(weight)
     need = _lib.gg_rms_norm_backward_workspace(m, n)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     _call(_lib.gg_rms_norm_backward, dev, stream, (dt, dt if wd == dtype else _FP32, m, n, grad_y.data_ptr(), gs,
                                                    h.data_ptr(), hs,
                                                    weight.data_ptr(), rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(),
-                                                   gw.data_ptr(), ws.data_ptr(), need),
+                                                   gw.data_ptr(), _ptr(ws), need),
           (grad_y, h, weight, rstd, grad_h, gx, gw, ws))
     return gx, gw
 

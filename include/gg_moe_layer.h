@@ -60,8 +60,10 @@ int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int6
  *   grad_x = grad_h + rstd * (weight * grad_y) - h * rstd^3 * mean(weight * grad_y * h)
  *   grad_weight = sum over rows of grad_y * h * rstd
  * grad_x [rows, hidden] contiguous is the gradient of x and of residual alike; grad_h (the gradient
- * that reaches h past the norm) may be NULL. grad_weight [hidden] is of weight_dtype.
- * workspace: gg_rms_norm_backward_workspace(rows, hidden) bytes, 16-byte aligned. Rules as above.
+ * that reaches h past the norm) may be NULL. grad_x may take the place of a contiguous grad_y, h or grad_h.
+ * grad_weight [hidden] is of weight_dtype.
+ * workspace: gg_rms_norm_backward_workspace(rows, hidden) bytes (0 for few rows: then it may be NULL), 16-byte aligned.
+ * Rules as above.
  */
 size_t gg_rms_norm_backward_workspace(int64_t rows, int64_t hidden);
 int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidden, const void *grad_y,
@@ -140,8 +142,9 @@ int gg_combine_backward(int dtype, int64_t tokens, int top_k, int64_t hidden, in
  * zero, in 0..15) for each `group` consecutive k; zero = 8 where zeros is NULL. x [total_m, k], out
  * [total_m, n], scales of dtype (bf16 or fp16), zeros bytes. For groups of few rows: decode, short prompts.
  * group_lens / group_offs: device sizes as in gg_prepare_device_lens_op; a group whose rows are not
- * inside [0, total_m) gets no work (and is not reported); rows of out that belong to no group are not written. The products are of 16 + q, less (16 + zero) times the sum of x,
- * exact but for the float32 sums: an infinity in x makes its row's outputs NaN.
+ * inside [0, total_m) gets no work (and is not reported); rows of out that belong to no group are not
+ * written. The products are of 16 + q, less (16 + zero) times the sum of x, exact but for the float32 sums:
+ * an infinity in x, or a value past 10^36, makes its row's outputs NaN or infinite.
  *
  * Storage: n in tiles of 16 and k in tiles of 128, padded with zeros:
  *   packed [group_num][ceil(n / 16)][ceil(k / 128)][64][16] bytes: piece 16 a + r of a tile is row r,

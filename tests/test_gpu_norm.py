@@ -172,6 +172,36 @@ def test_backward(pkg, dtype, m, n, grad_h):
     assert torch.equal(gx, again[0]) and torch.equal(gw, again[1])
 
 
+# Either side of the numbers of rows that choose how many waves take a row and how grad_weight is summed; every width of the
+# instances for many rows.
+@pytest.mark.parametrize("m,n", [(256, 1032), (257, 1032), (256, 2048), (256, 2056), (257, 2056), (257, 4104), (256, 5120), (512, 5128),
+                                 (513, 7168), (512, 8192), (513, 8200), (513, 14336), (512, 16384), (513, 20000)])
+def test_sizes_that_choose(pkg, m, n):
+    x, r, w = _data(m, n, BF, m + n)
+    o = pkg.rms_norm(x, w, r)
+    h, rstd, y = _reference(x, r, w, 1e-6)
+    assert torch.equal(o.h, h) and bool(((o.rstd.double() - rstd).abs() <= F * rstd).all())
+    _near(o.y, y, BF)
+    for scale in ("tensor", "row"):
+        q = pkg.rms_norm(x, w, r, out_dtype=E4, scale=scale)
+        top = y.abs().amax() if scale == "tensor" else y.abs().amax(1)
+        assert torch.equal(q.h, h) and bool(((q.scale.double() - top / 448).abs() <= 2 * F * top / 448).all())
+        back = q.y.double() * q.scale.double().view(-1, 1)
+        # half a unit of e4m3's last place, 2^-4 of a value, and of its smallest one, 2^-10 of the scale
+        assert bool(((back - y).abs() <= 2.0**-4 * (1 + 8 * F) * y.abs() + 2.0**-10 * (1 + F) * q.scale.double().view(-1, 1)).all())
+    g = _gen(m)
+    gy, gh = (torch.randn(m, n, device=DEV, generator=g).to(BF) for _ in range(2))
+    gx, gw = pkg.rms_norm_backward(gy, o.h, w, o.rstd, gh)
+    want, size, want_w, size_w = _backward_reference(gy, o.h, w, o.rstd, gh)
+    assert bool(((gx.double() - want).abs() <= HALF[BF] * want.abs() + F * size + TINY[BF]).all())
+    assert bool(((gw.double() - want_w).abs() <= HALF[BF] * want_w.abs() + F * size_w + TINY[BF]).all())
+    # grad_x in the place of an input
+    for i in range(3):
+        a = [gy.clone(), o.h.clone(), gh.clone()]
+        gx2, gw2 = pkg.rms_norm_backward(a[0], a[1], w, o.rstd, a[2], out=a[i])
+        assert gx2 is a[i] and torch.equal(gx2, gx) and torch.equal(gw2, gw)
+
+
 def test_backward_float32_weight_and_strides(pkg):
     m, n = 300, 2880
     x, r, w = _data(m, n, BF, 11, wdtype=torch.float32)
