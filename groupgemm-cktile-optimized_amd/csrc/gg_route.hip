@@ -14,10 +14,10 @@
 // probabilities' sums for the loss follow the same way, chunk by chunk in a fixed order.
 //
 // What bounds it: not the bytes (32768 tokens of 256 experts, float32: 7 us at 5.3 TB/s) but vector instructions and the
-// steps that wait for each other. Those tokens, top 8 with the loss: 27 us, 20 for the first launch (about 10 of them the
-// issue of its 6.1 million vector instructions, the rest loads, barriers and ranks with one workgroup a CU), 4 for the
-// second, 3.5 for the third. 33 tokens, one launch: 7.4; one token 5.5. Asking for the next turn's logits ahead
-// (29.6 us) loses: the registers are full. Backward 16640 tokens of 32 experts 3.7.
+// steps that wait for each other. Those tokens, top 8 with the loss: 24 us, 17 for the first launch (about 10 of them the
+// issue of its 6.2 million vector instructions, the rest loads, barriers and ranks with one workgroup a CU), 4 for the
+// second, 3.5 for the third. 33 tokens, one launch: 7.7; one token 5.7. Asking for the next turn's logits ahead
+// loses 2 us: the registers are full. Backward 16640 tokens of 32 experts 3.6.
 #include <algorithm>
 
 #include "gg_layer.h"
@@ -27,7 +27,7 @@ namespace layer {
 namespace {
 
 constexpr int kThreads  = 1024, kWaves = kThreads / 64;
-constexpr int kScanless = 32; // chunks whose histograms the last launch adds up itself (of 256: 30 us with the loss, scanned 26)
+constexpr int kScanless = 32; // chunks whose histograms the last launch adds up itself (of 256: 30 us with the loss where a scan took 26)
 constexpr int kMaxPairs = 1024, kMaxTokens = 128, kSegments = kMaxPairs / 64; // of a chunk
 
 struct RouteArgs {
@@ -197,8 +197,8 @@ __device__ __forceinline__ void write_loss(const RouteArgs &a, int64_t count, in
     }
 }
 
-// One chunk of tokens a workgroup. KEEP: values of its own that a lane may give (its share of the top_k + 1 largest);
-// SLOTS: of the top_k + 1, those that one lane keeps (lane s % L of the token the s-th).
+// One chunk of tokens a workgroup. KEEP: values of its own that a lane may give (its share of the top_k + 2 largest);
+// SLOTS: of the top_k + 2, those that one lane keeps (lane s % L of the token the s-th).
 template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(kThreads) route_kernel(const RouteArgs a) {
     constexpr int      kPer = 64 / L, kExperts = L * V; // tokens a wave has at a time
     constexpr unsigned kIndex = kExperts - 1;           // low bits of a packed value
@@ -215,6 +215,7 @@ template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(k
     unsigned      mask   = ~kIndex; // (in a register: the and-or below has a constant already)
     asm("" : "+v"(mask));
     const unsigned lane_bits = (L - 1 - sub) * V;
+    const int      rounds    = a.top_k + (a.dtype == GG_DTYPE_FP32 ? 2 : 0);
 
     float acc[V];
 #pragma unroll
@@ -247,7 +248,7 @@ template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(k
         }
         sum       = group_sum<L>(sum);
         bool live = wanted && top > kNegInf;
-        // the top_k + 1 largest packed values in order
+        // the top_k + 2 largest packed values in order (of 16-bit logits the top_k largest, see below)
         sort_descending(packed);
 #pragma unroll
         for (int j = 0; j < KEEP; ++j)
@@ -256,7 +257,7 @@ template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(k
 #pragma unroll
         for (int r = 0; r < SLOTS; ++r) {
             pick[r] = 0;
-            for (int i = 0; i < L && r * L + i <= a.top_k; ++i) {
+            for (int i = 0; i < L && r * L + i < rounds; ++i) {
                 const unsigned best = group_max<L>(packed[0]);
                 pick[r]             = sub == i ? best : pick[r];
                 const bool mine     = packed[0] == best;
@@ -267,17 +268,26 @@ template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(k
             }
         }
         // Packing cut the values' last bits: their order is right unless two that follow each other agree in the
-        // rest (top_k and the first one out among them). 16-bit logits have no such bits.
-        bool doubt = false;
+        // rest (top_k and the first one out among them). 16-bit logits have no such bits. Two such are put in order by
+        // their logits below; where there are more in a row the wave takes the values one by one, which takes so long that
+        // one token's need is seen in the time of a launch (32768 of 256 experts, where seven in a thousand have two:
+        // 27.6 us when those were taken so, 24.1 now; 4096 of 1024, top 32, 42.6 and 32.8). -infinity is never chosen, whatever its place.
+        bool doubt = false, tie = false; // tie: this lane's value with the next lane's
         if (__ballot(low != 0) != 0) {
 #pragma unroll
             for (int r = 0; r < SLOTS; ++r) {
                 const unsigned up   = static_cast<unsigned>(__shfl(static_cast<int>(pick[r]), base_lane + ((sub + 1) & (L - 1))));
                 const unsigned over = r + 1 < SLOTS ? static_cast<unsigned>(__shfl(static_cast<int>(pick[r + 1 < SLOTS ? r + 1 : r]), base_lane)) : 0;
                 const unsigned next = sub + 1 < L ? up : over;
-                doubt |= r * L + sub < a.top_k && ((pick[r] ^ next) & ~kIndex) == 0;
+                tie |= r * L + sub < a.top_k + (SLOTS == 1) && ((pick[r] ^ next) & ~kIndex) == 0 && pick[r] > (kNegInf | kIndex);
             }
-            doubt &= low != 0;
+            tie &= low != 0;
+            if constexpr (SLOTS > 1) {
+                doubt = tie;
+            } else {
+                const uint64_t ties = (__ballot(tie) >> base_lane) & (L == 64 ? ~0ull : (1ull << L) - 1); // of this token
+                doubt               = (ties & ties >> 1) != 0;
+            }
         }
         // A NaN sum: a NaN, an infinity, or nothing but -infinity. Then too the wave takes the values one by one.
         doubt |= sum != sum;
@@ -317,14 +327,29 @@ template <int L, int V, int KEEP, int SLOTS> __global__ void __launch_bounds__(k
                     slot[r] = sub == i ? e : slot[r];
                 }
         }
-        float chosen = 0.f;
 #pragma unroll
         for (int r = 0; r < SLOTS; ++r) {
             x[r] = -__builtin_inff();
-            if (live && r * L + sub < a.top_k && slot[r] < a.experts)
+            if (live && r * L + sub < a.top_k + (SLOTS == 1) && slot[r] < a.experts)
                 x[r] = load_one(a.dtype, a.logits, row + slot[r]);
-            chosen += x[r] != -__builtin_inff() ? exp_neg(x[r] - most) : 0.f;
         }
+        if constexpr (SLOTS == 1) {
+            const uint64_t firsts = __ballot(tie && !doubt); // (what was taken one by one is in order)
+            if (firsts != 0) {
+                const bool  first   = (firsts >> lane & 1) != 0, second = sub > 0 && (firsts << 1 >> lane & 1) != 0;
+                const int   other   = lane + (first ? 1 : second ? -1 : 0);
+                const float x_other = __shfl(x[0], other);
+                const int   e_other = __shfl(slot[0], other);
+                if (first ? x_other > x[0] : x_other < x[0]) { // equal ones stay: the lower expert is first
+                    x[0]    = x_other;
+                    slot[0] = e_other;
+                }
+            }
+        }
+        float chosen = 0.f;
+#pragma unroll
+        for (int r = 0; r < SLOTS; ++r)
+            chosen += r * L + sub < a.top_k && x[r] != -__builtin_inff() ? exp_neg(x[r] - most) : 0.f;
         const float inv = 1.f / sum, scale = a.renormalize ? 1.f / group_sum<L>(chosen) : inv;
         if (live && a.balance) {
 #pragma unroll
@@ -761,10 +786,10 @@ bool vector_rows(const void *p, int64_t stride, int64_t tokens, int dtype) {
 
 int run_route(const RouteArgs &a, hipStream_t s) {
     int st = with_lanes(a.experts, halves(a.tokens), [&](auto l, auto v) {
-        constexpr int few = v.value < 9 ? v.value : 9; // of top_k + 1 <= 9 values
-        constexpr int most = l.value * v.value < 32 ? l.value * v.value + 1 : 33; // top_k + 1
+        constexpr int few = v.value < 10 ? v.value : 10; // of top_k + 2 <= 10 values
+        constexpr int most = l.value * v.value < 32 ? l.value * v.value + 2 : 34; // top_k + 2
         return a.top_k <= 8
-                   ? launch("route", route_kernel<l.value, v.value, few, (9 + l.value - 1) / l.value>, a.chunks, kThreads, s, a)
+                   ? launch("route", route_kernel<l.value, v.value, few, (10 + l.value - 1) / l.value>, a.chunks, kThreads, s, a)
                    : launch("route", route_kernel<l.value, v.value, v.value, (most + l.value - 1) / l.value>, a.chunks, kThreads, s, a);
     });
     if (st == GG_OK && a.chunks > 1) {

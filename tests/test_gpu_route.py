@@ -123,6 +123,31 @@ def test_mask_hides_garbage(pkg, t, e, k):
     assert bool((grad[~mask] == 0).all()) and bool(grad.isfinite().all())
 
 
+@pytest.mark.parametrize("e", [40, 64, 100, 256, 300, 512, 1000])
+@pytest.mark.parametrize("k", [1, 5, 8, 12])
+@pytest.mark.parametrize("masked", [False, True])
+def test_values_that_differ_in_the_last_bits(pkg, e, k, masked):
+    """Float32 logits a unit or a few apart, in pairs, threes and more, among the chosen and at their end; equal ones too."""
+    t, g = 700, _gen(e + k)
+    logits = torch.randn(t, e, device=DEV, generator=g)
+    order = logits.argsort(1, descending=True)
+    bits = logits.view(torch.int32)
+    every = torch.arange(t, device=DEV)
+    for kind, tokens in enumerate(every.view(7, 100)):
+        if kind == 6:  # all of a token's logits within 64 units
+            bits[tokens] = 0x3f800000 + torch.randint(0, 64, (100, e), device=DEV, generator=g, dtype=torch.int32)
+            continue
+        for n in range(1, (2, 2, 3, 4, 2, 5)[kind]):  # the n values after the first of each run come near it
+            for at in ((0, 3), (k - 1,), (max(k - 2, 0),), (1,), (k,), (k // 2,))[kind]:
+                first, then = order[tokens, at], order[tokens, at + n]
+                off = torch.randint(-3, 4, (100,), device=DEV, generator=g, dtype=torch.int32)
+                bits[tokens, then] = bits[tokens, first] + off
+    if masked:
+        logits[torch.rand(t, e, device=DEV, generator=g) < 0.5] = -INF
+    r = pkg.route(logits, k, balance=True)
+    _check(r, _reference(logits, k, None, True), True)
+
+
 def test_special_values(pkg):
     l = torch.zeros(6, 8, device=DEV)
     l[0] = torch.tensor([0.0, -0.0, 0.0, -0.0, 0.0, 0.0, 0.0, 0.0])           # all equal: by index
