@@ -4,8 +4,8 @@
 // A token belongs to L lanes, each with V consecutive experts in registers. Logits are compared as unsigned numbers of
 // the same order. Packed into one word, the number's upper bits and the expert counted backwards (equal logits go to
 // the lower expert), each lane sorts its V with a network; then one value per round comes out: the largest of the
-// lanes' first ones, whose lane moves up. Where the bits that packing cuts could matter the wave takes them again by
-// their whole numbers. Softmax is taken of the values (max subtracted, float32).
+// lanes' first ones, whose lane moves up. Where the bits that packing cuts could matter, two are put in order by their
+// whole values, and for more the wave takes all again by whole numbers. Softmax is taken of the values (max subtracted, float32).
 //
 // Rows are a stable counting sort. A workgroup takes a chunk of consecutive tokens, lays the experts of
 // its pairs out in LDS and ranks 64 pairs at a time: lanes with the same expert find each other with one
@@ -14,8 +14,8 @@
 // probabilities' sums for the loss follow the same way, chunk by chunk in a fixed order.
 //
 // What bounds it: not the bytes (32768 tokens of 256 experts, float32: 7 us at 5.3 TB/s) but vector instructions and the
-// steps that wait for each other. Those tokens, top 8 with the loss: 24 us, 17 for the first launch (about 10 of them the
-// issue of its 6.2 million vector instructions, the rest loads, barriers and ranks with one workgroup a CU), 4 for the
+// steps that wait for each other. Those tokens, top 8 with the loss: 24 us, 17 for the first launch (about 11 of them the
+// issue of its 6.7 million vector instructions, the rest loads, barriers and ranks with one workgroup a CU), 4 for the
 // second, 3.5 for the third. 33 tokens, one launch: 7.7; one token 5.7. Asking for the next turn's logits ahead
 // loses 2 us: the registers are full. Backward 16640 tokens of 32 experts 3.6.
 #include <algorithm>
