@@ -55,13 +55,36 @@ template <typename T> __device__ __forceinline__ void load_w(const void *w, bool
 // Saturates (the conversion would give NaN past the largest value); a NaN stays one.
 __device__ __forceinline__ float saturate(float v, float top) { return v != v ? v : fminf(fmaxf(v, -top), top); }
 
-__device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], bool e5m2) {
+// Division by a scale, rounded as a float32 division is: the product with the rounded reciprocal, corrected once by its
+// remainder, which a fused multiply-add gives exactly (Markstein 1990). By the product alone one in sixty of the values
+// within two float32 units of a tie of the format went to the neighbouring code. The product is clamped first, far past
+// either format's range, so that the remainder stays finite; a NaN comes back with the remainder. Outside 2^-64 .. 2^64
+// the remainder could be subnormal, and `exact` divides.
+struct Divisor {
+    float s, inv;
+    bool  exact;
+    __device__ __forceinline__ explicit Divisor(float scale)
+        : s(scale), inv(1.f / scale), exact(!(fabsf(scale) >= 0x1p-64f && fabsf(scale) <= 0x1p64f)) {}
+    __device__ __forceinline__ float quotient(float v) const {
+        const float q = __builtin_amdgcn_fmed3f(v * inv, -131072.f, 131072.f);
+        return fmaf(-fmaf(q, s, -v), inv, q); // (in this order of signs a zero keeps its own)
+    }
+};
+
+// Eight values divided by the scale, as fp8.
+__device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], const Divisor &d, bool e5m2) {
     u32x2 w;
     const float top = e5m2 ? 57344.f : 448.f;
     float s[8];
+    if (d.exact) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        s[i] = saturate(v[i], top);
+        for (int i = 0; i < 8; ++i)
+            s[i] = saturate(v[i] / d.s, top);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            s[i] = saturate(d.quotient(v[i]), top);
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         int q = 0;
@@ -77,8 +100,8 @@ __device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], bool e5m2) {
     return w;
 }
 
-// Scale of the largest |y| (bits of a float >= 0 or NaN): 1 where the quotient is zero or subnormal, whose
-// reciprocal would be infinite.
+// Scale of the largest |y| (bits of a float >= 0 or NaN): 1 where the quotient is zero or subnormal, which a division
+// by it could turn into NaN or a value of few bits.
 __device__ __forceinline__ float scale_of(unsigned top_bits, bool e5m2) {
     const float s = __uint_as_float(top_bits) / (e5m2 ? 57344.f : 448.f);
     return s < 1.17549435e-38f ? 1.f : s;
@@ -179,15 +202,15 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
         if constexpr (FIRST) {
             top = max(top, row_top);
         } else {
-            float inv = 1.f;
+            float s = 1.f;
             if (a.mode == GG_NORM_SCALE_ROW) {
-                const float s = scale_of(row_max<WPR>(m, turn, row_top, wave, lane), a.e5m2);
-                inv           = 1.f / s;
+                s = scale_of(row_max<WPR>(m, turn, row_top, wave, lane), a.e5m2);
                 if (t == 0)
                     a.scale[row] = s;
             } else if (a.mode == GG_NORM_SCALE_GIVEN) {
-                inv = 1.f / a.scale[0];
+                s = a.scale[0];
             }
+            const Divisor by(s);
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int i = (u * 64 * WPR + t) * 8;
@@ -195,10 +218,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
                     if (a.mode == GG_NORM_PLAIN) {
                         *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.y) + row * a.hidden + i) = pack8<T>(v[u]);
                     } else {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j)
-                            v[u][j] *= inv;
-                        *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v[u], a.e5m2);
+                        *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v[u], by, a.e5m2);
                     }
                 }
             }
@@ -239,8 +259,8 @@ template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) qu
 #pragma unroll
     for (int i = 0; i < THREADS / 64; ++i)
         top = max(top, tops[i]);
-    const float s   = scale_of(top, a.e5m2);
-    const float inv = 1.f / s;
+    const float   s = scale_of(top, a.e5m2);
+    const Divisor by(s);
     if (blockIdx.x == 0 && threadIdx.x == 0)
         a.scale[0] = s;
     // from the last row backwards: the rows written last are still in the Infinity Cache
@@ -252,8 +272,8 @@ template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) qu
             load_w<T>(a.weight, a.w32, i, w);
 #pragma unroll
             for (int j = 0; j < 8; ++j)
-                v[j] = v[j] * rstd * w[j] * inv;
-            *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v, a.e5m2);
+                v[j] = v[j] * rstd * w[j];
+            *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v, by, a.e5m2);
         }
     }
 }
