@@ -3,9 +3,11 @@ ABI in include/gg_moe_layer.h: RMS norm with the residual's addition and an fp8 
 balance loss, dispatch and combine of the experts' rows, grouped products with 4-bit weights.
 
 Every function enqueues its kernels on the current stream of its tensors' device, or on `stream` (a
-raw hipStream_t handle), and returns without waiting. Outputs and workspaces come from torch's
-allocator. With `stream`, the caller orders that stream after whatever wrote the inputs; the
-allocator is told of the use, so a tensor may be dropped before the work is done.
+raw hipStream_t handle), and returns without waiting (but grouped_gemm_w4 with host group sizes, which
+copies them to the device and waits for that). Outputs and workspaces come from torch's allocator, from
+the memory of the stream that the kernels run on. With `stream`, the caller orders that stream after
+whatever wrote the inputs, and what reads the outputs on another stream after it; the allocator is told
+of both streams' uses, so a tensor may be dropped before the work is done.
 """
 from __future__ import annotations
 
@@ -27,23 +29,46 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 
-def _call(fn, dev, stream: Optional[int], args, tensors) -> None:
-    """fn(*args, stream): on the current stream of `dev` or on a given one, with `dev` the current device. A
-    stream that is not torch's current one is told of the tensors it uses."""
+def _call(fn, dev, args) -> None:
+    """fn(*args, stream) on the current stream of `dev`, with `dev` the current device."""
     current = _raw_stream(dev.index)
     if dev.index == _current_device():
-        st = fn(*args, current if stream is None else stream)
+        st = fn(*args, current)
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, current if stream is None else stream)
+            st = fn(*args, current)
     if st != GG_OK:
         raise GGError(st, _lib.gg_layer_last_error().decode())
-    if stream is not None and stream != current:
-        # (handle 0 is the default stream)
-        other = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
-        for t in tensors:
-            if t is not None:
-                t.record_stream(other)
+
+
+def _tensors(values):
+    for v in values:
+        if isinstance(v, torch.Tensor):
+            yield v
+        elif isinstance(v, tuple):
+            yield from _tensors(v)
+
+
+def _on(stream: int, f, *args):
+    """f(*args) with `stream` as torch's current one. Memory that torch hands out belongs to its current stream: a
+    dropped tensor's block is given out again while work queued there still uses it. So outputs and workspaces of
+    kernels on `stream` have to be allocated with that stream current, or nothing would order them after that work."""
+    dev = args[0].device
+    if dev.type != "cuda":
+        return f(*args)  # refused there
+    current = torch.cuda.current_stream(dev)
+    if stream == current.cuda_stream:
+        return f(*args)
+    # (handle 0 is the default stream)
+    other = torch.cuda.ExternalStream(stream, device=dev) if stream else torch.cuda.default_stream(dev)
+    with torch.cuda.stream(other):
+        out = f(*args)
+    for t in _tensors(args):
+        if t.is_cuda:
+            t.record_stream(other)
+    for t in _tensors((out,)):
+        t.record_stream(current)  # what the caller reads there
+    return out
 
 
 def _matrix(name: str, t):
@@ -105,6 +130,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
     "tensor": the x_scale of grouped_gemm_fp8), one for each row ("row"), or divided by a given device
     float32 scale [1]. out: y's buffer; out_h: h's, which may be x or residual itself.
     """
+    if stream is not None:
+        return _on(stream, rms_norm, x, weight, residual, eps, out_dtype, scale, out, out_h)
     dtype = x.dtype
     dt = _T16.get(dtype)
     if dt is None:
@@ -152,10 +179,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
                 raise ValueError("scale must be 'tensor', 'row' or a device float32 tensor of one value")
     y = _new_like(x) if out is None and mode == _PLAIN else _out(out, out_dtype, (m, n), dev)
     rstd = torch.empty(m, dtype=torch.float32, device=dev)
-    _call(_lib.gg_rms_norm, dev, stream, (dt, dt if wd == dtype else _FP32, od, mode, m, n, eps, x.data_ptr(), xs,
-                                          _ptr(residual), rs,
-                                          weight.data_ptr(), hp, hs, y.data_ptr(), rstd.data_ptr(), _ptr(s), _ptr(ws)),
-          (x, residual, weight, h, y, rstd, s, ws))
+    _call(_lib.gg_rms_norm, dev, (dt, dt if wd == dtype else _FP32, od, mode, m, n, eps, x.data_ptr(), xs, _ptr(residual), rs,
+                                  weight.data_ptr(), hp, hs, y.data_ptr(), rstd.data_ptr(), _ptr(s), _ptr(ws)))
     return NormOutput(y, h, rstd, s)
 
 
@@ -163,6 +188,8 @@ def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Op
     """(grad_x, grad_weight) of rms_norm from its h and rstd (gg_rms_norm_backward). grad_x is the gradient
     of x and of residual; grad_h, the gradient that reaches h past the norm, is added to it. grad_y and
     grad_h are of h's type (an fp8 y is differentiated as if it were not rounded)."""
+    if stream is not None:
+        return _on(stream, rms_norm_backward, grad_y, h, weight, rstd, grad_h, out)
     dtype = h.dtype
     dt = _T16.get(dtype)
     if dt is None:
@@ -183,11 +210,9 @@ def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Op
     gw = torch.empty_like(weight)
     need = _lib.gg_rms_norm_backward_workspace(m, n)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(_lib.gg_rms_norm_backward, dev, stream, (dt, dt if wd == dtype else _FP32, m, n, grad_y.data_ptr(), gs,
-                                                   h.data_ptr(), hs,
-                                                   weight.data_ptr(), rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(),
-                                                   gw.data_ptr(), _ptr(ws), need),
-          (grad_y, h, weight, rstd, grad_h, gx, gw, ws))
+    _call(_lib.gg_rms_norm_backward, dev, (dt, dt if wd == dtype else _FP32, m, n, grad_y.data_ptr(), gs, h.data_ptr(), hs,
+                                           weight.data_ptr(), rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(),
+                                           gw.data_ptr(), _ptr(ws), need))
     return gx, gw
 
 
@@ -225,6 +250,8 @@ def route(logits, top_k: int, mask=None, renormalize: bool = True, balance: bool
     (equal ones by the lower index), their softmax weights (divided by their sum with renormalize), the rows
     of each expert and of each pair, and with balance the loss E * sum(f * P) over the tokens that take part.
     mask [T] bool: False = the token takes no part (padding); its logits are not looked at."""
+    if stream is not None:
+        return _on(stream, route, logits, top_k, mask, renormalize, balance)
     dt, stride = _logits(logits)
     (t, e), dev = logits.shape, logits.device
     if mask is not None:
@@ -244,17 +271,17 @@ def route(logits, top_k: int, mask=None, renormalize: bool = True, balance: bool
     need = _lib.gg_route_workspace(t, e, top_k)
     if need:
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _call(_lib.gg_route, dev, stream, (dt, t, e, top_k, int(renormalize), logits.data_ptr(), stride, _ptr(mask),
-                                       experts.data_ptr(),
-                                       weights.data_ptr(), counts.data_ptr(), offs.data_ptr(), rows.data_ptr(), lse.data_ptr(),
-                                       _ptr(loss), _ptr(slope), _ptr(ws), need),
-          (logits, mask, experts, weights, counts, offs, rows, lse, loss, slope, ws))
+    _call(_lib.gg_route, dev, (dt, t, e, top_k, int(renormalize), logits.data_ptr(), stride, _ptr(mask), experts.data_ptr(),
+                               weights.data_ptr(), counts.data_ptr(), offs.data_ptr(), rows.data_ptr(), lse.data_ptr(),
+                               _ptr(loss), _ptr(slope), _ptr(ws), need))
     return Routing(experts, weights, counts, offs, rows, lse, slope, loss, bool(renormalize))
 
 
 def route_backward(logits, routing: Routing, grad_weights=None, grad_loss=None, out=None, stream: Optional[int] = None):
     """Gradient of the logits, in their type, from the gradients of routing.weights [T, k] float32 and of
     routing.loss (a device float32 tensor of one value), either of them None (gg_route_backward)."""
+    if stream is not None:
+        return _on(stream, route_backward, logits, routing, grad_weights, grad_loss, out)
     dt, stride = _logits(logits)
     (t, e), dev = logits.shape, logits.device
     r = routing
@@ -271,11 +298,9 @@ def route_backward(logits, routing: Routing, grad_weights=None, grad_loss=None, 
         if grad_loss.dtype != torch.float32 or grad_loss.numel() != 1 or grad_loss.device != dev:
             raise ValueError("grad_loss must be a device float32 tensor of one value")
     g = _new_like(logits) if out is None else _out(out, logits.dtype, (t, e), dev)
-    _call(_lib.gg_route_backward, dev, stream, (dt, t, e, k, int(r.renormalize), logits.data_ptr(), stride,
-                                                r.experts.data_ptr(),
-                                                r.weights.data_ptr(), r.lse.data_ptr(), _ptr(grad_weights), _ptr(grad_loss),
-                                                0 if grad_loss is None else r.slope.data_ptr(), g.data_ptr()),
-          (logits, r.experts, r.weights, r.lse, r.slope, grad_weights, grad_loss, g))
+    _call(_lib.gg_route_backward, dev, (dt, t, e, k, int(r.renormalize), logits.data_ptr(), stride, r.experts.data_ptr(),
+                                        r.weights.data_ptr(), r.lse.data_ptr(), _ptr(grad_weights), _ptr(grad_loss),
+                                        0 if grad_loss is None else r.slope.data_ptr(), g.data_ptr()))
     return g
 
 
@@ -302,6 +327,8 @@ def _offs(routing: Routing, dev):
 def dispatch(x, routing: Routing, out=None, stream: Optional[int] = None):
     """xs [T * k, H]: row routing.rows[t, s] is x[t]; rows past the last expert's are zero (gg_dispatch). x:
     [T, H] of any type of 1, 2 or 4 bytes, rows contiguous. xs with routing.counts is what grouped_gemm takes."""
+    if stream is not None:
+        return _on(stream, dispatch, x, routing, out)
     stride, dev = _matrix("x", x), x.device
     rows, t, k = _rows(routing, dev)
     offs = _offs(routing, dev)
@@ -311,9 +338,8 @@ def dispatch(x, routing: Routing, out=None, stream: Optional[int] = None):
     if x.element_size() not in (1, 2, 4):
         raise TypeError("x must be of a type of 1, 2 or 4 bytes")
     xs = _out(out, x.dtype, (t * k, n), dev)
-    _call(_lib.gg_dispatch, dev, stream, (x.element_size(), t, k, n, offs.numel() - 1, x.data_ptr(), stride,
-                                          rows.data_ptr(), offs.data_ptr(), xs.data_ptr()),
-          (x, rows, offs, xs))
+    _call(_lib.gg_dispatch, dev, (x.element_size(), t, k, n, offs.numel() - 1, x.data_ptr(), stride, rows.data_ptr(),
+                                  offs.data_ptr(), xs.data_ptr()))
     return xs
 
 
@@ -327,32 +353,35 @@ def _pairs(name: str, y, t: int, k: int):
 
 def dispatch_backward(grad_xs, routing: Routing, out=None, stream: Optional[int] = None):
     """grad_x [T, H]: the sum of each token's rows of grad_xs [T * k, H] (gg_dispatch_backward)."""
+    if stream is not None:
+        return _on(stream, dispatch_backward, grad_xs, routing, out)
     dev = grad_xs.device
     rows, t, k = _rows(routing, dev)
     n = _pairs("grad_xs", grad_xs, t, k)
     gx = _out(out, grad_xs.dtype, (t, n), dev)
-    _call(_lib.gg_dispatch_backward, dev, stream, (_T16[grad_xs.dtype], t, k, n, grad_xs.data_ptr(), rows.data_ptr(),
-                                                   gx.data_ptr()),
-          (grad_xs, rows, gx))
+    _call(_lib.gg_dispatch_backward, dev, (_T16[grad_xs.dtype], t, k, n, grad_xs.data_ptr(), rows.data_ptr(), gx.data_ptr()))
     return gx
 
 
 def combine(y, routing: Routing, out=None, stream: Optional[int] = None):
     """out [T, H]: the sum of each token's rows of y [T * k, H], times routing.weights (gg_combine)."""
+    if stream is not None:
+        return _on(stream, combine, y, routing, out)
     dev = y.device
     rows, t, k = _rows(routing, dev)
     n = _pairs("y", y, t, k)
     _flat("routing.weights", routing.weights, torch.float32, (t, k), dev)
     o = _out(out, y.dtype, (t, n), dev)
-    _call(_lib.gg_combine, dev, stream, (_T16[y.dtype], t, k, n, y.data_ptr(), rows.data_ptr(), routing.weights.data_ptr(),
-                                         o.data_ptr()),
-          (y, rows, routing.weights, o))
+    _call(_lib.gg_combine, dev, (_T16[y.dtype], t, k, n, y.data_ptr(), rows.data_ptr(), routing.weights.data_ptr(),
+                                 o.data_ptr()))
     return o
 
 
 def combine_backward(grad_out, y, routing: Routing, out=None, stream: Optional[int] = None):
     """(grad_y [T * k, H], grad_weights [T, k] float32) of combine (gg_combine_backward). grad_out: [T, H] of
     y's type, rows contiguous. Rows of grad_y past the last expert's are zero."""
+    if stream is not None:
+        return _on(stream, combine_backward, grad_out, y, routing, out)
     dev = y.device
     rows, t, k = _rows(routing, dev)
     offs = _offs(routing, dev)
@@ -363,10 +392,9 @@ def combine_backward(grad_out, y, routing: Routing, out=None, stream: Optional[i
     stride = _matrix("grad_out", grad_out)
     gy = _out(out, y.dtype, (t * k, n), dev)
     gw = torch.empty((t, k), dtype=torch.float32, device=dev)
-    _call(_lib.gg_combine_backward, dev, stream, (_T16[y.dtype], t, k, n, offs.numel() - 1, grad_out.data_ptr(), stride,
-                                                  y.data_ptr(), rows.data_ptr(), offs.data_ptr(),
-                                                  routing.weights.data_ptr(), gy.data_ptr(), gw.data_ptr()),
-          (grad_out, y, rows, offs, routing.weights, gy, gw))
+    _call(_lib.gg_combine_backward, dev, (_T16[y.dtype], t, k, n, offs.numel() - 1, grad_out.data_ptr(), stride, y.data_ptr(),
+                                          rows.data_ptr(), offs.data_ptr(), routing.weights.data_ptr(), gy.data_ptr(),
+                                          gw.data_ptr()))
     return gy, gw
 
 
@@ -448,6 +476,8 @@ def grouped_gemm_w4(x, w: W4Weights, group_m, out=None, stream: Optional[int] = 
     that is never read on the host (with optional device offsets); a device group that does not lie inside x
     gets no work, and rows of no group are not written. For groups of few rows: every 16 or 32 rows of a group read
     its weights once."""
+    if stream is not None:
+        return _on(stream, grouped_gemm_w4, x, w, group_m, out, None, group_offs)
     dt = _T16.get(x.dtype)
     if dt is None:
         raise TypeError("x must be bfloat16 or float16")
@@ -471,7 +501,6 @@ def grouped_gemm_w4(x, w: W4Weights, group_m, out=None, stream: Optional[int] = 
     elif group_m.device != dev or (group_offs is not None and group_offs.device != dev):
         raise ValueError("group sizes must be on x's device")
     o = _out(out, x.dtype, (m, n), dev)
-    _call(_lib.gg_gemm_w4, dev, stream, (dt, b, m, n, k, group, group_m.data_ptr(), _ptr(group_offs), x.data_ptr(),
-                                         packed.data_ptr(), scales.data_ptr(), _ptr(zeros), o.data_ptr()),
-          (x, packed, scales, zeros, group_m, group_offs, o))
+    _call(_lib.gg_gemm_w4, dev, (dt, b, m, n, k, group, group_m.data_ptr(), _ptr(group_offs), x.data_ptr(), packed.data_ptr(),
+                                 scales.data_ptr(), _ptr(zeros), o.data_ptr()))
     return o
