@@ -588,7 +588,7 @@ int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int6
         return fail(GG_ERR_INVALID, "scale_mode must be a gg_norm_scale");
     if (scale_mode == GG_NORM_PLAIN ? out_dtype != dtype : !is8(out_dtype))
         return fail(GG_ERR_INVALID, "out_dtype must be dtype, or an fp8 type with a scale");
-    if (scale_mode != GG_NORM_PLAIN && scale == nullptr)
+    if (scale_mode != GG_NORM_PLAIN && scale == nullptr && (rows > 0 || scale_mode != GG_NORM_SCALE_ROW)) // (a row scale of no rows)
         return fail(GG_ERR_INVALID, "scale is null");
     if (rows == 0 && scale_mode != GG_NORM_SCALE_TENSOR)
         return GG_OK;

@@ -45,7 +45,7 @@ typedef enum gg_norm_scale {
  *   GG_DTYPE_FP32. out_dtype: dtype, or an fp8 type with scale_mode 1-3.
  *   h: [rows, hidden]; may be x or residual itself. Not written (and may be NULL) without a residual.
  *   y: [rows, hidden] contiguous, overlapping no input. rstd: [rows], or NULL but for GG_NORM_SCALE_TENSOR.
- *   scale: written, [1] or [rows], or for GG_NORM_SCALE_GIVEN read, [1].
+ *   scale: written, [1] or [rows] (of no rows it may be NULL), or for GG_NORM_SCALE_GIVEN read, [1].
  *   workspace: GG_NORM_WORKSPACE bytes for GG_NORM_SCALE_TENSOR, else unused.
  * GG_ERR_UNSUPPORTED unless hidden % 8 == 0, hidden <= 32768, strides % 8 == 0 and 16-byte aligned
  * buffers (y of fp8: 8-byte).

@@ -57,3 +57,15 @@ def test_given_scales(pkg, out, scale):
     s = torch.tensor([scale], device=DEV)
     o = pkg.rms_norm(x, w, out_dtype=out, scale=s)
     _same(o, w, s, out)
+
+
+@pytest.mark.parametrize("out", [E4, E5])
+def test_no_rows_with_any_scale(pkg, out):
+    x, w = torch.empty(0, 64, device=DEV, dtype=BF), torch.ones(64, device=DEV, dtype=BF)
+    given = torch.full((1,), 0.5, device=DEV)
+    for residual in (None, x):
+        o = pkg.rms_norm(x, w, residual, out_dtype=out, scale="row")
+        assert o.y.shape == (0, 64) and o.y.dtype == out and o.scale.shape == (0,) and o.rstd.shape == (0,)
+        o = pkg.rms_norm(x, w, residual, out_dtype=out, scale=given)
+        assert o.y.shape == (0, 64) and o.scale is given and float(given) == 0.5
+        assert float(pkg.rms_norm(x, w, residual, out_dtype=out).scale) == 1.0

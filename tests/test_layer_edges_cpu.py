@@ -1,0 +1,20 @@
+"""The layer operators at the edges of their arguments, without a GPU."""
+import pytest
+import torch
+
+BF16, E4M3, E5M2 = 0, 2, 3
+INVALID = 2
+P = 4096  # an aligned address that is never dereferenced
+
+
+@pytest.mark.parametrize("out", [E4M3, E5M2])
+def test_norm_of_no_rows(pkg, out):
+    """An empty array of row scales may be NULL; one scale of the tensor, or a given one, may not."""
+    lib = pkg.load_library()
+
+    def call(mode, scale):
+        return lib.gg_rms_norm(BF16, BF16, out, mode, 0, 128, 1e-6, None, 128, None, 0, P, None, 0, None, None, scale, P, None)
+
+    assert call(2, None) == 0 and call(2, P) == 0 and call(3, P) == 0
+    for mode in (1, 3):
+        assert call(mode, None) == INVALID and "scale is null" in lib.gg_layer_last_error().decode()
