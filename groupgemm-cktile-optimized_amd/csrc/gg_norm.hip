@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_back_kernel(const Bac
             }
         }
         dot = row_sum<WPR>(m, turn, dot, wave, lane);
-        const float c = rstd * rstd * rstd * (dot / static_cast<float>(a.hidden));
+        const float c = rstd * (rstd * (rstd * (dot / static_cast<float>(a.hidden)))); // (rstd^3 alone may be past float32)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;

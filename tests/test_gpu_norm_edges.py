@@ -1,4 +1,4 @@
-"""RMS norm where it is easily off: the division by a scale, bit for bit.
+"""RMS norm where it is easily off: the division by a scale, bit for bit; no rows; rows of very large and small values.
 
 The kernels take y = (h * rstd) * weight in float32, divide it by the scale as float32 division rounds it, clamp and
 round to the format. Given rstd and the scale that a call returned, the same steps on the CPU give the same codes:
@@ -69,3 +69,24 @@ def test_no_rows_with_any_scale(pkg, out):
         o = pkg.rms_norm(x, w, residual, out_dtype=out, scale=given)
         assert o.y.shape == (0, 64) and o.scale is given and float(given) == 0.5
         assert float(pkg.rms_norm(x, w, residual, out_dtype=out).scale) == 1.0
+
+
+# rstd of 2^50 and 2^-50: its cube is past float32's range, the gradients are not.
+@pytest.mark.parametrize("power", [-50, 50])
+@pytest.mark.parametrize("m,n", [(5, 512), (5, 2880), (300, 1024), (300, 7168)])
+def test_backward_of_large_and_small_rows(pkg, power, m, n):
+    """Bounds as in the ordinary cases: float32 sums and products below 1e-5 of the terms' magnitudes, and half a unit
+    of bf16 in the stored value (2^-8 of it, or half the least subnormal)."""
+    g = torch.Generator(device=DEV).manual_seed(n)
+    h = (torch.randn(m, n, device=DEV, generator=g) * 2.0**power).to(BF)
+    w = (1 + 0.3 * torch.randn(n, device=DEV, generator=g)).to(BF)
+    gy = torch.randn(m, n, device=DEV, generator=g).to(BF)
+    o = pkg.rms_norm(h, w, None, 0.0)
+    gx, gw = pkg.rms_norm_backward(gy, h, w, o.rstd)
+    d, r, wg = h.double(), o.rstd.double()[:, None], gy.double() * w.double()
+    dot = (wg * d).sum(1, keepdim=True) / n
+    want = r * wg - d * r**3 * dot
+    size = (r * wg).abs() + d.abs() * r**3 * (wg * d).abs().sum(1, keepdim=True) / n
+    assert bool(((gx.double() - want).abs() <= 2.0**-8 * want.abs() + 1e-5 * size + 2.0**-134).all())
+    terms = gy.double() * d * r
+    assert bool(((gw.double() - terms.sum(0)).abs() <= 2.0**-8 * terms.sum(0).abs() + 1e-5 * terms.abs().sum(0) + 2.0**-134).all())
