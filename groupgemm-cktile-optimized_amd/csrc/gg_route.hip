@@ -702,7 +702,7 @@ template <typename T, int L, int V, bool VEC> __global__ void __launch_bounds__(
         dot = group_sum<L>(dot);
 #pragma unroll
         for (int j = 0; j < V; ++j)
-            x[j] = fmaf(v[j], g[j] - dot, x[j]);
+            x[j] = live ? fmaf(v[j], g[j] - dot, x[j]) : 0.f; // (0 of padding, also where the loss's gradient is infinite)
         wave_sync();
         if (!inside)
             continue;
