@@ -429,6 +429,8 @@ def pack_w4(q, scales, zeros=None) -> W4Weights:
     nt, kt = (n + 15) // 16, (k + 127) // 128
     packed = torch.empty((b, nt, kt, 64, 16), dtype=torch.uint8, device=q.device)
     for i in range(b):  # one matrix at a time: the layers' weights may fill the card
+        if bool((q[i] > 15).any()):  # would reach into the weight that shares its byte
+            raise ValueError("q must be uint8 [B, N, K] in 0..15")
         full = torch.zeros((nt * 16, kt * 128), dtype=torch.uint8, device=q.device)
         full[:n, :k] = q[i]
         # rows r, k = 128 c + 32 j + 8 a + 2 p + o -> piece 16 a + r, word j, half o, nibble p

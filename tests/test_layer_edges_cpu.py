@@ -18,3 +18,13 @@ def test_norm_of_no_rows(pkg, out):
     assert call(2, None) == 0 and call(2, P) == 0 and call(3, P) == 0
     for mode in (1, 3):
         assert call(mode, None) == INVALID and "scale is null" in lib.gg_layer_last_error().decode()
+
+
+@pytest.mark.parametrize("at", [(0, 0, 0), (1, 23, 127), (1, 5, 64)])
+def test_pack_w4_refuses_what_is_no_nibble(pkg, at):
+    q = torch.full((2, 24, 128), 15, dtype=torch.uint8)
+    s = torch.ones(2, 24, 2, dtype=torch.bfloat16)
+    pkg.pack_w4(q, s)
+    q[at] = 16
+    with pytest.raises(ValueError, match="0..15"):
+        pkg.pack_w4(q, s)
