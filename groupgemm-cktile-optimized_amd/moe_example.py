@@ -45,7 +45,8 @@ def _silu_product_backward(gu, grad):
 
 def _to_fp8(w):
     """Weights [E, N, K] as e4m3 with one scale for each expert."""
-    scale = w.float().abs().amax(dim=(1, 2)) / 448.0
+    top = w.float().abs().amax(dim=(1, 2))
+    scale = torch.where(top > 0, top / 448.0, torch.ones_like(top))  # (an expert of zeros)
     return (w.float() / scale[:, None, None]).to(torch.float8_e4m3fn), scale
 
 

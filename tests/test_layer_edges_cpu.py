@@ -1,4 +1,6 @@
 """The layer operators at the edges of their arguments, without a GPU."""
+import importlib
+
 import pytest
 import torch
 
@@ -28,3 +30,12 @@ def test_pack_w4_refuses_what_is_no_nibble(pkg, at):
     q[at] = 16
     with pytest.raises(ValueError, match="0..15"):
         pkg.pack_w4(q, s)
+
+
+def test_example_quantizes_an_expert_of_zeros(pkg):
+    w = torch.randn(3, 16, 32, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16)
+    w[1] = 0
+    q, scale = importlib.import_module(pkg.__name__ + ".moe_example")._to_fp8(w)
+    assert bool(q.float().isfinite().all()) and bool((q[1].float() == 0).all()) and bool((scale > 0).all())
+    back = q.float() * scale[:, None, None]  # e4m3: 2^-4 of a value, 2^-10 of the scale at least
+    assert bool(((back - w.float()).abs() <= 2.0**-4 * w.float().abs() + 2.0**-10 * scale[:, None, None]).all())
