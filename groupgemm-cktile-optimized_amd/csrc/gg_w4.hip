@@ -12,6 +12,7 @@
 #include <algorithm>
 
 #include "gg_layer.h"
+#include "gg_w4_choice.h"
 
 namespace gg {
 namespace layer {
@@ -534,13 +535,10 @@ __global__ void __launch_bounds__(256, 4) w4_rows_kernel(const W4Args a) {
     }
 }
 
-// How many pieces of `rows` rows the groups have at most.
-int64_t pieces_of(const W4Args &a, int rows) { return std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m) + a.total_m / rows); }
-
 template <typename K> int launch_w4(K kernel, int rows, int columns, int threads, const W4Args &a, hipStream_t s) {
     const int64_t blocks = (static_cast<int64_t>(a.n_tiles) * 16 + columns - 1) / columns;
     // HIP refuses grids of 2^32 threads: past them the pieces are walked in strides
-    const int64_t slots = std::min<int64_t>(pieces_of(a, rows), (int64_t(1) << 31) / threads / blocks);
+    const int64_t slots = std::min<int64_t>(w4_pieces(a.group_num, a.total_m, rows), (int64_t(1) << 31) / threads / blocks);
     return launch("gemm_w4", kernel, blocks * slots, threads, s, a);
 }
 
@@ -559,28 +557,17 @@ template <typename T, int MT, int NT> int launch_rows(const W4Args &a, int group
     return with_format(a, group, [&](auto g, auto z) { return launch_w4(w4_rows_kernel<T, MT, NT, g.value, z.value>, 16 * MT, 64 * NT, 256, a, s); });
 }
 
-// The instance by the rows that a group has on average and the workgroups there are. Measured (us; few-row instances of
-// 64, 32 and 16 columns a workgroup, then the many-row one, of 32 rows and 128 columns):
-//   rows per group (ragged; 32 groups of 2880 x 2880, k of a scale 32, zero points / 16 of 4096 x 4096, 128):
-//     8: 44.6, 54.6, 82.4, 47.4 / 32.5, 42.0, 57.4, 40.5          12: 50.1, 63.2, 100.9, 49.3 / 36.8, 48.7, 70.7, 38.0
-//     16: 54.5, 70.8, 114.9, 52.8 / 40.3, 56.1, 84.6, 41.6        20: 66.0, 84.0, 138.2, 58.9 / 49.0, 68.7, 104.7, 47.6
-//     24: 71.8, 95.5, 157.6, 65.2 / 52.7, 74.3, 118.0, 48.3       48: 120.1, 162.1, 269.7, 98.5 / 87.3, 133.5, 221.8, 63.1
-//     16 rows in every group of the first: 45.0, 60.3, 100.5, 50.0; 24: 71.0, 94.2, 157.3, 51.0
-//   Many-row instances of 16, 48 and 64 rows, or of 64, 192 and 256 columns, gain 3 to 17 % where their sizes fit and
-//   lose 5 to 50 % elsewhere.
-//   workgroups of 64 columns (one row): 8 of 512 x 7168: 11.9, 7.3, 6.1; 32 of 512 x 2048: 6.3, 5.0, 4.6; 128 of
-//     4096 x 1024: 5.2, 4.7, 5.5; 224 of 14336 x 4096: 10.8, 9.5, 12.0; 448 of 7168 x 2048: 9.7, 11.9, 13.8; 4 groups of 20
-//     rows, 2048 x 4096 (288): 11.6, 13.7, 18.8
-//   the many-row one does not split k: with few workgroups it loses (64-column few-row and many-row instance; workgroups of the
-//     latter): 160 of 24 rows, 4096 x 4096 17.6, 26.8; 320 27.5, 30.8 (k 9600: 63.7, 75.8; 1024: 12.2, 11.2); 448 of 14336 x
-//     4096 41.3, 34.6; 510 of 1280 x 5120 60.0, 50.5. Half a piece for each group and the rows / 32: about as many as there are.
 template <typename T> int run_w4(const W4Args &a, int group, hipStream_t s) {
-    const int64_t slots = std::max<int64_t>(1, std::min<int64_t>(a.group_num, a.total_m)), per = a.total_m / slots;
-    const int64_t wide = (a.n_tiles + 7) / 8 * (slots + a.total_m / 16) / 2, narrow = (a.n_tiles + 3) / 4 * pieces_of(a, 16);
-    return per > 16 && wide >= 384 ? launch_rows<T, 2, 2>(a, group, s)
-           : narrow >= 256          ? launch_few<T, 4, 4>(a, group, s)
-           : narrow >= 64           ? launch_few<T, 2, 8>(a, group, s)
-                                    : launch_few<T, 1, 8>(a, group, s);
+    switch (w4_choice(a.group_num, a.total_m, a.n)) {
+    case W4Choice::kRows:
+        return launch_rows<T, 2, 2>(a, group, s);
+    case W4Choice::kFew64:
+        return launch_few<T, 4, 4>(a, group, s);
+    case W4Choice::kFew32:
+        return launch_few<T, 2, 8>(a, group, s);
+    default:
+        return launch_few<T, 1, 8>(a, group, s);
+    }
 }
 
 } // namespace

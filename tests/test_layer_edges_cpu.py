@@ -1,9 +1,15 @@
 """The layer operators at the edges of their arguments, without a GPU."""
 import importlib
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
 
+import w4_cases
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 BF16, E4M3, E5M2 = 0, 2, 3
 INVALID = 2
 P = 4096  # an aligned address that is never dereferenced
@@ -39,3 +45,14 @@ def test_example_quantizes_an_expert_of_zeros(pkg):
     assert bool(q.float().isfinite().all()) and bool((q[1].float() == 0).all()) and bool((scale > 0).all())
     back = q.float() * scale[:, None, None]  # e4m3: 2^-4 of a value, 2^-10 of the scale at least
     assert bool(((back - w.float()).abs() <= 2.0**-4 * w.float().abs() + 2.0**-10 * scale[:, None, None]).all())
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="needs g++")
+def test_4_bit_sizes_reach_the_kernels_they_are_for(tmp_path):
+    """A threshold that moves must take the GPU tests' sizes with it."""
+    cases = w4_cases.CHOICES + w4_cases.TRIPS
+    exe = tmp_path / "w4_choice"
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-I", os.path.join(ROOT, "groupgemm-cktile-optimized_amd", "csrc"),
+                    os.path.join(ROOT, "tests", "w4_choice.cpp"), "-o", str(exe)], check=True)
+    r = subprocess.run([str(exe)] + [str(v) for c in cases for v in c[1:]], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0 and r.stdout.split() == [c[0] for c in cases]
