@@ -144,7 +144,8 @@ int gg_combine_backward(int dtype, int64_t tokens, int top_k, int64_t hidden, in
  * group_lens / group_offs: device sizes as in gg_prepare_device_lens_op; a group whose rows are not
  * inside [0, total_m) gets no work (and is not reported); rows of out that belong to no group are not
  * written. The products are of 16 + q, less (16 + zero) times the sum of x, exact but for the float32 sums:
- * an infinity in x, or a value past 10^36, makes its row's outputs NaN or infinite.
+ * an infinity in x makes its row's outputs NaN or infinite, and so may finite values of which 62 times the sum
+ * of |x| over the `group` k of a scale reaches 3.4e38 (4.3e34 in each of 128).
  *
  * Storage: n in tiles of 16 and k in tiles of 128, padded with zeros:
  *   packed [group_num][ceil(n / 16)][ceil(k / 128)][64][16] bytes: piece 16 a + r of a tile is row r,

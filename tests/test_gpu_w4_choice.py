@@ -1,5 +1,5 @@
-"""The 4-bit products at the sizes that choose a kernel, and in workgroups that take more than one piece of
-rows. Bounds as in test_gpu_w4.py."""
+"""The 4-bit products at the sizes that choose a kernel, in workgroups that take more than one piece of rows, and with
+values near the end of the stated range. Bounds as in test_gpu_w4.py."""
 import pytest
 import torch
 
@@ -68,3 +68,23 @@ def test_workgroups_that_come_back(pkg, dtype, zeros, group, k, kernel, b, m, n)
     pkg.grouped_gemm_w4(x, w4, torch.tensor(lens, device=DEV), out=out, group_offs=torch.tensor(offs + [0], device=DEV))
     written = _check(out, x, w, size, offs, [length if ok else 0 for length, ok in zip(lens, good)], dtype, k)
     assert bool((out[~written] == 9).all()) and int(written.sum()) == sum(length for length, ok in zip(lens, good) if ok)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("signs", ["one", "both"])
+@pytest.mark.parametrize("b,m,n", [(2, 3, 64), (32, 1024, 904)])
+def test_values_up_to_the_stated_limit(pkg, zeros, signs, b, m, n):
+    """62 times the sum of |x| over a scale's k just below 3.4e38: the sums on the way stay finite."""
+    k, group, dtype = 256, 128, torch.bfloat16
+    q, s, z = _weights(b, n, k, group, dtype, zeros, 5)
+    w4 = pkg.pack_w4(q, s, z)
+    w, size = _dense(q, s, z, group)
+    x = torch.full((m, k), 4.2e34, device=DEV)
+    if signs == "both":
+        x = torch.where(torch.rand(m, k, device=DEV, generator=_gen(3)) < 0.5, x, -x)
+    x = x.to(dtype)
+    assert float(x.double().abs().view(m, k // group, group).sum(2).max()) * 62 < 3.4e38
+    lens = [m // b + (g < m % b) for g in range(b)]
+    got = pkg.grouped_gemm_w4(x, w4, lens)
+    assert bool(got.isfinite().all())
+    assert bool(_check(got, x, w, size, [sum(lens[:g]) for g in range(b)], lens, dtype, k).all())
