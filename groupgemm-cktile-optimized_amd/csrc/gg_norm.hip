@@ -501,17 +501,17 @@ template <typename T, bool WIDE> int run_norm(const NormArgs &a, hipStream_t s) 
             return launch("rms_norm", norm_kernel<T, wpr.value, u.value, false>, std::min(blocks, kMaxBlocks),
                           block_threads(wpr.value), s, a);
         });
-    // The first pass: as many workgroups as fit at once, each with its share of the rows (32768 rows of 7168: 1280
-    // workgroups 405 us for both passes, 1024 439, 2048, 1.6 rounds of them, 465).
+    // The first pass: as many workgroups as fit at once, each with its share of the rows (32768 rows of 7168: 1792
+    // workgroups fit, 377 us for both passes; 1536 377, 1280 389, 1024 421, 2048, 1.1 rounds of them, 453).
     NormArgs b = a;
     if (b.residual == nullptr) { // h is x
         b.h        = const_cast<void *>(b.x);
         b.h_stride = b.x_stride;
     }
     const int st = with_shape<WIDE>(a.hidden, [&](auto wpr, auto u) {
-        constexpr auto   kernel = norm_kernel<T, wpr.value, u.value, true>;
-        static const int fit    = resident_blocks(kernel, block_threads(wpr.value));
-        b.n_parts               = static_cast<int>(std::min<int64_t>(blocks, std::min(fit, kMaxParts)));
+        constexpr auto kernel = norm_kernel<T, wpr.value, u.value, true>;
+        // (asked for each call, as devices differ; few workgroups fit in any case)
+        b.n_parts = static_cast<int>(blocks <= 256 ? blocks : std::min<int64_t>(blocks, std::min(resident_blocks(kernel, block_threads(wpr.value)), kMaxParts)));
         return launch("rms_norm", kernel, b.n_parts, block_threads(wpr.value), s, b);
     });
     constexpr int kThreads = WIDE ? 1024 : 256;

@@ -56,3 +56,15 @@ def test_4_bit_sizes_reach_the_kernels_they_are_for(tmp_path):
                     os.path.join(ROOT, "tests", "w4_choice.cpp"), "-o", str(exe)], check=True)
     r = subprocess.run([str(exe)] + [str(v) for c in cases for v in c[1:]], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0 and r.stdout.split() == [c[0] for c in cases]
+
+
+@pytest.mark.skipif(shutil.which("nm") is None, reason="needs nm")
+def test_the_library_keeps_nothing_of_a_call(pkg):
+    """No variable of the layer operators outlives a call but the thread's last message: what one device's call found
+    would else be used on another."""
+    r = subprocess.run(["nm", "-C", pkg.LIB_PATH], capture_output=True, text=True, timeout=120)
+    names = [line for line in r.stdout.splitlines() if "gg::layer::" in line]
+    assert r.returncode == 0 and any("g_error" in n for n in names)
+    # data and its guards (local, initialized, unique or weak), but for the kernels' handles, which have parameters
+    kept = [n for n in names if n.split(maxsplit=2)[1] in "bBdDuvV" and not n.endswith(")") and "g_error" not in n]
+    assert not kept, kept[:3]
