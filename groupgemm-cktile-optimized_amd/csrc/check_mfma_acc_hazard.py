@@ -14,10 +14,13 @@ every branch in it (two passes, so that loop back edges are followed too). It fa
 comes with fewer than 19 wait states. Exit status 1 with the offending lines.
 
 It also fails when a basic block with at least LOOP_MFMAS MFMAs (the unrolled K loop of six
-steps) holds v_readlane_b32 / v_writelane_b32: SGPR spill traffic inside the K loop.
+steps) holds v_readlane_b32 / v_writelane_b32: SGPR spill traffic inside the K loop. Kernels whose
+K loop is shorter name its MFMAs with --loop, and with --allow the lane operations that a block of
+them may hold.
 
-Usage: check_mfma_acc_hazard.py FILE.s [...]
+Usage: check_mfma_acc_hazard.py [--loop MFMAS] [--allow OPS] FILE.s [...]
 """
+import argparse
 import re
 import sys
 
@@ -92,7 +95,7 @@ def run_block(instrs, pending, where, bad):
     return pending, edges
 
 
-def scan_function(name, lines, bad, spills):
+def scan_function(name, lines, bad, spills, loop, allow):
     blocks = split_blocks(lines)
     entry = {}
     for _ in range(2):  # the second pass sees the pending MFMAs of back edges
@@ -105,24 +108,29 @@ def scan_function(name, lines, bad, spills):
     for label, instrs in blocks:
         mfmas = sum(1 for t in instrs if t.startswith("v_mfma"))
         lanes = [t for t in instrs if t.startswith(("v_readlane_b32", "v_writelane_b32"))]
-        if mfmas >= LOOP_MFMAS and lanes:
+        if mfmas >= loop and len(lanes) > allow:
             spills.append(f"{name[:80]} {label}: {len(lanes)} SGPR spill lane operations in a block of "
                           f"{mfmas} MFMAs, e.g. '{lanes[0]}'")
 
 
-def scan_text(text):
+def scan_text(text, loop=LOOP_MFMAS, allow=0):
     """(early accumulator reads, spill operations in K-loop blocks) of an assembly file's text."""
     bad, spills = set(), []
     for km in re.finditer(r"\n(_Z\w+):", text):
         end = text.find(".Lfunc_end", km.end())
-        scan_function(km.group(1), text[km.end():end].split("\n"), bad, spills)
+        scan_function(km.group(1), text[km.end():end].split("\n"), bad, spills, loop, allow)
     return sorted(bad), spills
 
 
 def main():
+    ap = argparse.ArgumentParser()
+    ap.add_argument("--loop", type=int, default=LOOP_MFMAS)
+    ap.add_argument("--allow", type=int, default=0)
+    ap.add_argument("files", nargs="+")
+    args = ap.parse_args()
     bad, spills = [], []
-    for path in sys.argv[1:]:
-        b, s = scan_text(open(path).read())
+    for path in args.files:
+        b, s = scan_text(open(path).read(), args.loop, args.allow)
         bad += [f"{path}: {x}" for x in b]
         spills += [f"{path}: {x}" for x in s]
     for b in (bad + spills)[:20]:
@@ -131,8 +139,8 @@ def main():
         print(f"check_mfma_acc_hazard: {len(bad)} accumulator reads too close to their MFMA, "
               f"{len(spills)} K-loop blocks with SGPR spill traffic")
         sys.exit(1)
-    print(f"check_mfma_acc_hazard: {' '.join(sys.argv[1:])}: no early accumulator reads, no spill "
-          f"traffic in the K loop")
+    print(f"check_mfma_acc_hazard: {' '.join(args.files)}: no early accumulator reads, "
+          f"{'no' if args.allow == 0 else f'at most {args.allow} lane operations of'} spill traffic in the K loop")
 
 
 if __name__ == "__main__":

@@ -1,6 +1,8 @@
 """The layer operators at the edges of their arguments, without a GPU."""
 import importlib
+import importlib.util
 import os
+import re
 import shutil
 import subprocess
 
@@ -68,3 +70,42 @@ def test_the_library_keeps_nothing_of_a_call(pkg):
     # data and its guards (local, initialized, unique or weak), but for the kernels' handles, which have parameters
     kept = [n for n in names if n.split(maxsplit=2)[1] in "bBdDuvV" and not n.endswith(")") and "g_error" not in n]
     assert not kept, kept[:3]
+
+
+def _spill_check():
+    spec = importlib.util.spec_from_file_location("acc", os.path.join(ROOT, "groupgemm-cktile-optimized_amd", "csrc",
+                                                                      "check_mfma_acc_hazard.py"))
+    acc = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(acc)
+    return acc
+
+
+def test_spill_check_of_short_loops():
+    """The check sees a K loop of few MFMAs where it is told of it, and allows no more lane operations than told."""
+    acc = _spill_check()
+    mfma = "    v_mfma_f32_16x16x32_bf16 a[0:3], v[0:3], v[8:11], a[0:3]\n"
+    lane = "    v_readlane_b32 s4, v185, 12\n"
+
+    def spills(lanes, mfmas, **options):
+        return acc.scan_text("\n_Zk:\n.LBB0_3:\n" + lane * lanes + mfma * mfmas + "\n.Lfunc_end0:\n", **options)[1]
+
+    assert not spills(1, 20) and spills(1, 20, loop=8) and not spills(1, 7, loop=8)
+    assert not spills(4, 20, loop=8, allow=4) and spills(5, 20, loop=8, allow=4)
+
+
+def test_layer_kernels_spill_no_vector_registers():
+    """The compiler's report of every kernel of the layer operators: no vector register spilled, no scratch."""
+    path = os.path.join(ROOT, "groupgemm-cktile-optimized_amd", "lib", "resource_usage.txt")
+    if not os.path.exists(path):
+        pytest.skip("library not built")
+    seen, bad, name = 0, [], None
+    with open(path, errors="replace") as f:
+        for line in f:
+            m = re.search(r"Function Name: (\S+)", line)
+            if m:
+                name = m.group(1) if "2gg5layer" in m.group(1) else None
+                seen += name is not None
+            m = re.search(r"\s(VGPRs Spill|ScratchSize \[bytes/lane\]): (\d+)", line)
+            if m and name and int(m.group(2)) != 0:
+                bad.append((name, m.group(1), int(m.group(2))))
+    assert seen >= 200 and not bad, (seen, bad)
