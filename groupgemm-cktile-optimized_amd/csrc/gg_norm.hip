@@ -10,8 +10,8 @@
 // The norm is taken of the rounded h, the value that later layers and the backward pass read, so the
 // passes agree whatever the scale.
 //
-// Measured: 32768 rows of 7168, bf16 with residual to fp8 with a tensor scale, 377 us: 248 for the first pass (x and r
-// read, h written: 5.7 TB/s) and 130 for the second (h read, y written: 5.4); 5 rows to bf16 3.9, the latency of a launch,
+// Measured: 32768 rows of 7168, bf16 with residual to fp8 with a tensor scale, 377 us: 245 for the first pass (x and r
+// read, h written: 5.8 TB/s) and 133 for the second (h read, y written: 5.3); 5 rows to bf16 3.8, the latency of a launch,
 // a row's loads and a barrier. Backward 16640 x 2880 with a gradient past the norm: 75 us, 5.1 TB/s (69 row by row, 6 for
 // the weight's gradient).
 #include "gg_layer.h"
@@ -518,8 +518,9 @@ template <typename T, bool WIDE> int run_norm(const NormArgs &a, hipStream_t s) 
     return st ? st : launch("rms_norm", quantize_kernel<T, kThreads>, std::min<int64_t>(b.rows, 8192), kThreads, s, b);
 }
 
-// Workgroups of the backward pass: at most those that the GPU holds at once (by the instances' registers, 72 to 224),
-// fewer where each would have less than four rows and their partial sums would cost more than they save. us at 1, 2
+// Workgroups of the backward pass: at most those that 256 CUs hold at once (by the instances' registers, 68 to 224: numbers
+// that a test holds to the compiler's report, as the size of the workspace is asked for without a device or a type; 1024
+// to two pieces and one wave a row, where 1280 fit), fewer where each would have less than four rows and their partial sums would cost more than they save. us at 1, 2
 // and 4 rows each, of 7168: 512 rows 19.9, 18.6, 21.6; 2048 46.8, 37.9, 34.2. At once against 1024:
 // 16640 rows of 2880 73.7 (1536) and 77.6, 4096 of 14336 108.5 (512) and 118.6.
 int64_t back_blocks(int64_t rows, int64_t hidden) {

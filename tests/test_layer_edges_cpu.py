@@ -109,3 +109,28 @@ def test_layer_kernels_spill_no_vector_registers():
             if m and name and int(m.group(2)) != 0:
                 bad.append((name, m.group(1), int(m.group(2))))
     assert seen >= 200 and not bad, (seen, bad)
+
+
+def test_backward_workgroups_fit_the_gpu(pkg):
+    """The RMS norm's gradient takes no more workgroups than 256 CUs hold at once, by the compiler's report of each
+    instance's waves for each of a CU's four SIMDs: the numbers are written down, as the workspace's size needs them."""
+    path = os.path.join(ROOT, "groupgemm-cktile-optimized_amd", "lib", "resource_usage.txt")
+    if not os.path.exists(path):
+        pytest.skip("library not built")
+    waves, name = {}, None
+    with open(path, errors="replace") as f:
+        for line in f:
+            m = re.search(r"Function Name: (\S+)", line)
+            if m:  # <type, waves of a row, pieces, with the sums>
+                name = re.search(r"norm_back_kernelINS0_\w+?ELi(\d+)ELi(\d+)ELb1E", m.group(1))
+            m = re.search(r"Occupancy \[waves/SIMD\]: (\d+)", line)
+            if m and name:
+                key = int(name.group(1)), int(name.group(2))
+                waves[key] = min(waves.get(key, 8), int(m.group(1)))
+    assert len(waves) >= 9
+    for hidden in (8, 512, 520, 1024, 1032, 2048, 2056, 4096, 4104, 6144, 6152, 8192, 8200, 12288, 12296, 16384, 16392, 32768):
+        wpr = 1 if hidden <= 1024 else 4 if hidden <= 16384 else 16
+        pieces = min(p for w, p in waves if w == wpr and p * 512 * w >= hidden)
+        of_block = 16 if wpr == 16 else 4
+        blocks = pkg.load_library().gg_rms_norm_backward_workspace(1 << 20, hidden) // (4 * hidden)
+        assert 256 <= blocks <= 256 * (waves[wpr, pieces] * 4 // of_block), (hidden, blocks, waves[wpr, pieces])
