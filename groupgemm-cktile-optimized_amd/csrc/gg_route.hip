@@ -126,7 +126,8 @@ __device__ __forceinline__ float value_of(unsigned k) {
     return __uint_as_float(k ^ (static_cast<int>(k) < 0 ? 0x80000000u : 0xffffffffu)); // NaN: 0x7fffffff, a NaN
 }
 
-// exp(x) for x <= 0: the product's rounding makes it off by |x| 2^-24 at most, v_exp_f32 by one unit.
+// exp(x) for x <= 0: the roundings of the product and of the constant make it off by 1.23 |x| 2^-24 at most, v_exp_f32 by
+// one unit.
 __device__ __forceinline__ float exp_neg(float x) { return __builtin_amdgcn_exp2f(x * 1.44269504f); }
 
 // Compare-exchanges of a sorting network for N = 4, 8 or 16 values (odd-even merges).

@@ -283,7 +283,8 @@ __device__ __forceinline__ void scale_sums(f32x4 (&acc)[MT][NT], f32x4 (&sum)[MT
 // Grid: workgroup (piece of 16 rows, block of 16 NT columns), G k of one scale. The W waves share out the 128-column tiles;
 // each loads weights, scales and x one tile ahead, into two sets of registers in turn. x comes through a buffer resource
 // that ends at the last row, so rows past it read as zeros and cost no traffic. Three workgroups a CU: 168 registers, which
-// the compiler passes into accumulation registers, with moves, unless it is told. 16 groups of 8 rows of 4096 x 4096 (k of
+// the compiler passes into accumulation registers, with moves, unless it is told; of the scalar registers the instances with
+// zero points reload four a tile from lanes. 16 groups of 8 rows of 4096 x 4096 (k of
 // a scale 128): 32.2 us, 4.3 TB/s of packed weights and scales; 32 of 8 rows of 2880 x 2880 (32, zero points) 42.7, 3.7 TB/s.
 // Long k comes nearer to the memory's 5.3 TB/s (32 of 8 rows, 2880 x 5632: 55.0 us, 4.9): a call spends 6 to 8 us on the
 // launch, the search for its rows, the first loads and the sum over the waves.

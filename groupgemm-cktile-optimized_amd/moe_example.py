@@ -96,7 +96,9 @@ class MoeLayer:
         return g
 
     def forward_fp8(self, x, residual):
-        """The forward pass with the gate and up products in e4m3: the norm gives their input and its scale."""
+        """The forward pass with the gate and up products in e4m3: the norm gives their input and its scale. The router reads
+        the rounded values, too, so tokens whose experts are close may choose others than in forward; and grouped_gemm_fp8
+        takes host sizes, so this pass waits for the counts."""
         y8, h, _, scale = rms_norm(x, self.norm, residual, out_dtype=torch.float8_e4m3fn)
         r = route((y8.float() * scale) @ self.router.float().t(), self.top_k)
         gu = grouped_gemm_fp8(dispatch(y8, r), self.gate_up8, r.counts.tolist(), scale, self.gate_up_scale)

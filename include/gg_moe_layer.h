@@ -39,6 +39,7 @@ typedef enum gg_norm_scale {
 /*
  * h = x + residual, rounded to x's type as the layers after this one read it (h = x without a
  * residual); rstd = 1 / sqrt(mean(h^2) + eps) of each row; y = h * rstd * weight, of the rounded h.
+ * (A row whose squares add up past 3.4e38, which values of some 10^17 and more can, has an rstd of 0.)
  * fp8: y = round(h * rstd * weight / scale), scale = max |h * rstd * weight| / (the format's largest
  * value), 1 where that is zero or subnormal. A NaN in a row makes its rstd, y and (for a tensor scale, every) scale NaN.
  *   dtype: GG_DTYPE_BF16 or GG_DTYPE_FP16 (x, residual, h; y unless fp8). weight_dtype: the same or
