@@ -95,6 +95,19 @@ C_API = {
                                             ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
                                             ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t,
                                             ctypes.c_void_p]),
+    "gg_layer_norm": (ctypes.c_int, [ctypes.c_int] * 4 + [ctypes.c_int64] * 2 + [ctypes.c_float, ctypes.c_void_p, ctypes.c_int64,
+                                     ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                     ctypes.c_int64] + [ctypes.c_void_p] * 6),
+    "gg_layer_norm_backward_workspace": (ctypes.c_size_t, [ctypes.c_int64] * 2),
+    "gg_layer_norm_backward": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_int64,
+                                              ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 4
+                               + [ctypes.c_int64] + [ctypes.c_void_p] * 4 + [ctypes.c_size_t, ctypes.c_void_p]),
+    "gg_silu_product": (ctypes.c_int, [ctypes.c_int] * 2 + [ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_int64]
+                        + [ctypes.c_void_p] * 3),
+    "gg_silu_product_backward": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_int64,
+                                                ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_void_p]),
+    "gg_quantize_rows": (ctypes.c_int, [ctypes.c_int] + [ctypes.c_int64] * 2 + [ctypes.c_void_p, ctypes.c_int64]
+                         + [ctypes.c_void_p] * 3),
     "gg_route_workspace": (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int, ctypes.c_int]),
     "gg_route": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                 ctypes.c_int64] + [ctypes.c_void_p] * 10 + [ctypes.c_size_t, ctypes.c_void_p]),
@@ -814,8 +827,9 @@ def grouped_gemm(x, w, group_m, out=None, stream: Optional[int] = None, group_of
 
 # The operators around the grouped GEMM in a mixture-of-experts layer (moe_layer.py). Loaded on first use: that
 # module imports torch, which a process that times the hipBLASLt baselines must not.
-_LAYER = ("NormOutput", "Routing", "W4Weights", "combine", "combine_backward", "dispatch", "dispatch_backward",
-          "grouped_gemm_w4", "pack_w4", "quantize_w4", "rms_norm", "rms_norm_backward", "route", "route_backward")
+_LAYER = ("LayerNormOutput", "NormOutput", "Routing", "ScaledRows", "W4Weights", "combine", "combine_backward", "dispatch",
+          "dispatch_backward", "grouped_gemm_w4", "layer_norm", "layer_norm_backward", "pack_w4", "quantize_rows", "quantize_w4",
+          "rms_norm", "rms_norm_backward", "route", "route_backward", "silu_product", "silu_product_backward")
 
 
 def __getattr__(name):

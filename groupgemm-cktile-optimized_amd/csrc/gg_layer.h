@@ -1,4 +1,4 @@
-// Shared pieces of the layer operators (gg_norm.hip, gg_route.hip, gg_rows.hip, gg_w4.hip): the
+// Shared pieces of the layer operators (gg_norm.hip, gg_act.hip, gg_route.hip, gg_rows.hip, gg_w4.hip): the
 // message of the last failed call, argument checks, 16-byte vectors of 16-bit values as float32 and
 // reductions over the lanes of a wave.
 #pragma once

@@ -1,7 +1,8 @@
-// RMS norm with the residual's addition, 16-bit or fp8 output, and its gradients (gg_rms_norm,
-// gg_rms_norm_backward in include/gg_moe_layer.h).
+// RMS norm and layer norm with the residual's addition, 16-bit, fp8 or int8 output, and their gradients (gg_rms_norm,
+// gg_layer_norm, .. in include/gg_moe_layer.h).
 //
-// Forward: h = round(x + r), rstd = (mean h^2 + eps)^-1/2, y = h rstd w. A row stays in the registers
+// Forward: h = round(x + r), rstd = (mean h^2 + eps)^-1/2, y = h rstd w; layer norm (CENTER) takes h less its mean, in
+// the mean square too, and adds a bias. A row stays in the registers
 // of the waves that work on it (one wave up to 1024 values, four up to 16384, of few rows up to 2048, else sixteen), so
 // x and r are read once and h and y written once: bound by HBM. The tensor scale needs the largest |y|
 // of all rows before the first value is rounded: a first pass writes h, rstd and one maximum per
@@ -14,7 +15,7 @@
 // read, h written: 5.8 TB/s) and 133 for the second (h read, y written: 5.3); 5 rows to bf16 3.8, the latency of a launch,
 // a row's loads and a barrier. Backward 16640 x 2880 with a gradient past the norm: 75 us, 5.1 TB/s (69 row by row, 6 for
 // the weight's gradient).
-#include "gg_layer.h"
+#include "gg_row.h"
 
 #include <algorithm>
 
@@ -28,122 +29,37 @@ namespace {
 constexpr int kMaxParts = GG_NORM_WORKSPACE / 4; // workgroups of a tensor scale's first pass
 
 struct NormArgs {
-    const void *x, *residual, *weight;
+    const void *x, *residual, *weight, *bias; // bias (layer norm only) may be null
     void       *h, *y;
-    float      *rstd, *scale, *parts;
+    float      *mean, *rstd, *scale, *parts; // mean: layer norm only
     int64_t     rows, x_stride, r_stride, h_stride;
     int         hidden, mode, n_parts;
     float       eps;
     bool        w32, e5m2;
 };
 
-// Eight weights from element i on, as float32.
-template <typename T> __device__ __forceinline__ void load_w(const void *w, bool w32, int i, float (&v)[8]) {
-    if (w32) {
-        const f32x4 *p = reinterpret_cast<const f32x4 *>(static_cast<const float *>(w) + i);
-        const f32x4  a = p[0], b = p[1];
+// y of eight values from element i on: v holds h (CENTER: less its mean) and then y.
+template <typename T, bool CENTER>
+__device__ __forceinline__ void scale_shift(const NormArgs &a, int i, float rstd, float (&v)[8]) {
+    float w[8], b[8];
+    load_w<T>(a.weight, a.w32, i, w);
+    if (CENTER && a.bias != nullptr) {
+        load_w<T>(a.bias, a.w32, i, b);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j]     = a[j];
-            v[4 + j] = b[j];
-        }
-    } else {
-        unpack8<T>(*reinterpret_cast<const u32x4 *>(static_cast<const uint16_t *>(w) + i), v);
-    }
-}
-
-// Saturates (the conversion would give NaN past the largest value); a NaN stays one.
-__device__ __forceinline__ float saturate(float v, float top) { return v != v ? v : fminf(fmaxf(v, -top), top); }
-
-// Division by a scale, rounded as a float32 division is: the product with the rounded reciprocal, corrected once by its
-// remainder, which a fused multiply-add gives exactly (Markstein 1990). By the product alone one in sixty of the values
-// within two float32 units of a tie of the format went to the neighbouring code. The product is clamped first, far past
-// either format's range, so that the remainder stays finite; a NaN comes back with the remainder. Outside 2^-64 .. 2^64
-// the remainder could be subnormal, and `exact` divides.
-struct Divisor {
-    float s, inv;
-    bool  exact;
-    __device__ __forceinline__ explicit Divisor(float scale)
-        : s(scale), inv(1.f / scale), exact(!(fabsf(scale) >= 0x1p-64f && fabsf(scale) <= 0x1p64f)) {}
-    __device__ __forceinline__ float quotient(float v) const {
-        const float q = __builtin_amdgcn_fmed3f(v * inv, -131072.f, 131072.f);
-        return fmaf(-fmaf(q, s, -v), inv, q); // (in this order of signs a zero keeps its own)
-    }
-};
-
-// Eight values divided by the scale, as fp8.
-__device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], const Divisor &d, bool e5m2) {
-    u32x2 w;
-    const float top = e5m2 ? 57344.f : 448.f;
-    float s[8];
-    if (d.exact) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            s[i] = saturate(v[i] / d.s, top);
+        for (int j = 0; j < 8; ++j)
+            v[j] = fmaf(v[j] * rstd, w[j], b[j]);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            s[i] = saturate(d.quotient(v[i]), top);
+        for (int j = 0; j < 8; ++j)
+            v[j] = v[j] * rstd * w[j];
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        int q = 0;
-        if (e5m2) {
-            q = __builtin_amdgcn_cvt_pk_bf8_f32(s[4 * i], s[4 * i + 1], q, false);
-            q = __builtin_amdgcn_cvt_pk_bf8_f32(s[4 * i + 2], s[4 * i + 3], q, true);
-        } else {
-            q = __builtin_amdgcn_cvt_pk_fp8_f32(s[4 * i], s[4 * i + 1], q, false);
-            q = __builtin_amdgcn_cvt_pk_fp8_f32(s[4 * i + 2], s[4 * i + 3], q, true);
-        }
-        w[i] = static_cast<unsigned>(q);
-    }
-    return w;
 }
 
-// Scale of the largest |y| (bits of a float >= 0 or NaN): 1 where the quotient is zero or subnormal, which a division
-// by it could turn into NaN or a value of few bits.
-__device__ __forceinline__ float scale_of(unsigned top_bits, bool e5m2) {
-    const float s = __uint_as_float(top_bits) / (e5m2 ? 57344.f : 448.f);
-    return s < 1.17549435e-38f ? 1.f : s;
-}
-
-// Reductions over the WPR waves of a row; `turn` alternates so that one barrier per call is enough.
-template <int WPR> struct RowReduce {
-    float    sums[2][WPR];
-    unsigned tops[2][WPR];
-};
-template <int WPR> __device__ __forceinline__ float row_sum(RowReduce<WPR> &m, int turn, float v, int wave, int lane) {
-    v = wave_sum(v);
-    if constexpr (WPR == 1)
-        return v;
-    if (lane == 0)
-        m.sums[turn][wave] = v;
-    __syncthreads();
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < WPR; ++i)
-        s += m.sums[turn][i];
-    return s;
-}
-template <int WPR> __device__ __forceinline__ unsigned row_max(RowReduce<WPR> &m, int turn, unsigned v, int wave, int lane) {
-    v = wave_max(v);
-    if constexpr (WPR == 1)
-        return v;
-    if (lane == 0)
-        m.tops[turn][wave] = v;
-    __syncthreads();
-    unsigned s = 0;
-#pragma unroll
-    for (int i = 0; i < WPR; ++i)
-        s = max(s, m.tops[turn][i]);
-    return s;
-}
-
-constexpr int block_threads(int wpr) { return wpr == 1 ? 256 : 64 * wpr; }
-constexpr int rows_per_block(int wpr) { return wpr == 1 ? 4 : 1; }
-
-// One pass over the rows. FIRST: the first pass of a tensor scale (no y; the workgroup's largest |y|).
-template <typename T, int WPR, int U, bool FIRST>
+// One pass over the rows: the whole norm in 16 bits or fp8, in int8 with a scale for each row (instances of its own: the
+// rounding's registers would cost the others a wave per SIMD), or the first pass of a tensor scale (no y; the workgroup's
+// largest |y|).
+enum Pass : int { kWhole = 0, kInt8 = 1, kFirst = 2 };
+template <typename T, bool CENTER, int WPR, int U, int PASS>
 __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs a) {
     __shared__ RowReduce<WPR> m;
     __shared__ unsigned       block_top[4];
@@ -156,7 +72,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0); row < a.rows;
          row += step, turn ^= 1) {
         float v[U][8];
-        float sq = 0.f;
+        float sq = 0.f; // CENTER: the plain sum first
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
@@ -178,8 +94,24 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    sq = fmaf(v[u][j], v[u][j], sq);
+                    sq = CENTER ? sq + v[u][j] : fmaf(v[u][j], v[u][j], sq);
             }
+        }
+        if constexpr (CENTER) {
+            // the row is in registers: its squares are summed about the mean, where nothing cancels
+            const float mean = row_sum<WPR>(m, turn, sq, wave, lane) / static_cast<float>(a.hidden);
+            if (t == 0 && a.mean != nullptr)
+                a.mean[row] = mean;
+            turn ^= 1;
+            sq = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if ((u * 64 * WPR + t) * 8 < a.hidden)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        v[u][j] -= mean;
+                        sq = fmaf(v[u][j], v[u][j], sq);
+                    }
         }
         sq = row_sum<WPR>(m, turn, sq, wave, lane);
         const float rstd = 1.f / sqrtf(sq / static_cast<float>(a.hidden) + a.eps);
@@ -190,21 +122,18 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
             if (i < a.hidden) {
-                float w[8];
-                load_w<T>(a.weight, a.w32, i, w);
+                scale_shift<T, CENTER>(a, i, rstd, v[u]);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    v[u][j] = v[u][j] * rstd * w[j];
+                for (int j = 0; j < 8; ++j)
                     row_top = max(row_top, __float_as_uint(fabsf(v[u][j])));
-                }
             }
         }
-        if constexpr (FIRST) {
+        if constexpr (PASS == kFirst) {
             top = max(top, row_top);
         } else {
             float s = 1.f;
-            if (a.mode == GG_NORM_SCALE_ROW) {
-                s = scale_of(row_max<WPR>(m, turn, row_top, wave, lane), a.e5m2);
+            if (PASS == kInt8 || a.mode == GG_NORM_SCALE_ROW) {
+                s = scale_of(row_max<WPR>(m, turn, row_top, wave, lane), PASS == kInt8 ? kTopI8 : a.e5m2 ? kTopE5M2 : kTopE4M3);
                 if (t == 0)
                     a.scale[row] = s;
             } else if (a.mode == GG_NORM_SCALE_GIVEN) {
@@ -215,7 +144,9 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
             for (int u = 0; u < U; ++u) {
                 const int i = (u * 64 * WPR + t) * 8;
                 if (i < a.hidden) {
-                    if (a.mode == GG_NORM_PLAIN) {
+                    if constexpr (PASS == kInt8) {
+                        *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_i8(v[u], by);
+                    } else if (a.mode == GG_NORM_PLAIN) {
                         *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.y) + row * a.hidden + i) = pack8<T>(v[u]);
                     } else {
                         *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v[u], by, a.e5m2);
@@ -224,7 +155,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
             }
         }
     }
-    if constexpr (FIRST) {
+    if constexpr (PASS == kFirst) {
         top = wave_max(top);
         constexpr int waves = block_threads(WPR) / 64;
         static_assert(waves <= 16, "");
@@ -247,7 +178,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
 }
 
 // The tensor scale's second pass: the largest of the first pass's maxima, then y from h and rstd.
-template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) quantize_kernel(const NormArgs a) {
+template <typename T, bool CENTER, int THREADS> __global__ void __launch_bounds__(THREADS) quantize_kernel(const NormArgs a) {
     __shared__ unsigned tops[THREADS / 64];
     unsigned            top = 0;
     for (int i = threadIdx.x; i < a.n_parts; i += THREADS)
@@ -259,20 +190,21 @@ template <typename T, int THREADS> __global__ void __launch_bounds__(THREADS) qu
 #pragma unroll
     for (int i = 0; i < THREADS / 64; ++i)
         top = max(top, tops[i]);
-    const float   s = scale_of(top, a.e5m2);
+    const float   s = scale_of(top, a.e5m2 ? kTopE5M2 : kTopE4M3);
     const Divisor by(s);
     if (blockIdx.x == 0 && threadIdx.x == 0)
         a.scale[0] = s;
     // from the last row backwards: the rows written last are still in the Infinity Cache
     for (int64_t row = a.rows - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
-        const float rstd = a.rstd[row];
+        const float rstd = a.rstd[row], mean = CENTER ? a.mean[row] : 0.f;
         for (int i = threadIdx.x * 8; i < a.hidden; i += THREADS * 8) {
-            float v[8], w[8];
+            float v[8];
             unpack8<T>(load_once(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i), v);
-            load_w<T>(a.weight, a.w32, i, w);
+            if constexpr (CENTER)
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                v[j] = v[j] * rstd * w[j];
+                for (int j = 0; j < 8; ++j)
+                    v[j] -= mean;
+            scale_shift<T, CENTER>(a, i, rstd, v);
             *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v, by, a.e5m2);
         }
     }
@@ -435,17 +367,18 @@ template <typename T> __global__ void __launch_bounds__(1024) weight_strip_kerne
     }
 }
 
-// grad_weight: the sum of the partial sums of each column, in a fixed order; 32 columns by 128 slices of the parts a
-// workgroup.
+// grad_weight, and grad_bias where parts hold `width` = 2 * hidden columns: the sum of the partial sums of each column, in
+// a fixed order; 32 columns by 128 slices of the parts a workgroup.
 template <typename T>
-__global__ void __launch_bounds__(1024) weight_sum_kernel(const float *parts, int n_parts, int hidden, void *out, bool w32) {
+__global__ void __launch_bounds__(1024) weight_sum_kernel(const float *parts, int n_parts, int width, int hidden, void *grad_weight,
+                                                          void *grad_bias, bool w32) {
     __shared__ f32x4 sums[128][8];
     const int c4 = threadIdx.x & 7, slice = threadIdx.x >> 3, col = blockIdx.x * 32 + c4 * 4; // hidden % 8 == 0
     f32x4     s{0.f, 0.f, 0.f, 0.f};
-    if (col < hidden)
+    if (col < width)
 #pragma unroll 8
         for (int p = slice; p < n_parts; p += 128)
-            s += *reinterpret_cast<const f32x4 *>(parts + static_cast<int64_t>(p) * hidden + col);
+            s += *reinterpret_cast<const f32x4 *>(parts + static_cast<int64_t>(p) * width + col);
     sums[slice][c4] = s;
     __syncthreads();
 #pragma unroll
@@ -454,52 +387,235 @@ __global__ void __launch_bounds__(1024) weight_sum_kernel(const float *parts, in
             sums[slice][c4] = s += sums[slice + half][c4];
         __syncthreads();
     }
-    if (slice == 0 && col < hidden) {
+    if (slice == 0 && col < width) {
+        void     *out = col < hidden ? grad_weight : grad_bias;
+        const int at  = col < hidden ? col : col - hidden;
         if (w32)
-            *reinterpret_cast<f32x4 *>(static_cast<float *>(out) + col) = s;
+            *reinterpret_cast<f32x4 *>(static_cast<float *>(out) + at) = s;
         else
-            *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + col) = u32x2{T::word(s[0], s[1]), T::word(s[2], s[3])};
+            *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(out) + at) = u32x2{T::word(s[0], s[1]), T::word(s[2], s[3])};
     }
 }
 
-// Few rows: a row's latency counts, and not how many are in flight. Then (WIDE) sixteen waves take a row of more than 2048
-// values, and grad_weight is summed from g and h again, which are in the caches, instead of from partial sums, which would be
-// as many bytes as the rows. us, sixteen waves and four: norm of 5 rows of 7168 3.9, 5.1, of 256 5.5, 7.3, 512 8.4, 10.8, 1024
-// 14.5, 14.8; of 512 rows of 4096 5.7, 5.6, 1024 10.8, 9.5; 256 of 14336 8.5, 14.0. Backward, with the sums and without:
-// 64 of 7168 7.1, 9.1, 481 of 13456 22.2, 34.3, 512 of 7168 16.6, 18.1, 512 of 4096 13.9, 12.4, 1024 of 8192 27.6, 27.4.
-bool few(int64_t rows, int64_t hidden) { return hidden > 1024 && rows <= (hidden > 5120 ? 512 : 256); }
+// ---- layer norm's gradients ----
 
-template <bool WIDE> int waves_per_row(int64_t hidden) {
-    return hidden <= 1024 ? 1 : hidden <= (WIDE ? 2048 : 16384) ? 4 : 16;
+struct CenterArgs {
+    BackArgs     b; // parts: [workgroups][2][hidden], grad_weight's and grad_bias's
+    const float *mean;
+};
+
+// The two sums of a row over its waves, with one barrier.
+template <int WPR> struct PairReduce {
+    float sums[2][2][WPR];
+};
+template <int WPR>
+__device__ __forceinline__ void row_sums(PairReduce<WPR> &m, int turn, float &p, float &q, int wave, int lane) {
+    p = wave_sum(p);
+    q = wave_sum(q);
+    if constexpr (WPR > 1) {
+        if (lane == 0) {
+            m.sums[turn][0][wave] = p;
+            m.sums[turn][1][wave] = q;
+        }
+        __syncthreads();
+        p = q = 0.f;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) {
+            p += m.sums[turn][0][i];
+            q += m.sums[turn][1][i];
+        }
+    }
 }
 
-int64_t row_blocks(int64_t rows, int64_t hidden) { return hidden <= 1024 ? (rows + 3) / 4 : rows; }
-
-// f(WPR, U) of the instance for `hidden` values a row: U pieces of 8 per lane.
-template <bool WIDE, typename F> int with_shape(int64_t hidden, F f) {
-    using std::integral_constant;
-    const int wpr = waves_per_row<WIDE>(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
-#define GG_SHAPE(W, N)                                                                                                 \
-    if (wpr == W && u <= N)                                                                                            \
-        return f(integral_constant<int, W>{}, integral_constant<int, N>{});
-    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1)
-    if constexpr (WIDE) {
-        GG_SHAPE(16, 1) GG_SHAPE(16, 2)
-    } else {
-        GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(4, 4) GG_SHAPE(4, 6) GG_SHAPE(4, 8)
+// With d = h - mean: grad_x = grad_h + rstd (w g - mean(w g)) - d rstd^3 mean(w g d), row by row; the partial sums of
+// g d rstd and of g stay in registers over the rows of a workgroup and are written once. Two sums a column are twice the
+// registers of the RMS norm's one, so rows past 8192 values take eight waves, and with more than four pieces a lane (past
+// 16384) load the inputs again, from the caches, instead of keeping them.
+template <typename T, int WPR, int U, bool SUMS>
+__global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const CenterArgs c) {
+    __shared__ PairReduce<WPR> m;
+    const BackArgs &a    = c.b;
+    constexpr bool  kKeep = U <= 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t    = WPR == 1 ? lane : static_cast<int>(threadIdx.x);
+    float     dw[U][8], db[U][8];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            dw[u][j] = db[u][j] = 0.f;
+    int           turn = 0;
+    const int64_t step = static_cast<int64_t>(gridDim.x) * rows_per_block(WPR);
+    // every wave of a block that shares a row makes the same trips, so the barriers match
+    for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0); row < a.rows;
+         row += step, turn ^= 1) {
+        const uint16_t *gp = static_cast<const uint16_t *>(a.g) + row * a.g_stride;
+        const uint16_t *hp = static_cast<const uint16_t *>(a.h) + row * a.h_stride;
+        const uint16_t *rp = a.gh == nullptr ? nullptr : static_cast<const uint16_t *>(a.gh) + row * a.gh_stride;
+        u32x4       gw[U], hw[U], rw[U];
+        float       sum = 0.f, dot = 0.f;
+        const float rstd = a.rstd[row], mean = c.mean[row];
+        if constexpr (kKeep) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int i = (u * 64 * WPR + t) * 8;
+                if (i < a.hidden) {
+                    gw[u] = load_once(gp + i);
+                    hw[u] = load_once(hp + i);
+                    if (rp != nullptr)
+                        rw[u] = load_once(rp + i);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * 64 * WPR + t) * 8;
+            if (i < a.hidden) {
+                float g[8], h[8], w[8];
+                unpack8<T>(kKeep ? gw[u] : *reinterpret_cast<const u32x4 *>(gp + i), g);
+                unpack8<T>(kKeep ? hw[u] : *reinterpret_cast<const u32x4 *>(hp + i), h);
+                load_w<T>(a.weight, a.w32, i, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float d = h[j] - mean, wg = g[j] * w[j];
+                    sum += wg;
+                    dot = fmaf(wg, d, dot);
+                    if constexpr (SUMS) {
+                        dw[u][j] = fmaf(g[j] * d, rstd, dw[u][j]);
+                        db[u][j] += g[j];
+                    }
+                }
+            }
+        }
+        row_sums<WPR>(m, turn, sum, dot, wave, lane);
+        const float n  = static_cast<float>(a.hidden);
+        const float c1 = rstd * (sum / n), c2 = rstd * (rstd * (rstd * (dot / n))); // (rstd^3 alone may be past float32)
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = (u * 64 * WPR + t) * 8;
+            if (i < a.hidden) {
+                float g[8], h[8], w[8], r[8];
+                unpack8<T>(kKeep ? gw[u] : load_once(gp + i), g);
+                unpack8<T>(kKeep ? hw[u] : load_once(hp + i), h);
+                load_w<T>(a.weight, a.w32, i, w);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    g[j] = rstd * (g[j] * w[j]) - c1 - (h[j] - mean) * c2;
+                if (rp != nullptr) {
+                    unpack8<T>(kKeep ? rw[u] : load_once(rp + i), r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        g[j] += r[j];
+                }
+                *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.gx) + row * a.hidden + i) = pack8<T>(g);
+            }
+        }
     }
-#undef GG_SHAPE
-    return f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    if constexpr (!SUMS)
+        return;
+    // a workgroup whose waves had rows of their own adds them up first, in their order
+    if constexpr (WPR == 1) {
+        __shared__ f32x4 mine[3][U][4][64];
+        if (wave > 0)
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    mine[wave - 1][u][q][lane]     = f32x4{dw[u][4 * q], dw[u][4 * q + 1], dw[u][4 * q + 2], dw[u][4 * q + 3]};
+                    mine[wave - 1][u][2 + q][lane] = f32x4{db[u][4 * q], db[u][4 * q + 1], db[u][4 * q + 2], db[u][4 * q + 3]};
+                }
+        __syncthreads();
+        if (wave > 0)
+            return;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                for (int o = 0; o < 3; ++o)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        dw[u][4 * q + j] += mine[o][u][q][lane][j];
+                        db[u][4 * q + j] += mine[o][u][2 + q][lane][j];
+                    }
+    }
+    float *part = a.parts + static_cast<int64_t>(blockIdx.x) * 2 * a.hidden;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int i = (u * 64 * WPR + t) * 8;
+        if (i < a.hidden) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                *reinterpret_cast<f32x4 *>(part + i + 4 * q) = f32x4{dw[u][4 * q], dw[u][4 * q + 1], dw[u][4 * q + 2], dw[u][4 * q + 3]};
+                *reinterpret_cast<f32x4 *>(part + a.hidden + i + 4 * q) =
+                    f32x4{db[u][4 * q], db[u][4 * q + 1], db[u][4 * q + 2], db[u][4 * q + 3]};
+            }
+        }
+    }
+}
+
+// grad_weight and grad_bias from g and h themselves: 64 columns (a line of 128 bytes a row) by 128 slices of the rows a workgroup.
+template <typename T> __global__ void __launch_bounds__(1024) center_strip_kernel(const CenterArgs c, void *grad_weight, void *grad_bias) {
+    __shared__ f32x4 sums[4][128][8];
+    const BackArgs &a = c.b;
+    const int c8 = threadIdx.x & 7, slice = threadIdx.x >> 3, col = blockIdx.x * 64 + c8 * 8; // hidden % 8 == 0
+    f32x4     s[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        s[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (col < a.hidden) {
+        const uint16_t *g = static_cast<const uint16_t *>(a.g) + col, *h = static_cast<const uint16_t *>(a.h) + col;
+#pragma unroll 4
+        for (int64_t row = slice; row < a.rows; row += 128) {
+            float gv[8], hv[8];
+            unpack8<T>(*reinterpret_cast<const u32x4 *>(g + row * a.g_stride), gv);
+            unpack8<T>(*reinterpret_cast<const u32x4 *>(h + row * a.h_stride), hv);
+            const float rstd = a.rstd[row], mean = c.mean[row];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                s[j / 4][j % 4] = fmaf(gv[j] * (hv[j] - mean), rstd, s[j / 4][j % 4]);
+                s[2 + j / 4][j % 4] += gv[j];
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        sums[q][slice][c8] = s[q];
+    __syncthreads();
+#pragma unroll
+    for (int half = 64; half > 0; half >>= 1) {
+        if (slice < half)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                sums[q][slice][c8] = s[q] += sums[q][slice + half][c8];
+        __syncthreads();
+    }
+    if (slice == 0 && col < a.hidden) {
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+            void *out = o == 0 ? grad_weight : grad_bias;
+            if (a.w32) {
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    reinterpret_cast<f32x4 *>(static_cast<float *>(out) + col)[q] = s[2 * o + q];
+            } else {
+                const f32x4 l = s[2 * o], r = s[2 * o + 1];
+                const float v[8] = {l[0], l[1], l[2], l[3], r[0], r[1], r[2], r[3]};
+                *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(out) + col) = pack8<T>(v);
+            }
+        }
+    }
 }
 
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;
 
-template <typename T, bool WIDE> int run_norm(const NormArgs &a, hipStream_t s) {
+template <typename T, bool CENTER, bool WIDE> int run_norm(const NormArgs &a, bool i8, hipStream_t s) {
+    constexpr const char *kWhat = CENTER ? "layer_norm" : "rms_norm";
     const int64_t blocks = row_blocks(a.rows, a.hidden);
     if (a.mode != GG_NORM_SCALE_TENSOR)
         return with_shape<WIDE>(a.hidden, [&](auto wpr, auto u) {
-            return launch("rms_norm", norm_kernel<T, wpr.value, u.value, false>, std::min(blocks, kMaxBlocks),
-                          block_threads(wpr.value), s, a);
+            return launch(kWhat, i8 ? norm_kernel<T, CENTER, wpr.value, u.value, kInt8> : norm_kernel<T, CENTER, wpr.value, u.value, kWhole>,
+                          std::min(blocks, kMaxBlocks), block_threads(wpr.value), s, a);
         });
     // The first pass: as many workgroups as fit at once, each with its share of the rows (32768 rows of 7168: 1792
     // workgroups fit, 377 us for both passes; 1536 377, 1280 389, 1024 421, 2048, 1.1 rounds of them, 453).
@@ -509,13 +625,13 @@ template <typename T, bool WIDE> int run_norm(const NormArgs &a, hipStream_t s) 
         b.h_stride = b.x_stride;
     }
     const int st = with_shape<WIDE>(a.hidden, [&](auto wpr, auto u) {
-        constexpr auto kernel = norm_kernel<T, wpr.value, u.value, true>;
+        constexpr auto kernel = norm_kernel<T, CENTER, wpr.value, u.value, kFirst>;
         // (asked for each call, as devices differ; few workgroups fit in any case)
         b.n_parts = static_cast<int>(blocks <= 256 ? blocks : std::min<int64_t>(blocks, std::min(resident_blocks(kernel, block_threads(wpr.value)), kMaxParts)));
-        return launch("rms_norm", kernel, b.n_parts, block_threads(wpr.value), s, b);
+        return launch(kWhat, kernel, b.n_parts, block_threads(wpr.value), s, b);
     });
     constexpr int kThreads = WIDE ? 1024 : 256;
-    return st ? st : launch("rms_norm", quantize_kernel<T, kThreads>, std::min<int64_t>(b.rows, 8192), kThreads, s, b);
+    return st ? st : launch(kWhat, quantize_kernel<T, CENTER, kThreads>, std::min<int64_t>(b.rows, 8192), kThreads, s, b);
 }
 
 // Workgroups of the backward pass: at most those that 256 CUs hold at once (by the instances' registers, 68 to 224: numbers
@@ -543,7 +659,44 @@ template <typename T> int run_back(const BackArgs &a, void *grad_weight, hipStre
                       block_threads(wpr.value), s, a);
     });
     return st ? st : launch("rms_norm_backward", weight_sum_kernel<T>, (a.hidden + 31) / 32, 1024, s, a.parts,
-                            static_cast<int>(back_blocks(a.rows, a.hidden)), a.hidden, grad_weight, a.w32);
+                            static_cast<int>(back_blocks(a.rows, a.hidden)), a.hidden, a.hidden, grad_weight, nullptr, a.w32);
+}
+
+// Layer norm's backward pass: waves of a row and pieces of a lane (see center_back_kernel), and workgroups: those that 256
+// CUs hold at once by the instances' registers (a test holds the numbers to the compiler's report), fewer of few rows.
+int center_waves(int64_t hidden) { return hidden <= 1024 ? 1 : hidden <= 8192 ? 4 : 8; }
+template <typename F> int with_center_shape(int64_t hidden, F f) {
+    using std::integral_constant;
+    const int wpr = center_waves(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+#define GG_SHAPE(W, N)                                                                                                 \
+    if (wpr == W && u <= N)                                                                                            \
+        return f(integral_constant<int, W>{}, integral_constant<int, N>{});
+    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(4, 4) GG_SHAPE(8, 3) GG_SHAPE(8, 4)
+#undef GG_SHAPE
+    return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+}
+int64_t center_blocks(int64_t rows, int64_t hidden) {
+    const int     wpr = center_waves(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+    const int64_t fit = wpr == 8 ? 256 : u == 1 ? 1280 : u == 2 && wpr == 4 ? 1024 : 768;
+    const int64_t b   = row_blocks(rows, hidden);
+    return std::min(fit, std::max(b / 4, b <= 256 ? b : std::min<int64_t>(b / 2, 512)));
+}
+
+template <typename T> int run_center_back(const CenterArgs &a, void *grad_weight, void *grad_bias, hipStream_t s) {
+    const int64_t rows = a.b.rows, hidden = a.b.hidden;
+    if (few(rows, hidden)) { // (the sums first: grad_x may take the place of an input)
+        const int st = launch("layer_norm_backward", center_strip_kernel<T>, (hidden + 63) / 64, 1024, s, a, grad_weight, grad_bias);
+        return st ? st : with_shape<true>(hidden, [&](auto wpr, auto u) {
+            return launch("layer_norm_backward", center_back_kernel<T, wpr.value, u.value, false>, row_blocks(rows, hidden),
+                          block_threads(wpr.value), s, a);
+        });
+    }
+    const int blocks = static_cast<int>(center_blocks(rows, hidden));
+    const int st     = with_center_shape(hidden, [&](auto wpr, auto u) {
+        return launch("layer_norm_backward", center_back_kernel<T, wpr.value, u.value, true>, blocks, block_threads(wpr.value), s, a);
+    });
+    return st ? st : launch("layer_norm_backward", weight_sum_kernel<T>, (2 * hidden + 31) / 32, 1024, s, a.b.parts, blocks,
+                            2 * a.b.hidden, a.b.hidden, grad_weight, grad_bias, a.b.w32);
 }
 
 // Rules shared by both passes.
@@ -558,17 +711,6 @@ int check_norm(int dtype, int weight_dtype, int64_t rows, int64_t hidden) {
         return fail(GG_ERR_UNSUPPORTED, "hidden must be a multiple of 8 and at most 32768");
     return GG_OK;
 }
-// A matrix operand: rows at least hidden apart, 16-byte pieces.
-int check_rows(const char *name, const void *p, int64_t stride, int64_t rows) {
-    if (rows > 0 && p == nullptr)
-        return fail(GG_ERR_INVALID, "%s is null", name);
-    if (rows > 1 && stride < 0)
-        return fail(GG_ERR_INVALID, "%s has a negative row stride", name);
-    if (!aligned(p, 16) || (rows > 1 && stride % 8 != 0))
-        return fail(GG_ERR_UNSUPPORTED, "%s must be 16-byte aligned with row strides of multiples of 8", name);
-    return GG_OK;
-}
-
 } // namespace
 } // namespace layer
 } // namespace gg
@@ -579,24 +721,27 @@ extern "C" {
 
 const char *gg_layer_last_error(void) { return g_error; }
 
-int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
-                const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight,
-                void *h, int64_t h_stride, void *y, float *rstd, float *scale, void *workspace, void *stream) {
+// Both norms' forward pass (center: layer norm).
+static int norm_forward(bool center, int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden,
+                        float eps, const void *x, int64_t x_stride, const void *residual, int64_t residual_stride,
+                        const void *weight, const void *bias, void *h, int64_t h_stride, void *y, float *mean, float *rstd,
+                        float *scale, void *workspace, void *stream) {
     g_error[0] = 0;
     if (const int st = check_norm(dtype, weight_dtype, rows, hidden))
         return st;
     if (scale_mode < GG_NORM_PLAIN || scale_mode > GG_NORM_SCALE_GIVEN)
         return fail(GG_ERR_INVALID, "scale_mode must be a gg_norm_scale");
-    if (scale_mode == GG_NORM_PLAIN ? out_dtype != dtype : !is8(out_dtype))
-        return fail(GG_ERR_INVALID, "out_dtype must be dtype, or an fp8 type with a scale");
+    if (scale_mode == GG_NORM_PLAIN ? out_dtype != dtype
+                                    : !is8(out_dtype) && !(out_dtype == GG_DTYPE_INT8 && scale_mode == GG_NORM_SCALE_ROW))
+        return fail(GG_ERR_INVALID, "out_dtype must be dtype, an fp8 type with a scale, or int8 with a scale for each row");
     if (scale_mode != GG_NORM_PLAIN && scale == nullptr && (rows > 0 || scale_mode != GG_NORM_SCALE_ROW)) // (a row scale of no rows)
         return fail(GG_ERR_INVALID, "scale is null");
     if (rows == 0 && scale_mode != GG_NORM_SCALE_TENSOR)
         return GG_OK;
     if (weight == nullptr || (rows > 0 && y == nullptr))
         return fail(GG_ERR_INVALID, "weight and y must be device pointers");
-    if (scale_mode == GG_NORM_SCALE_TENSOR && (workspace == nullptr || (rows > 0 && rstd == nullptr)))
-        return fail(GG_ERR_INVALID, "a tensor scale needs workspace and rstd");
+    if (scale_mode == GG_NORM_SCALE_TENSOR && (workspace == nullptr || (rows > 0 && (rstd == nullptr || (center && mean == nullptr)))))
+        return fail(GG_ERR_INVALID, center ? "a tensor scale needs workspace, mean and rstd" : "a tensor scale needs workspace and rstd");
     if (const int st = check_rows("x", x, x_stride, rows))
         return st;
     if (residual != nullptr) {
@@ -607,14 +752,16 @@ int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int6
         if (rows > 1 && h_stride < hidden)
             return fail(GG_ERR_INVALID, "rows of h overlap");
     }
-    if (!aligned(weight, 16) || !aligned(y, scale_mode == GG_NORM_PLAIN ? 16 : 8) || !aligned(workspace, 4))
-        return fail(GG_ERR_UNSUPPORTED, "weight and y must be 16-byte aligned (fp8 y: 8)");
+    if (!aligned(weight, 16) || !aligned(bias, 16) || !aligned(y, scale_mode == GG_NORM_PLAIN ? 16 : 8) || !aligned(workspace, 4))
+        return fail(GG_ERR_UNSUPPORTED, "weight%s and y must be 16-byte aligned (8-bit y: 8)", center ? ", bias" : "");
     NormArgs a{};
     a.x        = x;
     a.residual = residual;
     a.weight   = weight;
+    a.bias     = bias;
     a.h        = h;
     a.y        = y;
+    a.mean     = mean;
     a.rstd     = rstd;
     a.scale    = scale;
     a.parts    = static_cast<float *>(workspace);
@@ -627,14 +774,33 @@ int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int6
     a.eps      = eps;
     a.w32      = weight_dtype == GG_DTYPE_FP32;
     a.e5m2     = out_dtype == GG_DTYPE_FP8_E5M2;
-    if (rows == 0) { // no maximum: the scale alone
-        return launch("rms_norm", quantize_kernel<BF16, 256>, 1, 256, static_cast<hipStream_t>(stream), a);
-    }
+    const bool        i8 = out_dtype == GG_DTYPE_INT8;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const bool        wide = few(rows, hidden);
+    if (rows == 0) // no maximum: the scale alone
+        return launch(center ? "layer_norm" : "rms_norm", quantize_kernel<BF16, false, 256>, 1, 256, st, a);
+    const bool wide = few(rows, hidden);
+    const auto run  = [&](auto type, auto centered) {
+        using T = decltype(type);
+        return wide ? run_norm<T, centered.value, true>(a, i8, st) : run_norm<T, centered.value, false>(a, i8, st);
+    };
     if (dtype == GG_DTYPE_BF16)
-        return wide ? run_norm<BF16, true>(a, st) : run_norm<BF16, false>(a, st);
-    return wide ? run_norm<F16, true>(a, st) : run_norm<F16, false>(a, st);
+        return center ? run(BF16{}, std::true_type{}) : run(BF16{}, std::false_type{});
+    return center ? run(F16{}, std::true_type{}) : run(F16{}, std::false_type{});
+}
+
+int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
+                const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight,
+                void *h, int64_t h_stride, void *y, float *rstd, float *scale, void *workspace, void *stream) {
+    return norm_forward(false, dtype, weight_dtype, out_dtype, scale_mode, rows, hidden, eps, x, x_stride, residual,
+                        residual_stride, weight, nullptr, h, h_stride, y, nullptr, rstd, scale, workspace, stream);
+}
+
+int gg_layer_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
+                  const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight,
+                  const void *bias, void *h, int64_t h_stride, void *y, float *mean, float *rstd, float *scale,
+                  void *workspace, void *stream) {
+    return norm_forward(true, dtype, weight_dtype, out_dtype, scale_mode, rows, hidden, eps, x, x_stride, residual,
+                        residual_stride, weight, bias, h, h_stride, y, mean, rstd, scale, workspace, stream);
 }
 
 size_t gg_rms_norm_backward_workspace(int64_t rows, int64_t hidden) {
@@ -680,10 +846,61 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
     a.w32       = weight_dtype == GG_DTYPE_FP32;
     if (rows == 0) { // the sums of no rows
         return launch("rms_norm_backward", weight_sum_kernel<BF16>, (a.hidden + 31) / 32, 1024,
-                      static_cast<hipStream_t>(stream), nullptr, 0, a.hidden, grad_weight, a.w32);
+                      static_cast<hipStream_t>(stream), nullptr, 0, a.hidden, a.hidden, grad_weight, nullptr, a.w32);
     }
     return dtype == GG_DTYPE_BF16 ? run_back<BF16>(a, grad_weight, static_cast<hipStream_t>(stream))
                                   : run_back<F16>(a, grad_weight, static_cast<hipStream_t>(stream));
+}
+
+size_t gg_layer_norm_backward_workspace(int64_t rows, int64_t hidden) {
+    if (rows < 1 || hidden < 1 || hidden > 32768 || few(rows, hidden))
+        return 0;
+    return static_cast<size_t>(center_blocks(rows, hidden)) * static_cast<size_t>(hidden) * 8;
+}
+
+int gg_layer_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidden, const void *grad_y,
+                           int64_t grad_y_stride, const void *h, int64_t h_stride, const void *weight, const float *mean,
+                           const float *rstd, const void *grad_h, int64_t grad_h_stride, void *grad_x, void *grad_weight,
+                           void *grad_bias, void *workspace, size_t workspace_bytes, void *stream) {
+    g_error[0] = 0;
+    if (const int st = check_norm(dtype, weight_dtype, rows, hidden))
+        return st;
+    if (weight == nullptr || grad_weight == nullptr || grad_bias == nullptr ||
+        (rows > 0 && (grad_x == nullptr || mean == nullptr || rstd == nullptr)))
+        return fail(GG_ERR_INVALID, "weight, mean, rstd, grad_x, grad_weight and grad_bias must be device pointers");
+    if (const int st = check_rows("grad_y", grad_y, grad_y_stride, rows))
+        return st;
+    if (const int st = check_rows("h", h, h_stride, rows))
+        return st;
+    if (grad_h != nullptr)
+        if (const int st = check_rows("grad_h", grad_h, grad_h_stride, rows))
+            return st;
+    if (!aligned(weight, 16) || !aligned(grad_x, 16) || !aligned(grad_weight, 16) || !aligned(grad_bias, 16))
+        return fail(GG_ERR_UNSUPPORTED, "weight, grad_x, grad_weight and grad_bias must be 16-byte aligned");
+    const size_t need = gg_layer_norm_backward_workspace(rows, hidden);
+    if (workspace_bytes < need || (need > 0 && (workspace == nullptr || !aligned(workspace, 16))))
+        return fail(GG_ERR_WORKSPACE, "workspace must be 16-byte aligned and of gg_layer_norm_backward_workspace(rows, hidden) bytes");
+    CenterArgs a{};
+    a.b.g         = grad_y;
+    a.b.h         = h;
+    a.b.weight    = weight;
+    a.b.gh        = grad_h;
+    a.b.rstd      = rstd;
+    a.b.gx        = grad_x;
+    a.b.parts     = static_cast<float *>(workspace);
+    a.b.rows      = rows;
+    a.b.g_stride  = grad_y_stride;
+    a.b.h_stride  = h_stride;
+    a.b.gh_stride = grad_h_stride;
+    a.b.hidden    = static_cast<int>(hidden);
+    a.b.w32       = weight_dtype == GG_DTYPE_FP32;
+    a.mean        = mean;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (rows == 0) // the sums of no rows
+        return launch("layer_norm_backward", weight_sum_kernel<BF16>, (2 * a.b.hidden + 31) / 32, 1024, st, nullptr, 0,
+                      2 * a.b.hidden, a.b.hidden, grad_weight, grad_bias, a.b.w32);
+    return dtype == GG_DTYPE_BF16 ? run_center_back<BF16>(a, grad_weight, grad_bias, st)
+                                  : run_center_back<F16>(a, grad_weight, grad_bias, st);
 }
 
 } // extern "C"

@@ -19,7 +19,7 @@ from . import GG_OK, DType, GGError, _device_sizes, load_library
 
 _T16 = {torch.bfloat16: int(DType.BF16), torch.float16: int(DType.FP16)}
 _T8 = {torch.float8_e4m3fn: int(DType.FP8_E4M3), torch.float8_e5m2: int(DType.FP8_E5M2)}
-_FP32 = 4  # GG_DTYPE_FP32
+_FP32, _INT8 = 4, 5  # GG_DTYPE_FP32, GG_DTYPE_INT8
 _NORM_WORKSPACE = 8192  # GG_NORM_WORKSPACE
 _PLAIN, _TENSOR, _ROW, _GIVEN = 0, 1, 2, 3  # gg_norm_scale
 
@@ -114,24 +114,25 @@ def _ptr(t) -> int:
 
 class NormOutput(NamedTuple):
     """rms_norm's outputs: y; h = x + residual (x itself without one); rstd [M] float32; scale float32
-    ([1], or [M] for one a row) of an fp8 y, which stands for y * scale, else None."""
+    ([1], or [M] for one a row) of an 8-bit y, which stands for y * scale, else None."""
     y: "torch.Tensor"
     h: "torch.Tensor"
     rstd: "torch.Tensor"
     scale: "Optional[torch.Tensor]"
 
 
-def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=None, out=None, out_h=None,
-             stream: Optional[int] = None) -> NormOutput:
-    """y = h * rsqrt(mean(h^2) + eps) * weight over the rows of h = x + residual (gg_rms_norm).
+class LayerNormOutput(NamedTuple):
+    """layer_norm's outputs: y; h = x + residual (x itself without one); mean and rstd [M] float32; scale float32
+    ([1], or [M] for one a row) of an 8-bit y, which stands for y * scale, else None."""
+    y: "torch.Tensor"
+    h: "torch.Tensor"
+    mean: "torch.Tensor"
+    rstd: "torch.Tensor"
+    scale: "Optional[torch.Tensor]"
 
-    x, residual: [M, H] bf16 or fp16, rows contiguous at any stride; weight [H] of x's type or float32.
-    out_dtype float8_e4m3fn or float8_e5m2 gives an fp8 y: with one scale for the tensor (scale=None or
-    "tensor": the x_scale of grouped_gemm_fp8), one for each row ("row"), or divided by a given device
-    float32 scale [1]. out: y's buffer; out_h: h's, which may be x or residual itself.
-    """
-    if stream is not None:
-        return _on(stream, rms_norm, x, weight, residual, eps, out_dtype, scale, out, out_h)
+
+def _norm(center: bool, x, weight, bias, residual, eps, out_dtype, scale, out, out_h):
+    """(y, h, mean, rstd, scale) of either norm."""
     dtype = x.dtype
     dt = _T16.get(dtype)
     if dt is None:
@@ -142,6 +143,8 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
     if wd != dtype and wd != torch.float32:
         raise TypeError("weight must be of x's type or float32")
     _flat("weight", weight, wd, (n,), dev)
+    if bias is not None:
+        _flat("bias", bias, wd, (n,), dev)
     rs = hs = hp = 0
     h = x
     if residual is not None:
@@ -160,13 +163,17 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
     ws = s = None
     if out_dtype is None or out_dtype == dtype:
         if scale is not None:
-            raise ValueError("scale goes with an fp8 out_dtype")
+            raise ValueError("scale goes with an 8-bit out_dtype")
         out_dtype, od, mode = dtype, dt, _PLAIN
     else:
         od = _T8.get(out_dtype)
+        if od is None and out_dtype != torch.int8:
+            raise TypeError("out_dtype must be x's type, float8_e4m3fn, float8_e5m2 or int8")
         if od is None:
-            raise TypeError("out_dtype must be x's type, float8_e4m3fn or float8_e5m2")
-        if scale is None or isinstance(scale, str):
+            if not isinstance(scale, str) or scale != "row":
+                raise ValueError("int8 rows have a scale each: scale must be 'row'")
+            od, mode, s = _INT8, _ROW, torch.empty(m, dtype=torch.float32, device=dev)
+        elif scale is None or isinstance(scale, str):
             if scale not in (None, "tensor", "row"):
                 raise ValueError("scale must be 'tensor', 'row' or a device float32 tensor of one value")
             mode = _ROW if scale == "row" else _TENSOR
@@ -179,17 +186,44 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=
                 raise ValueError("scale must be 'tensor', 'row' or a device float32 tensor of one value")
     y = _new_like(x) if out is None and mode == _PLAIN else _out(out, out_dtype, (m, n), dev)
     rstd = torch.empty(m, dtype=torch.float32, device=dev)
-    _call(_lib.gg_rms_norm, dev, (dt, dt if wd == dtype else _FP32, od, mode, m, n, eps, x.data_ptr(), xs, _ptr(residual), rs,
-                                  weight.data_ptr(), hp, hs, y.data_ptr(), rstd.data_ptr(), _ptr(s), _ptr(ws)))
+    wt = dt if wd == dtype else _FP32
+    if not center:
+        _call(_lib.gg_rms_norm, dev, (dt, wt, od, mode, m, n, eps, x.data_ptr(), xs, _ptr(residual), rs, weight.data_ptr(),
+                                      hp, hs, y.data_ptr(), rstd.data_ptr(), _ptr(s), _ptr(ws)))
+        return y, h, None, rstd, s
+    mean = torch.empty_like(rstd)
+    _call(_lib.gg_layer_norm, dev, (dt, wt, od, mode, m, n, eps, x.data_ptr(), xs, _ptr(residual), rs, weight.data_ptr(), _ptr(bias),
+                                    hp, hs, y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(s), _ptr(ws)))
+    return y, h, mean, rstd, s
+
+
+def rms_norm(x, weight, residual=None, eps: float = 1e-6, out_dtype=None, scale=None, out=None, out_h=None,
+             stream: Optional[int] = None) -> NormOutput:
+    """y = h * rsqrt(mean(h^2) + eps) * weight over the rows of h = x + residual (gg_rms_norm).
+
+    x, residual: [M, H] bf16 or fp16, rows contiguous at any stride; weight [H] of x's type or float32.
+    out_dtype float8_e4m3fn or float8_e5m2 gives an fp8 y: with one scale for the tensor (scale=None or
+    "tensor": the x_scale of grouped_gemm_fp8), one for each row ("row"), or divided by a given device
+    float32 scale [1]; int8 with scale="row" the rows and scales of grouped_gemm_i8. out: y's buffer; out_h:
+    h's, which may be x or residual itself.
+    """
+    if stream is not None:
+        return _on(stream, rms_norm, x, weight, residual, eps, out_dtype, scale, out, out_h)
+    y, h, _, rstd, s = _norm(False, x, weight, None, residual, eps, out_dtype, scale, out, out_h)
     return NormOutput(y, h, rstd, s)
 
 
-def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Optional[int] = None):
-    """(grad_x, grad_weight) of rms_norm from its h and rstd (gg_rms_norm_backward). grad_x is the gradient
-    of x and of residual; grad_h, the gradient that reaches h past the norm, is added to it. grad_y and
-    grad_h are of h's type (an fp8 y is differentiated as if it were not rounded)."""
+def layer_norm(x, weight, bias=None, residual=None, eps: float = 1e-5, out_dtype=None, scale=None, out=None, out_h=None,
+               stream: Optional[int] = None) -> LayerNormOutput:
+    """y = (h - mean) * rstd * weight + bias over the rows of h = x + residual, rstd = rsqrt(mean((h - mean)^2) + eps)
+    (gg_layer_norm). bias [H] of weight's type or None; everything else as in rms_norm."""
     if stream is not None:
-        return _on(stream, rms_norm_backward, grad_y, h, weight, rstd, grad_h, out)
+        return _on(stream, layer_norm, x, weight, bias, residual, eps, out_dtype, scale, out, out_h)
+    return LayerNormOutput(*_norm(True, x, weight, bias, residual, eps, out_dtype, scale, out, out_h))
+
+
+def _norm_back(center: bool, grad_y, h, weight, mean, rstd, grad_h, out):
+    """(grad_x, grad_weight, grad_bias) of either norm."""
     dtype = h.dtype
     dt = _T16.get(dtype)
     if dt is None:
@@ -206,14 +240,107 @@ def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Op
         raise TypeError("weight must be of h's type or float32")
     _flat("weight", weight, wd, (n,), dev)
     _flat("rstd", rstd, torch.float32, (m,), dev)
+    if center:
+        _flat("mean", mean, torch.float32, (m,), dev)
     gx = _new_like(h) if out is None else _out(out, dtype, (m, n), dev)
     gw = torch.empty_like(weight)
-    need = _lib.gg_rms_norm_backward_workspace(m, n)
+    gb = torch.empty_like(weight) if center else None
+    need = (_lib.gg_layer_norm_backward_workspace if center else _lib.gg_rms_norm_backward_workspace)(m, n)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    _call(_lib.gg_rms_norm_backward, dev, (dt, dt if wd == dtype else _FP32, m, n, grad_y.data_ptr(), gs, h.data_ptr(), hs,
-                                           weight.data_ptr(), rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(),
-                                           gw.data_ptr(), _ptr(ws), need))
+    wt = dt if wd == dtype else _FP32
+    if center:
+        _call(_lib.gg_layer_norm_backward, dev, (dt, wt, m, n, grad_y.data_ptr(), gs, h.data_ptr(), hs, weight.data_ptr(),
+                                                 mean.data_ptr(), rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(),
+                                                 gw.data_ptr(), gb.data_ptr(), _ptr(ws), need))
+    else:
+        _call(_lib.gg_rms_norm_backward, dev, (dt, wt, m, n, grad_y.data_ptr(), gs, h.data_ptr(), hs, weight.data_ptr(),
+                                               rstd.data_ptr(), _ptr(grad_h), ghs, gx.data_ptr(), gw.data_ptr(), _ptr(ws), need))
+    return gx, gw, gb
+
+
+def rms_norm_backward(grad_y, h, weight, rstd, grad_h=None, out=None, stream: Optional[int] = None):
+    """(grad_x, grad_weight) of rms_norm from its h and rstd (gg_rms_norm_backward). grad_x is the gradient
+    of x and of residual; grad_h, the gradient that reaches h past the norm, is added to it. grad_y and
+    grad_h are of h's type (an 8-bit y is differentiated as if it were not rounded)."""
+    if stream is not None:
+        return _on(stream, rms_norm_backward, grad_y, h, weight, rstd, grad_h, out)
+    gx, gw, _ = _norm_back(False, grad_y, h, weight, None, rstd, grad_h, out)
     return gx, gw
+
+
+def layer_norm_backward(grad_y, h, weight, mean, rstd, grad_h=None, out=None, stream: Optional[int] = None):
+    """(grad_x, grad_weight, grad_bias) of layer_norm from its h, mean and rstd (gg_layer_norm_backward); as
+    rms_norm_backward. grad_bias is of weight's type, whether there was a bias or not."""
+    if stream is not None:
+        return _on(stream, layer_norm_backward, grad_y, h, weight, mean, rstd, grad_h, out)
+    return _norm_back(True, grad_y, h, weight, mean, rstd, grad_h, out)
+
+
+# ---- gated activation, rows of int8 ----
+
+
+class ScaledRows(NamedTuple):
+    """Rows y [M, N] and, where they are int8, scale [M] float32: row i stands for y[i] * scale[i]. Else scale is None."""
+    y: "torch.Tensor"
+    scale: "Optional[torch.Tensor]"
+
+
+def _gates(gu):
+    dt = _T16.get(gu.dtype)
+    if dt is None:
+        raise TypeError("gu must be bfloat16 or float16")
+    stride = _matrix("gu", gu)
+    if gu.shape[1] % 2:
+        raise ValueError("gu must hold as many gates as ups")
+    return dt, stride, gu.shape[1] // 2
+
+
+def silu_product(gu, out_dtype=None, out=None, stream: Optional[int] = None) -> ScaledRows:
+    """y = silu(gate) * up of rows gu [M, 2 N] that hold N gates and then N ups, rows contiguous at any stride
+    (gg_silu_product). y is of gu's type, or with out_dtype=int8 rounded to int8 rows with a scale each, as
+    grouped_gemm_i8 takes them."""
+    if stream is not None:
+        return _on(stream, silu_product, gu, out_dtype, out)
+    dt, stride, n = _gates(gu)
+    m, dev = gu.shape[0], gu.device
+    if out_dtype is None or out_dtype == gu.dtype:
+        y, s, od = _out(out, gu.dtype, (m, n), dev), None, dt
+    elif out_dtype == torch.int8:
+        y, s, od = _out(out, torch.int8, (m, n), dev), torch.empty(m, dtype=torch.float32, device=dev), _INT8
+    else:
+        raise TypeError("out_dtype must be gu's type or int8")
+    _call(_lib.gg_silu_product, dev, (dt, od, m, n, gu.data_ptr(), stride, y.data_ptr(), _ptr(s)))
+    return ScaledRows(y, s)
+
+
+def silu_product_backward(grad_y, gu, out=None, stream: Optional[int] = None):
+    """grad_gu [M, 2 N] of silu_product from grad_y [M, N] of gu's type (gg_silu_product_backward; an int8 y is
+    differentiated as if it were not rounded). out may be a contiguous gu itself."""
+    if stream is not None:
+        return _on(stream, silu_product_backward, grad_y, gu, out)
+    dt, stride, n = _gates(gu)
+    m, dev = gu.shape[0], gu.device
+    if grad_y.dtype != gu.dtype or grad_y.device != dev or tuple(grad_y.shape) != (m, n):
+        raise ValueError("grad_y must be [M, N] of gu's type")
+    gs = _matrix("grad_y", grad_y)
+    o = _new_like(gu) if out is None else _out(out, gu.dtype, (m, 2 * n), dev)
+    _call(_lib.gg_silu_product_backward, dev, (dt, m, n, grad_y.data_ptr(), gs, gu.data_ptr(), stride, o.data_ptr()))
+    return o
+
+
+def quantize_rows(x, out=None, stream: Optional[int] = None) -> ScaledRows:
+    """int8 rows of x [M, N] (bf16 or fp16, rows contiguous at any stride) and a scale for each (gg_quantize_rows):
+    scale = max |x| / 127 (1 for a row of zeros), y = x / scale rounded to the nearest, halves to even."""
+    if stream is not None:
+        return _on(stream, quantize_rows, x, out)
+    dt = _T16.get(x.dtype)
+    if dt is None:
+        raise TypeError("x must be bfloat16 or float16")
+    stride, dev = _matrix("x", x), x.device
+    m, n = x.shape
+    y, s = _out(out, torch.int8, (m, n), dev), torch.empty(m, dtype=torch.float32, device=dev)
+    _call(_lib.gg_quantize_rows, dev, (dt, m, n, x.data_ptr(), stride, y.data_ptr(), s.data_ptr()))
+    return ScaledRows(y, s)
 
 
 # ---- router ----

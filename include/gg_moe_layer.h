@@ -1,7 +1,7 @@
 /*
  * C ABI of the operators around the grouped GEMM in a mixture-of-experts layer (MI355X, gfx950):
- * RMS norm, router with balance loss, dispatch and combine of the experts' rows, and grouped
- * products with 4-bit weights. Same library and conventions as gg_grouped_gemm.h: plain pointers
+ * RMS norm, layer norm, gated activation, rows of int8, router with balance loss, dispatch and combine of the
+ * experts' rows, and grouped products with 4-bit weights and in 8-bit integers. Same library and conventions as gg_grouped_gemm.h: plain pointers
  * and sizes, `stream` a hipStream_t passed as void* (NULL = the default stream) of the current
  * device, every entry point returns a gg_status, none exits the process or throws.
  *
@@ -20,8 +20,8 @@
 extern "C" {
 #endif
 
-/* Beside gg_dtype: norm weights and router logits may be float32. */
-enum { GG_DTYPE_FP32 = 4 };
+/* Beside gg_dtype: norm weights and router logits may be float32, rows of 8 bits whole numbers in -127 .. 127. */
+enum { GG_DTYPE_FP32 = 4, GG_DTYPE_INT8 = 5 };
 
 /* Message of the last failed call of this header on the calling thread ("" if none). */
 const char *gg_layer_last_error(void);
@@ -32,7 +32,7 @@ const char *gg_layer_last_error(void);
 typedef enum gg_norm_scale {
     GG_NORM_PLAIN        = 0, /* y in the type of x */
     GG_NORM_SCALE_TENSOR = 1, /* y fp8, one scale for the tensor from its largest |y|: what the fp8 grouped GEMMs take */
-    GG_NORM_SCALE_ROW    = 2, /* y fp8, one scale for each row from its largest |y| */
+    GG_NORM_SCALE_ROW    = 2, /* y fp8 or int8, one scale for each row from its largest |y|: int8 is what gg_gemm_i8 takes */
     GG_NORM_SCALE_GIVEN  = 3  /* y fp8, divided by scale[0], which is read; values past the format's range saturate */
 } gg_norm_scale;
 
@@ -42,14 +42,17 @@ typedef enum gg_norm_scale {
  * (A row whose squares add up past 3.4e38, which values of some 10^17 and more can, has an rstd of 0.)
  * fp8: y = round(h * rstd * weight / scale), scale = max |h * rstd * weight| / (the format's largest
  * value), 1 where that is zero or subnormal. A NaN in a row makes its rstd, y and (for a tensor scale, every) scale NaN.
- *   dtype: GG_DTYPE_BF16 or GG_DTYPE_FP16 (x, residual, h; y unless fp8). weight_dtype: the same or
- *   GG_DTYPE_FP32. out_dtype: dtype, or an fp8 type with scale_mode 1-3.
+ * int8: the same with 127 for the format's largest value, rounded to the nearest whole number, halves to even. A row
+ * with a NaN or an infinity has a scale of NaN or infinity and holds no number past 127; where |y| is not finite or the
+ * scale is NaN it holds 0.
+ *   dtype: GG_DTYPE_BF16 or GG_DTYPE_FP16 (x, residual, h; y unless 8-bit). weight_dtype: the same or
+ *   GG_DTYPE_FP32. out_dtype: dtype, an fp8 type with scale_mode 1-3, or GG_DTYPE_INT8 with GG_NORM_SCALE_ROW.
  *   h: [rows, hidden]; may be x or residual itself. Not written (and may be NULL) without a residual.
  *   y: [rows, hidden] contiguous, overlapping no input. rstd: [rows], or NULL but for GG_NORM_SCALE_TENSOR.
  *   scale: written, [1] or [rows] (of no rows it may be NULL), or for GG_NORM_SCALE_GIVEN read, [1].
  *   workspace: GG_NORM_WORKSPACE bytes for GG_NORM_SCALE_TENSOR, else unused.
  * GG_ERR_UNSUPPORTED unless hidden % 8 == 0, hidden <= 32768, strides % 8 == 0 and 16-byte aligned
- * buffers (y of fp8: 8-byte).
+ * buffers (y of 8 bits: 8-byte).
  */
 enum { GG_NORM_WORKSPACE = 8192 };
 int gg_rms_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
@@ -71,6 +74,52 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
                          int64_t grad_y_stride, const void *h, int64_t h_stride, const void *weight, const float *rstd,
                          const void *grad_h, int64_t grad_h_stride, void *grad_x, void *grad_weight, void *workspace,
                          size_t workspace_bytes, void *stream);
+
+/* ---- layer norm with the residual's addition ---- */
+
+/*
+ * As gg_rms_norm, of h less its row's mean: mean = mean(h), rstd = 1 / sqrt(mean((h - mean)^2) + eps),
+ * y = (h - mean) * rstd * weight + bias. The squares are summed about the mean that was found, so rows of a
+ * large mean lose nothing. bias: [hidden] of weight_dtype, or NULL for none. mean, rstd: [rows], or NULL but for
+ * GG_NORM_SCALE_TENSOR. Types, scales, workspace and rules as there; bias 16-byte aligned.
+ */
+int gg_layer_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
+                  const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight,
+                  const void *bias, void *h, int64_t h_stride, void *y, float *mean, float *rstd, float *scale,
+                  void *workspace, void *stream);
+
+/*
+ * Gradients of gg_layer_norm from its h, mean and rstd (an 8-bit y is differentiated as if it were not rounded); with
+ * d = h - mean and g = weight * grad_y:
+ *   grad_x = grad_h + rstd * (g - mean(g)) - d * rstd^3 * mean(g * d)
+ *   grad_weight = sum over rows of grad_y * d * rstd, grad_bias = sum over rows of grad_y
+ * grad_weight, grad_bias: [hidden] of weight_dtype, both written. The rest as in gg_rms_norm_backward.
+ */
+size_t gg_layer_norm_backward_workspace(int64_t rows, int64_t hidden);
+int gg_layer_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidden, const void *grad_y,
+                           int64_t grad_y_stride, const void *h, int64_t h_stride, const void *weight, const float *mean,
+                           const float *rstd, const void *grad_h, int64_t grad_h_stride, void *grad_x, void *grad_weight,
+                           void *grad_bias, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ---- gated activation, rows of int8 ---- */
+
+/*
+ * y = silu(gate) * up, silu(v) = v / (1 + exp(-v)); gu [rows, 2 * inner] holds each row's gates and then its ups, as a
+ * product with the weights of both stacked writes them. out_dtype: dtype, or GG_DTYPE_INT8 with scale [rows] as
+ * gg_rms_norm's int8 rows (of the float32 values, which are not rounded to dtype first).
+ *   y: [rows, inner] contiguous, overlapping no input.
+ * gg_silu_product_backward: grad_gu [rows, 2 * inner] contiguous from grad_y [rows, inner]; with p = 1 / (1 + exp(-gate))
+ *   grad_gate = grad_y * up * p * (1 + gate * (1 - p)), grad_up = grad_y * gate * p
+ * grad_gu may take the place of a contiguous gu.
+ * GG_ERR_UNSUPPORTED unless inner % 8 == 0, inner <= 32768, strides % 8 == 0 and 16-byte aligned buffers (int8 y: 8-byte).
+ */
+int gg_silu_product(int dtype, int out_dtype, int64_t rows, int64_t inner, const void *gu, int64_t gu_stride, void *y,
+                    float *scale, void *stream);
+int gg_silu_product_backward(int dtype, int64_t rows, int64_t inner, const void *grad_y, int64_t grad_y_stride,
+                             const void *gu, int64_t gu_stride, void *grad_gu, void *stream);
+
+/* y [rows, n] int8 contiguous and scale [rows] of the rows of x (bf16 or fp16), as gg_rms_norm's int8 rows. Rules as above for n. */
+int gg_quantize_rows(int dtype, int64_t rows, int64_t n, const void *x, int64_t x_stride, int8_t *y, float *scale, void *stream);
 
 /* ---- router ---- */
 

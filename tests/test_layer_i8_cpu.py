@@ -1,0 +1,147 @@
+"""The operators of an int8 expert layer without a GPU: the C ABI refuses bad arguments and unsupported shapes before it
+touches the device, the torch functions check theirs."""
+import os
+import re
+
+import pytest
+import torch
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+BF16, FP16, E4M3, E5M2, FP32, INT8 = 0, 1, 2, 3, 4, 5
+INVALID, UNSUPPORTED, WORKSPACE = 2, 1, 4
+P = 4096  # an aligned address that is never dereferenced: every call below is refused first
+
+
+def _refused(pkg, status, want, text):
+    msg = pkg.load_library().gg_layer_last_error().decode()
+    assert status == want and text in msg, (status, msg)
+
+
+@pytest.mark.parametrize("change,want,text", [
+    (dict(dtype=FP32), INVALID, "dtype"),
+    (dict(wdtype=FP16), INVALID, "weight_dtype"),
+    (dict(mode=7), INVALID, "scale_mode"),
+    (dict(out=INT8), INVALID, "out_dtype"),
+    (dict(mode=1, out=INT8), INVALID, "out_dtype"),
+    (dict(mode=3, out=INT8), INVALID, "out_dtype"),
+    (dict(mode=2, out=BF16), INVALID, "out_dtype"),
+    (dict(mode=2, out=INT8, scale=None), INVALID, "scale is null"),
+    (dict(rows=-1), INVALID, "rows"),
+    (dict(hidden=100), UNSUPPORTED, "multiple of 8"),
+    (dict(hidden=32776), UNSUPPORTED, "at most 32768"),
+    (dict(x=None), INVALID, "x is null"),
+    (dict(xs=132), UNSUPPORTED, "row strides"),
+    (dict(h=None), INVALID, "h is null"),
+    (dict(hs=64), INVALID, "overlap"),
+    (dict(y=None), INVALID, "weight and y"),
+    (dict(b=P + 8), UNSUPPORTED, "aligned"),
+    (dict(mode=2, out=INT8, y=P + 4), UNSUPPORTED, "aligned"),
+    (dict(mode=1, out=E4M3, ws=None), INVALID, "workspace"),
+    (dict(mode=1, out=E4M3, mean=None), INVALID, "mean"),
+])
+def test_layer_norm_refusals(pkg, change, want, text):
+    a = dict(dtype=BF16, wdtype=BF16, out=BF16, mode=0, rows=4, hidden=128, x=P, xs=128, r=P, rs=128, w=P, b=P, h=P, hs=128, y=P,
+             mean=P, rstd=P, scale=P, ws=P)
+    a.update(change)
+    st = pkg.load_library().gg_layer_norm(a["dtype"], a["wdtype"], a["out"], a["mode"], a["rows"], a["hidden"], 1e-5, a["x"], a["xs"],
+                                          a["r"], a["rs"], a["w"], a["b"], a["h"], a["hs"], a["y"], a["mean"], a["rstd"], a["scale"],
+                                          a["ws"], None)
+    _refused(pkg, st, want, text)
+
+
+@pytest.mark.parametrize("change,want,text", [
+    (dict(dtype=INT8), INVALID, "dtype"),
+    (dict(hidden=12), UNSUPPORTED, "multiple of 8"),
+    (dict(g=None), INVALID, "grad_y is null"),
+    (dict(gx=None), INVALID, "grad_x"),
+    (dict(mean=None), INVALID, "mean"),
+    (dict(gb=None), INVALID, "grad_bias"),
+    (dict(gh=P + 2), UNSUPPORTED, "grad_h"),
+    (dict(gb=P + 8), UNSUPPORTED, "aligned"),
+    (dict(bytes=16), WORKSPACE, "workspace"),
+    (dict(ws=None), WORKSPACE, "workspace"),
+])
+def test_layer_norm_backward_refusals(pkg, change, want, text):
+    lib = pkg.load_library()
+    a = dict(dtype=BF16, hidden=128, g=P, h=P, w=P, mean=P, rstd=P, gh=P, gx=P, gw=P, gb=P, ws=P,
+             bytes=lib.gg_layer_norm_backward_workspace(2000, 128))
+    a.update(change)
+    st = lib.gg_layer_norm_backward(a["dtype"], a["dtype"], 2000, a["hidden"], a["g"], 128, a["h"], 128, a["w"], a["mean"], a["rstd"],
+                                    a["gh"], 128, a["gx"], a["gw"], a["gb"], a["ws"], a["bytes"], None)
+    _refused(pkg, st, want, text)
+
+
+@pytest.mark.parametrize("change,want,text", [
+    (dict(dtype=E4M3), INVALID, "dtype"),
+    (dict(out=FP16), INVALID, "out_dtype"),
+    (dict(rows=-1), INVALID, "rows"),
+    (dict(inner=20), UNSUPPORTED, "multiple of 8"),
+    (dict(inner=32776), UNSUPPORTED, "at most 32768"),
+    (dict(gu=None), INVALID, "gu is null"),
+    (dict(stride=132), UNSUPPORTED, "row strides"),
+    (dict(y=None), INVALID, "y must be"),
+    (dict(y=P + 8), UNSUPPORTED, "aligned"),
+    (dict(out=INT8, scale=None), INVALID, "scale"),
+    (dict(out=INT8, y=P + 4), UNSUPPORTED, "aligned"),
+])
+def test_silu_product_refusals(pkg, change, want, text):
+    a = dict(dtype=BF16, out=BF16, rows=4, inner=64, gu=P, stride=128, y=P, scale=P)
+    a.update(change)
+    st = pkg.load_library().gg_silu_product(a["dtype"], a["out"], a["rows"], a["inner"], a["gu"], a["stride"], a["y"], a["scale"], None)
+    _refused(pkg, st, want, text)
+
+
+def test_silu_backward_and_quantize_refusals(pkg):
+    lib = pkg.load_library()
+    _refused(pkg, lib.gg_silu_product_backward(BF16, 4, 64, None, 64, P, 128, P, None), INVALID, "grad_y is null")
+    _refused(pkg, lib.gg_silu_product_backward(BF16, 4, 64, P, 60, P, 128, P, None), UNSUPPORTED, "grad_y")
+    _refused(pkg, lib.gg_silu_product_backward(BF16, 4, 64, P, 64, P, 128, None, None), INVALID, "grad_gu")
+    _refused(pkg, lib.gg_silu_product_backward(BF16, 4, 64, P, 64, P, 128, P + 8, None), UNSUPPORTED, "grad_gu")
+    _refused(pkg, lib.gg_quantize_rows(FP32, 4, 64, P, 64, P, P, None), INVALID, "dtype")
+    _refused(pkg, lib.gg_quantize_rows(BF16, 4, 60, P, 64, P, P, None), UNSUPPORTED, "multiple of 8")
+    _refused(pkg, lib.gg_quantize_rows(BF16, 4, 64, P, -64, P, P, None), INVALID, "negative")
+    _refused(pkg, lib.gg_quantize_rows(BF16, 4, 64, P, 64, P, None, None), INVALID, "scale")
+    _refused(pkg, lib.gg_quantize_rows(BF16, 4, 64, P, 64, P + 4, P, None), UNSUPPORTED, "aligned")
+    for st in (lib.gg_silu_product(BF16, BF16, 0, 64, None, 0, None, None, None), lib.gg_quantize_rows(BF16, 0, 64, None, 0, None, None, None),
+               lib.gg_silu_product_backward(BF16, 0, 64, None, 0, None, 0, None, None)):
+        assert st == 0  # no rows: nothing to launch
+
+
+def test_torch_functions_refuse_host_tensors_and_types(pkg):
+    x, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.ones(64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="device"):
+        pkg.layer_norm(x, w)
+    with pytest.raises(TypeError, match="bfloat16"):
+        pkg.layer_norm(x.float(), w)
+    with pytest.raises(TypeError, match="bfloat16"):
+        pkg.layer_norm_backward(x, x.float(), w, None, None)
+    for f in (pkg.silu_product, pkg.quantize_rows):
+        with pytest.raises(ValueError, match="device"):
+            f(x)
+        with pytest.raises(TypeError, match="bfloat16"):
+            f(x.float())
+
+
+def test_backward_workgroups_fit_the_gpu(pkg):
+    """The layer norm's gradient takes no more workgroups than 256 CUs hold at once, by the compiler's report of each
+    instance's waves for each of a CU's four SIMDs: the numbers are written down, as the workspace's size needs them."""
+    path = os.path.join(ROOT, "groupgemm-cktile-optimized_amd", "lib", "resource_usage.txt")
+    if not os.path.exists(path):
+        pytest.skip("library not built")
+    waves, name = {}, None
+    with open(path, errors="replace") as f:
+        for line in f:
+            m = re.search(r"Function Name: (\S+)", line)
+            if m:  # <type, waves of a row, pieces, with the sums>
+                name = re.search(r"center_back_kernelINS0_\w+?ELi(\d+)ELi(\d+)ELb1E", m.group(1))
+            m = re.search(r"Occupancy \[waves/SIMD\]: (\d+)", line)
+            if m and name:
+                key = int(name.group(1)), int(name.group(2))
+                waves[key] = min(waves.get(key, 8), int(m.group(1)))
+    assert len(waves) >= 9
+    for hidden in (8, 512, 520, 1024, 1032, 2048, 2056, 4096, 4104, 6144, 6152, 8192, 8200, 12288, 12296, 16384, 16392, 32768):
+        wpr = 1 if hidden <= 1024 else 4 if hidden <= 8192 else 8
+        pieces = min(p for w, p in waves if w == wpr and p * 512 * w >= hidden)
+        of_block = max(wpr, 4)
+        blocks = pkg.load_library().gg_layer_norm_backward_workspace(1 << 20, hidden) // (8 * hidden)
+        assert 256 <= blocks <= 256 * (waves[wpr, pieces] * 4 // of_block), (hidden, blocks, waves[wpr, pieces])
