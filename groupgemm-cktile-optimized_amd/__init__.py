@@ -115,11 +115,16 @@ C_API = {
                                          ctypes.c_int64] + [ctypes.c_void_p] * 8),
     "gg_dispatch": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
                                    ctypes.c_int64] + [ctypes.c_void_p] * 4),
+    "gg_dispatch_scaled": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_void_p,
+                                          ctypes.c_int64] + [ctypes.c_void_p] * 6),
     "gg_dispatch_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64]
                              + [ctypes.c_void_p] * 4),
     "gg_combine": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64] + [ctypes.c_void_p] * 5),
     "gg_combine_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int, ctypes.c_int64, ctypes.c_int,
                                            ctypes.c_void_p, ctypes.c_int64] + [ctypes.c_void_p] * 7),
+    "gg_gemm_i8_workspace": (ctypes.c_size_t, [ctypes.c_int]),
+    "gg_gemm_i8": (ctypes.c_int, [ctypes.c_int, ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_void_p] * 8
+                   + [ctypes.c_size_t, ctypes.c_void_p]),
     "gg_gemm_w4": (ctypes.c_int, [ctypes.c_int, ctypes.c_int] + [ctypes.c_int64] * 3 + [ctypes.c_int] + [ctypes.c_void_p] * 8),
 }
 
@@ -827,9 +832,10 @@ def grouped_gemm(x, w, group_m, out=None, stream: Optional[int] = None, group_of
 
 # The operators around the grouped GEMM in a mixture-of-experts layer (moe_layer.py). Loaded on first use: that
 # module imports torch, which a process that times the hipBLASLt baselines must not.
-_LAYER = ("LayerNormOutput", "NormOutput", "Routing", "ScaledRows", "W4Weights", "combine", "combine_backward", "dispatch",
-          "dispatch_backward", "grouped_gemm_w4", "layer_norm", "layer_norm_backward", "pack_w4", "quantize_rows", "quantize_w4",
-          "rms_norm", "rms_norm_backward", "route", "route_backward", "silu_product", "silu_product_backward")
+_LAYER = ("I8Weights", "LayerNormOutput", "NormOutput", "Routing", "ScaledRows", "W4Weights", "combine", "combine_backward",
+          "dispatch", "dispatch_backward", "dispatch_scaled", "grouped_gemm_i8", "grouped_gemm_w4", "layer_norm",
+          "layer_norm_backward", "pack_w4", "quantize_i8", "quantize_rows", "quantize_w4", "rms_norm", "rms_norm_backward", "route",
+          "route_backward", "silu_product", "silu_product_backward")
 
 
 def __getattr__(name):

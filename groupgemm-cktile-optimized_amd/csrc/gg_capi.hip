@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "gg_few.h"
+#include "gg_i8.h"
 #include "gg_grouped_gemm.h"
 #include "gg_kernel.h"
 
@@ -52,6 +53,7 @@ struct gg_plan {
     gg::TableHeader    *d_header    = nullptr; // follows the table in the d_groups allocation
     bool                in_kernel_table = false; // the GEMM builds the table (no table launch)
     int64_t             in_rows     = 0;       // device-size plans: rows of the inputs
+    bool                i8          = false;   // device-size forward plans: int8 inputs (dtype: the output's)
     // Small-tile plans (use_small_tiles): the launch of gg_small.hip instead of the persistent one.
     bool                small       = false;
     gg::SmallArgs       sargs{};
@@ -682,6 +684,7 @@ int few_format(const gg_plan *plan) {
     case gg::kInE4M3: return gg::kFewE4M3;
     case gg::kInE5M2: return gg::kFewE5M2;
     case gg::kInE5M2xE4M3: return gg::kFewE5M2xE4M3;
+    case gg::kInI8: return plan->dtype == GG_DTYPE_FP16 ? gg::kFewI8F16 : gg::kFewI8;
     default: return plan->dtype == GG_DTYPE_FP16 ? gg::kFewF16 : gg::kFewBF16;
     }
 }
@@ -940,8 +943,10 @@ int plan_device_lens(gg_plan *plan, TableMemory memory, void *given, int op, int
         return fail(GG_ERR_INVALID, "group_lens is null");
     // Input formats: two equal 16-bit types, or fp8 (forward: both e4m3 or both e5m2; backward
     // also an e5m2 gradient with e4m3 w / x).
+    // int8 (plan->i8, gg::run_i8): the dtypes are the output's.
     const bool f8     = a_dtype == GG_DTYPE_FP8_E4M3 || a_dtype == GG_DTYPE_FP8_E5M2;
-    int        format = gg::kIn16;
+    const bool bytes  = f8 || plan->i8; // 1-byte inputs with scales
+    int        format = plan->i8 ? gg::kInI8 : gg::kIn16;
     if (f8) {
         if (a_dtype == GG_DTYPE_FP8_E4M3 && b_dtype == GG_DTYPE_FP8_E4M3)
             format = gg::kInE4M3;
@@ -967,7 +972,7 @@ int plan_device_lens(gg_plan *plan, TableMemory memory, void *given, int op, int
         return fail(GG_ERR_INVALID, "fp8 scales must be device pointers");
     // 16-byte rows; transposed fp8 operands move 16-column blocks
     const int64_t align_n = (f8 && op != GG_OP_FORWARD) ? 16 : 8;
-    const int64_t align_k = f8 ? 16 : 8;
+    const int64_t align_k = bytes ? 16 : 8;
     if (n % align_n != 0)
         return fail(GG_ERR_UNSUPPORTED, "N must be a multiple of " + std::to_string(align_n));
     if (k % align_k != 0)
@@ -977,8 +982,8 @@ int plan_device_lens(gg_plan *plan, TableMemory memory, void *given, int op, int
     if (k > (int64_t(1) << 21) || n > (int64_t(1) << 21))
         return fail(GG_ERR_UNSUPPORTED, "N and K must be at most 2097152");
     const int64_t lim   = int64_t(1) << 31;
-    const int64_t es    = f8 ? 1 : 2;
-    const int64_t steps = f8 ? 128 : gg::kTileK;
+    const int64_t es    = bytes ? 1 : 2;
+    const int64_t steps = bytes ? 128 : gg::kTileK;
     if (op == GG_OP_DGRAD && (n + steps) * k * es >= lim)
         return fail(GG_ERR_UNSUPPORTED, "one group's w must be smaller than 2 GiB");
     // wgrad: a group may hold every row
@@ -1056,8 +1061,8 @@ int plan_device_lens(gg_plan *plan, TableMemory memory, void *given, int op, int
     ka.tails = op == GG_OP_FORWARD ? (k_c % steps != 0)
                : op == GG_OP_DGRAD ? (k_c % steps != 0 || k % gg::kTileN != 0)
                                    : 1;
-    ka.x_scale         = f8 ? a_scale : nullptr;
-    ka.w_scale         = f8 ? b_scale : nullptr;
+    ka.x_scale         = bytes ? a_scale : nullptr;
+    ka.w_scale         = bytes ? b_scale : nullptr;
     if (op != GG_OP_FORWARD) {
         ka.lda = static_cast<int>(n);
         ka.ldb = static_cast<int>(k);
@@ -1184,6 +1189,30 @@ int run_plan(const gg_plan *plan, void *stream, bool zero_kernel) {
 }
 
 } // namespace
+
+size_t gg::i8_workspace(int group_num) { return device_table_bytes(group_num); }
+
+// The plan of device-size forward problems (plan_device_lens), run at once in the caller's workspace.
+int gg::run_i8(int out_dtype, int group_num, int64_t total_m, int64_t n, int64_t k, const int64_t *group_lens,
+               const int64_t *group_offs, const void *x, const void *w, const float *x_scale, const float *w_scale, void *out,
+               void *workspace, hipStream_t stream, char *why, size_t why_size) {
+    int st = GG_ERR_HIP;
+    why[0] = 0;
+    try {
+        g_last_error.clear();
+        gg_plan plan;
+        plan.i8 = true;
+        st      = plan_device_lens(&plan, kGiven, workspace, GG_OP_FORWARD, out_dtype, out_dtype, group_num, total_m, n, k, group_lens,
+                                   group_offs, x, w, x_scale, w_scale, out);
+        if (st == GG_OK)
+            st = run_plan(&plan, stream, true);
+        std::snprintf(why, why_size, "%s", g_last_error.c_str());
+    } catch (...) { // host memory
+        std::snprintf(why, why_size, "out of host memory");
+        st = GG_ERR_HIP;
+    }
+    return st;
+}
 
 extern "C" {
 

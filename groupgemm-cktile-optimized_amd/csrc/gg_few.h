@@ -1,13 +1,13 @@
 // Few-row kernels: forward and dgrad (gg_few.hip) and wgrad (gg_wfew.hip) of groups with few rows,
-// 16-bit and fp8. Host-side interface for the C ABI layer.
+// 16-bit and fp8, and the int8 forward. Host-side interface for the C ABI layer.
 #pragma once
 
 #include "gg_kernel.h"
 
 namespace gg {
 
-// Operand formats (A x B) of the few-row kernel.
-enum FewFormat : int { kFewBF16 = 0, kFewF16 = 1, kFewE4M3 = 2, kFewE5M2 = 3, kFewE5M2xE4M3 = 4 };
+// Operand formats (A x B) of the few-row kernel; int8 (forward only) by the type of its output.
+enum FewFormat : int { kFewBF16 = 0, kFewF16 = 1, kFewE4M3 = 2, kFewE5M2 = 3, kFewE5M2xE4M3 = 4, kFewI8 = 5, kFewI8F16 = 6 };
 
 // An instance: tiles of tile_m x tile_n, `waves` waves per workgroup that split the contraction,
 // a ring of `stages` chunks per wave; per_cu workgroups fit a CU (LDS), chunk_us is the time of one

@@ -1,5 +1,5 @@
 // Few-row kernel: forward (x w[g]^T) and dgrad (grad_out w[g]) of groups with few rows, 16-bit and
-// fp8, where the time is the reading of w or a problem is too small to fill the GPU with large tiles.
+// fp8, and the int8 forward, where the time is the reading of w or a problem is too small to fill the GPU with large tiles.
 //
 // What bounds it: w's bytes from HBM when the problem is large, and the latency of one tile's chain
 // (first loads, chunks, sums, stores) when it is small. So tiles are small (16-64 rows, 16-64
@@ -51,14 +51,20 @@ __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)"
 
 // Input formats of one instance (FewFormat in gg_kernel.h) as MFMA operands.
 template <int FMT> struct Fmt {
-    static constexpr bool f8  = FMT >= kFewE4M3;
-    static constexpr bool f16 = FMT == kFewF16;
-    static constexpr int  es  = f8 ? 1 : 2;
+    static constexpr bool i8  = FMT == kFewI8 || FMT == kFewI8F16;
+    static constexpr bool f8  = FMT >= kFewE4M3 && !i8;
+    static constexpr bool f16 = FMT == kFewF16 || FMT == kFewI8F16;
+    static constexpr int  es  = f8 || i8 ? 1 : 2;
+    using Sum = std::conditional_t<i8, i32x4, f32x4>;
     static constexpr int  kc  = 128 / es; // contraction values per chunk (128 bytes of a row)
     static constexpr bool a_e5m2 = FMT == kFewE5M2 || FMT == kFewE5M2xE4M3;
     static constexpr bool b_e5m2 = FMT == kFewE5M2;
 };
 
+// 16 x 16 products over 16 bytes of each row: 32 values of 16 bits or 64 of 8.
+__device__ __forceinline__ i32x4 mma_i8(const i32x4 &b, const i32x4 &a, const i32x4 &c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(b, a, c, 0, 0, 0);
+}
 template <bool F16> __device__ __forceinline__ f32x4 mma16(const i32x4 &b, const i32x4 &a, const f32x4 &c) {
     if constexpr (F16)
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(kf16x8, b), __builtin_bit_cast(kf16x8, a), c, 0, 0, 0);
@@ -69,6 +75,8 @@ template <bool F16> __device__ __forceinline__ f32x4 mma16(const i32x4 &b, const
 template <int FMT, bool MN, int MB, int NB, int W, int S>
 __global__ void __launch_bounds__(W * 64) few_gemm_kernel(const KernelArgs args) {
     using F = Fmt<FMT>;
+    using Sum = typename F::Sum;
+    static_assert(!F::i8 || !MN, "int8: forward only");
     constexpr int BM = 16 * MB, BN = 16 * NB;
     constexpr int kARegion = BM * 128, kChunk = (BM + BN) * 128; // bytes of one chunk: A, then B
     constexpr int kRing = W * S * kChunk;
@@ -179,12 +187,12 @@ __global__ void __launch_bounds__(W * 64) few_gemm_kernel(const KernelArgs args)
                       MN ? (boff + (c * F::kc + d * kBRowsPerDma) * ldb) | bcolbad : (boff + d * 8 * ldb + c * 128) | bad, br, 0);
         };
 
-        f32x4 acc[MB][NB];
+        Sum acc[MB][NB];
 #pragma unroll
         for (int i = 0; i < MB; ++i)
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-                acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+                acc[i][j] = Sum{0, 0, 0, 0};
 
         // ---- the K loop: chunk wave, wave + W, ...; a ring of S chunks per wave, no barrier ----
         const int chunks = (K + F::kc - 1) / F::kc;
@@ -260,7 +268,10 @@ __global__ void __launch_bounds__(W * 64) few_gemm_kernel(const KernelArgs args)
                         const i32x4 fa = a_piece(i, 4 * kh + fq);
 #pragma unroll
                         for (int j = 0; j < NB; ++j)
-                            acc[i][j] = mma16<F::f16>(fb[j], fa, acc[i][j]);
+                            if constexpr (F::i8)
+                                acc[i][j] = mma_i8(fb[j], fa, acc[i][j]);
+                            else
+                                acc[i][j] = mma16<F::f16>(fb[j], fa, acc[i][j]);
                     }
                 }
             }
@@ -282,7 +293,7 @@ __global__ void __launch_bounds__(W * 64) few_gemm_kernel(const KernelArgs args)
         for (int i = 0; i < MB; ++i)
 #pragma unroll
             for (int j = 0; j < NB; ++j)
-                *reinterpret_cast<f32x4 *>(sum + (wave * BM + 16 * i + fr) * kSumStride + 16 * j + 4 * fq) = acc[i][j];
+                *reinterpret_cast<Sum *>(sum + (wave * BM + 16 * i + fr) * kSumStride + 16 * j + 4 * fq) = acc[i][j];
         __syncthreads();
         float scale = 1.f;
         if constexpr (F::f8)
@@ -290,13 +301,21 @@ __global__ void __launch_bounds__(W * 64) few_gemm_kernel(const KernelArgs args)
         constexpr int kUnits = BM * BN / 4; // four columns each
         for (int u = tid; u < kUnits; u += W * 64) {
             const int row = u / (BN / 4), col = 4 * (u % (BN / 4));
-            f32x4     v   = *reinterpret_cast<const f32x4 *>(sum + row * kSumStride + col);
+            Sum       all = *reinterpret_cast<const Sum *>(sum + row * kSumStride + col);
 #pragma unroll
             for (int w = 1; w < W; ++w)
-                v += *reinterpret_cast<const f32x4 *>(sum + (w * BM + row) * kSumStride + col);
-            if constexpr (F::f8)
-                v *= scale;
+                all += *reinterpret_cast<const Sum *>(sum + (w * BM + row) * kSumStride + col);
             if (row < mv && tn * BN + col < N) {
+                f32x4 v = __builtin_convertvector(all, f32x4);
+                if constexpr (F::f8)
+                    v *= scale;
+                if constexpr (F::i8) {
+                    const f32x4 cs = *reinterpret_cast<const f32x4 *>(args.w_scale + static_cast<int64_t>(g) * N + static_cast<int64_t>(tn) * BN + col);
+                    const float rs = args.x_scale[row0 + row];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        v[e] = v[e] * cs[e] * rs;
+                }
                 uint16_t *o = static_cast<uint16_t *>(args.out) + (row0 + row) * static_cast<int64_t>(N) +
                               static_cast<int64_t>(tn) * BN + col;
                 *reinterpret_cast<u32x2 *>(o) = pack4<F::f16>(v);
@@ -338,6 +357,8 @@ hipError_t launch_few_gemm(const KernelArgs &a, int format, bool mn, int instanc
     case kFewE5M2: return mn ? launch_format<kFewE5M2, true>(a, instance, grid, s) : launch_format<kFewE5M2, false>(a, instance, grid, s);
     case kFewE5M2xE4M3: // an e5m2 gradient: dgrad only
         return mn ? launch_format<kFewE5M2xE4M3, true>(a, instance, grid, s) : hipErrorInvalidValue;
+    case kFewI8: return mn ? hipErrorInvalidValue : launch_format<kFewI8, false>(a, instance, grid, s);
+    case kFewI8F16: return mn ? hipErrorInvalidValue : launch_format<kFewI8F16, false>(a, instance, grid, s);
     default: return hipErrorInvalidValue;
     }
 }

@@ -1,13 +1,13 @@
 // One instance unit of the persistent grouped GEMM: the (input type, mode) pair GG_PART selects,
 // both variants (cross-tile and per-tile), (parts 14-17) the short-tile instances or (parts 18-19)
-// the short-wide forward instances. 16-bit forward units also hold the cross-tile instances with
-// the tail split (TAIL).
+// the short-wide forward instances; parts 20-21 are the int8 forward's, by the type of its output.
+// 16-bit forward units also hold the cross-tile instances with the tail split (TAIL).
 // The Makefile compiles this file once per part, in parallel; gg_kernel.hip's dispatch calls
 // launch_mode of every part.
 #include "gg_kernel_impl.h"
 
 #ifndef GG_PART
-#error "GG_PART selects the instance (0-19)"
+#error "GG_PART selects the instance (0-21)"
 #endif
 
 namespace gg {
@@ -81,7 +81,7 @@ void launch_short(const KernelArgs &args, bool cross, dim3 g, dim3 b, hipStream_
 }
 #endif
 
-#if GG_PART >= 18
+#if GG_PART == 18 || GG_PART == 19
 template <bool F16> void launch_short_wide(const KernelArgs &args, dim3 g, dim3 b, hipStream_t stream) {
     launch_cross<F16, make_mode(kFwd, kIn16), kShapeShortWide>(args, g, b, stream);
 }
@@ -100,7 +100,7 @@ extern "C" int GG_STAMP_CAT(gg_stamps_clear_p, GG_PART)() {
 }
 #endif
 
-// part -> (fp16 MFMA, mode); the dispatch's switch in gg_kernel.hip covers the same 14 pairs
+// part -> (fp16 MFMA, mode); the dispatch's switch in gg_kernel.hip covers the same 16 pairs
 #if GG_PART == 0
 template void launch_mode<false, make_mode(kFwd, kIn16)>(const KernelArgs &, bool, dim3, dim3, hipStream_t);
 #elif GG_PART == 1
@@ -141,6 +141,10 @@ template void launch_short<true, make_mode(kDgrad, kIn16)>(const KernelArgs &, b
 template void launch_short_wide<false>(const KernelArgs &, dim3, dim3, hipStream_t);
 #elif GG_PART == 19
 template void launch_short_wide<true>(const KernelArgs &, dim3, dim3, hipStream_t);
+#elif GG_PART == 20
+template void launch_mode<false, make_mode(kFwd, kInI8)>(const KernelArgs &, bool, dim3, dim3, hipStream_t);
+#elif GG_PART == 21
+template void launch_mode<true, make_mode(kFwd, kInI8)>(const KernelArgs &, bool, dim3, dim3, hipStream_t);
 #else
 #error "GG_PART out of range"
 #endif

@@ -15,7 +15,8 @@ enum InFormat : int {
     kIn16        = 0, // bf16 or fp16 inputs and output
     kInE4M3      = 1, // fp8 e4m3 A and B, bf16 output
     kInE5M2      = 2, // fp8 e5m2 A and B, bf16 output
-    kInE5M2xE4M3 = 3  // fp8 e5m2 A (the gradient), e4m3 B, bf16 output
+    kInE5M2xE4M3 = 3, // fp8 e5m2 A (the gradient), e4m3 B, bf16 output
+    kInI8        = 4  // int8 A and B (forward only), 16-bit output with a scale for each row and each column
 };
 constexpr int make_mode(int layout, int format) { return layout + 4 * format; }
 
@@ -38,6 +39,7 @@ constexpr int kInKernelTableGroups = 64;
 //   dgrad:   A = grad_out [sum(M), K], B^T = w[g] [K, N] (stored K x N), out = grad_x [sum(M), N]
 //   wgrad:   A^T = grad_out [M_g, m_out], B^T = x [M_g, N], out = grad_w [B, m_out, N], K = M_g
 // fp8 formats: 1-byte inputs, bf16 out scaled by a_scale[0] * b_scale[g] (x_scale / w_scale).
+// int8: 1-byte inputs, 16-bit out scaled by w_scale[g, n] and x_scale[m].
 struct KernelArgs {
     const void       *x;      // A operand storage (x, or grad_out for dgrad / wgrad)
     const void       *w;      // B operand storage (w, or x for wgrad)
@@ -55,8 +57,9 @@ struct KernelArgs {
     int               m_out;       // wgrad: output rows per group (0 otherwise)
     int               min_steps;   // wgrad: fewest K steps of a tile (kCrossMinStepsHost: a
                                    // cross-tile wgrad tile of a shorter group runs zero steps)
-    const float      *x_scale;     // fp8: device scale of the A operand (1 value)
-    const float      *w_scale;     // fp8: device scale of each group's B operand (group_num values)
+    const float      *x_scale;     // fp8: device scale of the A operand (1 value); int8: of each row
+    const float      *w_scale;     // fp8: device scale of each group's B operand (group_num values); int8: of each
+                                   // group's columns [group_num, n]
     const int        *d_total;     // device tile count (device-resident group sizes), or null:
                                    // then total_tiles holds it
     int               splits;      // split-K: K ranges per tile (1 = none; per-tile variant only)
@@ -128,7 +131,7 @@ constexpr bool has_short_tiles(int mode) {
 
 // Enqueue the persistent grouped GEMM: `grid` workgroups of 256 threads on `stream`.
 // fp16 selects the f16 MFMA, otherwise bf16 (16-bit formats); mode = make_mode(layout, format)
-// (fp8 formats write bf16, fp16 must be false).
+// (fp8 formats write bf16, fp16 must be false; int8: fp16 selects the output's type).
 // Returns the launch status.
 hipError_t launch_grouped_gemm(const KernelArgs &args, bool fp16, int grid, hipStream_t stream,
                                int mode = 0);

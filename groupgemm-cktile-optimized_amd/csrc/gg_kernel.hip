@@ -243,6 +243,7 @@ bool mode_supported(int mode, bool fp16) {
     case make_mode(kFwd, kIn16):
     case make_mode(kDgrad, kIn16):
     case make_mode(kWgrad, kIn16):
+    case make_mode(kFwd, kInI8):
         return true;
     case make_mode(kFwd, kInE4M3):
     case make_mode(kFwd, kInE5M2):
@@ -282,6 +283,7 @@ hipError_t launch_grouped_gemm(const KernelArgs &args, bool fp16, int grid, hipS
         case make_mode(kFwd, kIn16): launch_mode<true, make_mode(kFwd, kIn16)>(args, cross, g, b, stream); break;
         case make_mode(kDgrad, kIn16): launch_mode<true, make_mode(kDgrad, kIn16)>(args, cross, g, b, stream); break;
         case make_mode(kWgrad, kIn16): launch_mode<true, make_mode(kWgrad, kIn16)>(args, cross, g, b, stream); break;
+        case make_mode(kFwd, kInI8): launch_mode<true, make_mode(kFwd, kInI8)>(args, cross, g, b, stream); break;
         }
     } else {
         switch (mode) {
@@ -296,6 +298,7 @@ hipError_t launch_grouped_gemm(const KernelArgs &args, bool fp16, int grid, hipS
             GG_CASE(kWgrad, kInE4M3)
             GG_CASE(kWgrad, kInE5M2)
             GG_CASE(kWgrad, kInE5M2xE4M3)
+            GG_CASE(kFwd, kInI8)
         }
     }
 #undef GG_CASE

@@ -153,11 +153,15 @@ constexpr int b_stage(int s) { return (kAStages + s) * kOpBytes; }
 //   layout kDgrad: grad_x[g] = grad_out[g] @ w[g]             A = grad_out (K), B = w (MN)
 //   layout kWgrad: grad_w[g] = grad_out[g]^T @ x[g], K = M_g  A = grad_out (MN), B = x (MN)
 //   format kIn16 (bf16 / fp16), kInE4M3, kInE5M2 (both operands), kInE5M2xE4M3 (A e5m2, B
-//   e4m3); fp8 formats write bf16 out = (A B^T) * a_scale * b_scale[g].
+//   e4m3); fp8 formats write bf16 out = (A B^T) * a_scale * b_scale[g]. kInI8 (layout kFwd): int8 operands, int32
+//   sums, 16-bit out[m, n] = sum * b_scale[g, n] * a_scale[m]. v_mfma_i32_16x16x64_i8 takes 16 bytes of a row per lane
+//   in as many cycles as the 16-bit MFMAs, so a K step of 128 int8 values is, byte for byte and slot for slot, the
+//   16-bit forward's step of 64.
 // ---------------------------------------------------------------------------------------
 constexpr int  mode_layout(int m) { return m & 3; }
 constexpr int  mode_fmt(int m) { return m >> 2; }
-constexpr bool mode_f8(int m) { return mode_fmt(m) != kIn16; }
+constexpr bool mode_i8(int m) { return mode_fmt(m) == kInI8; }
+constexpr bool mode_f8(int m) { return mode_fmt(m) != kIn16 && !mode_i8(m); }
 constexpr bool mode_a_e5(int m) { return mode_fmt(m) == kInE5M2 || mode_fmt(m) == kInE5M2xE4M3; }
 constexpr bool mode_b_e5(int m) { return mode_fmt(m) == kInE5M2; }
 constexpr bool mode_a_mn(int m) { return mode_layout(m) == kWgrad; }
@@ -770,6 +774,16 @@ __device__ __forceinline__ void mfma_first(f32x4 &c, const i32x4 &a, const i32x4
         asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, 0" : "=a"(c) : "v"(a), "v"(b));
 }
 
+// int8 x int8 -> int32, 16 x 16 x 64; c holds the int32 sums' bits.
+template <bool FIRST> __device__ __forceinline__ void mfma_i8(f32x4 &c, const i32x4 &a, const i32x4 &b) {
+    if constexpr (FIRST)
+        asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, 0" : "=a"(c) : "v"(a), "v"(b));
+    else
+        asm volatile("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+}
+// An int32 sum as float32 (rounded to nearest even past 2^24).
+__device__ __forceinline__ float sum_value(float bits) { return static_cast<float>(__builtin_bit_cast(int, bits)); }
+
 // fp8 x fp8 -> fp32, 16 x 16 x 128 (gfx950): both sources are 32 bytes of a row per lane.
 // The kernel passes w (B) as src0 and x (A) as src1: cbsz gives src0's format, blgp src1's
 // (0 e4m3, 1 e5m2).
@@ -947,7 +961,8 @@ constexpr bool ct_instance(int mode, int shape, bool cross) {
     // modifiers follow the operands when x becomes its first source), 256-column tiles; and the
     // 16-bit forward's short-wide tiles, whose ninth column block keeps C^T accumulators
     return GG_CT && cross &&
-           (((mode == make_mode(kFwd, kIn16) || mode == make_mode(kFwd, kInE4M3) || mode == make_mode(kFwd, kInE5M2)) &&
+           (((mode == make_mode(kFwd, kIn16) || mode == make_mode(kFwd, kInE4M3) || mode == make_mode(kFwd, kInE5M2) ||
+              mode == make_mode(kFwd, kInI8)) &&
              shape == kShapeWide) ||
             (mode == make_mode(kFwd, kIn16) && shape == kShapeShortWide));
 }
@@ -986,8 +1001,9 @@ __global__ void __launch_bounds__(kThreads, 1) __attribute__((amdgpu_waves_per_e
 grouped_gemm_kernel(const KernelArgs args) {
     constexpr bool A_MN   = mode_a_mn(MODE), B_MN = mode_b_mn(MODE);
     constexpr bool F8     = mode_f8(MODE);
+    constexpr bool I8     = mode_i8(MODE);     // F16: the type of out
     constexpr int  LAYOUT = mode_layout(MODE);
-    constexpr int  ES     = F8 ? 1 : 2;        // input bytes per element
+    constexpr int  ES     = F8 || I8 ? 1 : 2;  // input bytes per element
     constexpr int  KS     = kRowBytes / ES;    // contraction values per K step
     // Row blocks of a wave: interleaved (wave wm's block mi is tile rows 16 (2 mi + wm) ..) when A
     // is K-major, so that the valid rows of a partial tile split evenly between the wm = 0 and
@@ -995,6 +1011,7 @@ grouped_gemm_kernel(const KernelArgs args) {
     constexpr bool NARROW = SHAPE == kShapeNarrow;
     constexpr bool SWIDE  = SHAPE == kShapeShortWide;
     constexpr bool SHORT  = SHAPE == kShapeShort || SWIDE; // at most 192 rows per tile
+    static_assert(!I8 || (LAYOUT == kFwd && SHAPE == kShapeWide && !TAIL), "int8: forward, 256 x 256 tiles");
     static_assert(!NARROW || (!CROSS && MODE == make_mode(kFwd, kIn16)), "narrow tiles: per-tile 16-bit forward");
     static_assert(!SHORT || MODE == make_mode(kFwd, kIn16) || MODE == make_mode(kDgrad, kIn16),
                   "short tiles: 16-bit forward and dgrad");
@@ -1081,7 +1098,7 @@ grouped_gemm_kernel(const KernelArgs args) {
                                                       : args.total_tiles;
     // Work units: a tile, or with split-K (per-tile variant only) one K range of a tile; unit
     // u = split * total_tiles + tile.
-    const int splits      = CROSS ? 1 : args.splits;
+    const int splits      = CROSS || I8 ? 1 : args.splits;
     // Tail split (cross-tile variant, host-size plans): the tiles of the last, partial round
     // (rem < half the grid) are cut into tail_s K ranges, one per workgroup, so every workgroup
     // ends the launch after its full rounds plus 1/tail_s of a tile instead of half the grid
@@ -1337,6 +1354,7 @@ grouped_gemm_kernel(const KernelArgs args) {
         int       tail;           // tail split: index of the last-round tile (-1: a whole tile)
         int       tail_k;         // tail split: the unit's K range (0 .. tail_s - 1)
         float     scale;          // fp8: x scale * w[g] scale (1 otherwise)
+        const float *row_scale, *col_scale; // int8: scales of the tile's first row and column
         uint32_t  rows;           // this wave's row blocks (bit mi) that hold a valid output
     };
     const int bad_off = static_cast<int>(0x80000000u);
@@ -1437,6 +1455,7 @@ grouped_gemm_kernel(const KernelArgs args) {
         tl.tail   = tail;
         tl.tail_k = split;
         tl.scale  = 1.0f;
+        tl.row_scale = tl.col_scale = nullptr;
         if constexpr (LAYOUT == kWgrad) {
             // A^T = grad_out rows of the group, columns tm*256..; B^T = x rows, columns tn*256..
             const int64_t o0a = static_cast<int64_t>(tm) * kTileM;
@@ -1470,6 +1489,10 @@ grouped_gemm_kernel(const KernelArgs args) {
                 tl.o0b = static_cast<int>(col0);
             }
             tl.c_ptr = static_cast<uint16_t *>(args.out) + row0 * N + col0;
+            if constexpr (I8) {
+                tl.row_scale = args.x_scale + row0;
+                tl.col_scale = args.w_scale + static_cast<int64_t>(g) * N + col0;
+            }
         }
         if constexpr (F8)
             tl.scale = to_const_space(args.x_scale)[0] * to_const_space(args.w_scale)[g];
@@ -1705,6 +1728,16 @@ grouped_gemm_kernel(const KernelArgs args) {
     auto stage_block = [&](const Tile &tl, int off, auto mi, auto ni, f32x4 v) {
         if constexpr (F8)
             v *= tl.scale;
+        if constexpr (I8) { // C^T: one row and four columns a lane (those past the tile's read zero: no branches here)
+            const auto  rr  = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(tl.row_scale), static_cast<short>(0), tl.m_valid * 4, 0x00020000);
+            const auto  rc  = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(tl.col_scale), static_cast<short>(0), tl.n_valid * 4, 0x00020000);
+            int row = wm * 16 + (lane & 15), col = wn * WCOLS + (lane >> 4) * 4;
+            fresh_v(row);
+            fresh_v(col);
+            const f32x4 cs = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rc, (col + ni * 16) * 4, 0, 0));
+            const float rs = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rr, (row + mi * A_BLK) * 4, 0, 0));
+            sfor<0, 4>([&](auto e) { v[int(e)] = sum_value(v[int(e)]) * cs[int(e)] * rs; });
+        }
         *reinterpret_cast<u32x2 *>(smem + off + mi * A_BLK * CSTR + ni * 16 * 2) = pack4<F16>(v);
     };
     // Second half of the LDS epilogue: the staged tile to global memory.
@@ -1817,9 +1850,48 @@ grouped_gemm_kernel(const KernelArgs args) {
     // the block at columns ecol .. +7, element s of its 8 column blocks' accumulators (column slot
     // l%16 of block ni is column 8 (l%16) + ni). Columns past n_valid get an out-of-range offset
     // (N % 8 == 0: a 16-byte chunk is all valid or all past N); rows past m_valid fall outside crs.
-    // fp8: scaled by the tile's x scale * w[g] scale (`scale`) before the conversion.
-    auto store_ct = [&](auto r, auto s_, const __amdgpu_buffer_rsrc_t &crs, int n_valid, float scale) {
+    // fp8: scaled by the tile's x scale * w[g] scale (`scale`) before the conversion. int8: by the columns' and the
+    // row's scales (`sc`).
+    //
+    // The scales of a tile travel as four registers a lane: entries l and 64 + l of the wave's 128 rows' scales (row
+    // block mi's row r is entry 16 mi + r) and of its 128 columns'. They are loaded when the tile begins, before the
+    // previous tile's 32 stores, and first read when the next one begins: by then more younger stores than operand DMAs
+    // are in flight, so the wait for them drains nothing. Where they are used, a lane gathers its eight columns' scales
+    // once a tile and each store's row scale from the lane that has it.
+    struct Scales {
+        float row[2], col[2];
+    };
+    auto load_scales = [&](const Tile &tl) {
+        Scales sc;
+        const auto rr = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(tl.row_scale), static_cast<short>(0), tl.m_valid * 4, 0x00020000);
+        const auto rc = __builtin_amdgcn_make_buffer_rsrc(const_cast<float *>(tl.col_scale), static_cast<short>(0), tl.n_valid * 4, 0x00020000);
+        sfor<0, 2>([&](auto h) {
+            const int e   = 64 * h + lane; // entries past the tile's rows or columns read zero
+            sc.row[int(h)] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rr, (2 * (e & ~15) + wm * 16 + (e & 15)) * 4, 0, 0));
+            sc.col[int(h)] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(rc, (wn * 128 + e) * 4, 0, 0));
+        });
+        return sc;
+    };
+    auto lane_value = [&](float v, int from4) { // v of lane from4 / 4
+        return __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(from4, __builtin_bit_cast(int, v)));
+    };
+    float col_scales[8]; // of the lane's columns 8 (l % 16) .. +7: entry 64 h + x is in half h of lanes x
+    auto  gather_cols = [&](const Scales &sc) {
+        int from4 = (lane & 7) * 32; // (opaque: the addresses are made here, not kept over the K loop)
+        fresh_v(from4);
+        sfor<0, 8>([&](auto ni) {
+            const float lo = lane_value(sc.col[0], from4 + 4 * ni), hi = lane_value(sc.col[1], from4 + 4 * ni);
+            col_scales[int(ni)] = lane & 8 ? hi : lo;
+        });
+    };
+    auto store_ct = [&](auto r, auto s_, const __amdgpu_buffer_rsrc_t &crs, int n_valid, float scale, const Scales &sc) {
         u32x4 d;
+        float row_scale = 1.f;
+        if constexpr (I8) { // entry 16 r + 4 q + s of the rows' scales
+            int from4 = q * 16;
+            fresh_v(from4);
+            row_scale = lane_value(sc.row[r >> 2], from4 + 64 * (r & 3) + 4 * s_);
+        }
         sfor<0, 4>([&](auto u) {
             // reads of these accumulators may not move above this point
             asm volatile("" : "+a"(acc[r][2 * u]), "+a"(acc[r][2 * u + 1]));
@@ -1827,6 +1899,10 @@ grouped_gemm_kernel(const KernelArgs args) {
             if constexpr (F8) {
                 v0 *= scale;
                 v1 *= scale;
+            }
+            if constexpr (I8) {
+                v0 = sum_value(v0) * col_scales[2 * u] * row_scale;
+                v1 = sum_value(v1) * col_scales[2 * u + 1] * row_scale;
             }
             if constexpr (F16)
                 d[int(u)] = __builtin_bit_cast(unsigned, f16x2{(_Float16)v0, (_Float16)v1});
@@ -1845,10 +1921,11 @@ grouped_gemm_kernel(const KernelArgs args) {
     // Store s (0-3) of the previous tile's row block r: packed with the next one for even s;
     // s = 4 (short-wide tiles): the ninth column block.
     constexpr int kEpiStores = SWIDE ? 5 : 4;
+    Scales        cur_scales{}, prev_scales{}; // int8
     auto epi_store = [&](auto r, auto s_) {
         sched_fence();
         if constexpr (CT && s_ < 4) {
-            store_ct(r, s_, prev_crs, prev_n, prev_scale);
+            store_ct(r, s_, prev_crs, prev_n, prev_scale, prev_scales);
         } else if constexpr (s_ == 4) {
             store_block9(r, prev_crs, prev_n);
         } else {
@@ -1864,6 +1941,11 @@ grouped_gemm_kernel(const KernelArgs args) {
         constexpr int kh = idx / P::nc, ni = idx % P::nc; // fp8: one MFMA per (mi, ni), kh = 0
         if constexpr (ni >= NBLK || mi >= RB) {
             // narrow tiles: no 8th column block; short tiles: no row blocks 6 and 7
+        } else if constexpr (I8) {
+            if constexpr (CT)
+                mfma_i8<FIRST && kh == 0>(acc[mi][ni], fa[mi & 1][kh], fb[SA][ni][kh]);
+            else
+                mfma_i8<FIRST && kh == 0>(acc[mi][ni], fb[SA][ni][kh], fa[mi & 1][kh]);
         } else if constexpr (F8) {
             const i32x8 bw = __builtin_shufflevector(fb[SA][ni][0], fb[SA][ni][1], 0, 1, 2, 3, 4, 5, 6, 7);
             const i32x8 ax = __builtin_shufflevector(fa[mi & 1][0], fa[mi & 1][1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -2034,6 +2116,11 @@ grouped_gemm_kernel(const KernelArgs args) {
         // with 5 or more rows it is no faster than a full step.) Loops in sequence, not branches
         // around whole steps, so the accumulators stay in place.
         const bool thin = kThin && __builtin_amdgcn_readfirstlane(cur.rows) <= 0xfu;
+        if constexpr (I8 && CROSS) {
+            prev_scales = cur_scales;
+            cur_scales  = load_scales(cur);
+            gather_cols(prev_scales);
+        }
         if constexpr (CROSS) {
             // First step: stores the previous tile's accumulators while it overwrites them (to
             // nowhere for the first tile). Always the same code, so the accumulators never
@@ -2112,7 +2199,9 @@ grouped_gemm_kernel(const KernelArgs args) {
             // Store this tile through LDS (split-K: its partial sums to the workspace); the next
             // one starts cold at the top of the loop (the stores were issued before its DMAs and
             // complete first).
-            if (splits > 1)
+            if constexpr (I8) // (never split)
+                epilogue_lds(cur);
+            else if (splits > 1)
                 store_partial(t);
             else
                 epilogue_lds(cur);
@@ -2137,6 +2226,8 @@ grouped_gemm_kernel(const KernelArgs args) {
         GG_STAMP(kStampSlots - 2);
         wait_vm_lds_barrier<0>();
         asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 3" ::: "memory"); // MFMA -> VALU read distance
+        if constexpr (I8)
+            gather_cols(cur_scales);
         Tile       tl   = cur;
         const bool part = TAIL && tl.tail >= 0;
         if constexpr (TAIL)
@@ -2159,7 +2250,7 @@ grouped_gemm_kernel(const KernelArgs args) {
                                                                poff + ((32 * mi + s_) * 256) * 4 + 16 * hf, 0, 0);
                     });
                 }
-                store_ct(mi, s_, crs, tl.n_valid, tl.scale);
+                store_ct(mi, s_, crs, tl.n_valid, tl.scale, cur_scales);
             });
         });
     } else if constexpr (CROSS) {

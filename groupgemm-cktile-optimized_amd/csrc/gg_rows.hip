@@ -20,6 +20,8 @@ struct RowArgs {
     const float   *weights;
     float         *grad_weights;
     const int64_t *offs;
+    const float   *scale;     // dispatch with scales: of each token's row,
+    float         *out_scale; // and of each row that is written
     int64_t        tokens, stride; // stride of the tokens' rows that are read, in bytes
     int            top_k, experts, pieces; // 16-byte pieces of a row
 };
@@ -44,11 +46,19 @@ __device__ __forceinline__ void zero_tail(const RowArgs &a) {
             static_cast<u32x4 *>(a.out)[row * a.pieces + i] = u32x4{0, 0, 0, 0};
 }
 
-// A token's row to the rows of its slots: read once, written top_k times. PAST: the stores go past the caches.
-template <bool PAST> __global__ void __launch_bounds__(1024) dispatch_kernel(const RowArgs a) {
+// A token's row to the rows of its slots: read once, written top_k times. PAST: the stores go past the caches. SCALED: the
+// row's scale goes with it (top_k <= 32, and a workgroup has 64 threads at least).
+template <bool PAST, bool SCALED> __global__ void __launch_bounds__(1024) dispatch_kernel(const RowArgs a) {
     for (int64_t t = blockIdx.x; t < a.tokens; t += gridDim.x) {
         const u32x4 *x    = reinterpret_cast<const u32x4 *>(static_cast<const char *>(a.in) + t * a.stride);
         const int   *rows = a.rows + t * a.top_k;
+        if constexpr (SCALED) {
+            if (static_cast<int>(threadIdx.x) < a.top_k) {
+                const int64_t row = rows[threadIdx.x];
+                if (has_row(a, row))
+                    a.out_scale[row] = a.scale[t];
+            }
+        }
         for (int i = threadIdx.x; i < a.pieces; i += blockDim.x) {
             const u32x4 v = x[i];
             for (int s = 0; s < a.top_k; ++s) {
@@ -59,6 +69,12 @@ template <bool PAST> __global__ void __launch_bounds__(1024) dispatch_kernel(con
         }
     }
     zero_tail(a);
+    if constexpr (SCALED) {
+        const int64_t pairs = a.tokens * a.top_k;
+        for (int64_t row = max(a.offs[a.experts], int64_t(0)) + static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; row < pairs;
+             row += static_cast<int64_t>(gridDim.x) * blockDim.x)
+            a.out_scale[row] = 0.f;
+    }
 }
 
 // out[t] = sum of the rows of its slots (WEIGHTED: times their weights), in the order of the slots, four of whose
@@ -162,8 +178,10 @@ using namespace gg::layer;
 
 extern "C" {
 
-int gg_dispatch(int elem_size, int64_t tokens, int top_k, int64_t hidden, int experts, const void *x, int64_t stride,
-                const int *rows, const int64_t *offs, void *xs, void *stream) {
+// Both forms of dispatch (scaled: scale and xs_scale).
+static int dispatch_rows(bool scaled, int elem_size, int64_t tokens, int top_k, int64_t hidden, int experts, const void *x,
+                         int64_t stride, const float *scale, const int *rows, const int64_t *offs, void *xs, float *xs_scale,
+                         void *stream) {
     g_error[0] = 0;
     if (elem_size != 1 && elem_size != 2 && elem_size != 4)
         return fail(GG_ERR_INVALID, "elem_size must be 1, 2 or 4");
@@ -175,6 +193,8 @@ int gg_dispatch(int elem_size, int64_t tokens, int top_k, int64_t hidden, int ex
         return fail(GG_ERR_INVALID, "rows and offs must be device pointers");
     if (tokens > 1 && stride < 0)
         return fail(GG_ERR_INVALID, "x has a negative row stride");
+    if (scaled && (scale == nullptr || xs_scale == nullptr))
+        return fail(GG_ERR_INVALID, "scale and xs_scale must be device pointers");
     if (!pieces(x) || !pieces(xs) || (tokens > 1 && stride * elem_size % 16 != 0))
         return fail(GG_ERR_UNSUPPORTED, "x and xs must be 16-byte aligned, strides multiples of 16 bytes");
     RowArgs a{};
@@ -187,8 +207,24 @@ int gg_dispatch(int elem_size, int64_t tokens, int top_k, int64_t hidden, int ex
     a.top_k   = top_k;
     a.experts = experts;
     a.pieces  = static_cast<int>(hidden * elem_size / 16);
-    return launch("dispatch", past_caches(a) ? dispatch_kernel<true> : dispatch_kernel<false>, std::min(tokens, kMaxGrid),
+    const bool past = past_caches(a);
+    const auto plain = past ? dispatch_kernel<true, false> : dispatch_kernel<false, false>;
+    if (!scaled)
+        return launch("dispatch", plain, std::min(tokens, kMaxGrid), row_threads(a.pieces), static_cast<hipStream_t>(stream), a);
+    a.scale     = scale;
+    a.out_scale = xs_scale;
+    return launch("dispatch_scaled", past ? dispatch_kernel<true, true> : dispatch_kernel<false, true>, std::min(tokens, kMaxGrid),
                   row_threads(a.pieces), static_cast<hipStream_t>(stream), a);
+}
+
+int gg_dispatch(int elem_size, int64_t tokens, int top_k, int64_t hidden, int experts, const void *x, int64_t stride,
+                const int *rows, const int64_t *offs, void *xs, void *stream) {
+    return dispatch_rows(false, elem_size, tokens, top_k, hidden, experts, x, stride, nullptr, rows, offs, xs, nullptr, stream);
+}
+
+int gg_dispatch_scaled(int elem_size, int64_t tokens, int top_k, int64_t hidden, int experts, const void *x, int64_t stride,
+                       const float *scale, const int *rows, const int64_t *offs, void *xs, float *xs_scale, void *stream) {
+    return dispatch_rows(true, elem_size, tokens, top_k, hidden, experts, x, stride, scale, rows, offs, xs, xs_scale, stream);
 }
 
 static int sum_rows(const char *what, bool weighted, int dtype, int64_t tokens, int top_k, int64_t hidden, const void *y,

@@ -1,10 +1,11 @@
 """The operators around the grouped GEMM in a mixture-of-experts layer, for torch tensors, over the C
-ABI in include/gg_moe_layer.h: RMS norm with the residual's addition and an fp8 output, router with
-balance loss, dispatch and combine of the experts' rows, grouped products with 4-bit weights.
+ABI in include/gg_moe_layer.h: RMS norm and layer norm with the residual's addition and an 8-bit output,
+gated activation, rows of int8, router with balance loss, dispatch and combine of the experts' rows,
+grouped products with 4-bit weights and in 8-bit integers.
 
 Every function enqueues its kernels on the current stream of its tensors' device, or on `stream` (a
-raw hipStream_t handle), and returns without waiting (but grouped_gemm_w4 with host group sizes, which
-copies them to the device and waits for that). Outputs and workspaces come from torch's allocator, from
+raw hipStream_t handle), and returns without waiting (but grouped_gemm_w4 and grouped_gemm_i8 with host
+group sizes, which copy them to the device and wait for that). Outputs and workspaces come from torch's allocator, from
 the memory of the stream that the kernels run on. With `stream`, the caller orders that stream after
 whatever wrote the inputs, and what reads the outputs on another stream after it; the allocator is told
 of both streams' uses, so a tensor may be dropped before the work is done.
@@ -470,6 +471,27 @@ def dispatch(x, routing: Routing, out=None, stream: Optional[int] = None):
     return xs
 
 
+def dispatch_scaled(x, scale, routing: Routing, out=None, stream: Optional[int] = None) -> ScaledRows:
+    """dispatch of rows that have a scale each (gg_dispatch_scaled): x [T, H] and scale [T] float32, as layer_norm,
+    rms_norm and quantize_rows give them, to xs [T * k, H] and its scales [T * k]; those of the zeroed rows are 0."""
+    if stream is not None:
+        return _on(stream, dispatch_scaled, x, scale, routing, out)
+    stride, dev = _matrix("x", x), x.device
+    rows, t, k = _rows(routing, dev)
+    offs = _offs(routing, dev)
+    if x.shape[0] != t:
+        raise ValueError("x must have a row for each token of the routing")
+    _flat("scale", scale, torch.float32, (t,), dev)
+    n = x.shape[1]
+    if x.element_size() not in (1, 2, 4):
+        raise TypeError("x must be of a type of 1, 2 or 4 bytes")
+    xs = _out(out, x.dtype, (t * k, n), dev)
+    s = torch.empty(t * k, dtype=torch.float32, device=dev)
+    _call(_lib.gg_dispatch_scaled, dev, (x.element_size(), t, k, n, offs.numel() - 1, x.data_ptr(), stride, scale.data_ptr(),
+                                         rows.data_ptr(), offs.data_ptr(), xs.data_ptr(), s.data_ptr()))
+    return ScaledRows(xs, s)
+
+
 def _pairs(name: str, y, t: int, k: int):
     if y.dtype not in _T16:
         raise TypeError(f"{name} must be bfloat16 or float16")
@@ -632,4 +654,82 @@ def grouped_gemm_w4(x, w: W4Weights, group_m, out=None, stream: Optional[int] = 
     o = _out(out, x.dtype, (m, n), dev)
     _call(_lib.gg_gemm_w4, dev, (dt, b, m, n, k, group, group_m.data_ptr(), _ptr(group_offs), x.data_ptr(), packed.data_ptr(),
                                  scales.data_ptr(), _ptr(zeros), o.data_ptr()))
+    return o
+
+
+# ---- 8-bit integers ----
+
+
+class I8Weights(NamedTuple):
+    """Weights [B, N, K] in int8 and a float32 scale for each output channel, scales [B, N]: w[b, n] * scales[b, n]."""
+    w: "torch.Tensor"
+    scales: "torch.Tensor"
+
+
+def quantize_i8(w) -> I8Weights:
+    """int8 form of weights [B, N, K] (bf16, fp16 or float32), one scale for each output channel: max |w| / 127 (1 for a
+    channel of zeros), values rounded to the nearest. Any device."""
+    if w.dim() != 3 or w.dtype not in (*_T16, torch.float32):
+        raise ValueError("w must be bfloat16, float16 or float32 [B, N, K]")
+    q = torch.empty(w.shape, dtype=torch.int8, device=w.device)
+    s = torch.empty(w.shape[:2], dtype=torch.float32, device=w.device)
+    for i in range(w.shape[0]):  # one matrix at a time: the layers' weights may fill the card
+        v = w[i].float()
+        top = v.abs().amax(1) / 127
+        s[i] = torch.where(top > 0, top, torch.ones_like(top))
+        q[i] = (v / s[i][:, None]).round().clamp(-127, 127).to(torch.int8)
+    return I8Weights(q, s)
+
+
+def grouped_gemm_i8(x, w: I8Weights, group_m, x_scale=None, out_dtype=None, out=None, stream: Optional[int] = None,
+                    group_offs=None):
+    """out [sum(M), N] = x[rows of g] @ w[g]^T in 8-bit integers (gg_gemm_i8): x int8 [sum(M), K] with x_scale [sum(M)]
+    float32, the ScaledRows of layer_norm, silu_product, quantize_rows or dispatch_scaled, to out_dtype (bfloat16 if None,
+    or float16); or x bfloat16 or float16, whose rows are first rounded by quantize_rows, to x's type. group_m as in
+    grouped_gemm: a host sequence of row counts, or a device int64 tensor [B] that is never read on the host (with
+    optional device offsets); a device group that does not lie inside x gets no work, and rows of no group are not
+    written. For any number of rows. No backward pass: train in 16 bits."""
+    if stream is not None:
+        return _on(stream, grouped_gemm_i8, x, w, group_m, x_scale, out_dtype, out, None, group_offs)
+    q, scales = w
+    if q.dim() != 3 or q.dtype != torch.int8 or not q.is_contiguous():
+        raise ValueError("w must be contiguous int8 [B, N, K] with its scales")
+    b, n, k = q.shape
+    dev = x.device
+    if x.dim() != 2 or not x.is_cuda or x.shape[1] != k:
+        raise ValueError("x must be a device matrix with K columns")
+    if x.dtype == torch.int8:
+        if x_scale is None:
+            raise ValueError("int8 x needs x_scale, a scale for each row")
+        if out_dtype is None:
+            out_dtype = torch.bfloat16
+        elif out_dtype not in _T16:
+            raise TypeError("out_dtype must be bfloat16 or float16")
+        if not x.is_contiguous():
+            raise ValueError("int8 x must be contiguous")
+    elif x.dtype in _T16:
+        if x_scale is not None or out_dtype not in (None, x.dtype):
+            raise ValueError("x_scale and out_dtype go with an int8 x")
+        out_dtype = x.dtype
+    else:
+        raise TypeError("x must be int8, bfloat16 or float16")
+    _flat("w.scales", scales, torch.float32, (b, n), dev)
+    if q.device != dev:
+        raise ValueError("w must be on x's device")
+    m = x.shape[0]
+    if not _device_sizes(group_m, group_offs, b):
+        if len(group_m) != b or any(r < 0 for r in group_m) or sum(group_m) != m:
+            raise ValueError("shape mismatch between x, w and group_m")
+        group_m = torch.tensor(list(group_m), dtype=torch.int64, device=dev)
+    elif group_m.device != dev or (group_offs is not None and group_offs.device != dev):
+        raise ValueError("group sizes must be on x's device")
+    if x.dtype != torch.int8:
+        x, x_scale = quantize_rows(x)
+    else:
+        _flat("x_scale", x_scale, torch.float32, (m,), dev)
+    o = _out(out, out_dtype, (m, n), dev)
+    need = _lib.gg_gemm_i8_workspace(b)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _call(_lib.gg_gemm_i8, dev, (_T16[out_dtype], b, m, n, k, group_m.data_ptr(), _ptr(group_offs), x.data_ptr(), q.data_ptr(),
+                                 x_scale.data_ptr(), scales.data_ptr(), o.data_ptr(), ws.data_ptr(), need))
     return o

@@ -166,6 +166,7 @@ int gg_route_backward(int dtype, int64_t tokens, int experts, int top_k, int ren
 /*
  * dispatch: xs[rows[t, s]] = x[t] for the rows a router gave (xs [tokens * top_k, hidden]); rows of xs
  * past the last expert's (slots of -1 leave as many) are zeroed. elem_size: bytes of an element (1, 2 or 4).
+ * dispatch_scaled: the same, and xs_scale[rows[t, s]] = scale[t] (float32) for rows that have a scale each; 0 for the zeroed rows.
  * dispatch_backward: grad_x[t] = sum over s of grad_xs[rows[t, s]] (bf16 or fp16).
  * combine: out[t] = sum over s of weights[t, s] * y[rows[t, s]] (bf16 or fp16); 0 for a token without rows.
  * combine_backward: grad_y[rows[t, s]] = weights[t, s] * grad_out[t] (rows past the last expert's
@@ -177,6 +178,8 @@ int gg_route_backward(int dtype, int64_t tokens, int experts, int top_k, int ren
  */
 int gg_dispatch(int elem_size, int64_t tokens, int top_k, int64_t hidden, int experts, const void *x, int64_t stride,
                 const int *rows, const int64_t *offs, void *xs, void *stream);
+int gg_dispatch_scaled(int elem_size, int64_t tokens, int top_k, int64_t hidden, int experts, const void *x, int64_t stride,
+                       const float *scale, const int *rows, const int64_t *offs, void *xs, float *xs_scale, void *stream);
 int gg_dispatch_backward(int dtype, int64_t tokens, int top_k, int64_t hidden, const void *grad_xs, const int *rows,
                          void *grad_x, void *stream);
 int gg_combine(int dtype, int64_t tokens, int top_k, int64_t hidden, const void *y, const int *rows,
@@ -209,6 +212,25 @@ int gg_combine_backward(int dtype, int64_t tokens, int top_k, int64_t hidden, in
 int gg_gemm_w4(int dtype, int group_num, int64_t total_m, int64_t n, int64_t k, int group, const int64_t *group_lens,
                const int64_t *group_offs, const void *x, const void *packed, const void *scales, const uint8_t *zeros,
                void *out, void *stream);
+
+/* ---- grouped products in 8-bit integers ---- */
+
+/*
+ * out[rows of g] = x[rows of g] @ w[g]^T * scales: out[m, n] = sum_k x[m, k] w[g, n, k] * w_scale[g, n] * x_scale[m]
+ * for x [total_m, k] and w [group_num, n, k] int8 (-128 .. 127), x_scale [total_m] and w_scale [group_num, n] float32,
+ * out [total_m, n] of out_dtype (bf16 or fp16), all contiguous. The sums are int32 and exact; each is made a float32,
+ * multiplied by w_scale and then by x_scale, and rounded to out_dtype once. Any number of rows a group, one to very many.
+ * group_lens / group_offs: device sizes as in gg_prepare_device_lens_op; a group whose rows are not inside
+ * [0, total_m) gets no work (and is not reported); rows of out that belong to no group are not written.
+ * workspace: gg_gemm_i8_workspace(group_num) bytes, 16-byte aligned, not shared by calls that may overlap.
+ * (The first call on a device looks up that device's properties, and so must run outside stream capture.)
+ * GG_ERR_UNSUPPORTED unless n % 8 == 0, k % 16 == 0, x, w, w_scale and out 16-byte aligned, n at most 2097152, k below
+ * 131072 (past it a sum may leave int32), group_num at most 8192 and total_m at most 134217728.
+ */
+size_t gg_gemm_i8_workspace(int group_num);
+int gg_gemm_i8(int out_dtype, int group_num, int64_t total_m, int64_t n, int64_t k, const int64_t *group_lens,
+               const int64_t *group_offs, const int8_t *x, const int8_t *w, const float *x_scale, const float *w_scale,
+               void *out, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

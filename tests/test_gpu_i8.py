@@ -1,0 +1,308 @@
+"""Grouped products in 8-bit integers, bit for bit.
+
+The int32 sums are exact, and what follows is one correctly rounded operation after the other: the sum as float32, times
+the channel's scale, times the row's scale, rounded to 16 bits. So the outputs are those of the same steps on exact sums
+(float64 products of int8 values are whole numbers below 2^53), with no tolerance.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs an MI355X", allow_module_level=True)
+
+DEV = torch.device("cuda:0")
+BF, FP, I8 = torch.bfloat16, torch.float16, torch.int8
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _ints(g, *shape):
+    return torch.randint(-128, 128, shape, device=DEV, generator=g).to(I8)
+
+
+def _data(b, m, n, k, seed):
+    g = _gen(seed)
+    x, w = _ints(g, m, k), _ints(g, b, n, k)
+    xs = torch.rand(m, device=DEV, generator=g) / 128 / k**0.5 + 1e-4
+    ws = torch.rand(b, n, device=DEV, generator=g) / 128 + 1e-4
+    return x, xs, w, ws
+
+
+def _want(x, xs, w, ws, lens, offs, dtype, fill):
+    out = torch.full((x.shape[0], w.shape[1]), fill, device=DEV, dtype=dtype)
+    for g, (m, o) in enumerate(zip(lens, offs)):
+        if m:
+            acc = x[o:o + m].double() @ w[g].double().t().contiguous()
+            out[o:o + m] = (acc.float() * ws[g] * xs[o:o + m, None]).to(dtype)
+    return out
+
+
+def _offs(lens, gap=0):
+    at, offs = gap, []
+    for m in lens:
+        offs.append(at)
+        at += m + gap
+    return offs, at
+
+
+def _run(pkg, x, xs, w, ws, lens, dtype, offs=None):
+    """The call over device sizes into a guarded output."""
+    m, n = x.shape[0], w.shape[1]
+    whole = torch.full((m * n + 64,), 3.0, device=DEV, dtype=dtype)
+    d = torch.tensor(lens, dtype=torch.int64, device=DEV)
+    o = None if offs is None else torch.tensor([*offs, 0], dtype=torch.int64, device=DEV)
+    got = pkg.grouped_gemm_i8(x, pkg.I8Weights(w, ws), d, xs, dtype, out=whole[:m * n].view(m, n), group_offs=o)
+    assert bool((whole[m * n:] == 3).all())
+    return got
+
+
+@pytest.fixture(params=["persistent", 0, 1, 2, 3, 4])
+def kernel(request, monkeypatch):
+    """The persistent kernel, or one instance of the few-row one."""
+    if request.param != "persistent":
+        monkeypatch.delenv("GG_SMALL")
+        monkeypatch.setenv("GG_FEW", str(request.param))
+    return request.param
+
+
+CASES = [  # n, k, rows of the groups
+    (8, 16, [1]),
+    (16, 48, [0, 1, 0]),
+    (24, 160, [3, 0, 16]),
+    (64, 128, [17, 1, 15, 0, 2]),
+    (256, 512, [256]),
+    (264, 192, [33, 64, 65, 257]),
+    (512, 1024, [1, 1, 0, 1, 1, 0, 0, 1]),
+    (520, 640, [300, 0, 700, 5, 129]),
+    (1000, 896, [100, 31, 513]),
+    (2880, 2880, [8, 0, 5]),
+    (136, 2048, [130, 0, 0, 7]),
+    (4096, 7168, [1, 2]),
+    (8, 131056, [3]),
+    (1032, 528, [40] * 70),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("n,k,lens", CASES)
+def test_every_kernel(pkg, kernel, dtype, n, k, lens):
+    offs, m = _offs(lens)
+    x, xs, w, ws = _data(len(lens), m, n, k, n + k)
+    want = _want(x, xs, w, ws, lens, offs, dtype, 3.0)
+    got = _run(pkg, x, xs, w, ws, lens, dtype)
+    assert torch.equal(got, want)
+    assert torch.equal(_run(pkg, x, xs, w, ws, lens, dtype), got)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("n,k,lens", [(264, 640, [33, 0, 300, 1]), (64, 144, [5, 17]), (512, 528, [9] * 66)])
+def test_groups_apart_and_outside(pkg, kernel, dtype, n, k, lens):
+    """Rows between the groups stay as they were; a group outside x, or of a negative length, gets no work."""
+    offs, m = _offs(lens, gap=3)
+    x, xs, w, ws = _data(len(lens), m, n, k, n * k)
+    assert torch.equal(_run(pkg, x, xs, w, ws, lens, dtype, offs), _want(x, xs, w, ws, lens, offs, dtype, 3.0))
+    bad_lens, bad_offs = list(lens), list(offs)
+    bad_offs[1] = m - lens[1] + 1  # ends one row behind x
+    if lens[1] == 0:
+        bad_lens[1], bad_offs[1] = 2, m - 1
+    bad_lens[0] = -4
+    ok = [0, 0] + list(lens[2:])
+    got = _run(pkg, x, xs, w, ws, bad_lens, dtype, bad_offs)
+    assert torch.equal(got, _want(x, xs, w, ws, ok, offs, dtype, 3.0))
+
+
+def test_largest_sums(pkg, kernel):
+    """-128 x -128 over the longest contraction: the largest sum there is, 16384 * 131056."""
+    k = 131056
+    x, w = torch.full((5, k), -128, device=DEV, dtype=I8), torch.full((2, 8, k), -128, device=DEV, dtype=I8)
+    w[1] = 127
+    xs, ws = torch.full((5,), 2.0**-16, device=DEV), torch.full((2, 8), 2.0**-8, device=DEV)
+    lens, offs = [2, 3], [0, 2]
+    got = _run(pkg, x, xs, w, ws, lens, BF)
+    assert torch.equal(got, _want(x, xs, w, ws, lens, offs, BF, 0.0)) and float(got[0, 0]) > 0 > float(got[2, 0])
+
+
+def test_scales_that_are_not_finite(pkg, kernel):
+    x, xs, w, ws = _data(2, 300, 512, 640, 5)
+    xs[7], xs[200], xs[250] = float("nan"), float("inf"), 0.0
+    ws[1, 33] = float("nan")
+    lens, offs = [150, 150], [0, 150]
+    got, want = _run(pkg, x, xs, w, ws, lens, BF), _want(x, xs, w, ws, lens, offs, BF, 0.0)
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got.nan_to_num(0), want.nan_to_num(0))
+    assert bool(got[7].isnan().all()) and bool((got[250] == 0).logical_or(got[250].isnan()).all())
+
+
+def _lens(b, m, seed):
+    g = torch.Generator().manual_seed(seed)
+    share = torch.rand(b, generator=g) ** 2
+    lens = (share / share.sum() * m).int().tolist()
+    lens[seed % b] += m - sum(lens)
+    return lens
+
+
+# The choice is the planner's here: small and large problems, contractions that end in every part of a step of 128 and steps
+# of every number modulo six, tiles in every state, more tiles than workgroups and more groups than the kernel's own table.
+@pytest.mark.parametrize("b,m,n,k", [
+    (1, 1, 4096, 7168), (3, 5, 520, 12256), (32, 250, 2880, 2880), (8, 600, 1024, 2064), (4, 2048, 2048, 1024),
+    (8, 4160, 1536, 1104), (16, 9000, 1000, 512), (16, 9000, 520, 656), (6, 5000, 2304, 784), (6, 5000, 2304, 896),
+    (6, 5000, 2304, 1024), (6, 5000, 2304, 1152), (6, 5000, 2304, 1280), (5, 3333, 4104, 1408), (96, 20000, 512, 768),
+    (300, 7000, 264, 384), (2, 9000, 2880, 2880)])
+def test_the_planners_choice(pkg, monkeypatch, b, m, n, k):
+    monkeypatch.delenv("GG_SMALL")
+    lens = _lens(b, m, n + k)
+    offs, _ = _offs(lens)
+    x, xs, w, ws = _data(b, m, n, k, m + n)
+    for dtype in (BF, FP):
+        assert torch.equal(_run(pkg, x, xs, w, ws, lens, dtype), _want(x, xs, w, ws, lens, offs, dtype, 3.0))
+    # the sizes on the host
+    got = pkg.grouped_gemm_i8(x, pkg.I8Weights(w, ws), lens, xs)
+    assert got.dtype == BF and torch.equal(got, _want(x, xs, w, ws, lens, offs, BF, 3.0))
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("m,n,k", [(5, 264, 640), (700, 1024, 1040), (1, 64, 16)])
+def test_rows_in_16_bits(pkg, dtype, m, n, k):
+    """The call's rounding of the rows is quantize_rows', whatever their stride."""
+    g = _gen(m)
+    x = torch.randn(m, k + 8, device=DEV, generator=g).to(dtype)[:, :k]
+    w = pkg.quantize_i8((torch.randn(3, n, k, device=DEV, generator=g) * k**-0.5).to(dtype))
+    lens = [m // 2, 0, m - m // 2]
+    d = torch.tensor(lens, dtype=torch.int64, device=DEV)
+    q = pkg.quantize_rows(x)
+    got = pkg.grouped_gemm_i8(x, w, d)
+    assert got.dtype == dtype and torch.equal(got, pkg.grouped_gemm_i8(q.y, w, d, q.scale, dtype))
+    offs, _ = _offs(lens)
+    assert torch.equal(got, _want(q.y, q.scale, w.w, w.scales, lens, offs, dtype, 0.0))
+
+
+def test_quantize_i8(pkg):
+    w = (torch.randn(3, 40, 256, device=DEV, generator=_gen(1))).to(BF)
+    w[1, 3] = 0
+    q = pkg.quantize_i8(w)
+    s = w.float().abs().amax(2) / 127
+    s[1, 3] = 1.0
+    assert torch.equal(q.scales, s) and torch.equal(q.w, (w.float() / s[..., None]).round().to(I8))
+    assert bool(((q.w.double() * q.scales.double()[..., None] - w.double()).abs() <= 0.5001 * s.double()[..., None]).all())
+
+
+def test_no_rows_and_no_groups(pkg):
+    w = pkg.I8Weights(torch.zeros(2, 64, 128, device=DEV, dtype=I8), torch.ones(2, 64, device=DEV))
+    none = torch.empty(0, 128, device=DEV, dtype=I8)
+    lens = torch.zeros(2, dtype=torch.int64, device=DEV)
+    assert pkg.grouped_gemm_i8(none, w, lens, torch.empty(0, device=DEV)).shape == (0, 64)
+    x, xs = torch.ones(3, 128, device=DEV, dtype=I8), torch.ones(3, device=DEV)
+    out = torch.full((3, 64), 7.0, device=DEV, dtype=BF)
+    assert bool((pkg.grouped_gemm_i8(x, w, lens, xs, out=out) == 7).all())  # no group has them: left as they were
+
+
+@pytest.mark.parametrize("b,m,n,k", [(4, 40, 264, 640), (70, 3000, 512, 1024), (4, 3000, 512, 1024)])
+def test_captured(pkg, monkeypatch, b, m, n, k):
+    """Replays read the rows, scales and sizes of the time; two graphs and eager calls between share nothing."""
+    monkeypatch.delenv("GG_SMALL")
+    x, xs, w, ws = _data(b, m, n, k, 9)
+    w8, lens = pkg.I8Weights(w, ws), torch.zeros(b, dtype=torch.int64, device=DEV)
+    x16 = torch.randn(m, k, device=DEV, generator=_gen(10)).to(BF)
+
+    def step():
+        return pkg.grouped_gemm_i8(x, w8, lens, xs), pkg.grouped_gemm_i8(x16, w8, lens)
+
+    step()
+    torch.cuda.synchronize()
+    graphs, held = [torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()], []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            held.append(step())
+    for i in range(3):
+        lens.copy_(torch.tensor(_lens(b, m, 20 + i)))
+        x.copy_(_ints(_gen(30 + i), m, k))
+        torch.cuda.synchronize()
+        for g in graphs:
+            g.replay()
+        want = step()
+        torch.cuda.synchronize()
+        for h in held:
+            assert torch.equal(h[0], want[0]) and torch.equal(h[1], want[1])
+
+
+def test_torch_level_refusals(pkg):
+    x, xs, w, ws = _data(2, 4, 64, 128, 3)
+    w8, lens = pkg.I8Weights(w, ws), torch.tensor([2, 2], device=DEV)
+    for args, err, text in (
+            ((x, w8, lens), ValueError, "x_scale"), ((x.float(), w8, lens), TypeError, "int8, bfloat16"),
+            ((x, w8, lens, xs[:3]), ValueError, "x_scale"), ((x, w8, lens, xs.double()), TypeError, "x_scale"),
+            ((x, w8, lens, xs, torch.float32), TypeError, "out_dtype"), ((x[:, :64], w8, lens, xs), ValueError, "K columns"),
+            ((x.t().contiguous().t(), w8, lens, xs), ValueError, "contiguous"), ((x.to(BF), w8, lens, xs), ValueError, "int8 x"),
+            ((x, pkg.I8Weights(w, ws[:, :8]), lens, xs), ValueError, "scales"), ((x, w8, [2, 1], xs), ValueError, "shape mismatch"),
+            ((x, pkg.I8Weights(w.float(), ws), lens, xs), ValueError, "int8")):
+        with pytest.raises(err, match=text):
+            pkg.grouped_gemm_i8(*args)
+    with pytest.raises(pkg.GGError, match="multiple of 8"):
+        pkg.grouped_gemm_i8(x, pkg.I8Weights(w[:, :60].contiguous(), ws[:, :60].contiguous()), lens, xs)
+    with pytest.raises(pkg.GGError, match="K of 16"):
+        pkg.grouped_gemm_i8(x[:, :120].contiguous(), pkg.I8Weights(w[:, :, :120].contiguous(), ws), lens, xs)
+
+
+# ---- rows with their scales to the experts ----
+
+
+@pytest.mark.parametrize("t,k,h,masked", [(1, 1, 16, False), (33, 4, 1040, True), (700, 8, 2880, True), (5000, 2, 7168, False)])
+def test_dispatch_scaled(pkg, t, k, h, masked):
+    g = _gen(t)
+    mask = torch.rand(t, device=DEV, generator=g) < 0.6 if masked else None
+    r = pkg.route(torch.randn(t, 16, device=DEV, generator=g), k, mask)
+    x, s = _ints(g, t, h + 16)[:, :h], torch.rand(t, device=DEV, generator=g)
+    xs = pkg.dispatch_scaled(x, s, r)
+    assert torch.equal(xs.y, pkg.dispatch(x, r))
+    want = torch.zeros(t * k, device=DEV)
+    ok = r.rows >= 0
+    want[r.rows[ok].long()] = s[:, None].expand(t, k)[ok]
+    assert torch.equal(xs.scale, want)
+
+
+def test_int8_layer(pkg):
+    """Norm, dispatch, product, activation, product and combine on int8 rows against the same layer in 64 bits on the
+    rounded weights and rows: every step's output is compared on that step's own inputs."""
+    t, h, inner, e, k = 300, 512, 320, 6, 2
+    g = _gen(77)
+
+    def randn(*s):
+        return torch.randn(s, device=DEV, generator=g)
+
+    x, res = randn(t, h).to(BF), randn(t, h).to(BF)
+    w, b = (1 + 0.1 * randn(h)).to(BF), (0.1 * randn(h)).to(BF)
+    up, down = pkg.quantize_i8(randn(e, 2 * inner, h) * h**-0.5), pkg.quantize_i8(randn(e, h, inner) * inner**-0.5)
+    mask = torch.rand(t, device=DEV, generator=g) < 0.9
+    o = pkg.layer_norm(x, w, b, res, out_dtype=I8, scale="row")
+    r = pkg.route((o.y.float() * o.scale[:, None]) @ randn(h, e), k, mask)
+    xs = pkg.dispatch_scaled(o.y, o.scale, r)
+    gu = pkg.grouped_gemm_i8(xs.y, up, r.counts, xs.scale)
+    act = pkg.silu_product(gu, I8)
+    ys = pkg.grouped_gemm_i8(act.y, down, r.counts, act.scale)
+    out = pkg.combine(ys, r)
+    lens, used = r.counts.tolist(), int(r.offs[-1])
+    offs = r.offs.tolist()[:-1]
+    want = _want(xs.y, xs.scale, up.w, up.scales, lens, offs, BF, 0.0)
+    assert torch.equal(gu[:used], want[:used])
+    want = _want(act.y, act.scale, down.w, down.scales, lens, offs, BF, 0.0)
+    assert torch.equal(ys[:used], want[:used])
+    # and the whole against 64 bits without any rounding of rows. A row's values are off by half a step of its scale, the
+    # largest over 127; relative to a row's norm, with values up to 5 of its standard deviations, that is 5 / 127 / 12^0.5 =
+    # 0.011 after each of the two roundings, which a product passes on as it is and the activation at most 1.1 times;
+    # bf16's roundings (2^-9 each) are small beside it. Twice that, as norms over the whole output are.
+    hd = x.double() + res.double()
+    hd = hd.to(BF).double()
+    c = hd - hd.mean(1, keepdim=True)
+    y = c * (c.square().mean(1, keepdim=True) + 1e-5).rsqrt() * w.double() + b.double()
+    ref = torch.zeros(t, h, device=DEV, dtype=torch.float64)
+    wu, wd = up.w.double() * up.scales.double()[..., None], down.w.double() * down.scales.double()[..., None]
+    for s in range(k):
+        for i in range(e):
+            at = (r.experts[:, s] == i).nonzero()[:, 0]
+            v, u = (y[at] @ wu[i].t().contiguous()).chunk(2, dim=1)
+            ref[at] += (v * torch.sigmoid(v) * u @ wd[i].t().contiguous()) * r.weights[at, s, None].double()
+    assert float((out.double() - ref).norm() / ref.norm()) <= 2 * 0.011 * (1.1 + 1)
+    assert bool((out[~mask] == 0).all())

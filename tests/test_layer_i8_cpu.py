@@ -1,5 +1,6 @@
 """The operators of an int8 expert layer without a GPU: the C ABI refuses bad arguments and unsupported shapes before it
 touches the device, the torch functions check theirs."""
+import ctypes
 import os
 import re
 
@@ -145,3 +146,65 @@ def test_backward_workgroups_fit_the_gpu(pkg):
         of_block = max(wpr, 4)
         blocks = pkg.load_library().gg_layer_norm_backward_workspace(1 << 20, hidden) // (8 * hidden)
         assert 256 <= blocks <= 256 * (waves[wpr, pieces] * 4 // of_block), (hidden, blocks, waves[wpr, pieces])
+
+
+# ---- 8-bit integer products ----
+
+
+@pytest.mark.parametrize("change,want,text", [
+    (dict(out_dtype=INT8), INVALID, "out_dtype"),
+    (dict(b=-1), INVALID, "group_num"),
+    (dict(k=0), INVALID, "k >= 1"),
+    (dict(n=60), UNSUPPORTED, "multiple of 8"),
+    (dict(k=24), UNSUPPORTED, "K of 16"),
+    (dict(k=131072), UNSUPPORTED, "below 131072"),
+    (dict(n=2097160), UNSUPPORTED, "2097152"),
+    (dict(b=8193), UNSUPPORTED, "8192"),
+    (dict(m=(1 << 27) + 1), UNSUPPORTED, "134217728"),
+    (dict(m=1 << 27, n=2097152), UNSUPPORTED, "tiles"),
+    (dict(lens=None), INVALID, "device pointers"),
+    (dict(xs=None), INVALID, "device pointers"),
+    (dict(ws=None), INVALID, "device pointers"),
+    (dict(x=P + 8), UNSUPPORTED, "aligned"),
+    (dict(ws=P + 4), UNSUPPORTED, "aligned"),
+    (dict(mem=None), WORKSPACE, "workspace"),
+    (dict(mem=P + 8), WORKSPACE, "workspace"),
+    (dict(bytes=32), WORKSPACE, "workspace"),
+])
+def test_gemm_i8_refusals(pkg, change, want, text):
+    lib = pkg.load_library()
+    a = dict(out_dtype=BF16, b=4, m=16, n=64, k=128, lens=P, x=P, w=P, xs=P, ws=P, out=P, mem=P, bytes=lib.gg_gemm_i8_workspace(4))
+    a.update(change)
+    st = lib.gg_gemm_i8(a["out_dtype"], a["b"], a["m"], a["n"], a["k"], a["lens"], None, a["x"], a["w"], a["xs"], a["ws"], a["out"],
+                        a["mem"], a["bytes"], None)
+    _refused(pkg, st, want, text)
+
+
+def test_int8_is_no_type_of_the_other_products(pkg):
+    """The int8 products have an entry point of their own: the plans of the others refuse the type."""
+    lib = pkg.load_library()
+    assert lib.gg_gemm_i8_workspace(0) == 0 and lib.gg_gemm_i8(BF16, 0, 16, 64, 128, *[None] * 8, 0, None) == 0
+    status = ctypes.create_string_buffer(16)  # host memory, which the call writes
+    assert lib.gg_call_device_lens(0, INT8, INT8, 2, 16, 64, 128, P, None, P, P, P, P, P, P, 4096, ctypes.addressof(status), None) == INVALID
+
+
+def test_dispatch_scaled_refusals(pkg):
+    lib = pkg.load_library()
+    _refused(pkg, lib.gg_dispatch_scaled(1, 4, 2, 64, 8, P, 64, None, P, P, P, P, None), INVALID, "scale")
+    _refused(pkg, lib.gg_dispatch_scaled(1, 4, 2, 64, 8, P, 64, P, P, P, P, None, None), INVALID, "scale")
+    _refused(pkg, lib.gg_dispatch_scaled(1, 4, 2, 60, 8, P, 64, P, P, P, P, P, None), UNSUPPORTED, "16 bytes")
+    _refused(pkg, lib.gg_dispatch_scaled(3, 4, 2, 64, 8, P, 64, P, P, P, P, P, None), INVALID, "elem_size")
+
+
+def test_quantize_i8_on_the_host(pkg):
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(2, 24, 64, generator=g)
+    w[1, 5] = 0
+    q = pkg.quantize_i8(w)
+    s = w.abs().amax(2) / 127
+    s[1, 5] = 1.0
+    assert q.w.dtype == torch.int8 and torch.equal(q.scales, s) and torch.equal(q.w, (w / s[..., None]).round().to(torch.int8))
+    with pytest.raises(ValueError, match="w must be"):
+        pkg.quantize_i8(w[0])
+    with pytest.raises(ValueError, match="device"):
+        pkg.grouped_gemm_i8(torch.zeros(3, 64, dtype=torch.int8), q, [1, 2], torch.ones(3))
