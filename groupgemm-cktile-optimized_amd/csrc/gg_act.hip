@@ -22,7 +22,9 @@ struct ActArgs {
     int         inner; // values of a row of y
 };
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + __expf(-v)); }
+// By the reciprocal instruction, which is off by a unit in the last place, as the exponential's is (a division rounded as
+// IEEE asks takes ten instructions, and the int8 rows' kernel is held up by what it computes as much as by what it reads).
+__device__ __forceinline__ float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
 // y of the eight values from element i of a row on.
 template <typename T, bool GATED> __device__ __forceinline__ void load_y(const ActArgs &a, const uint16_t *x, int i, float (&v)[8]) {
@@ -60,7 +62,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) round_rows_kernel(const Ac
                     top = max(top, __float_as_uint(fabsf(v[u][j])));
             }
         }
-        const float s = scale_of(row_max<WPR>(m, turn, top, wave, lane), kTopI8);
+        const float s = uniform(scale_of(row_max<WPR>(m, turn, top, wave, lane), kTopI8));
         if (t == 0)
             a.scale[row] = s;
         const Divisor by(s);
@@ -104,17 +106,28 @@ template <typename T, bool BACK> __global__ void __launch_bounds__(256) silu_ker
 
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;
 
-template <typename T, bool GATED, bool WIDE> int run_round(const char *what, const ActArgs &a, hipStream_t s) {
-    return with_shape<WIDE>(a.inner, [&](auto wpr, auto u) {
-        return launch(what, round_rows_kernel<T, GATED, wpr.value, u.value>, std::min(row_blocks(a.rows, a.inner), kMaxBlocks),
-                      block_threads(wpr.value), s, a);
+// f(waves of a row, pieces of a lane). Of many rows, one wave takes a row of up to 2048 values, whose four pieces it has
+// under way together and which needs no barrier: at four waves the kernel waited (us, four waves and one: 32768 rows of
+// 2048 69.4, 56.8, rounding alone 50.6, 35.7). Of few rows the norms' shapes.
+template <typename F> int with_round_shape(int64_t rows, int64_t n, F f) {
+    using std::integral_constant;
+    if (few(rows, n))
+        return with_shape<true>(n, f);
+    if (n > 2048)
+        return with_shape<false>(n, f);
+    return n <= 512    ? f(integral_constant<int, 1>{}, integral_constant<int, 1>{})
+           : n <= 1024 ? f(integral_constant<int, 1>{}, integral_constant<int, 2>{})
+           : n <= 1536 ? f(integral_constant<int, 1>{}, integral_constant<int, 3>{})
+                       : f(integral_constant<int, 1>{}, integral_constant<int, 4>{});
+}
+template <typename T, bool GATED> int run_round(const char *what, const ActArgs &a, hipStream_t s) {
+    return with_round_shape(a.rows, a.inner, [&](auto wpr, auto u) {
+        const int64_t blocks = wpr.value == 1 ? (a.rows + 3) / 4 : a.rows;
+        return launch(what, round_rows_kernel<T, GATED, wpr.value, u.value>, std::min(blocks, kMaxBlocks), block_threads(wpr.value), s, a);
     });
 }
 template <bool GATED> int run_round(const char *what, int dtype, const ActArgs &a, hipStream_t s) {
-    const bool wide = few(a.rows, a.inner);
-    if (dtype == GG_DTYPE_BF16)
-        return wide ? run_round<BF16, GATED, true>(what, a, s) : run_round<BF16, GATED, false>(what, a, s);
-    return wide ? run_round<F16, GATED, true>(what, a, s) : run_round<F16, GATED, false>(what, a, s);
+    return dtype == GG_DTYPE_BF16 ? run_round<BF16, GATED>(what, a, s) : run_round<F16, GATED>(what, a, s);
 }
 
 template <bool BACK> int run_silu(const char *what, int dtype, const ActArgs &a, hipStream_t s) {

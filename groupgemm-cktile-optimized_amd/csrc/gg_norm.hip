@@ -38,20 +38,26 @@ struct NormArgs {
     bool        w32, e5m2;
 };
 
-// y of eight values from element i on: v holds h (CENTER: less its mean) and then y.
-template <typename T, bool CENTER>
-__device__ __forceinline__ void scale_shift(const NormArgs &a, int i, float rstd, float (&v)[8]) {
-    float w[8], b[8];
-    load_w<T>(a.weight, a.w32, i, w);
-    if (CENTER && a.bias != nullptr) {
-        load_w<T>(a.bias, a.w32, i, b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = fmaf(v[j] * rstd, w[j], b[j]);
+// The largest |y| of a workgroup's rows, for a tensor scale's second pass.
+template <int WPR>
+__device__ __forceinline__ void store_top(const NormArgs &a, unsigned top, unsigned (&block_top)[4], RowReduce<WPR> &m, int wave, int lane) {
+    top                 = wave_max(top);
+    constexpr int waves = block_threads(WPR) / 64;
+    static_assert(waves <= 16, "");
+    if constexpr (WPR == 1) {
+        if (lane == 0)
+            block_top[wave] = top;
     } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            v[j] = v[j] * rstd * w[j];
+        __syncthreads(); // the last row's tops are read
+        if (lane == 0)
+            m.tops[0][wave] = top;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        unsigned s = 0;
+        for (int i = 0; i < waves; ++i)
+            s = max(s, WPR == 1 ? block_top[i & 3] : m.tops[0][i % WPR]);
+        reinterpret_cast<unsigned *>(a.parts)[blockIdx.x] = s;
     }
 }
 
@@ -59,7 +65,7 @@ __device__ __forceinline__ void scale_shift(const NormArgs &a, int i, float rstd
 // rounding's registers would cost the others a wave per SIMD), or the first pass of a tensor scale (no y; the workgroup's
 // largest |y|).
 enum Pass : int { kWhole = 0, kInt8 = 1, kFirst = 2 };
-template <typename T, bool CENTER, int WPR, int U, int PASS>
+template <typename T, int WPR, int U, int PASS>
 __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs a) {
     __shared__ RowReduce<WPR> m;
     __shared__ unsigned       block_top[4];
@@ -72,7 +78,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
     for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0); row < a.rows;
          row += step, turn ^= 1) {
         float v[U][8];
-        float sq = 0.f; // CENTER: the plain sum first
+        float sq = 0.f;
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
@@ -94,24 +100,8 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    sq = CENTER ? sq + v[u][j] : fmaf(v[u][j], v[u][j], sq);
+                    sq = fmaf(v[u][j], v[u][j], sq);
             }
-        }
-        if constexpr (CENTER) {
-            // the row is in registers: its squares are summed about the mean, where nothing cancels
-            const float mean = row_sum<WPR>(m, turn, sq, wave, lane) / static_cast<float>(a.hidden);
-            if (t == 0 && a.mean != nullptr)
-                a.mean[row] = mean;
-            turn ^= 1;
-            sq = 0.f;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
-                if ((u * 64 * WPR + t) * 8 < a.hidden)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        v[u][j] -= mean;
-                        sq = fmaf(v[u][j], v[u][j], sq);
-                    }
         }
         sq = row_sum<WPR>(m, turn, sq, wave, lane);
         const float rstd = 1.f / sqrtf(sq / static_cast<float>(a.hidden) + a.eps);
@@ -122,10 +112,13 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
             if (i < a.hidden) {
-                scale_shift<T, CENTER>(a, i, rstd, v[u]);
+                float w[8];
+                load_w<T>(a.weight, a.w32, i, w);
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 8; ++j) {
+                    v[u][j] = v[u][j] * rstd * w[j];
                     row_top = max(row_top, __float_as_uint(fabsf(v[u][j])));
+                }
             }
         }
         if constexpr (PASS == kFirst) {
@@ -134,6 +127,8 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
             float s = 1.f;
             if (PASS == kInt8 || a.mode == GG_NORM_SCALE_ROW) {
                 s = scale_of(row_max<WPR>(m, turn, row_top, wave, lane), PASS == kInt8 ? kTopI8 : a.e5m2 ? kTopE5M2 : kTopE4M3);
+                if constexpr (PASS == kInt8)
+                    s = uniform(s);
                 if (t == 0)
                     a.scale[row] = s;
             } else if (a.mode == GG_NORM_SCALE_GIVEN) {
@@ -155,26 +150,221 @@ __global__ void __launch_bounds__(block_threads(WPR)) norm_kernel(const NormArgs
             }
         }
     }
-    if constexpr (PASS == kFirst) {
-        top = wave_max(top);
-        constexpr int waves = block_threads(WPR) / 64;
-        static_assert(waves <= 16, "");
-        if constexpr (WPR == 1) {
-            if (lane == 0)
-                block_top[wave] = top;
-        } else {
-            __syncthreads(); // the last row's tops are read
-            if (lane == 0)
-                m.tops[0][wave] = top;
+    if constexpr (PASS == kFirst)
+        store_top<WPR>(a, top, block_top, m, wave, lane);
+}
+
+// ---- layer norm ----
+
+// The two sums of a row over its waves, with one barrier.
+template <int WPR> struct PairReduce {
+    float sums[2][2][WPR];
+};
+template <int WPR>
+__device__ __forceinline__ void row_sums(PairReduce<WPR> &m, int turn, float &p, float &q, int wave, int lane) {
+    p = wave_sum(p);
+    q = wave_sum(q);
+    if constexpr (WPR > 1) {
+        if (lane == 0) {
+            m.sums[turn][0][wave] = p;
+            m.sums[turn][1][wave] = q;
         }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            unsigned s = 0;
-            for (int i = 0; i < waves; ++i)
-                s = max(s, WPR == 1 ? block_top[i & 3] : m.tops[0][i % WPR]);
-            reinterpret_cast<unsigned *>(a.parts)[blockIdx.x] = s;
+        p = q = 0.f;
+#pragma unroll
+        for (int i = 0; i < WPR; ++i) {
+            p += m.sums[turn][0][i];
+            q += m.sums[turn][1][i];
         }
     }
+}
+
+// Mean and sum of squares about it of a row, with one barrier. A wave finds the mean m_w of its own n_w values, the sum of
+// their squares about that, and what rounding left of their sum, e = sum (x - m_w); the waves' are put together exactly,
+// sum (x - m)^2 = sum (x - m_w)^2 + 2 (m_w - m) e + n_w (m_w - m)^2, each by a lane of every wave. So nothing cancels but
+// what a second pass over the row would lose, too.
+template <int WPR> struct Moments {
+    f32x4 of_wave[2][WPR]; // m_w n_w, m_w, squares, e
+};
+template <int WPR, int U> struct RowMoments {
+    float own, inv_own, n; // values of this wave, and of wave lane % WPR
+    float inv_hidden;
+    __device__ __forceinline__ RowMoments(int hidden, int wave, int lane) {
+        // in each of the U rounds the waves take 512 values one after the other
+        const auto count = [&](int w) {
+            int c = 0;
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                c += min(max(hidden - (u * WPR + w) * 512, 0), 512);
+            return static_cast<float>(c);
+        };
+        own        = count(WPR == 1 ? 0 : wave);
+        inv_own    = own > 0.f ? 1.f / own : 0.f;
+        n          = count(lane & (WPR - 1));
+        inv_hidden = 1.f / static_cast<float>(hidden);
+    }
+    // v holds zeros past the row's end; mine: the lane's pieces of 8 that are not.
+    __device__ __forceinline__ void operator()(Moments<WPR> &m, int turn, const float (&v)[U][8], const bool (&mine)[U], int wave,
+                                               int lane, float &mean, float &square) const {
+        float s[2] = {0.f, 0.f}, q[2] = {0.f, 0.f};
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                s[j & 1] += v[u][j];
+        const float sum = wave_sum(s[0] + s[1]), mw = sum * inv_own;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (mine[u])
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float d = v[u][j] - mw;
+                    q[j & 1] = fmaf(d, d, q[j & 1]);
+                }
+        const float sq = wave_sum(q[0] + q[1]);
+        if constexpr (WPR == 1) {
+            mean   = mw;
+            square = sq;
+        } else {
+            if (lane == 0)
+                m.of_wave[turn][wave] = f32x4{sum, mw, sq, fmaf(-own, mw, sum)};
+            __syncthreads();
+            const f32x4 w = m.of_wave[turn][lane & (WPR - 1)];
+            mean          = group_sum<WPR>(w[0]) * inv_hidden;
+            const float d = w[1] - mean;
+            square        = group_sum<WPR>(n > 0.f ? fmaf(d, fmaf(n, d, 2.f * w[3]), w[2]) : 0.f);
+        }
+    }
+};
+
+// As norm_kernel. A workgroup takes one row after the other and, where a lane has at most four pieces of one, has the next
+// one's values under way while it works on a row and keeps weight and bias (as many bytes as a row each, or in float32
+// twice as many) in registers.
+template <typename T, int WPR, int U, int PASS>
+__global__ void __launch_bounds__(block_threads(WPR)) center_norm_kernel(const NormArgs a) {
+    __shared__ Moments<WPR>  mom;
+    __shared__ RowReduce<WPR> m;
+    __shared__ unsigned       block_top[4];
+    constexpr bool kHold = U <= 4;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int t    = WPR == 1 ? lane : static_cast<int>(threadIdx.x); // thread of the row
+    unsigned  top  = 0;
+    int       turn = 0;
+    bool      mine[U];
+    u32x4     xw[U], rw[U];
+    const RowMoments<WPR, U> moments(a.hidden, wave, lane);
+    const int64_t step = static_cast<int64_t>(gridDim.x) * rows_per_block(WPR);
+    int64_t       row  = static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0);
+    const auto fetch = [&](int64_t r) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (mine[u]) {
+                const int i = (u * 64 * WPR + t) * 8;
+                xw[u]       = load_once(static_cast<const uint16_t *>(a.x) + r * a.x_stride + i);
+                if (a.residual != nullptr)
+                    rw[u] = load_once(static_cast<const uint16_t *>(a.residual) + r * a.r_stride + i);
+            }
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+        mine[u] = (u * 64 * WPR + t) * 8 < a.hidden;
+    if (kHold && row < a.rows)
+        fetch(row);
+    float w[kHold ? U : 1][8], b[kHold ? U : 1][8];
+    if constexpr (kHold) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                w[u][j] = b[u][j] = 0.f;
+            if (mine[u]) {
+                load_w<T>(a.weight, a.w32, (u * 64 * WPR + t) * 8, w[u]);
+                if (a.bias != nullptr)
+                    load_w<T>(a.bias, a.w32, (u * 64 * WPR + t) * 8, b[u]);
+            }
+        }
+    }
+    // every wave of a block that shares a row makes the same trips, so the barriers match
+    for (; row < a.rows; row += step, turn ^= 1) {
+        float v[U][8];
+        if constexpr (!kHold)
+            fetch(row);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                v[u][j] = 0.f;
+            if (mine[u]) {
+                unpack8<T>(xw[u], v[u]);
+                if (a.residual != nullptr) {
+                    float r[8];
+                    unpack8<T>(rw[u], r);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        v[u][j] += r[j];
+                    const u32x4 hw = pack8<T>(v[u]);
+                    *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.h) + row * a.h_stride + (u * 64 * WPR + t) * 8) = hw;
+                    unpack8<T>(hw, v[u]);
+                }
+            }
+        }
+        if (kHold && row + step < a.rows)
+            fetch(row + step);
+        float mean, square;
+        moments(mom, turn, v, mine, wave, lane, mean, square);
+        const float rstd = 1.f / sqrtf(square * moments.inv_hidden + a.eps);
+        if (t == 0) {
+            if (a.mean != nullptr)
+                a.mean[row] = mean;
+            if (a.rstd != nullptr)
+                a.rstd[row] = rstd;
+        }
+        unsigned row_top = 0;
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (mine[u]) {
+                if constexpr (!kHold) {
+                    load_w<T>(a.weight, a.w32, (u * 64 * WPR + t) * 8, w[0]);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        b[0][j] = 0.f;
+                    if (a.bias != nullptr)
+                        load_w<T>(a.bias, a.w32, (u * 64 * WPR + t) * 8, b[0]);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    v[u][j] = fmaf((v[u][j] - mean) * rstd, w[kHold ? u : 0][j], b[kHold ? u : 0][j]);
+                    if (PASS != kWhole || a.mode == GG_NORM_SCALE_ROW)
+                        row_top = max(row_top, __float_as_uint(fabsf(v[u][j])));
+                }
+            }
+        if constexpr (PASS == kFirst) {
+            top = max(top, row_top);
+        } else {
+            float s = 1.f;
+            if (PASS == kInt8 || a.mode == GG_NORM_SCALE_ROW) {
+                s = uniform(scale_of(row_max<WPR>(m, turn, row_top, wave, lane), PASS == kInt8 ? kTopI8 : a.e5m2 ? kTopE5M2 : kTopE4M3));
+                if (t == 0)
+                    a.scale[row] = s;
+            } else if (a.mode == GG_NORM_SCALE_GIVEN) {
+                s = a.scale[0];
+            }
+            const Divisor by(s);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (mine[u]) {
+                    const int64_t at = row * a.hidden + (u * 64 * WPR + t) * 8;
+                    if constexpr (PASS == kInt8)
+                        *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + at) = pack_i8(v[u], by);
+                    else if (a.mode == GG_NORM_PLAIN)
+                        *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.y) + at) = pack8<T>(v[u]);
+                    else
+                        *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + at) = pack_fp8(v[u], by, a.e5m2);
+                }
+        }
+    }
+    if constexpr (PASS == kFirst)
+        store_top<WPR>(a, top, block_top, m, wave, lane);
 }
 
 // The tensor scale's second pass: the largest of the first pass's maxima, then y from h and rstd.
@@ -198,13 +388,21 @@ template <typename T, bool CENTER, int THREADS> __global__ void __launch_bounds_
     for (int64_t row = a.rows - 1 - blockIdx.x; row >= 0; row -= gridDim.x) {
         const float rstd = a.rstd[row], mean = CENTER ? a.mean[row] : 0.f;
         for (int i = threadIdx.x * 8; i < a.hidden; i += THREADS * 8) {
-            float v[8];
+            float v[8], w[8];
             unpack8<T>(load_once(static_cast<const uint16_t *>(a.h) + row * a.h_stride + i), v);
-            if constexpr (CENTER)
+            load_w<T>(a.weight, a.w32, i, w);
+            if constexpr (CENTER) {
+                float b[8] = {};
+                if (a.bias != nullptr)
+                    load_w<T>(a.bias, a.w32, i, b);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    v[j] -= mean;
-            scale_shift<T, CENTER>(a, i, rstd, v);
+                    v[j] = fmaf((v[j] - mean) * rstd, w[j], b[j]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    v[j] = v[j] * rstd * w[j];
+            }
             *reinterpret_cast<u32x2 *>(static_cast<uint8_t *>(a.y) + row * a.hidden + i) = pack_fp8(v, by, a.e5m2);
         }
     }
@@ -404,29 +602,6 @@ struct CenterArgs {
     const float *mean;
 };
 
-// The two sums of a row over its waves, with one barrier.
-template <int WPR> struct PairReduce {
-    float sums[2][2][WPR];
-};
-template <int WPR>
-__device__ __forceinline__ void row_sums(PairReduce<WPR> &m, int turn, float &p, float &q, int wave, int lane) {
-    p = wave_sum(p);
-    q = wave_sum(q);
-    if constexpr (WPR > 1) {
-        if (lane == 0) {
-            m.sums[turn][0][wave] = p;
-            m.sums[turn][1][wave] = q;
-        }
-        __syncthreads();
-        p = q = 0.f;
-#pragma unroll
-        for (int i = 0; i < WPR; ++i) {
-            p += m.sums[turn][0][i];
-            q += m.sums[turn][1][i];
-        }
-    }
-}
-
 // With d = h - mean: grad_x = grad_h + rstd (w g - mean(w g)) - d rstd^3 mean(w g d), row by row; the partial sums of
 // g d rstd and of g stay in registers over the rows of a workgroup and are written once. Two sums a column are twice the
 // registers of the RMS norm's one, so rows past 8192 values take eight waves, and with more than four pieces a lane (past
@@ -490,6 +665,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const C
         row_sums<WPR>(m, turn, sum, dot, wave, lane);
         const float n  = static_cast<float>(a.hidden);
         const float c1 = rstd * (sum / n), c2 = rstd * (rstd * (rstd * (dot / n))); // (rstd^3 alone may be past float32)
+        const float c3 = fmaf(c2, mean, -c1);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
@@ -500,7 +676,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const C
                 load_w<T>(a.weight, a.w32, i, w);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    g[j] = rstd * (g[j] * w[j]) - c1 - (h[j] - mean) * c2;
+                    g[j] = fmaf(rstd, g[j] * w[j], fmaf(-c2, h[j], c3));
                 if (rp != nullptr) {
                     unpack8<T>(kKeep ? rw[u] : load_once(rp + i), r);
 #pragma unroll
@@ -609,13 +785,51 @@ template <typename T> __global__ void __launch_bounds__(1024) center_strip_kerne
 
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;
 
+// The layer norm's shapes: of many rows eight waves for a row of 6145 to 8192 values and sixteen for up to 16384, which keep
+// weight and bias in registers and have a next row's values under way, where four would have to choose. us at four, eight and
+// sixteen waves: 8192 rows of 7168 to int8 81.6, 71.9, 90.7, to bf16 82.3, 74.6, 79.3; 4096 of 5120 31.3, 33.3, 33.2; at four
+// and sixteen: 8000 of 12288 97.6, 74.5.
+template <typename F> int with_center_forward(bool few_rows, int64_t hidden, F f) {
+    using std::integral_constant;
+    const int wpr = hidden <= 1024    ? 1
+                    : hidden > 16384  ? 8
+                    : few_rows        ? (hidden <= 2048 ? 4 : 16)
+                    : hidden <= 6144  ? 4
+                    : hidden <= 8192  ? 8
+                                      : 16;
+    const int u   = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+#define GG_SHAPE(W, N)                                                                                                 \
+    if (wpr == W && u <= N)                                                                                            \
+        return f(integral_constant<int, W>{}, integral_constant<int, N>{});
+    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(8, 2) GG_SHAPE(16, 1) GG_SHAPE(16, 2)
+#undef GG_SHAPE
+    return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+}
+// The shape of either norm's forward pass.
+template <bool CENTER, bool WIDE, typename F> int with_norm_shape(int64_t hidden, F f) {
+    if constexpr (CENTER)
+        return with_center_forward(WIDE, hidden, f);
+    else
+        return with_shape<WIDE>(hidden, f);
+}
+
+// The kernel of either norm for one pass.
+template <typename T, bool CENTER, int WPR, int U, int PASS> constexpr auto norm_pass() {
+    if constexpr (CENTER)
+        return center_norm_kernel<T, WPR, U, PASS>;
+    else
+        return norm_kernel<T, WPR, U, PASS>;
+}
+
 template <typename T, bool CENTER, bool WIDE> int run_norm(const NormArgs &a, bool i8, hipStream_t s) {
     constexpr const char *kWhat = CENTER ? "layer_norm" : "rms_norm";
     const int64_t blocks = row_blocks(a.rows, a.hidden);
     if (a.mode != GG_NORM_SCALE_TENSOR)
-        return with_shape<WIDE>(a.hidden, [&](auto wpr, auto u) {
-            return launch(kWhat, i8 ? norm_kernel<T, CENTER, wpr.value, u.value, kInt8> : norm_kernel<T, CENTER, wpr.value, u.value, kWhole>,
-                          std::min(blocks, kMaxBlocks), block_threads(wpr.value), s, a);
+        return with_norm_shape<CENTER, WIDE>(a.hidden, [&](auto wpr, auto u) {
+            const auto kernel = i8 ? norm_pass<T, CENTER, wpr.value, u.value, kInt8>() : norm_pass<T, CENTER, wpr.value, u.value, kWhole>();
+            // the layer norm's workgroups go from row to row: as many as fit at once
+            const int64_t grid = !CENTER || blocks <= 256 ? blocks : std::min<int64_t>(blocks, resident_blocks(kernel, block_threads(wpr.value)));
+            return launch(kWhat, kernel, std::min(grid, kMaxBlocks), block_threads(wpr.value), s, a);
         });
     // The first pass: as many workgroups as fit at once, each with its share of the rows (32768 rows of 7168: 1792
     // workgroups fit, 377 us for both passes; 1536 377, 1280 389, 1024 421, 2048, 1.1 rounds of them, 453).
@@ -624,8 +838,8 @@ template <typename T, bool CENTER, bool WIDE> int run_norm(const NormArgs &a, bo
         b.h        = const_cast<void *>(b.x);
         b.h_stride = b.x_stride;
     }
-    const int st = with_shape<WIDE>(a.hidden, [&](auto wpr, auto u) {
-        constexpr auto kernel = norm_kernel<T, CENTER, wpr.value, u.value, kFirst>;
+    const int st = with_norm_shape<CENTER, WIDE>(a.hidden, [&](auto wpr, auto u) {
+        constexpr auto kernel = norm_pass<T, CENTER, wpr.value, u.value, kFirst>();
         // (asked for each call, as devices differ; few workgroups fit in any case)
         b.n_parts = static_cast<int>(blocks <= 256 ? blocks : std::min<int64_t>(blocks, std::min(resident_blocks(kernel, block_threads(wpr.value)), kMaxParts)));
         return launch(kWhat, kernel, b.n_parts, block_threads(wpr.value), s, b);
@@ -677,7 +891,7 @@ template <typename F> int with_center_shape(int64_t hidden, F f) {
 }
 int64_t center_blocks(int64_t rows, int64_t hidden) {
     const int     wpr = center_waves(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
-    const int64_t fit = wpr == 8 ? 256 : u == 1 ? 1280 : u == 2 && wpr == 4 ? 1024 : 768;
+    const int64_t fit = wpr == 8 ? 256 : u == 1 ? (wpr == 4 ? 1536 : 1280) : u == 2 && wpr == 4 ? 1024 : 768;
     const int64_t b   = row_blocks(rows, hidden);
     return std::min(fit, std::max(b / 4, b <= 256 ? b : std::min<int64_t>(b / 2, 512)));
 }

@@ -41,8 +41,13 @@ struct Divisor {
     }
 };
 
-// Eight values divided by the scale, within +-top.
-__device__ __forceinline__ void quotients(const float (&v)[8], const Divisor &d, float top, float (&s)[8]) {
+constexpr float kTopE4M3 = 448.f, kTopE5M2 = 57344.f, kTopI8 = 127.f; // largest values
+
+// Eight values divided by the scale, as fp8.
+__device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], const Divisor &d, bool e5m2) {
+    u32x2 w;
+    const float top = e5m2 ? kTopE5M2 : kTopE4M3;
+    float s[8];
     if (d.exact) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
@@ -52,15 +57,6 @@ __device__ __forceinline__ void quotients(const float (&v)[8], const Divisor &d,
         for (int i = 0; i < 8; ++i)
             s[i] = saturate(d.quotient(v[i]), top);
     }
-}
-
-constexpr float kTopE4M3 = 448.f, kTopE5M2 = 57344.f, kTopI8 = 127.f; // largest values
-
-// Eight values divided by the scale, as fp8.
-__device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], const Divisor &d, bool e5m2) {
-    u32x2 w;
-    float s[8];
-    quotients(v, d, e5m2 ? kTopE5M2 : kTopE4M3, s);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         int q = 0;
@@ -76,20 +72,33 @@ __device__ __forceinline__ u32x2 pack_fp8(const float (&v)[8], const Divisor &d,
     return w;
 }
 
-// Eight values divided by the scale, as int8: rounded to the nearest whole number, halves to even; a NaN becomes 0.
-// Next to 1.5 * 2^23 a float32 steps by one: the sum is rounded to it, and its low byte is the number.
+// Eight values of a row divided by the row's scale, as int8: quotients as float32 division rounds them (Divisor), to the
+// nearest whole number, halves to even. With a finite scale no value of the row is more than 127 scales (and a float32's
+// rounding), so nothing needs to be clamped, and in a row without one, which has a NaN or an infinity, all are 0: four
+// operations a value where clamps and checks for each would be twelve. Next to 1.5 * 2^23 a float32 steps by one: the sum
+// is rounded to it, and its low byte is the number.
 __device__ __forceinline__ u32x2 pack_i8(const float (&v)[8], const Divisor &d) {
-    u32x2 w;
-    float s[8];
-    quotients(v, d, kTopI8, s);
+    u32x2 w{0, 0};
+    if (!(d.s < __builtin_inff()))
+        return w;
+    float y[8];
+    if (d.exact) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            y[i] = v[i] / d.s;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            y[i] = v[i] * d.inv;
+            y[i] = fmaf(-fmaf(y[i], d.s, -v[i]), d.inv, y[i]);
+        }
+    }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         unsigned q[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float x = s[4 * i + j];
-            q[j]          = __float_as_uint((x == x ? x : 0.f) + 12582912.f);
-        }
+        for (int j = 0; j < 4; ++j)
+            q[j] = __float_as_uint(y[4 * i + j] + 12582912.f);
         w[i] = __builtin_amdgcn_perm(q[1], q[0], 0x0c0c0400u) | __builtin_amdgcn_perm(q[3], q[2], 0x04000c0cu);
     }
     return w;
@@ -100,6 +109,10 @@ __device__ __forceinline__ u32x2 pack_i8(const float (&v)[8], const Divisor &d) 
 __device__ __forceinline__ float scale_of(unsigned top_bits, float format_top) {
     const float s = __uint_as_float(top_bits) / format_top;
     return s < 1.17549435e-38f ? 1.f : s;
+}
+// A value that every lane of the wave has, as a scalar (what depends on it branches for the wave).
+__device__ __forceinline__ float uniform(float v) {
+    return __uint_as_float(static_cast<unsigned>(__builtin_amdgcn_readfirstlane(static_cast<int>(__float_as_uint(v)))));
 }
 
 // Reductions over the WPR waves of a row; `turn` alternates so that one barrier per call is enough.
