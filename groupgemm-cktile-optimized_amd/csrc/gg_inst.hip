@@ -31,6 +31,12 @@ void launch_mode(const KernelArgs &args, bool cross, dim3 g, dim3 b, hipStream_t
             return;
         }
     }
+    if constexpr (MODE == make_mode(kFwd, kInI8)) { // short tiles: cross-tile only (launch_grouped_gemm checks)
+        if (args.tile_m != kTileM) {
+            launch_cross<F16, MODE, kShapeShort>(args, g, b, stream);
+            return;
+        }
+    }
     if (cross) {
         if constexpr (MODE == make_mode(kFwd, kIn16)) {
             if (args.tail_splits > 1) {

@@ -263,9 +263,14 @@ hipError_t launch_grouped_gemm(const KernelArgs &args, bool fp16, int grid, hipS
     if (!mode_supported(mode, fp16))
         return hipErrorInvalidValue;
     // short tiles: forward and 16-bit dgrad plans with a host-built group table, never split;
-    // short-wide tiles (288 columns): short cross-tile 16-bit forward plans without a tail split
+    // short-wide tiles (288 columns): short cross-tile 16-bit forward plans without a tail split;
+    // int8: cross-tile with the in-kernel table
     const bool wide_n = args.tile_n == kShortWideTileN;
-    if (args.tile_m != kTileM &&
+    if (args.tile_m != kTileM && mode_i8(mode)) {
+        if (args.tile_m != kShortTileM || args.tile_n != kTileN || args.d_lens == nullptr || args.splits > 1 ||
+            !uses_cross_tile(args, grid, mode))
+            return hipErrorInvalidValue;
+    } else if (args.tile_m != kTileM &&
         (args.tile_m <= 0 || args.tile_m > kShortTileM || args.tile_m % 16 != 0 || !has_short_tiles(mode) ||
          args.d_lens != nullptr || args.d_total != nullptr || args.splits > 1 ||
          (args.tile_n != kTileN && !wide_n)))

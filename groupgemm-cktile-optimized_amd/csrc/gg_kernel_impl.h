@@ -964,7 +964,8 @@ constexpr bool ct_instance(int mode, int shape, bool cross) {
            (((mode == make_mode(kFwd, kIn16) || mode == make_mode(kFwd, kInE4M3) || mode == make_mode(kFwd, kInE5M2) ||
               mode == make_mode(kFwd, kInI8)) &&
              shape == kShapeWide) ||
-            (mode == make_mode(kFwd, kIn16) && shape == kShapeShortWide));
+            (mode == make_mode(kFwd, kIn16) && shape == kShapeShortWide) ||
+            (mode == make_mode(kFwd, kInI8) && shape == kShapeShort));
 }
 
 
@@ -1011,10 +1012,11 @@ grouped_gemm_kernel(const KernelArgs args) {
     constexpr bool NARROW = SHAPE == kShapeNarrow;
     constexpr bool SWIDE  = SHAPE == kShapeShortWide;
     constexpr bool SHORT  = SHAPE == kShapeShort || SWIDE; // at most 192 rows per tile
-    static_assert(!I8 || (LAYOUT == kFwd && SHAPE == kShapeWide && !TAIL), "int8: forward, 256 x 256 tiles");
+    static_assert(!I8 || (LAYOUT == kFwd && (SHAPE == kShapeWide || (SHAPE == kShapeShort && CROSS)) && !TAIL),
+                  "int8: forward, 256 x 256 tiles or (cross-tile) short ones");
     static_assert(!NARROW || (!CROSS && MODE == make_mode(kFwd, kIn16)), "narrow tiles: per-tile 16-bit forward");
-    static_assert(!SHORT || MODE == make_mode(kFwd, kIn16) || MODE == make_mode(kDgrad, kIn16),
-                  "short tiles: 16-bit forward and dgrad");
+    static_assert(!SHORT || MODE == make_mode(kFwd, kIn16) || MODE == make_mode(kDgrad, kIn16) || I8,
+                  "short tiles: 16-bit forward and dgrad, int8 forward");
     static_assert(!SWIDE || (CROSS && !TAIL && MODE == make_mode(kFwd, kIn16)),
                   "short-wide tiles: cross-tile 16-bit forward, no tail split");
     constexpr int  TN     = NARROW ? kNarrowTileN : SWIDE ? kShortWideTileN : kTileN; // output columns per tile
@@ -1036,8 +1038,8 @@ grouped_gemm_kernel(const KernelArgs args) {
     static_assert(!SWIDE || (NBLK == P::nc && RB == P::rows), "short-wide plan");
     // row-major accumulators (GG_CT): whole 256 x 256 tiles of the 16-bit forward, cross-tile
     constexpr bool CT = ct_instance(MODE, SHAPE, CROSS);
-    static_assert(!CT || (RB == 8 && NBLK == 8 && P::nc == 8) || (SWIDE && NBLK == 9 && P::nc == 9),
-                  "row-major accumulators: whole tiles, or short-wide tiles (ninth block C^T)");
+    static_assert(!CT || (NBLK == 8 && P::nc == 8) || (SWIDE && NBLK == 9 && P::nc == 9),
+                  "row-major accumulators: 256-column tiles, or short-wide tiles (ninth block C^T)");
     constexpr int B_BLK = CT ? 1 : 16; // LDS rows between the w fragments of consecutive column blocks
     constexpr int NC   = P::nc;                                     // column blocks in the registers
     constexpr int A_ST = P::la * kWaves * 1024;                     // bytes of an A stage
@@ -1060,17 +1062,18 @@ grouped_gemm_kernel(const KernelArgs args) {
     int       T = args.k_tiles; // K steps of the current tile (per group for wgrad)
     // In-kernel group table (device-resident sizes, at most 64 groups): every wave builds it,
     // lane g holding group g; workgroup 0 reports the tile count and the first invalid group.
-    // Short tiles and the per-tile fp8 wgrad instances take host-built tables only: the host never
-    // plans them with an in-kernel table (a device-size wgrad plan runs cross-tile), and the lane
+    // The 16-bit short tiles and the per-tile fp8 wgrad instances take host-built tables only: the host
+    // never plans them with an in-kernel table (a device-size wgrad plan runs cross-tile), and the lane
     // table's registers would push the fp8 wgrad instance with tail masks past 256 VGPRs.
-    constexpr bool kLaneTable = !SHORT && !(F8 && !CROSS && LAYOUT == kWgrad);
+    constexpr bool kLaneTable = (!SHORT || I8) && !(F8 && !CROSS && LAYOUT == kWgrad);
     const bool     in_kernel_table = kLaneTable && args.d_lens != nullptr;
     LaneGroup  lgrp{0, 0, 0, 0};
     int        lg_total = 0;
     if (in_kernel_table) {
         int first_bad, overflow;
         lgrp = lane_group_table(args.d_lens, args.d_offs, args.group_num, args.lens_rows, args.n_tiles,
-                                LAYOUT == kWgrad ? args.m_out : 0, lane, &lg_total, &first_bad, &overflow);
+                                LAYOUT == kWgrad ? args.m_out : 0, lane, &lg_total, &first_bad, &overflow,
+                                SHORT ? args.tile_m : kTileM);
         if constexpr (LAYOUT == kWgrad) {
             // Every group owns the same number of tiles, of as many K steps as its rows fill: dealt
             // round by round in the groups' own order, the busiest workgroup of a router's ragged
@@ -1432,7 +1435,8 @@ grouped_gemm_kernel(const KernelArgs args) {
                       (static_cast<int64_t>(__builtin_amdgcn_readlane(static_cast<int>(lgrp.row0 >> 32), g)) << 32);
             ge.m     = __builtin_amdgcn_readlane(lgrp.m, g);
             ge.tile0 = __builtin_amdgcn_readlane(lgrp.tile0, g);
-            const int m_tiles = ((LAYOUT == kWgrad ? args.m_out : ge.m) + kTileM - 1) / kTileM;
+            const int tile_m  = SHORT ? args.tile_m : kTileM;
+            const int m_tiles = ((LAYOUT == kWgrad ? args.m_out : ge.m) + tile_m - 1) / tile_m;
             band_coords(L - ge.tile0, m_tiles, args.n_tiles, args.band, &tm, &tn);
         } else {
             locate_tile(L, const_table, args.group_num, args.n_tiles, args.band, &g, &tm, &tn,

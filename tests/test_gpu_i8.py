@@ -60,10 +60,13 @@ def _run(pkg, x, xs, w, ws, lens, dtype, offs=None):
     return got
 
 
-@pytest.fixture(params=["persistent", 0, 1, 2, 3, 4])
+@pytest.fixture(params=["persistent", "short", 0, 1, 2, 3, 4])
 def kernel(request, monkeypatch):
-    """The persistent kernel, or one instance of the few-row one."""
-    if request.param != "persistent":
+    """The persistent kernel, on tiles of 256 rows or (short; up to 64 groups, 512 values of k and more) 192, or one
+    instance of the few-row one."""
+    if isinstance(request.param, str):
+        monkeypatch.setenv("GG_SHORT", "1" if request.param == "short" else "0")
+    else:
         monkeypatch.delenv("GG_SMALL")
         monkeypatch.setenv("GG_FEW", str(request.param))
     return request.param
@@ -84,6 +87,8 @@ CASES = [  # n, k, rows of the groups
     (4096, 7168, [1, 2]),
     (8, 131056, [3]),
     (1032, 528, [40] * 70),
+    (776, 1424, [192, 193, 384, 0, 1, 191, 575]),
+    (264, 512, [150] * 64),
 ]
 
 
