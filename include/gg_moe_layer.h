@@ -43,8 +43,7 @@ typedef enum gg_norm_scale {
  * fp8: y = round(h * rstd * weight / scale), scale = max |h * rstd * weight| / (the format's largest
  * value), 1 where that is zero or subnormal. A NaN in a row makes its rstd, y and (for a tensor scale, every) scale NaN.
  * int8: the same with 127 for the format's largest value, rounded to the nearest whole number, halves to even. A row
- * with a NaN or an infinity has a scale of NaN or infinity and holds no number past 127; where |y| is not finite or the
- * scale is NaN it holds 0.
+ * whose largest |y| is a NaN or an infinity has that (a NaN first) for a scale and holds zeros.
  *   dtype: GG_DTYPE_BF16 or GG_DTYPE_FP16 (x, residual, h; y unless 8-bit). weight_dtype: the same or
  *   GG_DTYPE_FP32. out_dtype: dtype, an fp8 type with scale_mode 1-3, or GG_DTYPE_INT8 with GG_NORM_SCALE_ROW.
  *   h: [rows, hidden]; may be x or residual itself. Not written (and may be NULL) without a residual.
@@ -79,8 +78,8 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
 
 /*
  * As gg_rms_norm, of h less its row's mean: mean = mean(h), rstd = 1 / sqrt(mean((h - mean)^2) + eps),
- * y = (h - mean) * rstd * weight + bias. The squares are summed about the mean that was found, so rows of a
- * large mean lose nothing. bias: [hidden] of weight_dtype, or NULL for none. mean, rstd: [rows], or NULL but for
+ * y = (h - mean) * rstd * weight + bias. The squares are summed about means, so rows of a large mean lose nothing
+ * (a row of one value gives its bias, with eps = 0 NaN). bias: [hidden] of weight_dtype, or NULL for none. mean, rstd: [rows], or NULL but for
  * GG_NORM_SCALE_TENSOR. Types, scales, workspace and rules as there; bias 16-byte aligned.
  */
 int gg_layer_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
@@ -118,7 +117,8 @@ int gg_silu_product(int dtype, int out_dtype, int64_t rows, int64_t inner, const
 int gg_silu_product_backward(int dtype, int64_t rows, int64_t inner, const void *grad_y, int64_t grad_y_stride,
                              const void *gu, int64_t gu_stride, void *grad_gu, void *stream);
 
-/* y [rows, n] int8 contiguous and scale [rows] of the rows of x (bf16 or fp16), as gg_rms_norm's int8 rows. Rules as above for n. */
+/* y [rows, n] int8 contiguous, overlapping no input, and scale [rows] of the rows of x (bf16 or fp16), as gg_rms_norm's int8
+ * rows. Rules as above for n. */
 int gg_quantize_rows(int dtype, int64_t rows, int64_t n, const void *x, int64_t x_stride, int8_t *y, float *scale, void *stream);
 
 /* ---- router ---- */

@@ -250,10 +250,9 @@ def test_backward(pkg, dtype, m, n, grad_h, w32):
     assert all(torch.equal(a, c) for a, c in zip(got, again))
 
 
-@pytest.mark.parametrize("m", [5, 700])
+@pytest.mark.parametrize("m,n", [(5, 1544), (700, 1544), (600, 20000), (530, 12296)])
 @pytest.mark.parametrize("place", ["grad_y", "h", "grad_h"])
-def test_backward_strides_and_in_place(pkg, m, place):
-    n = 1544
+def test_backward_strides_and_in_place(pkg, m, n, place):
     x, r, w, b = _data(m, n, BF, 11)
     g = _gen(12)
     t = {"grad_y": torch.randn(m, n, device=DEV, generator=g).to(BF), "grad_h": torch.randn(m, n, device=DEV, generator=g).to(BF)}
