@@ -580,6 +580,8 @@ int allocate_plan(gg_plan *p, hipStream_t s) {
 // tiles, the staged bytes (each small tile stages its own operands) decide against it.
 // Plans of more than kFewMaxSmallTiles 128 x 128 tiles whose groups average over 64 rows keep them:
 // the few-row tiles ran 0.73-1.28x there (7 of the 300 problems), and the model is no better than that.
+// int8 plans take the fp8 constants (the bytes and cycles are the same): of 17 problems of 8 to 1600 rows, 7 to 206 MB of w,
+// the choice was the best instance or within 7 % of it on 15, 10 % off on two (4 x 128 rows, 4096 x 7168 31 us, best 28).
 // GG_SMALL in the environment (0: no small tiles, 1: 128 x 128 tiles) turns it off; without it,
 // GG_FEW=<i> takes instance i (GG_FEW=-1: none).
 constexpr double kFewFixedUs = 1.6, kFewRoundUs = 1.9;
@@ -938,8 +940,8 @@ size_t device_table_bytes(int group_num) { return size_t(group_num) * sizeof(gg:
 // groups as a router spreads them (the octiles' means of a gamma distribution of shape 6), and the count is sure to
 // about n_tiles sqrt(group_num / 12), the spread of the groups' last tiles: rounds are averaged over three counts that
 // far apart, and a gain of 5 % on average is taken if the worst case loses no more than 12 %. us, 256 and 192 rows:
-// taken 8 groups of 4160 rows, 7168 x 2048 88 -> 72; the same, 4096 x 7168 144 -> 124; 8320 rows 220 -> 200; 1200 78 ->
-// 70; left 32768 rows 696 (707), 32 x 16640, 2880 x 2880 164 (169), 1 x 2048, 7168 x 2048 32 (43), 16 x 20000,
+// taken 8 groups of 4160 rows in all, 7168 x 2048 88 -> 72; the same, 4096 x 7168 144 -> 124; 8320 rows 220 -> 200;
+// 1200 78 -> 70; left 32768 rows 696 (707), 32 x 16640, 2880 x 2880 164 (169), 1 x 2048, 7168 x 2048 32 (43), 16 x 20000,
 // 1408 x 2048 58 (66); missed 64 x 8192, 2048 x 1408 66 (58). GG_SHORT=0 or 1 in the environment decides it.
 constexpr double kShortStep = 0.83;
 bool use_short_i8(int group_num, int64_t rows, int64_t n_tiles, int64_t k_tiles, int cus) {

@@ -28,7 +28,8 @@
 // Measured (MI355X, us per launch back to back, the plans that ran before -> this kernel): bf16
 // forward 4 x 256 rows, 512 x 1024 12.3 -> 6.4; 36 x 16, 2048 x 1024 35.9 -> 23.4 (6.4 TB/s of w, part of
 // it from the Infinity Cache); 1 x 512, 2880 x 2880 28.5 -> 20.3; 3 x 5 (device sizes), 3328 x 12256 130 -> 38;
-// fp8 forward 4 x 3, 9840 x 800 14.7 -> 6.0; dgrad bf16 3 x 14, 1208 x 2048 25.3 ->
+// fp8 forward 4 x 3, 9840 x 800 14.7 -> 6.0; int8 forward 8 of 32 groups with one row each, 4096 x 7168 (w from HBM) 57 -> 41,
+// 5.7 TB/s; dgrad bf16 3 x 14, 1208 x 2048 25.3 ->
 // 6.0, fp8 32 x 64, 2512 x 768 26.4 -> 17.3. The ring's depth and the waves were swept (29
 // combinations of 1-8 row blocks, 1-4 column blocks, 1-16 waves, 1-4 chunks): what pays is many
 // small workgroups per CU, not a deep ring (16 rows: 4 waves x 2 chunks, 2 per CU, 29.1 against

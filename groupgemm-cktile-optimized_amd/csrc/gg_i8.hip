@@ -4,6 +4,8 @@
 // The sums are exact in int32; each is made a float32 once, takes both scales and is rounded to 16 bits. They run on the
 // grouped GEMM's own kernels: many rows on the persistent 256 x 256 one (gg_kernel_impl.h, mode kInI8), few on the
 // few-row one (gg_few.hip), chosen by the launch-time model of the device-size plans (choose_few_rows).
+// What bounds it: few rows, the reading of w (8 of 32 groups with a row each, 4096 x 7168: 41 us, 5.7 TB/s); many, the
+// matrix pipes (8 groups of 32768 rows in all, 4096 x 7168: 690 us, 2.8 POP/s).
 #include "gg_i8.h"
 
 #include "gg_layer.h"
