@@ -96,9 +96,9 @@ template <typename T, bool BACK> __global__ void __launch_bounds__(256) silu_ker
             unpack8<T>(load_once(static_cast<const uint16_t *>(a.grad) + row * a.grad_stride + i), g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float s = sigmoid(v[j]);
-                d[j]          = g[j] * u[j] * s * (1.f + v[j] * (1.f - s));
-                g[j]          = g[j] * v[j] * s;
+                const float s = sigmoid(v[j]); // (grad_y last: its product with a large gate or up may be past float32)
+                d[j]          = s * (1.f + v[j] * (1.f - s)) * u[j] * g[j];
+                g[j]          = v[j] * s * g[j];
             }
             uint16_t *o = static_cast<uint16_t *>(a.y) + row * 2 * a.inner + i;
             *reinterpret_cast<u32x4 *>(o)           = pack8<T>(d);

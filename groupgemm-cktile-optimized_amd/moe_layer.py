@@ -668,16 +668,17 @@ class I8Weights(NamedTuple):
 
 def quantize_i8(w) -> I8Weights:
     """int8 form of weights [B, N, K] (bf16, fp16 or float32), one scale for each output channel: max |w| / 127 (1 for a
-    channel of zeros), values rounded to the nearest. Any device."""
+    channel of zeros), values rounded to the nearest. A channel with a NaN or an infinity has that for a scale and holds
+    zeros, so that what is multiplied by it is NaN. Any device."""
     if w.dim() != 3 or w.dtype not in (*_T16, torch.float32):
         raise ValueError("w must be bfloat16, float16 or float32 [B, N, K]")
     q = torch.empty(w.shape, dtype=torch.int8, device=w.device)
     s = torch.empty(w.shape[:2], dtype=torch.float32, device=w.device)
     for i in range(w.shape[0]):  # one matrix at a time: the layers' weights may fill the card
-        v = w[i].float()
+        v = w[i].detach().float()
         top = v.abs().amax(1) / 127
-        s[i] = torch.where(top > 0, top, torch.ones_like(top))
-        q[i] = (v / s[i][:, None]).round().clamp(-127, 127).to(torch.int8)
+        s[i] = torch.where(top == 0, torch.ones_like(top), top)
+        q[i] = torch.where(top.isfinite()[:, None], v / s[i][:, None], torch.zeros_like(v)).round().clamp(-127, 127).to(torch.int8)
     return I8Weights(q, s)
 
 

@@ -208,3 +208,24 @@ def test_captured(pkg):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+def test_gradient_of_large_values(pkg):
+    """grad_y * up or grad_y * gate past float32 where the gradient itself is not (the sigmoid is far below one)."""
+    n = 64
+    gy = torch.full((3, n), 2.0**100, device=DEV)
+    v = torch.linspace(-60, -20, n, device=DEV).repeat(3, 1)
+    u = torch.full((3, n), 2.0**100, device=DEV)
+    u[0], gy[1], u[1] = 2.0**60, 2.0**126, 1.0
+    v[2] = -200.0
+    gu, gy = torch.cat([v, u], 1).to(BF), gy.to(BF)
+    got = pkg.silu_product_backward(gy, gu).double()
+    v, u = gu.double().chunk(2, dim=1)
+    p, g = torch.sigmoid(v), gy.double()
+    rel = (12 + 3 * v.abs()) * E * (1 + v.abs())  # as above, by the size of the terms of 1 + v (1 - p)
+    for part, want in ((got[:, :n], g * u * p * (1 + v * (1 - p))), (got[:, n:], g * v * p)):
+        here = want.abs() < 2.0**127
+        off = rel * want.abs()
+        assert int(here[:2].sum()) > n and not bool(part.isnan().any())
+        assert bool(((part - want).abs() <= HALF[BF] * (want.abs() + off) + off + TINY[BF])[:2][here[:2]].all())
+    assert bool((got[2] == 0).all())  # exp(200) is past float32: the sigmoid is 0

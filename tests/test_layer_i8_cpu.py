@@ -208,3 +208,14 @@ def test_quantize_i8_on_the_host(pkg):
         pkg.quantize_i8(w[0])
     with pytest.raises(ValueError, match="device"):
         pkg.grouped_gemm_i8(torch.zeros(3, 64, dtype=torch.int8), q, [1, 2], torch.ones(3))
+
+
+def test_quantize_i8_of_what_is_not_finite(pkg):
+    """A channel with a NaN or an infinity must not come out as finite numbers; a leaf's scales are no part of its graph."""
+    w = torch.ones(1, 4, 16)
+    w[0, 1, 3], w[0, 2, 5], w[0, 3] = float("nan"), -float("inf"), 0.0
+    q = pkg.quantize_i8(w.requires_grad_())
+    s = q.scales[0]
+    assert not q.scales.requires_grad and float(s[3]) == 1.0 and bool((q.w[0, 0] == 127).all())
+    assert bool(s[1].isnan()) and float(s[2]) == float("inf") and bool((q.w[0, 1:] == 0).all())
+    assert bool((q.w[0].float() * s[:, None])[1:3].isnan().all())
