@@ -251,6 +251,24 @@ def test_torch_level_refusals(pkg):
         pkg.grouped_gemm_i8(x[:, :120].contiguous(), pkg.I8Weights(w[:, :, :120].contiguous(), ws), lens, xs)
 
 
+def test_offsets_past_32_bits(pkg, kernel):
+    """x, w and out of more than 2^32 bytes: the last group, at their ends, comes out as it does alone."""
+    b, m, n, k = 40, 300000, 8192, 16384
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    rows, (x1, xs1, w1, ws1) = 5, _data(1, 5, n, k, 4)
+    want = pkg.grouped_gemm_i8(x1, pkg.I8Weights(w1, ws1), torch.tensor([rows], device=DEV), xs1)
+    assert torch.equal(want, _want(x1, xs1, w1, ws1, [rows], [0], BF, 0.0))
+    x, w = torch.zeros(m, k, device=DEV, dtype=I8), torch.zeros(b, n, k, device=DEV, dtype=I8)
+    xs, ws = torch.zeros(m, device=DEV), torch.zeros(b, n, device=DEV)
+    x[-rows:], xs[-rows:], w[-1], ws[-1] = x1, xs1, w1[0], ws1[0]
+    lens = torch.zeros(b, dtype=torch.int64, device=DEV)
+    lens[-1] = rows
+    offs = torch.zeros(b + 1, dtype=torch.int64, device=DEV)
+    offs[b - 1:] = torch.tensor([m - rows, m], device=DEV)
+    assert torch.equal(pkg.grouped_gemm_i8(x, pkg.I8Weights(w, ws), lens, xs, group_offs=offs)[-rows:], want)
+
+
 # ---- rows with their scales to the experts ----
 
 

@@ -336,3 +336,22 @@ def test_captured_forward_and_backward(pkg, m, n):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, c) for a, c in zip(got, want)), i
+
+
+def test_more_rows_than_32_bits_of_bytes(pkg):
+    """Offsets past 2^32: the last rows are those of a call of as many as take the same kernels."""
+    m, n, k = 140000, 16384, 600
+    if torch.cuda.mem_get_info()[0] < 30 << 30:
+        pytest.skip("needs 30 GB")
+    g = torch.Generator(device=DEV).manual_seed(6)
+    h, gy = torch.zeros(m, n, device=DEV, dtype=BF), torch.zeros(m, n, device=DEV, dtype=BF)
+    for t in (h, gy):
+        t[-k:] = torch.randn(k, n, device=DEV, generator=g).to(BF)
+    w, b = torch.randn(2, n, device=DEV, generator=g).to(BF)
+    o, last = pkg.layer_norm(h, w, b), pkg.layer_norm(h[-k:], w, b)
+    assert all(torch.equal(o[i][-k:], last[i]) for i in (0, 2, 3))
+    gx, gx_last = (pkg.layer_norm_backward(gy[i:], h[i:], w, o.mean[i:], o.rstd[i:])[0] for i in (0, m - k))
+    assert torch.equal(gx[-k:], gx_last)
+    del gx
+    q, last = pkg.layer_norm(h, w, b, out_dtype=torch.int8, scale="row"), pkg.layer_norm(h[-k:], w, b, out_dtype=torch.int8, scale="row")
+    assert torch.equal(q.y[-k:], last.y) and torch.equal(q.scale[-k:], last.scale)
