@@ -604,16 +604,16 @@ struct CenterArgs {
 };
 
 // With d = h - mean: grad_x = grad_h + rstd (w g - mean(w g)) - d rstd^3 mean(w g d), row by row; the partial sums of
-// g d rstd and of g stay in registers over the rows of a workgroup and are written once. Two sums a column are twice the
-// registers of the RMS norm's one, so rows past 8192 values take eight waves, and with more than four pieces a lane (past
+// g d rstd and of g stay in registers over the rows of a workgroup, which has R at a time, and are written once. Two sums a
+// column are twice the registers of the RMS norm's one, so rows past 8192 values take eight waves, and with more than four pieces a lane (past
 // 16384) load the inputs again, from the caches, instead of keeping them.
-template <typename T, int WPR, int U, bool SUMS>
-__global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const CenterArgs c) {
-    __shared__ PairReduce<WPR> m;
+template <typename T, int WPR, int U, bool SUMS, int R>
+__global__ void __launch_bounds__(64 * WPR * R) center_back_kernel(const CenterArgs c) {
+    __shared__ PairReduce<WPR> m[R];
     const BackArgs &a    = c.b;
     constexpr bool  kKeep = U <= 4;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int t    = WPR == 1 ? lane : static_cast<int>(threadIdx.x);
+    const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) % WPR, own = __builtin_amdgcn_readfirstlane(threadIdx.x / (64 * WPR));
+    const int t    = static_cast<int>(threadIdx.x) % (64 * WPR);
     float     dw[U][8], db[U][8];
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -621,10 +621,11 @@ __global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const C
         for (int j = 0; j < 8; ++j)
             dw[u][j] = db[u][j] = 0.f;
     int           turn = 0;
-    const int64_t step = static_cast<int64_t>(gridDim.x) * rows_per_block(WPR);
-    // every wave of a block that shares a row makes the same trips, so the barriers match
-    for (int64_t row = static_cast<int64_t>(blockIdx.x) * rows_per_block(WPR) + (WPR == 1 ? wave : 0); row < a.rows;
-         row += step, turn ^= 1) {
+    const int64_t step = static_cast<int64_t>(gridDim.x) * R;
+    // every wave of the workgroup makes the same trips, so the barriers match; past the last row they have no values
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * R; first < a.rows; first += step, turn ^= 1) {
+        const int64_t   row  = R == 1 ? first : std::min(first + own, a.rows - 1);
+        const int       here = R == 1 || first + own < a.rows ? a.hidden : 0;
         const uint16_t *gp = static_cast<const uint16_t *>(a.g) + row * a.g_stride;
         const uint16_t *hp = static_cast<const uint16_t *>(a.h) + row * a.h_stride;
         const uint16_t *rp = a.gh == nullptr ? nullptr : static_cast<const uint16_t *>(a.gh) + row * a.gh_stride;
@@ -635,7 +636,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const C
 #pragma unroll
             for (int u = 0; u < U; ++u) {
                 const int i = (u * 64 * WPR + t) * 8;
-                if (i < a.hidden) {
+                if (i < here) {
                     gw[u] = load_once(gp + i);
                     hw[u] = load_once(hp + i);
                     if (rp != nullptr)
@@ -646,7 +647,7 @@ __global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const C
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
-            if (i < a.hidden) {
+            if (i < here) {
                 float g[8], h[8], w[8];
                 unpack8<T>(kKeep ? gw[u] : *reinterpret_cast<const u32x4 *>(gp + i), g);
                 unpack8<T>(kKeep ? hw[u] : *reinterpret_cast<const u32x4 *>(hp + i), h);
@@ -663,14 +664,14 @@ __global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const C
                 }
             }
         }
-        row_sums<WPR>(m, turn, sum, dot, wave, lane);
+        row_sums<WPR>(m[own], turn, sum, dot, wave, lane);
         const float n  = static_cast<float>(a.hidden);
         const float c1 = rstd * (sum / n), c2 = rstd * (rstd * (rstd * (dot / n))); // (rstd^3 alone may be past float32)
         const float c3 = fmaf(c2, mean, -c1);
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
-            if (i < a.hidden) {
+            if (i < here) {
                 float g[8], h[8], w[8], r[8];
                 unpack8<T>(kKeep ? gw[u] : load_once(gp + i), g);
                 unpack8<T>(kKeep ? hw[u] : load_once(hp + i), h);
@@ -690,30 +691,30 @@ __global__ void __launch_bounds__(block_threads(WPR)) center_back_kernel(const C
     }
     if constexpr (!SUMS)
         return;
-    // a workgroup whose waves had rows of their own adds them up first, in their order
-    if constexpr (WPR == 1) {
-        __shared__ f32x4 mine[3][U][4][64];
-        if (wave > 0)
+    // the sums of a workgroup's R rows are added up first, in their order
+    if constexpr (R > 1) {
+        __shared__ f32x4 mine[R - 1][U][4][64 * WPR];
+        if (own > 0)
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
-                    mine[wave - 1][u][q][lane]     = f32x4{dw[u][4 * q], dw[u][4 * q + 1], dw[u][4 * q + 2], dw[u][4 * q + 3]};
-                    mine[wave - 1][u][2 + q][lane] = f32x4{db[u][4 * q], db[u][4 * q + 1], db[u][4 * q + 2], db[u][4 * q + 3]};
+                    mine[own - 1][u][q][t]     = f32x4{dw[u][4 * q], dw[u][4 * q + 1], dw[u][4 * q + 2], dw[u][4 * q + 3]};
+                    mine[own - 1][u][2 + q][t] = f32x4{db[u][4 * q], db[u][4 * q + 1], db[u][4 * q + 2], db[u][4 * q + 3]};
                 }
         __syncthreads();
-        if (wave > 0)
+        if (own > 0)
             return;
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int q = 0; q < 2; ++q)
 #pragma unroll
-                for (int o = 0; o < 3; ++o)
+                for (int o = 0; o < R - 1; ++o)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        dw[u][4 * q + j] += mine[o][u][q][lane][j];
-                        db[u][4 * q + j] += mine[o][u][2 + q][lane][j];
+                        dw[u][4 * q + j] += mine[o][u][q][t][j];
+                        db[u][4 * q + j] += mine[o][u][2 + q][t][j];
                     }
     }
     float *part = a.parts + static_cast<int64_t>(blockIdx.x) * 2 * a.hidden;
@@ -877,26 +878,41 @@ template <typename T> int run_back(const BackArgs &a, void *grad_weight, hipStre
                             static_cast<int>(back_blocks(a.rows, a.hidden)), a.hidden, a.hidden, grad_weight, nullptr, a.w32);
 }
 
-// Layer norm's backward pass: waves of a row and pieces of a lane (see center_back_kernel), and workgroups: those that 256
-// CUs hold at once by the instances' registers (a test holds the numbers to the compiler's report), fewer of few rows as in
-// back_blocks. (The next row's values under way while a row is worked on cost registers, and so workgroups: 16640 x 2880
-// 102 us instead of 79; forcing five waves a SIMD where the registers give four spilled: 90.)
-int center_waves(int64_t hidden) { return hidden <= 1024 ? 1 : hidden <= 8192 ? 4 : 8; }
-template <typename F> int with_center_shape(int64_t hidden, F f) {
-    using std::integral_constant;
-    const int wpr = center_waves(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
-#define GG_SHAPE(W, N)                                                                                                 \
-    if (wpr == W && u <= N)                                                                                            \
-        return f(integral_constant<int, W>{}, integral_constant<int, N>{});
-    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(4, 4) GG_SHAPE(8, 3) GG_SHAPE(8, 4)
-#undef GG_SHAPE
-    return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
+// Layer norm's backward pass: waves of a row, pieces of a lane and rows of a workgroup (see center_back_kernel). Rows that
+// share a workgroup share its partial sums, but wait for each other at the barriers. us at one, two and three rows:
+// 1000 x 2880 17.6, 14.8, 14.5; 1500 x 4096 24.8, 22.9, 20.3; 16640 x 2048 61.3, 63.6, 56.6; of 6144 163, 170, 160; but 8192 x
+// 4096 61.8, 59.3, 60.9; 16640 x 2880 82.1, 81.4, 87.2; at one and two (three are short of registers) 2500 x 7168 48.8, 43.9,
+// 8192 x 7168 104, 110. So two rows past 2048 with two pieces, with four two up to 4096 and then one.
+struct CenterShape {
+    int waves, pieces, rows;
+};
+CenterShape center_shape(int64_t rows, int64_t hidden) {
+    const int wpr = hidden <= 1024 ? 1 : hidden <= 8192 ? 4 : 8, u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
+    return {wpr, wpr == 8 ? (u <= 3 ? 3 : u == 4 ? 4 : 8) : u,
+            wpr == 1 ? 4 : wpr == 8 ? 1 : u == 2 ? (rows <= 2048 ? 3 : 2) : u == 4 ? (rows <= 4096 ? 2 : 1) : 3};
 }
+template <typename F> int with_center_shape(int64_t rows, int64_t hidden, F f) {
+    using std::integral_constant;
+    const CenterShape c = center_shape(rows, hidden);
+#define GG_SHAPE(W, N, R)                                                                                              \
+    if (c.waves == W && c.pieces == N && c.rows == R)                                                                  \
+        return f(integral_constant<int, W>{}, integral_constant<int, N>{}, integral_constant<int, R>{});
+    GG_SHAPE(1, 1, 4) GG_SHAPE(1, 2, 4) GG_SHAPE(4, 1, 3) GG_SHAPE(4, 2, 2) GG_SHAPE(4, 2, 3) GG_SHAPE(4, 3, 3) GG_SHAPE(4, 4, 1)
+    GG_SHAPE(4, 4, 2) GG_SHAPE(8, 3, 1) GG_SHAPE(8, 4, 1)
+#undef GG_SHAPE
+    return f(integral_constant<int, 8>{}, integral_constant<int, 8>{}, integral_constant<int, 1>{});
+}
+// Its workgroups: at most those that 256 CUs hold at once by the instances' registers (a test holds the numbers to the
+// compiler's report). Of up to eight turns each has as many as the others (3200 x 6144 46.1 -> 44.0; of many, what the
+// last turn leaves idle is less than what fewer workgroups lose, 16640 x 2880 81.4, 83.5), and past 256 two turns at least,
+// which halves the partial sums (1500 x 1536 13.0 -> 11.5). (The next row's values under way while a row is worked on cost registers, and so workgroups:
+// 16640 x 2880 102 us instead of 79; forcing five waves a SIMD where the registers give four spilled: 90.)
 int64_t center_blocks(int64_t rows, int64_t hidden) {
-    const int     wpr = center_waves(hidden), u = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
-    const int64_t fit = wpr == 8 ? 256 : u == 1 ? (wpr == 4 ? 1536 : 1280) : u == 2 && wpr == 4 ? 1024 : 768;
-    const int64_t b   = row_blocks(rows, hidden);
-    return std::min(fit, std::max(b / 4, b <= 256 ? b : std::min<int64_t>(b / 2, 512)));
+    const CenterShape c     = center_shape(rows, hidden);
+    const int64_t     fit   = c.waves == 8 ? 256 : c.waves == 1 ? (c.pieces == 1 ? 1280 : 768) : c.rows == 1 ? 768 : c.pieces == 1 || (c.pieces == 2 && c.rows == 2) ? 512 : 256;
+    const int64_t     b     = (rows + c.rows - 1) / c.rows;
+    const int64_t     turns = std::max<int64_t>((b + fit - 1) / fit, b <= 256 ? 1 : 2);
+    return turns > 8 ? fit : (b + turns - 1) / turns;
 }
 
 template <typename T> int run_center_back(const CenterArgs &a, void *grad_weight, void *grad_bias, hipStream_t s) {
@@ -904,13 +920,14 @@ template <typename T> int run_center_back(const CenterArgs &a, void *grad_weight
     if (few(rows, hidden)) { // (the sums first: grad_x may take the place of an input)
         const int st = launch("layer_norm_backward", center_strip_kernel<T>, (hidden + 63) / 64, 1024, s, a, grad_weight, grad_bias);
         return st ? st : with_shape<true>(hidden, [&](auto wpr, auto u) {
-            return launch("layer_norm_backward", center_back_kernel<T, wpr.value, u.value, false>, row_blocks(rows, hidden),
-                          block_threads(wpr.value), s, a);
+            constexpr int r = rows_per_block(wpr.value);
+            return launch("layer_norm_backward", center_back_kernel<T, wpr.value, u.value, false, r>, row_blocks(rows, hidden),
+                          64 * wpr.value * r, s, a);
         });
     }
     const int blocks = static_cast<int>(center_blocks(rows, hidden));
-    const int st     = with_center_shape(hidden, [&](auto wpr, auto u) {
-        return launch("layer_norm_backward", center_back_kernel<T, wpr.value, u.value, true>, blocks, block_threads(wpr.value), s, a);
+    const int st     = with_center_shape(rows, hidden, [&](auto wpr, auto u, auto r) {
+        return launch("layer_norm_backward", center_back_kernel<T, wpr.value, u.value, true, r.value>, blocks, 64 * wpr.value * r.value, s, a);
     });
     return st ? st : launch("layer_norm_backward", weight_sum_kernel<T>, (2 * hidden + 31) / 32, 1024, s, a.b.parts, blocks,
                             2 * a.b.hidden, a.b.hidden, grad_weight, grad_bias, a.b.w32);

@@ -250,6 +250,23 @@ def test_backward(pkg, dtype, m, n, grad_h, w32):
     assert all(torch.equal(a, c) for a, c in zip(got, again))
 
 
+@pytest.mark.parametrize("m,n", [(601, 1536), (602, 2880), (2047, 2056), (2050, 2880), (599, 6144), (1027, 8192), (4097, 7168), (4096, 6152),
+                                 (4099, 1032), (3100, 4104)])
+def test_backward_with_a_last_workgroup_that_is_not_full(pkg, m, n):
+    """Workgroups have two or three rows at a time: those that are not there change nothing, in place as well."""
+    x, r, w, b = _data(m, n, BF, m + n, F32)
+    g = _gen(m)
+    gy, gh = (torch.randn(m, n, device=DEV, generator=g).to(BF) for _ in range(2))
+    o = pkg.layer_norm(x, w, b, r)
+    whole = torch.full((m + 3, n), 7.0, device=DEV, dtype=BF)
+    got = pkg.layer_norm_backward(gy, o.h, w, o.mean, o.rstd, gh, out=whole[:m])
+    _check_back(got, _back_reference(gy, o.h, w, o.mean, o.rstd, gh), BF, F32)
+    assert bool((whole[m:] == 7).all())
+    own = o.h.clone()
+    again = pkg.layer_norm_backward(gy, own, w, o.mean, o.rstd, gh, out=own)
+    assert all(torch.equal(a, c) for a, c in zip(got, again))
+
+
 @pytest.mark.parametrize("m,n", [(5, 1544), (700, 1544), (600, 20000), (530, 12296)])
 @pytest.mark.parametrize("place", ["grad_y", "h", "grad_h"])
 def test_backward_strides_and_in_place(pkg, m, n, place):

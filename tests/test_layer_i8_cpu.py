@@ -123,29 +123,35 @@ def test_torch_functions_refuse_host_tensors_and_types(pkg):
             f(x.float())
 
 
-def test_backward_workgroups_fit_the_gpu(pkg):
+@pytest.mark.parametrize("rows", [600, 1500, 2048, 2049, 4096, 4097, 16640, 1 << 20])
+def test_backward_workgroups_fit_the_gpu(pkg, rows):
     """The layer norm's gradient takes no more workgroups than 256 CUs hold at once, by the compiler's report of each
-    instance's waves for each of a CU's four SIMDs: the numbers are written down, as the workspace's size needs them."""
+    instance's waves for each of a CU's four SIMDs and its LDS: the numbers are written down, as the workspace's size needs
+    them. Every workgroup has rows."""
     path = os.path.join(ROOT, "groupgemm-cktile-optimized_amd", "lib", "resource_usage.txt")
     if not os.path.exists(path):
         pytest.skip("library not built")
-    waves, name = {}, None
+    report, name = {}, None
     with open(path, errors="replace") as f:
         for line in f:
             m = re.search(r"Function Name: (\S+)", line)
-            if m:  # <type, waves of a row, pieces, with the sums>
-                name = re.search(r"center_back_kernelINS0_\w+?ELi(\d+)ELi(\d+)ELb1E", m.group(1))
-            m = re.search(r"Occupancy \[waves/SIMD\]: (\d+)", line)
+            if m:  # <type, waves of a row, pieces, with the sums, rows>
+                name = re.search(r"center_back_kernelINS0_\w+?ELi(\d+)ELi(\d+)ELb1ELi(\d+)E", m.group(1))
+            m = re.search(r"(Occupancy \[waves/SIMD\]|LDS Size \[bytes/block\]): (\d+)", line)
             if m and name:
-                key = int(name.group(1)), int(name.group(2))
-                waves[key] = min(waves.get(key, 8), int(m.group(1)))
-    assert len(waves) >= 9
+                report.setdefault(tuple(map(int, name.groups())), {}).setdefault(m.group(1)[:3], []).append(int(m.group(2)))
+    assert len(report) >= 11
     for hidden in (8, 512, 520, 1024, 1032, 2048, 2056, 4096, 4104, 6144, 6152, 8192, 8200, 12288, 12296, 16384, 16392, 32768):
+        lib = pkg.load_library()
+        if lib.gg_layer_norm_backward_workspace(rows, hidden) == 0:
+            continue  # few rows
         wpr = 1 if hidden <= 1024 else 4 if hidden <= 8192 else 8
-        pieces = min(p for w, p in waves if w == wpr and p * 512 * w >= hidden)
-        of_block = max(wpr, 4)
-        blocks = pkg.load_library().gg_layer_norm_backward_workspace(1 << 20, hidden) // (8 * hidden)
-        assert 256 <= blocks <= 256 * (waves[wpr, pieces] * 4 // of_block), (hidden, blocks, waves[wpr, pieces])
+        pieces = min(p for w, p, _ in report if w == wpr and p * 512 * w >= hidden)
+        held = {1: 4, 8: 1}.get(wpr) or {2: 3 if rows <= 2048 else 2, 4: 2 if rows <= 4096 else 1}.get(pieces, 3)
+        at = report[wpr, pieces, held]
+        of_cu = min(min(at["Occ"]) * 4 // max(wpr * held, 4), 160 * 1024 // max(max(at["LDS"]), 1))
+        blocks = lib.gg_layer_norm_backward_workspace(rows, hidden) // (8 * hidden)
+        assert of_cu >= 1 and (256 if rows >= 1 << 20 else 1) <= blocks <= min(256 * of_cu, -(-rows // held)), (hidden, blocks, at)
 
 
 # ---- 8-bit integer products ----
