@@ -15,7 +15,7 @@
 // read, h written: 5.8 TB/s) and 133 for the second (h read, y written: 5.3); 5 rows to bf16 3.8, the latency of a launch,
 // a row's loads and a barrier. Backward 16640 x 2880 with a gradient past the norm: 75 us, 5.1 TB/s (69 row by row, 6 for
 // the weight's gradient). Layer norm: 32768 rows of 4096 bf16 86 us (6.2 TB/s), 8192 of 7168 with residual to int8 72 (5.7),
-// 6 of 7168 4.4; backward 16640 x 2880 with a gradient past the norm 79 (4.9 TB/s; 73 row by row, 6 for the two sums).
+// 6 of 7168 4.4; backward 16640 x 2880 with a gradient past the norm 79 (4.9 TB/s; 5 of it for the two sums), 1024 x 8192 27.
 #include "gg_row.h"
 
 #include <algorithm>
