@@ -111,12 +111,13 @@ constexpr int64_t kMaxBlocks = int64_t(1) << 20;
 
 // f(waves of a row, pieces of a lane). Of many rows, one wave takes a row of up to 2048 values, whose four pieces it has
 // under way together and which needs no barrier: at four waves the kernel waited (us, four waves and one: 32768 rows of
-// 2048 69.4, 56.8, rounding alone 50.6, 35.7). Of few rows the norms' shapes.
+// 2048 69.4, 56.8, rounding alone 50.6, 35.7; 3000 9.9, 8.3; but 1000 5.1, 5.6, 400 3.7, 5.5). Up to 8192 values four waves
+// take one, past it sixteen where there are few (512 of 12288 11.9, 8.3; 1400 18.7, 18.0; 3000 36, 33; rounding alone 23, 24).
 template <typename F> int with_round_shape(int64_t rows, int64_t n, F f) {
     using std::integral_constant;
-    if (few(rows, n))
+    if (n > 8192 && rows <= 1024)
         return with_shape<true>(n, f);
-    if (n > 2048)
+    if (n > 2048 || (n > 1024 && rows <= 1280))
         return with_shape<false>(n, f);
     return n <= 512    ? f(integral_constant<int, 1>{}, integral_constant<int, 1>{})
            : n <= 1024 ? f(integral_constant<int, 1>{}, integral_constant<int, 2>{})

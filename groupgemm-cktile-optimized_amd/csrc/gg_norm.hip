@@ -787,30 +787,29 @@ template <typename T> __global__ void __launch_bounds__(1024) center_strip_kerne
 
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;
 
-// The layer norm's shapes: of many rows eight waves for a row of 6145 to 8192 values and sixteen for up to 16384, which keep
-// weight and bias in registers and have a next row's values under way, where four would have to choose. us at four, eight and
-// sixteen waves: 8192 rows of 7168 to int8 81.6, 71.9, 90.7, to bf16 82.3, 74.6, 79.3; 4096 of 5120 31.3, 33.3, 33.2; at four
-// and sixteen: 8000 of 12288 97.6, 74.5.
-template <typename F> int with_center_forward(bool few_rows, int64_t hidden, F f) {
+// The layer norm's shapes: eight waves for a row of 6145 to 8192 values and sixteen for up to 16384, which keep weight and
+// bias in registers and have a next row's values under way, where four would have to choose; eight for 4097 to 6144 in few
+// rows. us at four, eight and sixteen waves: 8192 rows of 7168 to int8 81.6, 71.9, 90.7, to bf16 82.3, 74.6, 79.3; 4096 of
+// 5120 31.3, 33.3, 33.2; at four and sixteen: 8000 of 12288 97.6, 74.5; at eight and sixteen, with residual to int8, 64 of
+// 7168 5.0, 5.8, 512 9.2, 11.6; at four and sixteen 512 of 4096 6.2, 7.5, 64 4.8, 4.7.
+template <typename F> int with_center_forward(int64_t rows, int64_t hidden, F f) {
     using std::integral_constant;
-    const int wpr = hidden <= 1024    ? 1
-                    : hidden > 16384  ? 8
-                    : few_rows        ? (hidden <= 2048 ? 4 : 16)
-                    : hidden <= 6144  ? 4
-                    : hidden <= 8192  ? 8
-                                      : 16;
+    const int wpr = hidden <= 1024                                      ? 1
+                    : hidden <= 4096 || (hidden <= 6144 && rows > 256) ? 4
+                    : hidden <= 8192 || hidden > 16384                  ? 8
+                                                                        : 16;
     const int u   = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
 #define GG_SHAPE(W, N)                                                                                                 \
     if (wpr == W && u <= N)                                                                                            \
         return f(integral_constant<int, W>{}, integral_constant<int, N>{});
-    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(8, 2) GG_SHAPE(16, 1) GG_SHAPE(16, 2)
+    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(8, 2) GG_SHAPE(16, 2)
 #undef GG_SHAPE
     return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
 }
 // The shape of either norm's forward pass.
-template <bool CENTER, bool WIDE, typename F> int with_norm_shape(int64_t hidden, F f) {
+template <bool CENTER, bool WIDE, typename F> int with_norm_shape(int64_t rows, int64_t hidden, F f) {
     if constexpr (CENTER)
-        return with_center_forward(WIDE, hidden, f);
+        return with_center_forward(rows, hidden, f);
     else
         return with_shape<WIDE>(hidden, f);
 }
@@ -827,7 +826,7 @@ template <typename T, bool CENTER, bool WIDE> int run_norm(const NormArgs &a, bo
     constexpr const char *kWhat = CENTER ? "layer_norm" : "rms_norm";
     const int64_t blocks = row_blocks(a.rows, a.hidden);
     if (a.mode != GG_NORM_SCALE_TENSOR)
-        return with_norm_shape<CENTER, WIDE>(a.hidden, [&](auto wpr, auto u) {
+        return with_norm_shape<CENTER, WIDE>(a.rows, a.hidden, [&](auto wpr, auto u) {
             const auto kernel = i8 ? norm_pass<T, CENTER, wpr.value, u.value, kInt8>() : norm_pass<T, CENTER, wpr.value, u.value, kWhole>();
             // the layer norm's workgroups go from row to row: as many as fit at once
             const int64_t grid = !CENTER || blocks <= 256 ? blocks : std::min<int64_t>(blocks, resident_blocks(kernel, block_threads(wpr.value)));
@@ -840,7 +839,7 @@ template <typename T, bool CENTER, bool WIDE> int run_norm(const NormArgs &a, bo
         b.h        = const_cast<void *>(b.x);
         b.h_stride = b.x_stride;
     }
-    const int st = with_norm_shape<CENTER, WIDE>(a.hidden, [&](auto wpr, auto u) {
+    const int st = with_norm_shape<CENTER, WIDE>(a.rows, a.hidden, [&](auto wpr, auto u) {
         constexpr auto kernel = norm_pass<T, CENTER, wpr.value, u.value, kFirst>();
         // (asked for each call, as devices differ; few workgroups fit in any case)
         b.n_parts = static_cast<int>(blocks <= 256 ? blocks : std::min<int64_t>(blocks, std::min(resident_blocks(kernel, block_threads(wpr.value)), kMaxParts)));
