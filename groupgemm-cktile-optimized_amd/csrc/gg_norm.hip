@@ -15,7 +15,7 @@
 // read, h written: 5.8 TB/s) and 133 for the second (h read, y written: 5.3); 5 rows to bf16 3.8, the latency of a launch,
 // a row's loads and a barrier. Backward 16640 x 2880 with a gradient past the norm: 75 us, 5.1 TB/s (69 row by row, 6 for
 // the weight's gradient). Layer norm: 32768 rows of 4096 bf16 86 us (6.2 TB/s), 8192 of 7168 with residual to int8 72 (5.7),
-// 6 of 7168 4.4; backward 16640 x 2880 with a gradient past the norm 79 (4.9 TB/s; 5 of it for the two sums), 1024 x 8192 27.
+// 6 of 7168 4.7; backward 16640 x 2880 with a gradient past the norm 79 (4.9 TB/s; 5 of it for the two sums), 1024 x 8192 27.
 #include "gg_row.h"
 
 #include <algorithm>
@@ -788,21 +788,21 @@ template <typename T> __global__ void __launch_bounds__(1024) center_strip_kerne
 constexpr int64_t kMaxBlocks = int64_t(1) << 20;
 
 // The layer norm's shapes: eight waves for a row of 6145 to 8192 values and sixteen for up to 16384, which keep weight and
-// bias in registers and have a next row's values under way, where four would have to choose; eight for 4097 to 6144 in few
+// bias in registers and have a next row's values under way, where four would have to choose; eight from 2049 on in few
 // rows. us at four, eight and sixteen waves: 8192 rows of 7168 to int8 81.6, 71.9, 90.7, to bf16 82.3, 74.6, 79.3; 4096 of
 // 5120 31.3, 33.3, 33.2; at four and sixteen: 8000 of 12288 97.6, 74.5; at eight and sixteen, with residual to int8, 64 of
-// 7168 5.0, 5.8, 512 9.2, 11.6; at four and sixteen 512 of 4096 6.2, 7.5, 64 4.8, 4.7.
+// 7168 5.0, 5.8, 512 9.2, 11.6; at four and eight 64 of 4096 4.3, 4.0, 256 4.8, 4.6, 600 7.1, 8.4.
 template <typename F> int with_center_forward(int64_t rows, int64_t hidden, F f) {
     using std::integral_constant;
     const int wpr = hidden <= 1024                                      ? 1
-                    : hidden <= 4096 || (hidden <= 6144 && rows > 256) ? 4
+                    : hidden <= 2048 || (hidden <= 6144 && rows > 256) ? 4
                     : hidden <= 8192 || hidden > 16384                  ? 8
                                                                         : 16;
     const int u   = static_cast<int>((hidden + 512 * wpr - 1) / (512 * wpr));
 #define GG_SHAPE(W, N)                                                                                                 \
     if (wpr == W && u <= N)                                                                                            \
         return f(integral_constant<int, W>{}, integral_constant<int, N>{});
-    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(8, 2) GG_SHAPE(16, 2)
+    GG_SHAPE(1, 1) GG_SHAPE(1, 2) GG_SHAPE(4, 1) GG_SHAPE(4, 2) GG_SHAPE(4, 3) GG_SHAPE(8, 1) GG_SHAPE(8, 2) GG_SHAPE(16, 2)
 #undef GG_SHAPE
     return f(integral_constant<int, 8>{}, integral_constant<int, 8>{});
 }
