@@ -21,7 +21,8 @@ TINY = {BF: 2.0**-134, FP: 2.0**-25}
 E = 2.0**-23
 
 SHAPES = [(1, 8), (3, 64), (5, 512), (7, 520), (4, 1024), (2, 1032), (9, 2048), (3, 2056), (6, 2880), (5, 7168), (2, 8200),
-          (3, 14336), (2, 16392), (1, 32768), (2100, 256), (1025, 1544), (257, 1032), (513, 5128)]
+          (3, 14336), (2, 16392), (1, 32768), (2100, 256), (1025, 1544), (257, 1032), (513, 5128),
+          (1290, 1544), (1300, 2048), (1030, 12288), (1026, 16400), (1024, 9000)]
 
 
 def _gen(seed):

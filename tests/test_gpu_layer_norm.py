@@ -71,7 +71,8 @@ def _check_i8(q, scale, y, off):
 
 
 SHAPES = [(1, 8), (3, 64), (5, 512), (7, 520), (4, 1024), (2, 1032), (9, 2048), (3, 2056), (6, 4096), (5, 7168), (2, 8200),
-          (3, 14336), (2, 16384), (2, 16392), (1, 32768), (2100, 256), (1025, 1544), (520, 5128)]
+          (3, 14336), (2, 16384), (2, 16392), (1, 32768), (2100, 256), (1025, 1544), (520, 5128), (256, 4096), (257, 4096), (256, 6144),
+          (300, 8192)]
 
 
 @pytest.mark.parametrize("dtype", [BF, FP])
@@ -105,7 +106,7 @@ def test_int8_rows(pkg, dtype, m, n):
 @pytest.mark.parametrize("out", [E4, E5])
 @pytest.mark.parametrize("mode", ["tensor", "row", "given"])
 @pytest.mark.parametrize("dtype,m,n", [(BF, 1, 8), (BF, 5, 512), (FP, 3, 1040), (BF, 33, 7168), (FP, 2500, 264), (BF, 2049, 2880),
-                                       (FP, 2, 16400)])
+                                       (FP, 2, 16400), (BF, 256, 2880), (FP, 40, 4096), (BF, 257, 4104), (FP, 30, 6144)])
 def test_fp8(pkg, out, mode, dtype, m, n):
     x, r, w, b = _data(m, n, dtype, m + n)
     ref = _reference(x, r, w, b, 1e-5)
