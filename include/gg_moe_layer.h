@@ -78,9 +78,10 @@ int gg_rms_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hidd
 
 /*
  * As gg_rms_norm, of h less its row's mean: mean = mean(h), rstd = 1 / sqrt(mean((h - mean)^2) + eps),
- * y = (h - mean) * rstd * weight + bias. The squares are summed about means, so rows of a large mean lose nothing
- * (a row of one value gives its bias, with eps = 0 NaN). bias: [hidden] of weight_dtype, or NULL for none. mean, rstd: [rows], or NULL but for
- * GG_NORM_SCALE_TENSOR. Types, scales, workspace and rules as there; bias 16-byte aligned.
+ * y = (h - mean) * rstd * weight + bias. The squares are summed about means, so a large mean costs the variance nothing,
+ * and y no more than the mean's own rounding to float32 times rstd * weight; a row of one value has that value for its mean
+ * and gives its bias (with eps = 0 NaN). bias: [hidden] of weight_dtype, or NULL for none. mean, rstd: [rows], or NULL but
+ * for GG_NORM_SCALE_TENSOR. Types, scales, workspace and rules as there; bias 16-byte aligned.
  */
 int gg_layer_norm(int dtype, int weight_dtype, int out_dtype, int scale_mode, int64_t rows, int64_t hidden, float eps,
                   const void *x, int64_t x_stride, const void *residual, int64_t residual_stride, const void *weight,

@@ -1,0 +1,57 @@
+"""Layer norm where float32 could lose what its definition keeps: rows of one value at widths whose reciprocal is rounded.
+
+A 16-bit value has at most 11 significant bits and a width is 8 * m with m <= 4096, so every sum of equal values of a row is
+a float32 and their quotient is the value itself: mean, y and scale are compared bit for bit.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs an MI355X", allow_module_level=True)
+
+DEV = torch.device("cuda:0")
+BF, FP, F32, E4, I8 = torch.bfloat16, torch.float16, torch.float32, torch.float8_e4m3fn, torch.int8
+# one wave a row, four, eight and sixteen waves, rows that a lane cannot hold; each of widths that are no power of two
+WIDTHS = [56, 520, 1000, 1032, 1992, 2056, 2880, 5000, 6152, 7168, 8200, 14336, 16392, 20000, 32760]
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _constant(m, n, dtype):
+    values = torch.tensor([3.0, 7.0, 1000.0, -0.3, 2.0**-14, -30000.0, 0.0], device=DEV).to(dtype)
+    return values.repeat(-(-m // 7))[:m, None].expand(m, n).contiguous()
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+@pytest.mark.parametrize("m", [7, 600])
+@pytest.mark.parametrize("n", WIDTHS)
+def test_a_row_of_one_value_is_its_bias(pkg, dtype, m, n):
+    x = _constant(m, n, dtype)
+    g = _gen(n)
+    w, b = (1 + torch.randn(n, device=DEV, generator=g)).to(dtype), torch.randn(n, device=DEV, generator=g).to(dtype)
+    o = pkg.layer_norm(x, w, b)
+    assert torch.equal(o.mean, x[:, 0].float()) and bool((o.rstd == o.rstd[0]).all())
+    assert torch.equal(o.y, b.expand(m, n))
+    # of sums that are rounded to one value, too
+    h = pkg.layer_norm(x, w, b, x)
+    assert torch.equal(h.mean, h.h[:, 0].float()) and torch.equal(h.y, b.expand(m, n))
+    # 8-bit outputs: nothing but zeros without a bias
+    q = pkg.layer_norm(x, w, None, None, 1e-5, I8, "row")
+    assert bool((q.y == 0).all()) and bool((q.scale == 1).all())
+    e = pkg.layer_norm(x, w, None, None, 1e-5, E4)
+    assert bool((e.y.float() == 0).all()) and float(e.scale) == 1.0
+
+
+@pytest.mark.parametrize("m", [7, 600])
+@pytest.mark.parametrize("n", WIDTHS)
+def test_a_row_of_one_value_without_eps_is_nan(pkg, m, n):
+    x = _constant(m, n, FP)
+    w = torch.ones(n, device=DEV, dtype=FP)
+    o = pkg.layer_norm(x, w, None, None, 0.0)
+    assert torch.equal(o.mean, x[:, 0].float()) and bool(o.y.isnan().all())
+    q = pkg.layer_norm(x, w, None, None, 0.0, I8, "row")
+    assert bool(q.scale.isnan().all()) and bool((q.y == 0).all())
