@@ -3,6 +3,8 @@
 //
 // y = gate s(gate) up with s(v) = 1 / (1 + exp(-v)); a row holds its gates, then its ups. With p = s(gate):
 // grad_gate = g up p (1 + gate (1 - p)), grad_up = g gate p. Everything in float32 from the 16-bit inputs, rounded once.
+// A sigmoid below 2^-126, that of gates below -87.3, may come out as 0: then y and the gradients lose less than that part of
+// gate up, of g up (1 - gate) and of g gate.
 // Bound by HBM: every value is read once and written once. 16-bit outputs need nothing of the rest of their row, so the
 // pieces of 8 values are dealt to the lanes one after the other. An int8 row's scale needs its largest |y| before the
 // first value is rounded: the row's values stay in registers, as in the norms.
@@ -96,8 +98,10 @@ template <typename T, bool BACK> __global__ void __launch_bounds__(256) silu_ker
             unpack8<T>(load_once(static_cast<const uint16_t *>(a.grad) + row * a.grad_stride + i), g);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const float s = sigmoid(v[j]); // (grad_y last: its product with a large gate or up may be past float32)
-                d[j]          = s * (1.f + v[j] * (1.f - s)) * u[j] * g[j];
+                // (grad_y last: its product with a large gate or up may be past float32; half of the slope, which is up to
+                // 1.1, and twice the result: up times it may be, too)
+                const float s = sigmoid(v[j]);
+                d[j]          = (0.5f * s) * (1.f + v[j] * (1.f - s)) * u[j] * g[j] * 2.f;
                 g[j]          = v[j] * s * g[j];
             }
             uint16_t *o = static_cast<uint16_t *>(a.y) + row * 2 * a.inner + i;

@@ -110,6 +110,7 @@ int gg_layer_norm_backward(int dtype, int weight_dtype, int64_t rows, int64_t hi
  *   y: [rows, inner] contiguous, overlapping no input.
  * gg_silu_product_backward: grad_gu [rows, 2 * inner] contiguous from grad_y [rows, inner]; with p = 1 / (1 + exp(-gate))
  *   grad_gate = grad_y * up * p * (1 + gate * (1 - p)), grad_up = grad_y * gate * p
+ * In both, a sigmoid below 2^-126 (a gate below -87.3) may be taken as 0.
  * grad_gu may take the place of a contiguous gu.
  * GG_ERR_UNSUPPORTED unless inner % 8 == 0, inner <= 32768, strides % 8 == 0 and 16-byte aligned buffers (int8 y: 8-byte).
  */
