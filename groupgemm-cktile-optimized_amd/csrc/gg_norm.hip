@@ -612,7 +612,7 @@ struct CenterArgs {
     const float *mean;
 };
 
-// With d = h - mean: grad_x = grad_h + rstd (w g - mean(w g)) - d rstd^3 mean(w g d), row by row; the partial sums of
+// With d = h - mean: grad_x = grad_h + rstd (w g - mean(w g) - d rstd^2 mean(w g d)), row by row; the partial sums of
 // g d rstd and of g stay in registers over the rows of a workgroup, which has R at a time, and are written once. Two sums a
 // column are twice the registers of the RMS norm's one, so rows past 8192 values take eight waves, and with more than four pieces a lane (past
 // 16384) load the inputs again, from the caches, instead of keeping them.
@@ -674,9 +674,11 @@ __global__ void __launch_bounds__(64 * WPR * R) center_back_kernel(const CenterA
             }
         }
         row_sums<WPR>(m[own], turn, sum, dot, wave, lane);
+        // The row's loads are all back (vmcnt 0) for lanes past its end, too: else the compiler lets each of the next row's
+        // wait for the one before it (4096 x 14336 105 instead of 100 us).
+        __builtin_amdgcn_s_waitcnt(0x0f70);
         const float n  = static_cast<float>(a.hidden);
-        const float c1 = rstd * (sum / n), c2 = rstd * (rstd * (rstd * (dot / n))); // (rstd^3 alone may be past float32)
-        const float c3 = fmaf(c2, mean, -c1);
+        const float c1 = sum / n, c2 = rstd * (rstd * (dot / n)); // of w g and of d in grad_x / rstd (rstd^2 alone may be past float32)
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int i = (u * 64 * WPR + t) * 8;
@@ -685,14 +687,19 @@ __global__ void __launch_bounds__(64 * WPR * R) center_back_kernel(const CenterA
                 unpack8<T>(kKeep ? gw[u] : load_once(gp + i), g);
                 unpack8<T>(kKeep ? hw[u] : load_once(hp + i), h);
                 load_w<T>(a.weight, a.w32, i, w);
+// (h - mean first: c2 h - c2 mean would cancel where the mean is large)
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
-                    g[j] = fmaf(rstd, g[j] * w[j], fmaf(-c2, h[j], c3));
+                    g[j] = fmaf(-c2, h[j] - mean, fmaf(g[j], w[j], -c1));
                 if (rp != nullptr) {
                     unpack8<T>(kKeep ? rw[u] : load_once(rp + i), r);
 #pragma unroll
                     for (int j = 0; j < 8; ++j)
-                        g[j] += r[j];
+                        g[j] = fmaf(rstd, g[j], r[j]);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        g[j] *= rstd;
                 }
                 *reinterpret_cast<u32x4 *>(static_cast<uint16_t *>(a.gx) + row * a.hidden + i) = pack8<T>(g);
             }

@@ -1,4 +1,5 @@
-"""Layer norm where float32 could lose what its definition keeps: rows of one value at widths whose reciprocal is rounded.
+"""Layer norm where float32 could lose what its definition keeps: rows of one value at widths whose reciprocal is rounded,
+gradients of rows of a large mean.
 
 A 16-bit value has at most 11 significant bits and a width is 8 * m with m <= 4096, so every sum of equal values of a row is
 a float32 and their quotient is the value itself: mean, y and scale are compared bit for bit.
@@ -55,3 +56,31 @@ def test_a_row_of_one_value_without_eps_is_nan(pkg, m, n):
     assert torch.equal(o.mean, x[:, 0].float()) and bool(o.y.isnan().all())
     q = pkg.layer_norm(x, w, None, None, 0.0, I8, "row")
     assert bool(q.scale.isnan().all()) and bool((q.y == 0).all())
+
+
+HALF = {BF: 2.0**-8, FP: 2.0**-11, F32: 2.0**-24}
+TINY = {BF: 2.0**-134, FP: 2.0**-25, F32: 2.0**-150}  # half the least subnormal
+F = 1e-5  # of the sum of magnitudes: a float32 chain of at most 64 terms a lane and a tree, below 100 * 2^-24
+
+
+# few rows, many rows of each number of waves and pieces, and rows whose inputs are loaded again
+@pytest.mark.parametrize("mean", [1000.0, -2000.0])
+@pytest.mark.parametrize("m,n", [(8, 520), (1300, 1024), (8, 2880), (600, 2880), (8, 4096), (600, 4096), (4100, 6152), (600, 7168),
+                                 (600, 12288), (8, 20000), (600, 20000)])
+def test_gradient_of_rows_of_a_large_mean(pkg, mean, m, n):
+    """A gradient along the normalised row, of which grad_x takes nearly all away again. h - mean is exact to its own last
+    bit whatever the mean, so each of grad_x's terms is off by a few 2^-24 and the sums by F of their own magnitudes."""
+    g = _gen(n)
+    h = (mean + torch.randn(m, n, device=DEV, generator=g)).to(FP)
+    w = torch.ones(n, device=DEV)
+    o = pkg.layer_norm(h, w)
+    d, r = h.double() - o.mean.double()[:, None], o.rstd.double()[:, None]
+    gy = (d * r + 0.01 * torch.randn(m, n, device=DEV, generator=g)).to(FP)
+    gx, gw, gb = pkg.layer_norm_backward(gy, h, w, o.mean, o.rstd)
+    v = gy.double()
+    want = r * (v - v.mean(1, keepdim=True)) - d * r**3 * (v * d).mean(1, keepdim=True)
+    size = r * (v.abs() + v.abs().mean(1, keepdim=True)) + d.abs() * r**3 * (v * d).abs().mean(1, keepdim=True)
+    assert bool(((gx.double() - want).abs() <= HALF[FP] * (want.abs() + F * size) + F * size + TINY[FP]).all())
+    for got, t in ((gw, v * d * r), (gb, v)):
+        off = F * t.abs().sum(0)
+        assert bool(((got.double() - t.sum(0)).abs() <= HALF[F32] * (t.sum(0).abs() + off) + off).all())
