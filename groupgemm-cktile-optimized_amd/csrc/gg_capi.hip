@@ -20,6 +20,7 @@
 
 #include "gg_few.h"
 #include "gg_i8.h"
+#include "gg_i8_choice.h"
 #include "gg_grouped_gemm.h"
 #include "gg_kernel.h"
 
@@ -934,36 +935,15 @@ int noalloc_scratch(void **out) {
 enum TableMemory { kOwned, kScratch, kGiven };
 size_t device_table_bytes(int group_num) { return size_t(group_num) * sizeof(gg::GroupEntry) + sizeof(gg::TableHeader); }
 
-// Short tiles (192 x 256) for an int8 plan, whose sizes only the device knows. A K step of one takes kShortStep of a
-// 256 x 256 tile's, so they pay where they need no more rounds of workgroups (and not where the GPU is full of rows:
-// every byte of w is staged for fewer of them). The tiles of a group are expected from `rows` rows spread over the
-// groups as a router spreads them (the octiles' means of a gamma distribution of shape 6), and the count is sure to
-// about n_tiles sqrt(group_num / 12), the spread of the groups' last tiles: rounds are averaged over three counts that
-// far apart, and a gain of 5 % on average is taken if the worst case loses no more than 12 %. us, 256 and 192 rows:
-// taken 8 groups of 4160 rows in all, 7168 x 2048 88 -> 72; the same, 4096 x 7168 144 -> 124; 8320 rows 220 -> 200;
-// 1200 78 -> 70; left 32768 rows 696 (707), 32 x 16640, 2880 x 2880 164 (169), 1 x 2048, 7168 x 2048 32 (43), 16 x 20000,
-// 1408 x 2048 58 (66); missed 64 x 8192, 2048 x 1408 66 (58). GG_SHORT=0 or 1 in the environment decides it.
-constexpr double kShortStep = 0.83;
+// Short tiles (192 x 256) for an int8 plan, whose sizes only the device knows (short_tiles_pay). GG_SHORT=0 or 1 in the
+// environment decides it.
+static_assert(gg::kTileM == 256 && gg::kShortTileM == 192, "short_tiles_pay");
 bool use_short_i8(int group_num, int64_t rows, int64_t n_tiles, int64_t k_tiles, int cus) {
     if (group_num > gg::kInKernelTableGroups || k_tiles < gg::kCrossMinStepsHost)
         return false;
     if (const char *env = std::getenv("GG_SHORT"); env != nullptr && *env != '\0')
         return std::atoi(env) != 0;
-    const auto rounds = [&](int tile_m, double *all) { // on average; all: of the three counts
-        constexpr double kShare[8] = {0.45, 0.62, 0.75, 0.87, 0.99, 1.13, 1.32, 1.78};
-        const double     average   = double(rows) / group_num;
-        double           tiles     = 0.0;
-        for (double share : kShare)
-            tiles += std::ceil(group_num == 1 ? average / tile_m : share * average / tile_m);
-        tiles *= double(group_num) / 8 * n_tiles;
-        const double spread = group_num == 1 ? 0.0 : std::sqrt(group_num / 12.0) * std::min(1.0, average / tile_m) * n_tiles;
-        for (int i = 0; i < 3; ++i)
-            all[i] = std::max(1.0, std::ceil((tiles + 1.22 * (i - 1) * spread) / cus));
-        return (all[0] + all[1] + all[2]) / 3;
-    };
-    double       wide[3], narrow[3];
-    const double w = rounds(gg::kTileM, wide), s = rounds(gg::kShortTileM, narrow);
-    return kShortStep * s < 0.95 * w && kShortStep * narrow[2] < 1.12 * wide[0];
+    return gg::short_tiles_pay(group_num, rows, n_tiles, cus);
 }
 
 int plan_device_lens(gg_plan *plan, TableMemory memory, void *given, int op, int a_dtype, int b_dtype, int group_num,
