@@ -16,7 +16,7 @@ from typing import NamedTuple, Optional
 
 import torch
 
-from . import GG_OK, DType, GGError, _device_sizes, load_library
+from . import GG_ERR_UNSUPPORTED, GG_OK, DType, GGError, _device_sizes, load_library
 
 _T16 = {torch.bfloat16: int(DType.BF16), torch.float16: int(DType.FP16)}
 _T8 = {torch.float8_e4m3fn: int(DType.FP8_E4M3), torch.float8_e5m2: int(DType.FP8_E5M2)}
@@ -331,7 +331,7 @@ def silu_product_backward(grad_y, gu, out=None, stream: Optional[int] = None):
 
 def quantize_rows(x, out=None, stream: Optional[int] = None) -> ScaledRows:
     """int8 rows of x [M, N] (bf16 or fp16, rows contiguous at any stride) and a scale for each (gg_quantize_rows):
-    scale = max |x| / 127 (1 for a row of zeros), y = x / scale rounded to the nearest, halves to even."""
+    scale = max |x| / 127 (1 for a row of zeros), y = x / scale rounded to the nearest, halves to even. N at most 32768."""
     if stream is not None:
         return _on(stream, quantize_rows, x, out)
     dt = _T16.get(x.dtype)
@@ -686,10 +686,10 @@ def grouped_gemm_i8(x, w: I8Weights, group_m, x_scale=None, out_dtype=None, out=
                     group_offs=None):
     """out [sum(M), N] = x[rows of g] @ w[g]^T in 8-bit integers (gg_gemm_i8): x int8 [sum(M), K] with x_scale [sum(M)]
     float32, the ScaledRows of layer_norm, silu_product, quantize_rows or dispatch_scaled, to out_dtype (bfloat16 if None,
-    or float16); or x bfloat16 or float16, whose rows are first rounded by quantize_rows, to x's type. group_m as in
-    grouped_gemm: a host sequence of row counts, or a device int64 tensor [B] that is never read on the host (with
-    optional device offsets); a device group that does not lie inside x gets no work, and rows of no group are not
-    written. For any number of rows. No backward pass: train in 16 bits."""
+    or float16), K below 131072; or x bfloat16 or float16, whose rows are first rounded by quantize_rows, to x's type, K at
+    most 32768. group_m as in grouped_gemm: a host sequence of row counts, or a device int64 tensor [B] that is never read
+    on the host (with optional device offsets); a device group that does not lie inside x gets no work, and rows of no group
+    are not written. For any number of rows. No backward pass: train in 16 bits."""
     if stream is not None:
         return _on(stream, grouped_gemm_i8, x, w, group_m, x_scale, out_dtype, out, None, group_offs)
     q, scales = w
@@ -711,6 +711,8 @@ def grouped_gemm_i8(x, w: I8Weights, group_m, x_scale=None, out_dtype=None, out=
     elif x.dtype in _T16:
         if x_scale is not None or out_dtype not in (None, x.dtype):
             raise ValueError("x_scale and out_dtype go with an int8 x")
+        if k > 32768:  # quantize_rows' limit, in this call's words
+            raise GGError(GG_ERR_UNSUPPORTED, "K must be at most 32768 for x of 16 bits; int8 x may have K below 131072")
         out_dtype = x.dtype
     else:
         raise TypeError("x must be int8, bfloat16 or float16")
