@@ -9,8 +9,8 @@
 // pieces of 8 values are dealt to the lanes one after the other. An int8 row's scale needs its largest |y| before the
 // first value is rounded: the row's values stay in registers, as in the norms.
 //
-// Measured (us): 32768 rows of 2048 bf16 60 (6.7 TB/s), to int8 57 (5.9), backward 98 (6.8); 16640 of 2880 fp16 to int8 40.5
-// (5.9); 33 of 2048 to int8 3.4, a launch and a row's latency. Rounding alone, 4160 of 2048: 8.
+// Measured (us): 32768 rows of 2048 bf16 60 (6.7 TB/s), to int8 57 (5.9), backward 97 (6.9); 16640 of 2880 fp16 to int8 40.6
+// (5.9); 33 of 2048 to int8 3.3, a launch and a row's latency. Rounding alone, 4160 of 2048: 8.
 #include <algorithm>
 
 #include "gg_row.h"

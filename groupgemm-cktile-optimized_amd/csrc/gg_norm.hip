@@ -3,8 +3,9 @@
 //
 // Forward: h = round(x + r), rstd = (mean h^2 + eps)^-1/2, y = h rstd w; layer norm (CENTER) takes h less its mean, in
 // the mean square too, and adds a bias. A row stays in the registers
-// of the waves that work on it (one wave up to 1024 values, four up to 16384, of few rows up to 2048, else sixteen), so
-// x and r are read once and h and y written once: bound by HBM. The tensor scale needs the largest |y|
+// of the waves that work on it (the RMS norm's: one wave up to 1024 values, four up to 16384, of few rows up to 2048, else
+// sixteen, with_shape; the layer norm's: with_center_forward, and center_shape for its gradients), so x and r are read once
+// and h and y written once: bound by HBM. The tensor scale needs the largest |y|
 // of all rows before the first value is rounded: a first pass writes h, rstd and one maximum per
 // workgroup, a second reads h again and rounds.
 //
@@ -14,8 +15,9 @@
 // Measured: 32768 rows of 7168, bf16 with residual to fp8 with a tensor scale, 377 us: 245 for the first pass (x and r
 // read, h written: 5.8 TB/s) and 133 for the second (h read, y written: 5.3); 5 rows to bf16 3.8, the latency of a launch,
 // a row's loads and a barrier. Backward 16640 x 2880 with a gradient past the norm: 75 us, 5.1 TB/s (69 row by row, 6 for
-// the weight's gradient). Layer norm: 32768 rows of 4096 bf16 86 us (6.2 TB/s), 8192 of 7168 with residual to int8 72 (5.7),
-// 6 of 7168 4.7; backward 16640 x 2880 with a gradient past the norm 79 (4.9 TB/s; 5 of it for the two sums), 1024 x 8192 27.
+// the weight's gradient). 8192 of 7168 with residual to int8 73 (5.6). Layer norm: 32768 rows of 4096 bf16 87.5 us (6.2 TB/s),
+// 8192 of 7168 with residual to int8 75 (5.5), to fp8 with a scale a row 85 (4.8), for the tensor 62 + 36; 6 of 7168 4.7;
+// backward 16640 x 2880 with a gradient past the norm 76 + 5 for the two sums (5.2 TB/s), 1024 x 8192 26.
 #include "gg_row.h"
 
 #include <algorithm>

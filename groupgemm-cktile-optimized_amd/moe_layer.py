@@ -331,7 +331,8 @@ def silu_product_backward(grad_y, gu, out=None, stream: Optional[int] = None):
 
 def quantize_rows(x, out=None, stream: Optional[int] = None) -> ScaledRows:
     """int8 rows of x [M, N] (bf16 or fp16, rows contiguous at any stride) and a scale for each (gg_quantize_rows):
-    scale = max |x| / 127 (1 for a row of zeros), y = x / scale rounded to the nearest, halves to even. N at most 32768."""
+    scale = max |x| / 127 (1 where that is zero or subnormal), y = x / scale rounded to the nearest, halves to even. A row with
+    a NaN or an infinity has that for a scale and holds zeros. N at most 32768."""
     if stream is not None:
         return _on(stream, quantize_rows, x, out)
     dt = _T16.get(x.dtype)
