@@ -676,8 +676,8 @@ __global__ void __launch_bounds__(64 * WPR * R) center_back_kernel(const CenterA
             }
         }
         row_sums<WPR>(m[own], turn, sum, dot, wave, lane);
-        // The row's loads are all back (vmcnt 0) for lanes past its end, too: else the compiler lets each of the next row's
-        // wait for the one before it (4096 x 14336 105 instead of 100 us).
+        // vmcnt 0: the row's loads are back. Said once here, or the compiler, which sees lanes past the row's end that wait for
+        // none, has each of the next row's loads wait for the one before it (4096 x 14336 105 instead of 101 us).
         __builtin_amdgcn_s_waitcnt(0x0f70);
         const float n  = static_cast<float>(a.hidden);
         const float c1 = sum / n, c2 = rstd * (rstd * (dot / n)); // of w g and of d in grad_x / rstd (rstd^2 alone may be past float32)
@@ -689,9 +689,8 @@ __global__ void __launch_bounds__(64 * WPR * R) center_back_kernel(const CenterA
                 unpack8<T>(kKeep ? gw[u] : load_once(gp + i), g);
                 unpack8<T>(kKeep ? hw[u] : load_once(hp + i), h);
                 load_w<T>(a.weight, a.w32, i, w);
-// (h - mean first: c2 h - c2 mean would cancel where the mean is large)
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 8; ++j) // h - mean first: c2 h - c2 mean would cancel where the mean is large
                     g[j] = fmaf(-c2, h[j] - mean, fmaf(g[j], w[j], -c1));
                 if (rp != nullptr) {
                     unpack8<T>(kKeep ? rw[u] : load_once(rp + i), r);
